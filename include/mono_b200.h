@@ -629,8 +629,95 @@ int mono_gqa_score_launch(const mono_gqa_args* a, void* stream);
 int mono_gqa_select_launch(const mono_gqa_args* a, void* stream);
 int mono_gqa_attn_launch(const mono_gqa_args* a, void* stream);
 
+/* ---- q | k | v rows -> normed, rotated queries and the paged K / V caches --------------
+ * Per q and k head RMSNorm over 128 dims with weight 1 + g (g_q / g_k NULL: none), rotation of
+ * the first rot_dim dims (a multiple of 16) with table row positions[t] (clamped to the table) in pairs (i, i + rot_dim / 2)
+ * or, interleaved, (2i, 2i + 1).  q goes to q_out as bf16; k and v as E4M3 of value / scale, saturating, to cache slot
+ * slots[t] = page * 64 + offset of caches [page][64][kv_heads][128]; a slot outside the cache (negative: a pad row), or
+ * slots == NULL, inserts nothing.  f32 arithmetic, one rounding at each store.  Slots of one launch are distinct. */
+typedef struct mono_qkv_append_args {
+    int tokens, q_heads, kv_heads, rot_dim, interleaved;
+    const void* src_bf16; /* bf16 [tokens][src_ld]: q heads | k heads | v heads; or NULL and */
+    const float* src_f32; /* f32 partial sums [nsum][..][src_ld], sum_stride apart; at most 16 tokens */
+    int nsum;
+    long src_ld, sum_stride; /* multiples of 8 and 4 values */
+    const void* g_q;         /* bf16 [128] */
+    const void* g_k;
+    float eps;
+    const void* cos; /* [table_rows][rot_dim / 2], bf16 or f32 */
+    const void* sin;
+    int table_f32;
+    int64_t table_rows;
+    const int64_t* positions; /* [tokens] */
+    const int64_t* slots;     /* [tokens] */
+    float k_scale, v_scale;
+    uint8_t* k_cache;
+    uint8_t* v_cache;
+    int64_t n_pages;
+    void* q_out; /* bf16 [tokens][q_heads][128] */
+} mono_qkv_append_args;
+int mono_qkv_append_launch(const mono_qkv_append_args* a, void* stream);
+
+/* ---- attention of a batch whose sequences share prefixes, over the paged K / V caches ----
+ * Sequence b has query tokens q_start[b] .. q_start[b + 1] - 1 and lens[b] keys of its own (those of its query tokens
+ * included) in pages page_table[b][..]; group g's sequences group_start[g] .. group_start[g + 1] - 1 share the first
+ * prefix_lens[g] keys in pages prefix_table[g][..].  Token j of a sequence's n sees its group's prefix and the
+ * sequence's keys 0 .. lens[b] - n + j.  out = softmax((q . k) k_scale sm_scale) v v_scale; a token that sees no key
+ * gives zeros, tokens of no sequence keep their output row.  A page number outside the cache counts as a page without
+ * keys.  Lengths beyond their table's columns are cut.  Both starts must never fall and stay in range: otherwise the
+ * guard's argument word is set and the output is not valid.  The tables are device data: a captured launch follows them. */
+typedef struct mono_prefix_attn_args {
+    int tokens, q_heads, kv_heads, seqs, groups; /* at most 16 q heads per kv head, seqs + groups <= 2048 */
+    const void* q;                               /* bf16 [tokens][q_ld]: q_heads x 128 */
+    long q_ld;
+    const uint8_t* k_cache; /* [n_pages][64][kv_heads][128] E4M3 */
+    const uint8_t* v_cache;
+    int64_t n_pages;
+    const int32_t* q_start;    /* [seqs + 1] */
+    const int32_t* page_table; /* [seqs][pt_ld] */
+    int pt_ld;
+    const int32_t* lens;         /* [seqs] */
+    const int32_t* group_start;  /* [groups + 1] */
+    const int32_t* prefix_table; /* [groups][prefix_ld] */
+    int prefix_ld;
+    const int32_t* prefix_lens; /* [groups] */
+    float k_scale, v_scale, sm_scale;
+    void* scratch; /* mono_prefix_attn_scratch_bytes(tokens, q_heads, kv_heads, seqs, groups); one launch at a time */
+    size_t scratch_bytes;
+    void* out; /* bf16 [tokens][q_heads][128] */
+    int32_t* guard;
+    uint64_t wait_ns; /* limit of every device wait; 0 = default */
+} mono_prefix_attn_args;
+size_t mono_prefix_attn_scratch_bytes(int tokens, int q_heads, int kv_heads, int seqs, int groups);
+int mono_prefix_attn_launch(const mono_prefix_attn_args* a, void* stream);
+
+/* ---- next tokens from logits and given random numbers ------------------------------------
+ * Row r: w_i = exp((l_i - max) / T), T = temperature[r]; the tokens in order of (logit descending, index ascending); kept is
+ * the front part with rank < top_k, mass before the token < top_p x the whole mass, and w_i >= min_p, at least the first
+ * token.  The drawn token is the first, by index, whose running kept mass passes u x the kept mass.  T <= 0 (or NaN) takes the
+ * first of the order; top_k < 1, top_p >= 1 (or NaN) and min_p <= 0 (or NaN) filter nothing, and so do NULL arrays
+ * (temperature NULL: 1).  logprobs[r] = log(w / whole mass) of the drawn token before any filter (T <= 0: at T = 1).
+ * NaN logits count as -inf; a row without a logit above -inf gives token -1 and logprob -inf.  u is taken as 0 below 0
+ * (or NaN), and at 1 or above draws the last kept token. */
+#define MONO_SAMPLE_MAX_VOCAB 393216
+typedef struct mono_sample_args {
+    int rows, vocab;
+    const void* logits; /* f32 or bf16 [rows][ld] */
+    int logits_bf16;
+    long ld;
+    const float* u; /* [rows] in [0, 1) */
+    const float* temperature;
+    const int32_t* top_k;
+    const float* top_p;
+    const float* min_p;
+    int64_t* tokens; /* [rows] */
+    float* logprobs; /* [rows] or NULL */
+} mono_sample_args;
+int mono_sample_launch(const mono_sample_args* a, void* stream);
+
 /* sizeof() of the argument structs, by index (0 gemv_job, 1 gemv_args, 2 act_prep,
- * 3 route, 4 mid, 5 sparse_mla, 6 reduce, 7 rowdot, ..., 11 gqa, 12 logits_gather): lets a binding check its mirror. */
+ * 3 route, 4 mid, 5 sparse_mla, 6 reduce, 7 rowdot, ..., 11 gqa, 12 logits_gather, 13 prefetch,
+ * 14 qkv_append, 15 prefix_attn, 16 sample): lets a binding check its mirror. */
 size_t mono_struct_size(int which);
 
 #ifdef __cplusplus

@@ -163,8 +163,39 @@ class LogitsGatherArgs(C.Structure):
     ]
 
 
+class QkvAppendArgs(C.Structure):
+    _fields_ = [
+        ("tokens", i32), ("q_heads", i32), ("kv_heads", i32), ("rot_dim", i32), ("interleaved", i32),
+        ("src_bf16", vp), ("src_f32", vp), ("nsum", i32), ("src_ld", i64), ("sum_stride", i64),
+        ("g_q", vp), ("g_k", vp), ("eps", f32), ("cos", vp), ("sin", vp), ("table_f32", i32),
+        ("table_rows", C.c_int64), ("positions", vp), ("slots", vp), ("k_scale", f32), ("v_scale", f32),
+        ("k_cache", vp), ("v_cache", vp), ("n_pages", C.c_int64), ("q_out", vp),
+    ]
+
+
+class PrefixAttnArgs(C.Structure):
+    _fields_ = [
+        ("tokens", i32), ("q_heads", i32), ("kv_heads", i32), ("seqs", i32), ("groups", i32),
+        ("q", vp), ("q_ld", i64), ("k_cache", vp), ("v_cache", vp), ("n_pages", C.c_int64),
+        ("q_start", vp), ("page_table", vp), ("pt_ld", i32), ("lens", vp),
+        ("group_start", vp), ("prefix_table", vp), ("prefix_ld", i32), ("prefix_lens", vp),
+        ("k_scale", f32), ("v_scale", f32), ("sm_scale", f32), ("scratch", vp), ("scratch_bytes", C.c_size_t),
+        ("out", vp), ("guard", vp), ("wait_ns", u64),
+    ]
+
+
+class SampleArgs(C.Structure):
+    _fields_ = [
+        ("rows", i32), ("vocab", i32), ("logits", vp), ("logits_bf16", i32), ("ld", i64), ("u", vp),
+        ("temperature", vp), ("top_k", vp), ("top_p", vp), ("min_p", vp), ("tokens", vp), ("logprobs", vp),
+    ]
+
+
+SAMPLE_MAX_VOCAB = 393216
+
 _STRUCTS = [GemvJob, GemvArgs, ActPrepArgs, RouteArgs, MidArgs, SparseMlaArgs, ReduceArgs, RowdotArgs,
-            MlaMidArgs, QPostArgs, IndexArgs, GqaArgs, LogitsGatherArgs, PrefetchArgs]
+            MlaMidArgs, QPostArgs, IndexArgs, GqaArgs, LogitsGatherArgs, PrefetchArgs,
+            QkvAppendArgs, PrefixAttnArgs, SampleArgs]
 
 # every symbol include/mono_b200.h declares: name -> (restype, argtypes)
 SYMBOLS = {
@@ -206,6 +237,10 @@ SYMBOLS = {
     "mono_gqa_score_launch": (i32, [C.POINTER(GqaArgs), vp]),
     "mono_gqa_select_launch": (i32, [C.POINTER(GqaArgs), vp]),
     "mono_gqa_attn_launch": (i32, [C.POINTER(GqaArgs), vp]),
+    "mono_qkv_append_launch": (i32, [C.POINTER(QkvAppendArgs), vp]),
+    "mono_prefix_attn_scratch_bytes": (C.c_size_t, [i32, i32, i32, i32, i32]),
+    "mono_prefix_attn_launch": (i32, [C.POINTER(PrefixAttnArgs), vp]),
+    "mono_sample_launch": (i32, [C.POINTER(SampleArgs), vp]),
     "mono_struct_size": (C.c_size_t, [i32]),
     "mono_launch_count": (C.c_ulonglong, []),
     "mono_peer_alloc": (i32, [C.c_size_t, C.POINTER(vp)]),

@@ -234,6 +234,9 @@ extern "C" size_t mono_struct_size(int which) {
         case 11: return sizeof(mono_gqa_args);
         case 12: return sizeof(mono_logits_gather_args);
         case 13: return sizeof(mono_prefetch_args);
+        case 14: return sizeof(mono_qkv_append_args);
+        case 15: return sizeof(mono_prefix_attn_args);
+        case 16: return sizeof(mono_sample_args);
         default: return 0;
     }
 }

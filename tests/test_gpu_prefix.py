@@ -1,0 +1,415 @@
+"""Cache append and shared-prefix attention on the GPU through the public ops, against the 64-bit restatement."""
+
+import pytest
+import torch
+
+from oracle import prefix as OP
+from sgl_amd_mono_b200 import _lib as L
+from sgl_amd_mono_b200 import ops
+from sgl_amd_mono_b200.prefix import PrefixTables, QkvAppendOp, SharedPrefixAttnOp
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+K_SCALE, V_SCALE = 0.0625, 0.046875
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+# ---------------------------------------------------------------- append
+def _append_inputs(tokens, hq, hk, rot, table=torch.bfloat16, seed=0, pages=None):
+    g = _gen(seed)
+    pages = pages or -(-tokens // 64) + 2
+    x = torch.randn(tokens, (hq + 2 * hk) * 128, generator=g)
+    ang = torch.arange(512, dtype=torch.float64)[:, None] / 1e4 ** (torch.arange(0, rot, 2, dtype=torch.float64) / rot)
+    d = dict(x=x.bfloat16(), g_q=(torch.randn(128, generator=g) * 0.2).bfloat16(), g_k=(torch.randn(128, generator=g) * 0.2).bfloat16(),
+             cos=ang.cos().to(table), sin=ang.sin().to(table), positions=torch.randint(0, 512, (tokens,), generator=g),
+             slots=torch.randperm(pages * 64, generator=g)[:tokens])
+    caches = [(torch.randn(pages, 64, hk, 128, generator=g) * 16).to(torch.float8_e4m3fn).view(torch.uint8) for _ in range(2)]
+    return d, caches
+
+
+def _check_append(q, kc, vc, x, d, caches, hq, hk, interleaved, norm=True, eps=1e-6):
+    gq, gk = (d["g_q"], d["g_k"]) if norm else (None, None)
+    rq, rk, rv = OP.append_rows(x, hq, hk, gq, gk, eps, d["cos"], d["sin"], d["positions"], interleaved)
+    # f32 arithmetic: a norm is a 128-term sum, a root and two products (relative 2^-20 of the value at most), a
+    # rotation adds two products of the pair's size
+    slack = 2.0**-19
+    top = rq.abs().amax(-1, keepdim=True)
+    assert torch.isfinite(q.float()).all()
+    assert ((q.cpu().double() - rq).abs() <= rq.abs() * 2.0**-8 + top * slack).all()
+    for got, before, ref, scale in ((kc, caches[0], rk, K_SCALE), (vc, caches[1], rv, V_SCALE)):
+        want = OP.cache_values(before).reshape(-1, hk, 128)
+        tol = torch.zeros_like(want)
+        live = (d["slots"] >= 0) & (d["slots"] < want.shape[0])
+        v = (ref / scale).clamp(-448, 448)
+        at = d["slots"][live]
+        want[at] = v[live]
+        # E4M3: half a step is 2^-4 of the value, or 2^-10 below the smallest normal number
+        tol[at] = (v.abs() * 2.0**-4).clamp(min=2.0**-10)[live] + v.abs().amax(-1, keepdim=True)[live] * slack
+        have = OP.cache_values(got.cpu()).reshape(-1, hk, 128)
+        assert ((have - want).abs() <= tol).all()
+        # the other slots keep their bytes
+        rest = torch.ones(want.shape[0], dtype=torch.bool)
+        rest[at] = False
+        assert torch.equal(got.cpu().reshape(-1, hk, 128)[rest], before.reshape(-1, hk, 128)[rest])
+
+
+@pytest.mark.parametrize("tokens,hq,hk,rot,interleaved,table", [
+    (1, 1, 1, 64, False, torch.bfloat16), (1, 12, 2, 64, False, torch.float32), (5, 3, 3, 16, True, torch.bfloat16),
+    (16, 12, 2, 128, False, torch.bfloat16), (33, 7, 1, 48, False, torch.float32), (33, 5, 5, 96, True, torch.float32),
+    (700, 48, 8, 64, True, torch.bfloat16), (1203, 20, 4, 112, False, torch.bfloat16)])
+def test_append_rows(tokens, hq, hk, rot, interleaved, table):
+    d, caches = _append_inputs(tokens, hq, hk, rot, table)
+    op = QkvAppendOp(hq, hk, DEV, max_tokens=tokens, rot_dim=rot, interleaved=interleaved, k_scale=K_SCALE, v_scale=V_SCALE)
+    kc, vc = (c.to(DEV) for c in caches)
+    q = op(d["x"].to(DEV), *(d[k].to(DEV) for k in ("g_q", "g_k", "cos", "sin", "positions", "slots")), kc, vc)
+    _check_append(q, kc, vc, d["x"], d, caches, hq, hk, interleaved)
+
+
+def test_append_strided_rows_pads_far_positions_and_no_norm():
+    tokens, hq, hk = 70, 12, 2
+    d, caches = _append_inputs(tokens, hq, hk, 64)
+    wide = torch.full((tokens, 2048 + 24), float("nan"), dtype=torch.bfloat16)
+    wide[:, 8 : 8 + 2048] = d["x"]
+    d["slots"][[0, 3]] = -1
+    d["slots"][5] = caches[0].shape[0] * 64  # behind the cache: inserts nothing
+    d["positions"][[1, 2]] = torch.tensor([-7, 10**12])
+    op = QkvAppendOp(hq, hk, DEV, max_tokens=128, k_scale=K_SCALE, v_scale=V_SCALE)
+    kc, vc = (c.to(DEV) for c in caches)
+    q = op(wide.to(DEV)[:, 8 : 8 + 2048], None, None, *(d[k].to(DEV) for k in ("cos", "sin", "positions", "slots")), kc, vc)
+    _check_append(q, kc, vc, d["x"], d, caches, hq, hk, False, norm=False)
+    # without slots nothing is inserted
+    k2 = kc.clone()
+    op(d["x"].to(DEV), None, None, *(d[k].to(DEV) for k in ("cos", "sin", "positions")), None, kc, vc)
+    assert torch.equal(k2, kc)
+
+
+@pytest.mark.parametrize("tokens,nsum", [(1, 1), (16, 3), (9, 7)])
+def test_append_from_partial_sums(tokens, nsum):
+    hq, hk = 12, 2
+    d, caches = _append_inputs(tokens, hq, hk, 64)
+    parts = torch.randn(nsum, 16, 2048, generator=_gen(3))
+    op = QkvAppendOp(hq, hk, DEV, max_tokens=16, k_scale=K_SCALE, v_scale=V_SCALE)
+    kc, vc = (c.to(DEV) for c in caches)
+    q = op(parts.to(DEV), *(d[k].to(DEV) for k in ("g_q", "g_k", "cos", "sin", "positions", "slots")), kc, vc, tokens=tokens)
+    # the f32 sum of the parts is the operator's input: added in order, as the kernel does
+    x = torch.zeros(16, 2048)
+    for p in parts:
+        x = x + p
+    _check_append(q, kc, vc, x[:tokens], d, caches, hq, hk, False)
+
+
+def test_append_extreme_values():
+    hq, hk = 2, 1
+    d, caches = _append_inputs(4, hq, hk, 64)
+    x = d["x"].float().view(4, 4, 128)
+    x[0] = 0  # a zero head stays zero under eps
+    x[1] *= 1e4  # saturates V
+    x[2, 3, 5] = float("inf")
+    x[3, 3, 7] = float("nan")
+    op = QkvAppendOp(hq, hk, DEV, max_tokens=4, k_scale=K_SCALE, v_scale=V_SCALE)
+    kc, vc = (c.to(DEV) for c in caches)
+    q = op(x.bfloat16().view(4, -1).to(DEV), *(d[k].to(DEV) for k in ("g_q", "g_k", "cos", "sin", "positions", "slots")), kc, vc)
+    v = OP.cache_values(vc.cpu()).reshape(-1, 128)[d["slots"]]
+    assert (q[0] == 0).all() and (v[0] == 0).all()
+    assert v[1].abs().max() == 448
+    assert v[2, 5] == 448 and torch.isfinite(v[2]).all()
+    assert torch.isnan(v[3, 7]) and torch.isnan(v[3]).sum() == 1
+    assert torch.isfinite(q).all()
+
+
+def test_append_far_cache_offsets():
+    """Slots behind 2^31 bytes of a cache (and the attention that reads them) use 64-bit offsets."""
+    pages, hk, hq = 33000, 8, 8  # 2.16 GB a cache
+    kc, vc = (torch.zeros(pages, 64, hk, 128, dtype=torch.uint8, device=DEV) for _ in range(2))
+    d, _ = _append_inputs(64, hq, hk, 64, pages=4)
+    d["slots"] = (pages - 1) * 64 + torch.arange(64)
+    op = QkvAppendOp(hq, hk, DEV, max_tokens=64, k_scale=K_SCALE, v_scale=V_SCALE)
+    q = op(d["x"].to(DEV), *(d[k].to(DEV) for k in ("g_q", "g_k", "cos", "sin", "positions", "slots")), kc, vc)
+    last = [c[-1:].cpu() for c in (kc, vc)]
+    d2 = dict(d, slots=torch.arange(64))
+    _check_append(q, last[0], last[1], d["x"], d2, [torch.zeros(1, 64, hk, 128, dtype=torch.uint8)] * 2, hq, hk, False)
+    assert int(kc[:-1].count_nonzero()) == 0
+    attn = SharedPrefixAttnOp(hq, hk, DEV, max_tokens=1, max_seqs=1, k_scale=K_SCALE, v_scale=V_SCALE)
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32)  # noqa: E731
+    t = PrefixTables(i32(0, 1), i32(pages - 1).view(1, 1), i32(64))
+    out = attn(q[63:64], kc, vc, _dev(t))
+    _check_attend(out, q[63:64].cpu(), last, PrefixTables(t.q_start, i32(0).view(1, 1), t.lens), attn)
+
+
+# ---------------------------------------------------------------- attention
+def _dev(t: PrefixTables) -> PrefixTables:
+    return PrefixTables(*(None if x is None else x.to(DEV) for x in (t.q_start, t.page_table, t.lens, t.group_start, t.prefix_table, t.prefix_lens)))
+
+
+def _tables(ntok, own, starts, prefix, seed=0, spare=1, columns=0):
+    """Tables over pages in random order; returns (tables, pages)."""
+    need = [-(-n // 64) for n in list(prefix) + list(own)]
+    pages = sum(need) + spare
+    order = torch.randperm(pages, generator=_gen(seed)).to(torch.int32)
+    rows, at = [], 0
+    for n in need:
+        rows.append(order[at : at + n])
+        at += n
+
+    def table(part, extra):
+        w = max([len(r) for r in part] + [1]) + extra
+        t = torch.full((len(part), w), -1, dtype=torch.int32)
+        for i, r in enumerate(part):
+            t[i, : len(r)] = r
+        return t
+
+    i32 = lambda v: torch.tensor(list(v), dtype=torch.int32)  # noqa: E731
+    q_start = i32([0] + torch.tensor(ntok).cumsum(0).tolist())
+    p = len(prefix)
+    if not p:
+        return PrefixTables(q_start, table(rows, columns), i32(own)), pages
+    return PrefixTables(q_start, table(rows[p:], columns), i32(own), i32(starts), table(rows[:p], columns), i32(prefix)), pages
+
+
+def _caches(pages, hk, seed=1):
+    g = _gen(seed)
+    return [(torch.randn(pages, 64, hk, 128, generator=g) * 16).to(torch.float8_e4m3fn).view(torch.uint8) for _ in range(2)]
+
+
+def _check_attend(out, q, caches, t, op, rows=None):
+    ref, mag, big, seen = OP.attend(q, *caches, t.q_start, t.page_table, t.lens, t.group_start, t.prefix_table, t.prefix_lens,
+                                    op.k_scale, op.v_scale, op.sm_scale)
+    # weights: f16 rounding 2^-11; a score is 128 products added in f32 steps that may truncate (2^-23 of the running
+    # sum each) and enters numerator and denominator; the value sums add one step per 16 keys; the store rounds to bf16
+    tol = ref.abs() * 2.0**-8 + mag * (2.0**-11 + 2 * (128 * 2.0**-23 * big[..., None] + 2.0**-20) + (seen[:, None, None] / 16 + 16) * 2.0**-23)
+    live = ~torch.isnan(ref) if rows is None else rows
+    err = (out.cpu().double() - ref).abs()
+    assert (err[live] <= tol[live]).all(), f"off by {(err - tol)[live].max():.3g} beyond the bound, {int((err > tol)[live].sum())} values"
+    return ref
+
+
+def _attend(hq, hk, ntok, own, starts, prefix, seed=0, columns=0, qmul=2.0, **kw):
+    t, pages = _tables(ntok, own, starts, prefix, seed, columns=columns)
+    caches = _caches(pages, hk)
+    tokens = sum(ntok)
+    q = (torch.randn(tokens, hq, 128, generator=_gen(seed + 5)) * qmul).bfloat16()
+    op = SharedPrefixAttnOp(hq, hk, DEV, max_tokens=tokens, max_seqs=len(own), max_groups=max(1, len(prefix)), k_scale=K_SCALE, v_scale=V_SCALE, **kw)
+    dc = [c.to(DEV) for c in caches]
+    out = op(q.to(DEV), *dc, _dev(t))
+    torch.cuda.synchronize()
+    rc, words = ops.guard_read(op.guard)
+    assert rc == 0, f"guard words {words}"
+    _check_attend(out, q, caches, t, op)
+    return op, q, caches, dc, t, out
+
+
+@pytest.mark.parametrize("hq,hk,ntok,own,starts,prefix", [
+    (1, 1, [1], [1], [0, 1], [1]),                                   # one key each
+    (12, 2, [1], [64], [], []),                                      # no prefix, a whole page
+    (12, 2, [1] * 4, [1, 63, 64, 65], [0, 4], [129]),                # page borders
+    (8, 8, [1] * 3, [7, 200, 31], [0, 3], [64]),                     # one q head per kv head
+    (16, 1, [1] * 5, [3, 70, 128, 1, 33], [0, 5], [700]),            # sixteen q heads on one
+    (20, 4, [1] * 9, list(range(1, 200, 23))[:9], [0, 2, 3, 9], [300, 1, 65]),  # three groups
+    (12, 2, [1] * 6, [5, 6, 7, 8, 9, 10], [1, 4], [100]),            # some sequences have no group
+    (12, 2, [3, 1, 5, 2], [40, 1, 5, 130], [0, 4], [500]),           # several query tokens, causal
+    (6, 1, [1] * 40, [1 + 7 * i for i in range(40)], [0, 40], [190]),   # more rows than one tile of the prefix
+    (6, 3, [70, 1, 200], [70, 65, 333], [0, 2, 3], [77, 130]),       # prompt chunks
+    (24, 2, [1] * 33, [9] * 33, [0, 33], [1111])])
+def test_attend(hq, hk, ntok, own, starts, prefix):
+    _attend(hq, hk, ntok, own, starts, prefix, columns=2)
+
+
+def test_attend_empty_sides():
+    """No prefix keys, no own keys, neither: the last gives zeros."""
+    hq, hk = 6, 2
+    t, pages = _tables([1, 1, 2, 1], [5, 1, 1, 1], [0, 2, 4], [64, 1], spare=2)
+    t.lens[:] = torch.tensor([5, 0, 1, 0])   # sequence 2: its first token comes before its only key
+    t.prefix_lens[:] = torch.tensor([64, 0])
+    caches = _caches(pages, hk)
+    q = torch.randn(5, hq, 128, generator=_gen(9)).bfloat16()
+    op = SharedPrefixAttnOp(hq, hk, DEV, max_tokens=5, max_seqs=4, max_groups=2, k_scale=K_SCALE, v_scale=V_SCALE)
+    out = op(q.to(DEV), *(c.to(DEV) for c in caches), _dev(t))
+    ref = _check_attend(out, q, caches, t, op)
+    assert (ref[2] == 0).all() and (out[2] == 0).all() and (out[4] == 0).all() and (ref[3] != 0).all()
+
+
+def test_attend_rows_of_no_sequence_keep_their_values():
+    hq, hk = 12, 2
+    t, pages = _tables([1, 2], [30, 70], [0, 2], [100])
+    t.q_start += 1  # token 0 and the tokens behind the last sequence belong to nobody
+    caches = _caches(pages, hk)
+    q = torch.randn(7, hq, 128, generator=_gen(2)).bfloat16()
+    op = SharedPrefixAttnOp(hq, hk, DEV, max_tokens=7, max_seqs=2, k_scale=K_SCALE, v_scale=V_SCALE)
+    mine = torch.full((7, hq, 128), 3.25, dtype=torch.bfloat16, device=DEV)
+    out = op(q.to(DEV), *(c.to(DEV) for c in caches), _dev(t), out=mine)
+    assert out.data_ptr() == mine.data_ptr()
+    _check_attend(out, q, caches, t, op)
+    assert (out[0] == 3.25).all() and (out[4:] == 3.25).all()
+
+
+def test_attend_ignores_what_lies_in_masked_places():
+    """Keys and values behind a length, pages outside the cache and unused columns: NaN bytes there change nothing."""
+    hq, hk = 12, 2
+    op, q, caches, dc, t, out = _attend(hq, hk, [1, 2, 1], [10, 70, 129], [0, 3], [200])
+    want = out.clone()
+    n = [c.clone() for c in caches]
+    for tab, lens in ((t.page_table, t.lens), (t.prefix_table, t.prefix_lens)):
+        for row, ln in zip(tab, lens):
+            full, part = divmod(int(ln), 64)
+            if part:
+                for c in n:
+                    c[int(row[full]), part:] = 0x7F
+    used = set(int(p) for tab in (t.page_table, t.prefix_table) for p in tab.flatten() if p >= 0)
+    for c in n:
+        c[[p for p in range(c.shape[0]) if p not in used]] = 0xFF
+    assert torch.equal(op(q.to(DEV), *(c.to(DEV) for c in n), _dev(t)), want)
+    # a page number outside the cache is a page without keys
+    t2 = PrefixTables(t.q_start, t.page_table.clone(), t.lens, t.group_start, t.prefix_table.clone(), t.prefix_lens)
+    t2.prefix_table[0, 1] = caches[0].shape[0]
+    t2.page_table[2, 0] = -5
+    got = op(q.to(DEV), *dc, _dev(t2))
+    _check_attend(got, q, caches, t2, op)
+    # lengths beyond the columns are cut
+    t3 = PrefixTables(t.q_start, t.page_table[:, :1].contiguous(), t.lens, t.group_start, t.prefix_table, t.prefix_lens)
+    got = op(q.to(DEV), *dc, _dev(t3))
+    _check_attend(got, q, caches, t3, op)
+
+
+def test_attend_sharp_scores_and_nan_rows():
+    """Scores far apart (one key takes all the weight, a sink in another block), and a NaN query: its own rows only."""
+    hq, hk = 12, 2
+    t, pages = _tables([1, 1], [100, 30], [0, 2], [640])
+    caches = _caches(pages, hk)
+    q = (torch.randn(2, hq, 128, generator=_gen(2)) * 30).bfloat16()
+    q[0, 3] = float("nan")
+    q[1, 5] *= 1e-30
+    q[1, 6] = 0
+    op = SharedPrefixAttnOp(hq, hk, DEV, max_tokens=2, max_seqs=2, k_scale=K_SCALE, v_scale=V_SCALE)
+    out = op(q.to(DEV), *(c.to(DEV) for c in caches), _dev(t))
+    assert torch.isnan(out[0, 3]).all() and int(torch.isnan(out).any(-1).sum()) == 1
+    _check_attend(out, q, caches, t, op)
+
+
+def test_attend_strided_queries_and_repeats_to_the_bit():
+    hq, hk = 12, 2
+    op, q, caches, dc, t, out = _attend(hq, hk, [1] * 5, [70] * 5, [0, 5], [900])
+    want = out.clone()
+    wide = torch.full((5, hq * 128 + 512), float("nan"), dtype=torch.bfloat16, device=DEV)
+    wide[:, : hq * 128] = q.to(DEV).view(5, -1)
+    again = op(wide[:, : hq * 128].unflatten(1, (hq, 128)), *dc, _dev(t))
+    assert torch.equal(again, want)
+
+
+def test_attend_in_a_graph_follows_the_tables():
+    hq, hk = 12, 2
+    op, q, caches, dc, t, _ = _attend(hq, hk, [1] * 3, [70, 10, 64], [0, 3], [300], columns=2)
+    dt, qd = _dev(t), q.to(DEV)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            out = op(qd, *dc, dt)
+    torch.cuda.current_stream().wait_stream(side)
+    for lens, plen in (([70, 10, 64], 300), ([3, 1, 2], 17), ([70, 9, 33], 0)):
+        t.lens[:], t.prefix_lens[:] = torch.tensor(lens), plen
+        dt.lens.copy_(t.lens)
+        dt.prefix_lens.copy_(t.prefix_lens)
+        g.replay()
+        torch.cuda.synchronize()
+        _check_attend(out, q, caches, t, op)
+
+
+def test_attend_refuses_starts_that_fall():
+    hq, hk = 12, 2
+    op, q, caches, dc, t, _ = _attend(hq, hk, [1] * 3, [70, 10, 64], [0, 3], [300])
+    bad = _dev(t)
+    bad.q_start.copy_(torch.tensor([0, 3, 0, 3]))
+    op(q.to(DEV), *dc, bad)
+    torch.cuda.synchronize()
+    rc, words = ops.guard_read(op.guard)
+    assert rc != 0 and words[2] == 105  # argument word: the tables' site + 1
+    op.guard.zero_()
+    bad = _dev(t)
+    bad.group_start.copy_(torch.tensor([0, 9]))
+    op(q.to(DEV), *dc, bad)
+    rc, words = ops.guard_read(op.guard)
+    assert rc != 0 and words[2] == 105
+    op.guard.zero_()
+    _check_attend(op(q.to(DEV), *dc, _dev(t)), q, caches, t, op)
+
+
+def test_attend_on_a_side_stream_with_its_own_op():
+    hq, hk = 12, 2
+    a = _attend(hq, hk, [1] * 8, [70] * 8, [0, 8], [2000])
+    b = SharedPrefixAttnOp(hq, hk, DEV, max_tokens=8, max_seqs=8, k_scale=K_SCALE, v_scale=V_SCALE)
+    op, q, caches, dc, t, out = a
+    want, qd, dt = out.clone(), q.to(DEV), _dev(t)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for _ in range(5):
+        with torch.cuda.stream(side):
+            o2 = b(qd, *dc, dt)
+        o1 = op(qd, *dc, dt)
+    torch.cuda.synchronize()
+    assert torch.equal(o1, want) and torch.equal(o2, want)
+
+
+def test_append_then_attend_then_append():
+    """A prompt's rows go to the cache once; three samples of it then take two steps each on the same pages."""
+    hq, hk, eps = 12, 2, 1e-6
+    prompt, seqs = 150, 3
+    pages = 3 + seqs
+    g = _gen(4)
+    width = (hq + 2 * hk) * 128
+    ang = torch.arange(512, dtype=torch.float64)[:, None] / 1e6 ** (torch.arange(0, 64, 2, dtype=torch.float64) / 64)
+    cos, sin = ang.cos().bfloat16(), ang.sin().bfloat16()
+    gq, gk = ((torch.randn(128, generator=g) * 0.1).bfloat16() for _ in range(2))
+    kc, vc = (torch.zeros(pages, 64, hk, 128, dtype=torch.uint8, device=DEV) for _ in range(2))
+    app = QkvAppendOp(hq, hk, DEV, max_tokens=prompt, k_scale=K_SCALE, v_scale=V_SCALE)
+    att = SharedPrefixAttnOp(hq, hk, DEV, max_tokens=prompt, max_seqs=seqs, k_scale=K_SCALE, v_scale=V_SCALE)
+    w = [x.to(DEV) for x in (gq, gk, cos, sin)]
+    order = torch.tensor([4, 0, 2])
+    at = torch.arange(prompt)
+    x = torch.randn(prompt, width, generator=g).bfloat16()
+    q = app(x.to(DEV), *w, at.to(DEV), (order[at // 64] * 64 + at % 64).to(DEV), kc, vc)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32)  # noqa: E731
+    # the prompt attends itself: one sequence, causal, no prefix
+    t = PrefixTables(i32([0, prompt]), order.to(torch.int32).view(1, 3), i32([prompt]))
+    out = att(q, kc, vc, _dev(t))
+    _check_attend(out, q.cpu(), [kc.cpu(), vc.cpu()], t, att)
+    own = torch.tensor([1, 3, 5])
+    for step in range(2):
+        x = torch.randn(seqs, width, generator=g).bfloat16()
+        q = app(x.to(DEV), *w, torch.full((seqs,), prompt + step, device=DEV), (own * 64 + step).to(DEV), kc, vc)
+        t = PrefixTables(i32([0, 1, 2, 3]), own.to(torch.int32).view(3, 1), i32([step + 1] * 3), i32([0, 3]), order.to(torch.int32).view(1, 3), i32([prompt]))
+        out = att(q, kc, vc, _dev(t))
+        _check_attend(out, q.cpu(), [kc.cpu(), vc.cpu()], t, att)
+
+
+def test_ops_refuse_other_shapes_types_and_devices():
+    app = QkvAppendOp(12, 2, DEV, max_tokens=8)
+    att = SharedPrefixAttnOp(12, 2, DEV, max_tokens=8, max_seqs=2)
+    d, caches = _append_inputs(8, 12, 2, 64)
+    kc, vc = (c.to(DEV) for c in caches)
+    good = dict(qkv=d["x"].to(DEV), g_q=None, g_k=None, cos=d["cos"].to(DEV), sin=d["sin"].to(DEV), positions=d["positions"].to(DEV),
+                slots=d["slots"].to(DEV), k_cache=kc, v_cache=vc)
+    app(**good)
+    for name, bad in [("qkv", good["qkv"].half()), ("qkv", good["qkv"].cpu()), ("qkv", good["qkv"][:, :-128]), ("qkv", good["qkv"].repeat(2, 1)),
+                      ("qkv", good["qkv"].float()), ("g_q", torch.zeros(64, device=DEV).bfloat16()), ("cos", good["cos"][:, :16]),
+                      ("sin", good["sin"].float()), ("positions", good["positions"].int()), ("slots", good["slots"][:4]),
+                      ("k_cache", kc[:, :32]), ("v_cache", vc[:1].contiguous()), ("k_cache", kc.cpu())]:
+        with pytest.raises(ValueError, match=name):
+            app(**{**good, name: bad})
+    t, pages = _tables([1, 1], [9, 9], [0, 2], [70])
+    kc, vc = (c.to(DEV) for c in _caches(pages, 2))
+    q, dt = torch.zeros(2, 12, 128, device=DEV).bfloat16(), _dev(t)
+    att(q, kc, vc, dt)
+    for bad_q in (q.float(), q[:, :6], q.repeat(5, 1, 1), q.transpose(0, 1), q.cpu()):
+        with pytest.raises(ValueError, match="q"):
+            att(bad_q, kc, vc, dt)
+    for field, bad in [("q_start", dt.q_start[:2]), ("page_table", dt.page_table.long()), ("lens", dt.lens.repeat(2)), ("group_start", dt.group_start[:1]),
+                       ("prefix_table", dt.prefix_table[0]), ("prefix_lens", None), ("prefix_lens", dt.prefix_lens.repeat(2))]:
+        with pytest.raises(ValueError, match=field):
+            att(q, kc, vc, PrefixTables(**{**dt.__dict__, field: bad}))
+    with pytest.raises(ValueError, match="out"):
+        att(q, kc, vc, dt, out=torch.zeros(2, 12, 128, device=DEV))
+    assert L.load().mono_prefix_attn_scratch_bytes(8, 12, 2, 2, 1) == att.scratch.numel()

@@ -5,25 +5,41 @@
 //   token = first i by index with (running kept mass) > u (kept mass)
 //
 // Every filter keeps a front part of one order, so together they keep everything above one logit and, of the tokens
-// with exactly that logit, the first m by index.  That logit is found by a radix descent on the monotone image of the
-// f32 bits, on counts and masses.  Masses are fixed point, w * 2^44 rounded to an integer, and exact from there on: sums
-// do not depend on the order they are taken in, so a launch repeats to the bit, and a border is decided to 2^-44 of
-// the largest weight (f32 sums would decide it to 2^-20 or so, which draws other tokens where many are alike).
+// with exactly that logit, the first m by index.  Masses are fixed point, w * 2^44 rounded to an integer, and exact from
+// there on: sums do not depend on the order they are taken in, so a launch repeats to the bit, and a border is decided
+// to 2^-44 of the largest weight (f32 sums would decide it to 2^-20 or so, which draws other tokens where many are
+// alike).  A token whose weight rounds to 0 is never drawn, so it counts in no rank either.
+//
+// Layout: a cluster of eight CTAs per row; each reads its eighth of the row once from HBM into shared memory and all
+// passes run on that.  The border is found in steps that all eight CTAs decide alike from merged histograms (read over
+// distributed shared memory; one cluster barrier a step):
+//   1. the largest logit;
+//   2. Z, and a histogram of token counts over 1024 equal steps of log2 w.  The weights of a step differ by 3 %, so the
+//      counts bound the masses, and the border lies in a few neighbouring steps;
+//   3. those steps' range of keys (the order-preserving image of the f32 bits) by 1024 bins with counts and masses,
+//      again on the bin that holds the border, until one key or one token is left (two rounds as a rule).
+// Then each warp's run of kept mass says which warp walks to the token.
+#include <cooperative_groups.h>
+
 #include "mono_common.cuh"
 
 extern void mono_set_error(const char* fmt, ...);
 
 namespace sampling {
 using namespace mono;
+namespace cg = cooperative_groups;
 
-constexpr int kThreads = 1024;
+constexpr int kCtas = 8;  // of a row: the portable cluster size; a slice of the largest vocabulary fits shared memory
+constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
+constexpr int kBins = 1024;
+constexpr int kPerThread = kBins / kThreads;
 constexpr double kOne = 17592186044416.0;  // 2^44
+constexpr float kSteps = kBins / 44.001f;  // histogram steps per factor of two: weights down to 2^-44
 typedef unsigned long long u64;
 
-// Order-preserving image of a logit; NaN goes with -inf.
+// Order-preserving image of a logit (NaN has been taken to -inf).
 __device__ __forceinline__ uint32_t key_of(float x) {
-    if (!(x == x)) x = -INFINITY;
     const uint32_t b = __float_as_uint(x == 0.f ? 0.f : x);  // -0 counts as 0
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
@@ -31,22 +47,47 @@ __device__ __forceinline__ float logit_of(uint32_t key) { return __uint_as_float
 constexpr uint32_t kKeyNegInf = 0x007FFFFFu;
 
 struct Row {
-    float mx;        // largest logit
-    double inv_t;
-    u64 k;           // rank below this
-    double p;        // < 1: share of the mass
-    u64 floor_w;     // weight at least this
-    float u;
-    bool greedy;
+    float mx;          // largest logit
+    float c;           // log2(e) / T, f32: for histogram steps only
+    double c64;        // the same
+    u64 k;             // rank below this
+    u64 floor_w;       // weight at least this
+    const double* tab; // 2^(i / 16)
 };
 
+// f32 -> f64 by bits (conversions between the two run at a quarter of the rate of the arithmetic): normal numbers; a
+// subnormal f32 gives another number below 2^-126, which no difference of logits notices
+__device__ __forceinline__ double widen(float x) {
+    const uint32_t b = __float_as_uint(x);
+    return __hiloint2double((int)((b & 0x80000000u) | (((b & 0x7FFFFFFFu) >> 3) + 0x38000000u)), (int)(b << 29));
+}
+
+// round(2^44 exp((x - mx) / T)).  y = (x - mx) log2(e) / T = n + i / 16 + r, 0 <= i < 16, |r| <= 1/32:
+// 2^y = 2^n 2^(i/16) exp(r ln 2), the last by its Taylor series (r ln 2 <= 0.0217: the seventh power's term is below
+// 2^-51), all in f64; then the mantissa is shifted to its place.
 __device__ __forceinline__ u64 weight_of(float x, const Row& r) {
     if (x == r.mx) return (u64)kOne;
-    const double d = ((double)x - (double)r.mx) * r.inv_t;
-    if (!(d > -31.0)) return 0;  // below 2^-44; also -inf and NaN
-    return (u64)(exp(d) * kOne + 0.5);
+    const double y = (widen(x) - widen(r.mx)) * r.c64;
+    if (!(y > -45.0) || x == -INFINITY) return 0;
+    const double shifted = y * 16.0 + 6755399441055744.0;  // 2^52 + 2^51: the low word holds round(16 y)
+    const int q = __double2loint(shifted);
+    const double t = fma(shifted - 6755399441055744.0, -0.0625, y) * 0.69314718055994530942;
+    double e = fma(t, 1.0 / 720, 1.0 / 120);
+    e = fma(t, e, 1.0 / 24);
+    e = fma(t, e, 1.0 / 6);
+    e = fma(t, e, 0.5);
+    e = fma(t, e, 1.0);
+    e = fma(t, e, 1.0);
+    e *= r.tab[q & 15];                       // in (0.97, 2.0)
+    const double v = e + 1.0;                 // exponent 0 or 1: e + 1 in (1.97, 3.0); 51 bits below the point at least
+    const u64 m = (u64)__double_as_longlong(v);
+    // v = (2^52 + frac) 2^(E - 52), so 2^52 e = ((2^52 + frac) << E) - 2^52
+    const int E = (int)(m >> 52) - 1023;
+    const u64 fix = (((m & 0xFFFFFFFFFFFFFull) | 0x10000000000000ull) << E) - 0x10000000000000ull;
+    const int sh = 8 - (q >> 4);  // 2^52 e 2^n / 2^8
+    return sh > 62 ? 0 : (fix + (1ull << (sh - 1))) >> sh;
 }
-// floor(u W) for a 24-bit u below 1
+// floor(u W) for 0 <= u < 1
 __device__ __forceinline__ u64 share_of(float u, u64 W) {
     const int e = (int)((__float_as_uint(u) >> 23) & 0xFF);
     if (e == 0) return 0;  // below 2^-126
@@ -57,179 +98,435 @@ __device__ __forceinline__ u64 share_of(float u, u64 W) {
     if (sh >= 64) return hi >> (sh - 64);
     return (hi << (64 - sh)) | (lo >> sh);
 }
-
-__device__ __forceinline__ u64 block_sum_u64(u64 v, u64* red) {
+__device__ __forceinline__ u64 warp_sum_u64(u64 v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-    __syncthreads();
-    u64 s = 0;
-    for (int i = 0; i < kWarps; ++i) s += red[i];
-    return s;
+    return v;
 }
 
-template <typename T>
-__device__ __forceinline__ float load_logit(const T* p, int i);
-template <>
-__device__ __forceinline__ float load_logit<float>(const float* p, int i) { return __ldg(p + i); }
-template <>
-__device__ __forceinline__ float load_logit<__nv_bfloat16>(const __nv_bfloat16* p, int i) { return __bfloat162float(p[i]); }
+struct Hist {
+    uint32_t n[2][kBins], lo[2][kBins], hi[2][kBins];  // counts, and masses in two words; two sets, used in turn
+};
+// One word atomics are native in shared memory, 64-bit ones are not: the carry is taken from the value that was there.
+__device__ __forceinline__ void hist_add(Hist& h, int set, int bin, uint32_t n, u64 w) {
+    atomicAdd(&h.n[set][bin], n);
+    const uint32_t wl = (uint32_t)w, old = atomicAdd(&h.lo[set][bin], wl);
+    const uint32_t wh = (uint32_t)(w >> 32) + (old + wl < old ? 1u : 0u);
+    if (wh) atomicAdd(&h.hi[set][bin], wh);
+}
 
-// One CTA per row.
+// Sums of the threads before this one (exclusive), and all threads' bins are in thread order.
+template <typename A>
+__device__ __forceinline__ A block_before(A v, A* red) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    A s = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const A t = __shfl_up_sync(0xffffffffu, s, o);
+        if (lane >= o) s += t;
+    }
+    if (lane == 31) red[warp] = s;
+    __syncthreads();
+    A b = s - v;
+    for (int i = 0; i < warp; ++i) b += red[i];
+    return b;
+}
+
+// `slice`: logits of a CTA (a multiple of 4); runs: a warp's consecutive logits (a multiple of 128)
 template <typename T>
-__global__ void __launch_bounds__(kThreads) sample_kernel(const mono_sample_args a) {
+__global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 2) sample_kernel(const mono_sample_args a, int slice, int run) {
+    extern __shared__ __align__(16) float xs[];  // [slice], then the histograms
+    Hist& h = *reinterpret_cast<Hist*>(xs + slice);
+    __shared__ u64 s_wsum[kWarps], red64[kWarps], s_z[kCtas], s_part[kCtas], s_cut[2];
+    __shared__ uint32_t s_wties[kWarps], red32[kWarps], s_key[kCtas], s_num[kCtas], s_cnt[2];
+    __shared__ float redf[2][kWarps];
+    __shared__ int s_bin[2];
+    __shared__ double s_tab[16];
+    cg::cluster_group cluster = cg::this_cluster();
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, row = blockIdx.x / kCtas, V = a.vocab;
+    const int rank = (int)cluster.block_rank();
+    if (tid < 16) s_tab[tid] = exp2(tid / 16.0);
+    for (int i = tid; i < kBins; i += kThreads) h.n[0][i] = 0;
+    if (tid == 0) { s_bin[0] = kBins; s_bin[1] = kBins; }
     pdl_prologue();
-    __shared__ u64 red[kWarps], hist_m[256];
-    __shared__ uint32_t hist_n[256], red32[kWarps];
-    __shared__ u64 s_above, s_bin_mass;
-    __shared__ uint32_t s_count, s_bin, s_bin_n;
-    __shared__ int s_token;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, row = blockIdx.x, V = a.vocab;
-    const T* x = reinterpret_cast<const T*>(a.logits) + (size_t)row * a.ld;
-    // ---- the largest logit and its first index
+    const int first = min(rank * slice, V), count = min(slice, V - first);  // this CTA's tokens
+    const T* x = reinterpret_cast<const T*>(a.logits) + (size_t)row * a.ld + first;
+    const float temp = a.temperature ? a.temperature[row] : 1.f;
+    const int tk = a.top_k ? a.top_k[row] : 0;
+    const float tp = a.top_p ? a.top_p[row] : 1.f, mp = a.min_p ? a.min_p[row] : 0.f;
+    float u = a.u[row];
+    // ---- the slice into shared memory, and its largest logit; places behind the vocabulary hold -inf
     uint32_t kmax = 0;
-    for (int i = tid; i < V; i += kThreads) kmax = max(kmax, key_of(load_logit(x, i)));
+    {
+        constexpr int N = sizeof(T) == 4 ? 4 : 8;  // logits of a 16-byte load
+        auto put = [&](int i, float v) {
+            v = v == v ? v : -INFINITY;
+            kmax = max(kmax, key_of(v));
+            xs[i] = v;
+        };
+        const int vecs = (reinterpret_cast<uintptr_t>(x) & 15) ? 0 : count / N;
+        constexpr int B = 4;
+        for (int i0 = tid; i0 < vecs; i0 += kThreads * B) {
+            uint4 w[B];
+#pragma unroll
+            for (int j = 0; j < B; ++j) w[j] = __ldg(reinterpret_cast<const uint4*>(x) + min(i0 + j * kThreads, vecs - 1));
+#pragma unroll
+            for (int j = 0; j < B; ++j) {
+                const int i = i0 + j * kThreads;
+                if (i >= vecs) break;
+                const uint32_t ws[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    if (sizeof(T) == 4) {
+                        put(i * 4 + q, __uint_as_float(ws[q]));
+                    } else {
+                        put(i * 8 + 2 * q, __uint_as_float(ws[q] << 16));
+                        put(i * 8 + 2 * q + 1, __uint_as_float(ws[q] & 0xFFFF0000u));
+                    }
+                }
+            }
+        }
+        for (int i = vecs * N + tid; i < slice; i += kThreads) put(i, i < count ? (float)x[i] : -INFINITY);
+    }
     kmax = __reduce_max_sync(0xffffffffu, kmax);
     if (lane == 0) red32[warp] = kmax;
-    if (tid == 0) s_token = INT32_MAX;
     __syncthreads();
-    for (int i = 0; i < kWarps; ++i) kmax = max(kmax, red32[i]);
-    if (kmax <= kKeyNegInf) {  // no logit above -inf
-        if (tid == 0) {
+    if (tid < kCtas) {
+        for (int i = 0; i < kWarps; ++i) kmax = max(kmax, red32[i]);
+        *cluster.map_shared_rank(&s_key[rank], tid) = kmax;
+    }
+    cluster.sync();
+    kmax = 0;
+    for (int i = 0; i < kCtas; ++i) kmax = max(kmax, s_key[i]);
+    if (kmax <= kKeyNegInf) {  // no logit above -inf: all CTAs of the row leave
+        if (tid == 0 && rank == 0) {
             a.tokens[row] = -1;
             if (a.logprobs) a.logprobs[row] = -INFINITY;
         }
         return;
     }
     Row r;
+    r.tab = s_tab;
     r.mx = logit_of(kmax);
-    const float temp = a.temperature ? a.temperature[row] : 1.f;
-    r.greedy = !(temp > 0.f);
-    r.inv_t = r.greedy ? 1.0 : 1.0 / (double)temp;
-    const int tk = a.top_k ? a.top_k[row] : 0;
-    r.k = tk < 1 || tk > V ? (u64)V : (u64)tk;
-    r.p = a.top_p && a.top_p[row] < 1.f ? fmax((double)a.top_p[row], 0.0) : 1.0;
-    const float mp = a.min_p && a.min_p[row] > 0.f ? fminf(a.min_p[row], 1.f) : 0.f;
-    r.floor_w = (u64)ceil((double)mp * kOne);
-    r.u = a.u[row];
-    if (!(r.u > 0.f)) r.u = 0.f;
-    if (r.greedy) r.k = 1;
-    // ---- the whole mass
-    u64 z = 0;
-    for (int i = tid; i < V; i += kThreads) z += weight_of(load_logit(x, i), r);
-    z = block_sum_u64(z, red);
-    // ---- the border: keys above `lo` bits in all, the bin [lo, lo + 2^shift) holds it
-    // "mass before < top_p Z" for a whole number of units of mass: before < ceil(top_p Z)
-    const u64 limit = r.p < 1.0 ? max((u64)ceil(r.p * (double)z), 1ull) : ~0ull;
-    uint32_t lo = 0;      // the border key's known high bits
-    uint32_t count = 0;   // tokens above
-    u64 above = 0;        // their mass
-    uint32_t ties = 0;    // tokens at the border key that are kept
-    if (r.k < (u64)V || r.p < 1.0 || r.floor_w) {
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            __syncthreads();
-            if (tid < 256) { hist_n[tid] = 0; hist_m[tid] = 0; }
-            __syncthreads();
-            for (int i = tid; i < V; i += kThreads) {
-                const float v = load_logit(x, i);
-                const uint32_t k = key_of(v);
-                if (shift == 24 || (k >> (shift + 8)) == (lo >> (shift + 8))) {
-                    atomicAdd(&hist_n[(k >> shift) & 255], 1u);
-                    atomicAdd(&hist_m[(k >> shift) & 255], weight_of(v, r));
-                }
-            }
-            __syncthreads();
-            if (tid == 0) {
-                // down to the first bin that is not kept whole
-                uint32_t c = count;
-                u64 m = above;
-                int b = 255;
-                for (; b > 0; --b) {
-                    const uint32_t low_key = lo | ((uint32_t)b << shift);
-                    if (hist_n[b] == 0) continue;
-                    if (c + hist_n[b] > r.k || m + hist_m[b] >= limit || weight_of(logit_of(low_key), r) < r.floor_w) break;
-                    c += hist_n[b];
-                    m += hist_m[b];
-                }
-                s_bin = b;
-                s_count = c;
-                s_above = m;
-                s_bin_n = hist_n[b];
-                s_bin_mass = hist_m[b];
-            }
-            __syncthreads();
-            lo |= s_bin << shift;
-            count = s_count;
-            above = s_above;
-        }
-        // of the tokens with the border's logit: rank and mass before the j-th are count + j and above + j w
-        const u64 w = weight_of(logit_of(lo), r);
-        u64 m = s_bin_n;
-        if (w < r.floor_w) m = 0;
-        m = min(m, r.k - count);
-        if (limit != ~0ull) m = above >= limit ? 0 : w == 0 ? m : min(m, (limit - above + w - 1) / w);
-        ties = (uint32_t)m;
-        if (count + ties == 0) ties = 1;
-    }
-    const u64 tie_w = weight_of(logit_of(lo), r);
-    const u64 kept = (r.k < (u64)V || r.p < 1.0 || r.floor_w) ? above + ties * tie_w : z;
-    const u64 target = r.u >= 1.f ? kept - 1 : share_of(r.u, kept);
-    // ---- the draw: every warp sums a run of consecutive tokens; the run that holds the target walks itself
-    const int run = (V + kWarps - 1) / kWarps, i0 = min(warp * run, V), i1 = min(i0 + run, V);
-    const bool all = !(r.k < (u64)V || r.p < 1.0 || r.floor_w);
-    uint32_t my_ties = 0;
-    u64 mine = 0;
-    for (int i = i0 + lane; i < i1; i += 32) {
-        const float v = load_logit(x, i);
-        const uint32_t k = key_of(v);
-        if (all || k > lo) mine += weight_of(v, r);
-        else if (k == lo) ++my_ties;
-    }
+    const bool greedy = !(temp > 0.f);
+    // temperatures below 2^-100 tell no more logits apart than 2^-100 does; beside an infinite logit nothing has weight
+    r.c64 = r.mx == INFINITY ? 1e30 : greedy ? 1.4426950408889634 : 1.4426950408889634 / fmax((double)temp, 7.888609052210118e-31);
+    r.c = (float)r.c64;
+    r.k = greedy ? 1ull : tk < 1 || tk > V ? (u64)V : (u64)tk;
+    const double p = !greedy && tp < 1.f ? fmax((double)tp, 0.0) : 1.0;
+    r.floor_w = !greedy && mp > 0.f ? (u64)ceil((double)fminf(mp, 1.f) * kOne) : 0ull;
+    const bool filtered = r.k < (u64)V || p < 1.0 || r.floor_w;
+    // ---- Z, and the histogram of counts over steps of log2 w
+    const int i0 = min(warp * run, slice), i1 = min(i0 + run, slice);
+    {
+        u64 z = 0;
+        for (int i = i0 + lane * 4; i < i1; i += 128) {
+            const float4 v4 = *reinterpret_cast<const float4*>(xs + i);
+            const float v[4] = {v4.x, v4.y, v4.z, v4.w};
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-    my_ties = __reduce_add_sync(0xffffffffu, my_ties);
-    __syncthreads();
-    if (lane == 0) { red32[warp] = my_ties; red[warp] = mine; }
-    __syncthreads();
-    u64 before = 0;
-    uint32_t ties_before = 0;
-    auto kept_ties = [&](uint32_t first, uint32_t n) { return first >= ties ? 0u : min(n, ties - first); };
-    for (int w = 0; w < warp; ++w) {
-        before += red[w] + (all ? 0ull : kept_ties(ties_before, red32[w]) * tie_w);
-        ties_before += red32[w];
+            for (int j = 0; j < 4; ++j) {
+                const u64 w = weight_of(v[j], r);
+                z += w;
+                if (filtered && w) {
+                    const float y = v[j] == r.mx ? 0.f : (r.mx - v[j]) * r.c;
+                    atomicAdd(&h.n[0][min((int)(y * kSteps), kBins - 1)], 1u);
+                }
+            }
+        }
+        z = warp_sum_u64(z);
+        if (lane == 0) s_wsum[warp] = z;
     }
-    const u64 after = before + mine + (all ? 0ull : kept_ties(ties_before, my_ties) * tie_w);
-    if (before <= target && target < after) {  // one warp
-        for (int b = i0; b < i1; b += 32) {
-            const int i = b + lane;
-            const float v = i < i1 ? load_logit(x, i) : -INFINITY;
-            const uint32_t k = i < i1 ? key_of(v) : 0;
-            const uint32_t tie_mask = __ballot_sync(0xffffffffu, !all && i < i1 && k == lo);
-            const bool tie_kept = ties_before + __popc(tie_mask & ((1u << lane) - 1)) < ties;
-            u64 w = 0;
-            if (i < i1 && (all || k > lo || (k == lo && tie_kept))) w = weight_of(v, r);
-            u64 s = w;
+    __syncthreads();
+    if (tid < kCtas) {
+        u64 z = 0;
+        for (int i = 0; i < kWarps; ++i) z += s_wsum[i];
+        *cluster.map_shared_rank(&s_z[rank], tid) = z;
+    }
+    cluster.sync();
+    u64 Z = 0;
+    for (int i = 0; i < kCtas; ++i) Z += s_z[i];
+    // kept: keys above khi; of the keys klo .. khi (one key, or one token) the first `ties` of `tied`
+    uint32_t khi = 0, klo = 1, tied = 0, ties = 0;
+    u64 kept = Z, tie_w = 0;
+    bool all = !filtered;
+    if (filtered) {
+        // "mass before < p Z", for masses in whole units
+        const u64 limit = p < 1.0 ? max((u64)ceil(p * (double)Z), 1ull) : ~0ull;
+        // ---- bounds of the border among the steps
+        {
+            uint32_t n[kPerThread] = {};
+            for (int c = 0; c < kCtas; ++c) {
+                const uint2 v = *reinterpret_cast<const uint2*>(cluster.map_shared_rank(&h.n[0][tid * kPerThread], c));
+                n[0] += v.x;
+                n[1] += v.y;
+            }
+            static_assert(kPerThread == 2, "two bins per thread");
+            // a step's weights lie in (2^-((b + 1) / kSteps), 2^-(b / kSteps)], in units of the largest
+            float top[kPerThread + 1];
+#pragma unroll
+            for (int j = 0; j <= kPerThread; ++j) top[j] = exp2f(-(float)(tid * kPerThread + j) / kSteps);
+            const float m_hi = n[0] * top[0] + n[1] * top[1], m_lo = n[0] * top[1] + n[1] * top[2];
+            uint32_t c = block_before<uint32_t>(n[0] + n[1], red32);
+            float hi = block_before<float>(m_hi, redf[0]), lo = block_before<float>(m_lo, redf[1]);
+            // f32 sums of at most 1024 terms, and steps that f32 places to a few 2^-24 of their number: 0.1 % covers both
+            const float lim = limit == ~0ull ? INFINITY : (float)((double)limit / kOne), fl = (float)((double)r.floor_w / kOne);
+#pragma unroll
+            for (int j = 0; j < kPerThread; ++j) {
+                c += n[j];
+                hi += n[j] * top[j];
+                lo += n[j] * top[j + 1];
+                const int b = tid * kPerThread + j;
+                if (c > r.k || hi * 1.001f >= lim || top[j + 1] * 0.999f < fl) atomicMin(&s_bin[0], b);  // may not be kept whole
+                if (c > r.k || lo * 0.999f >= lim || top[j] * 1.001f < fl) atomicMin(&s_bin[1], b);      // the border is not behind it
+            }
+        }
+        __syncthreads();
+        const int b0 = s_bin[0], b1 = min(s_bin[1], kBins - 1);
+        __syncthreads();
+        if (b0 >= kBins) {
+            all = true;
+            cluster.sync();  // no CTA leaves while another reads its histogram
+        } else {
+            // the steps' range of logits, with room for the rounding of the step's number
+            const double per = 1.0 / ((double)r.c * (double)kSteps);
+            float xh = b0 == 0 ? r.mx : (float)((double)r.mx - (double)b0 * per * (1.0 - 4e-6));
+            float xl = (float)((double)r.mx - (double)(b1 + 1) * per * (1.0 + 4e-6));
+            if (!(xh <= r.mx)) xh = r.mx;
+            if (!(xl <= xh)) xl = -INFINITY;  // no number: infinite temperature, infinite logits
+            khi = min(key_of(xh) + 2u, kmax);
+            // (the last step also holds what lies behind it)
+            klo = b1 < kBins - 1 && key_of(xl) > kKeyNegInf + 2u ? key_of(xl) - 2u : kKeyNegInf + 1u;
+            u64 above = 0;
+            uint32_t n_above = 0;
+            for (int level = 1;; ++level) {
+                const int set = level & 1;
+                const uint32_t width = khi - klo;
+                const int sh = width < kBins ? 0 : 22 - __clz(width);
+                for (int i = tid; i < kBins; i += kThreads) { h.n[set][i] = 0; h.lo[set][i] = 0; h.hi[set][i] = 0; }
+                if (tid == 0) s_bin[set] = kBins;  // not the one that slower threads may still read
+                __syncthreads();
+                u64 m_ab = 0;
+                uint32_t n_ab = 0;
+                for (int b = i0; b < i1; b += 128) {  // whole warps: the lanes vote
+                    const int i = b + lane * 4;
+                    const float4 v4 = i < i1 ? *reinterpret_cast<const float4*>(xs + i) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+                    const float v[4] = {v4.x, v4.y, v4.z, v4.w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint32_t k = key_of(v[j]);
+                        u64 w = 0;
+                        if (k >= klo && (k <= khi || level == 1)) w = weight_of(v[j], r);
+                        if (level == 1 && k > khi) {
+                            m_ab += w;
+                            n_ab += w != 0;
+                            w = 0;
+                        }
+                        const unsigned in = __ballot_sync(0xffffffffu, w != 0);
+                        if (in == 0) continue;
+                        const int bin = (int)((khi - k) >> sh), lead = __ffs(in) - 1;
+                        const int lb = __shfl_sync(0xffffffffu, bin, lead);
+                        if (__popc(in) > 4 && __all_sync(0xffffffffu, w == 0 || bin == lb)) {  // many equal logits: one addition for all
+                            const u64 sum = warp_sum_u64(w);
+                            if (lane == lead) hist_add(h, set, bin, __popc(in), sum);
+                        } else if (w) {
+                            hist_add(h, set, bin, 1, w);
+                        }
+                        __syncwarp();
+                    }
+                }
+                if (level == 1) {
+                    m_ab = warp_sum_u64(m_ab);
+                    n_ab = __reduce_add_sync(0xffffffffu, n_ab);
+                    if (lane == 0) { red64[warp] = m_ab; red32[warp] = n_ab; }
+                }
+                __syncthreads();
+                if (level == 1 && tid < kCtas) {
+                    u64 m = 0;
+                    uint32_t n = 0;
+                    for (int i = 0; i < kWarps; ++i) { m += red64[i]; n += red32[i]; }
+                    *cluster.map_shared_rank(&s_part[rank], tid) = m;
+                    *cluster.map_shared_rank(&s_num[rank], tid) = n;
+                }
+                cluster.sync();
+                if (level == 1)
+                    for (int i = 0; i < kCtas; ++i) { above += s_part[i]; n_above += s_num[i]; }
+                uint32_t n[kPerThread] = {};
+                u64 m[kPerThread] = {};
+                for (int c = 0; c < kCtas; ++c) {
+                    const uint2 vn = *reinterpret_cast<const uint2*>(cluster.map_shared_rank(&h.n[set][tid * kPerThread], c));
+                    const uint2 vl = *reinterpret_cast<const uint2*>(cluster.map_shared_rank(&h.lo[set][tid * kPerThread], c));
+                    const uint2 vh = *reinterpret_cast<const uint2*>(cluster.map_shared_rank(&h.hi[set][tid * kPerThread], c));
+                    n[0] += vn.x;
+                    n[1] += vn.y;
+                    m[0] += ((u64)vh.x << 32) + vl.x;
+                    m[1] += ((u64)vh.y << 32) + vl.y;
+                }
+                uint32_t c = n_above + block_before<uint32_t>(n[0] + n[1], red32);
+                u64 mass = above + block_before<u64>(m[0] + m[1], red64);
+                uint32_t c_at[kPerThread];
+                u64 m_at[kPerThread];
+                int mine = -1;
+#pragma unroll
+                for (int j = 0; j < kPerThread; ++j) {
+                    c_at[j] = c;
+                    m_at[j] = mass;
+                    c += n[j];
+                    mass += m[j];
+                    const int b = tid * kPerThread + j;
+                    if (n[j] == 0 || mine >= 0) continue;
+                    const uint32_t top = khi - ((uint32_t)b << sh);
+                    const uint32_t low = top - klo < (1u << sh) ? klo : top - ((1u << sh) - 1);
+                    if (c > r.k || mass >= limit || weight_of(logit_of(low), r) < r.floor_w) mine = j;
+                }
+                if (mine >= 0) atomicMin(&s_bin[set], tid * kPerThread + mine);
+                __syncthreads();
+                const int b = s_bin[set];
+                if (b >= kBins) {  // everything in the range is kept
+                    if (tid == kThreads - 1) { s_cut[set] = mass; s_cnt[set] = c; }
+                    __syncthreads();
+                    kept = s_cut[set];
+                    khi = klo - 1;  // and nobody is tied
+                    break;
+                }
+                if (tid == b / kPerThread) {
+                    const int j = b % kPerThread;
+                    s_cut[set] = j ? m_at[1] : m_at[0];
+                    s_cnt[set] = j ? c_at[1] : c_at[0];
+                    red64[0] = j ? m[1] : m[0];
+                    red32[0] = j ? n[1] : n[0];
+                }
+                __syncthreads();
+                above = s_cut[set];
+                n_above = s_cnt[set];
+                const u64 bin_m = red64[0];
+                tied = red32[0];
+                khi -= (uint32_t)b << sh;
+                klo = khi - klo < (1u << sh) ? klo : khi - ((1u << sh) - 1);
+                if (sh == 0 || tied == 1) {
+                    tie_w = bin_m / tied;
+                    // rank and mass before the j-th of them are n_above + j and above + j tie_w
+                    u64 t = tied;
+                    if (tie_w < r.floor_w) t = 0;
+                    t = min(t, r.k - n_above);
+                    if (limit != ~0ull) t = above >= limit ? 0 : min(t, (limit - above + tie_w - 1) / tie_w);
+                    if (n_above + t == 0) t = 1;
+                    ties = (uint32_t)t;
+                    kept = above + t * tie_w;
+                    break;
+                }
+                __syncthreads();  // red32 / red64 have been read
+            }
+        }
+    }
+    if (!(u > 0.f)) u = 0.f;
+    const u64 target = u >= 1.f ? kept - 1 : share_of(u, kept);
+    // ---- the draw: every warp's run of kept mass; where only some of the tied tokens are kept, their number apart
+    const bool some = !all && ties > 0 && ties < tied;
+    if (!all && !some && ties == tied) khi = klo - 1;  // all of the tied are kept: so is every key from klo on
+    if (!all) {
+        u64 m = 0;
+        uint32_t t = 0;
+        for (int i = i0 + lane * 4; i < i1; i += 128) {
+            const float4 v4 = *reinterpret_cast<const float4*>(xs + i);
+            const float v[4] = {v4.x, v4.y, v4.z, v4.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t k = key_of(v[j]);
+                if (k > khi) m += weight_of(v[j], r);
+                else if (some && k >= klo) ++t;
+            }
+        }
+        m = warp_sum_u64(m);
+        t = __reduce_add_sync(0xffffffffu, t);
+        if (lane == 0) { s_wsum[warp] = m; s_wties[warp] = t; }
+        __syncthreads();
+        if (tid < kCtas) {
+            u64 sm = 0;
+            uint32_t st = 0;
+            for (int i = 0; i < kWarps; ++i) { sm += s_wsum[i]; st += s_wties[i]; }
+            *cluster.map_shared_rank(&s_z[rank], tid) = sm;  // Z has been taken
+            *cluster.map_shared_rank(&s_key[rank], tid) = st;
+        }
+        cluster.sync();
+    }
+    // from here on a CTA reads only what is its own
+    u64 before = 0;
+    uint32_t t_before = 0;
+    auto kept_of = [&](uint32_t from, uint32_t n) { return some && from < ties ? (u64)min(n, ties - from) * tie_w : 0ull; };
+    for (int c = 0; c < rank; ++c) {
+        before += s_z[c];
+        if (some) { before += kept_of(t_before, s_key[c]); t_before += s_key[c]; }
+    }
+    for (int w = 0; w < warp; ++w) {
+        before += s_wsum[w];
+        if (some) { before += kept_of(t_before, s_wties[w]); t_before += s_wties[w]; }
+    }
+    const u64 after = before + s_wsum[warp] + (some ? kept_of(t_before, s_wties[warp]) : 0ull);
+    if (before <= target && target < after) {  // one warp of the eight CTAs
+        for (int b = i0; b < i1; b += 128) {
+            const float4 v4 = *reinterpret_cast<const float4*>(xs + min(b + lane * 4, i1 - 4));
+            const float v[4] = {v4.x, v4.y, v4.z, v4.w};
+            const bool in = b + lane * 4 < i1;
+            u64 w[4];
+            uint32_t tie = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t k = key_of(v[j]);
+                w[j] = in && (all || k > khi) ? weight_of(v[j], r) : 0;
+                if (in && some && k <= khi && k >= klo) tie |= 1u << j;
+            }
+            if (some) {
+                uint32_t n = __popc(tie), s = n;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const uint32_t t = __shfl_up_sync(0xffffffffu, s, o);
+                    if (lane >= o) s += t;
+                }
+                uint32_t at = t_before + s - n;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (tie >> j & 1) w[j] = at++ < ties ? tie_w : 0;
+                t_before += __shfl_sync(0xffffffffu, s, 31);
+            }
+            const u64 own = w[0] + w[1] + w[2] + w[3];
+            u64 s = own;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const u64 t = __shfl_up_sync(0xffffffffu, s, o);
                 if (lane >= o) s += t;
             }
-            const uint32_t hit = __ballot_sync(0xffffffffu, w > 0 && before + s > target);
+            const uint32_t hit = __ballot_sync(0xffffffffu, before + s > target);
             if (hit) {
-                const int token = b + __ffs(hit) - 1;
-                if (lane == 0) {
-                    const float xt = load_logit(x, token);
-                    const double y = xt == r.mx ? 0.0 : ((double)xt - (double)r.mx) * r.inv_t;
-                    a.tokens[row] = token;
-                    if (a.logprobs) a.logprobs[row] = (float)(y - log((double)z / kOne));
+                if (lane == __ffs(hit) - 1) {
+                    u64 at = before + s - own;
+                    int j = 0;
+                    while (j < 3 && at + w[j] <= target) at += w[j++];
+                    const float xt = v[j];
+                    const double y = xt == r.mx ? 0.0 : ((double)xt - (double)r.mx) * r.c64 * 0.69314718055994530942;
+                    a.tokens[row] = first + b + lane * 4 + j;
+                    if (a.logprobs) a.logprobs[row] = (float)(y - log((double)Z / kOne));
                 }
                 break;
             }
             before += __shfl_sync(0xffffffffu, s, 31);
-            ties_before += __popc(tie_mask);
         }
     }
+}
+
+template <typename T>
+static cudaError_t launch(const mono_sample_args* a, cudaStream_t st) {
+    int slice = (a->vocab + kCtas - 1) / kCtas;
+    slice = (slice + 7) & ~7;  // slices start on 16-byte addresses where the row does
+    int run = (slice + kWarps - 1) / kWarps;
+    run = (run + 127) & ~127;
+    const size_t smem = (size_t)slice * 4 + sizeof(Hist);
+    static std::atomic<uint64_t> attr_once{0};  // bit d: set on device d
+    if (attr_needed(attr_once)) {
+        const cudaError_t e = cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, MONO_SAMPLE_MAX_VOCAB / kCtas * 4 + (int)sizeof(Hist));
+        if (e != cudaSuccess) return e;
+        attr_done(attr_once);
+    }
+    return launch_k(sample_kernel<T>, a->rows * kCtas, kThreads, smem, st, *a, slice, run);
 }
 
 }  // namespace sampling
@@ -248,8 +545,7 @@ extern "C" int mono_sample_launch(const mono_sample_args* a, void* stream) {
         mono_set_error("%s: logits and tokens must be aligned to their type", who);
         return MONO_E_ARG;
     }
-    const cudaError_t e = a->logits_bf16 ? mono::launch_k(sampling::sample_kernel<__nv_bfloat16>, a->rows, sampling::kThreads, 0, (cudaStream_t)stream, *a)
-                                         : mono::launch_k(sampling::sample_kernel<float>, a->rows, sampling::kThreads, 0, (cudaStream_t)stream, *a);
+    const cudaError_t e = a->logits_bf16 ? sampling::launch<__nv_bfloat16>(a, (cudaStream_t)stream) : sampling::launch<float>(a, (cudaStream_t)stream);
     if (e != cudaSuccess) mono_set_error("%s: %s", who, cudaGetErrorString(e));
     return (int)e;
 }

@@ -4,7 +4,8 @@
 //               (q[t][h] . k) k_scale sm_scale,  times v v_scale
 //
 // A prefix is read once for all tokens of its group: the rows of a tile come from every sequence of the group.
-// prefix_attn.cuh says how the work is cut.  This file holds the kernel for few rows and the merge.
+// prefix_attn.cuh says how the work is cut.  This file holds the kernel for few rows and the merge; prefix_attn_tc.cu
+// the kernel for many.
 #include "prefix_attn.cuh"
 
 extern void mono_set_error(const char* fmt, ...);
@@ -17,12 +18,6 @@ constexpr int kStages = 4;
 constexpr int kTileBytes = kPage * kDim;             // one page of one kv head: 64 keys x 128 bytes
 constexpr int kPitch = kDim + 4;                     // floats of a combine row
 constexpr float kPBias = 14.f;                       // P is formed as 2^14 p, so that f16 keeps small weights
-
-struct alignas(64) Params {
-    CUtensorMap kmap, vmap;
-    mono_prefix_attn_args a;
-    Scratch s;
-};
 
 // D(16x8,f32) += A(16x16,f16,row) * B(16x8,f16,col)
 __device__ __forceinline__ void mma_f16(float d[4], const uint32_t a[4], uint32_t b0, uint32_t b1) {
@@ -298,7 +293,7 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_narrow_kernel(const __grid
                         float sum = 0.f;
 #pragma unroll
                         for (int w = 0; w < kConsumers; ++w) sum += s_m[w][tid] == -INFINITY ? 0.f : s_l[w][tid] * exp2f(s_m[w][tid] - M);
-                        seg[tid] = M;
+                        seg[tid] = M - kPBias;
                         seg[16 + tid] = sum;
                     }
                     for (int r = 0; r < rows; ++r) {
@@ -342,7 +337,7 @@ __global__ void __launch_bounds__(128) prefix_merge_kernel(const mono_prefix_att
     const int G = a.q_heads / a.kv_heads, E = a.groups + a.seqs;
     // the segments of the row's two items: `count` segments `stride` floats apart
     const float* base[2] = {nullptr, nullptr};
-    int count[2] = {0, 0}, stride[2] = {0, 0}, tile_rows[2] = {0, 0}, row_in[2] = {0, 0};
+    int count[2] = {0, 0}, stride[2] = {0, 0}, tile_rows[2] = {0, 0}, row_in[2] = {0, 0}, twice[2] = {0, 0};
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
         const int e = k ? s_seq : s_grp;
@@ -361,20 +356,25 @@ __global__ void __launch_bounds__(128) prefix_merge_kernel(const mono_prefix_att
         const uint32_t c0 = owner(U, first, ctas), c1 = owner(U, first + units - 1, ctas);
         stride[k] = w ? Shape<true>::kSegFloats : Shape<false>::kSegFloats;
         base[k] = s.seg[w] + (size_t)(c0 + s.item[w][e] + it_in) * stride[k];
-        count[k] = (int)(c1 - c0) + 1;
         tile_rows[k] = tr;
         row_in[k] = row % tr;
+        twice[k] = w && n.ntok * G - (row / tr) * tr <= kWideHalf;
+        count[k] = ((int)(c1 - c0) + 1) << twice[k];
     }
     const int total = count[0] + count[1];
-    auto seg_of = [&](int i, int* k) {
-        *k = i >= count[0];
-        return base[*k] + (size_t)(i - (*k ? count[0] : 0)) * stride[*k];
+    // part i of the row: where its segment lies, and the row in that segment
+    auto part_of = [&](int i, const float** sg, int* rows, int* r) {
+        const int k = i >= count[0], j = i - (k ? count[0] : 0);
+        *sg = base[k] + (size_t)(j >> twice[k]) * stride[k];
+        *rows = tile_rows[k];
+        *r = row_in[k] + (twice[k] ? (j & 1) * kWideHalf : 0);
     };
     float M = -INFINITY;
     for (int i = lane; i < total; i += 32) {
-        int k;
-        const float* sg = seg_of(i, &k);
-        M = fmaxf(M, __ldcg(sg + row_in[k]));
+        const float* sg;
+        int rows, rr;
+        part_of(i, &sg, &rows, &rr);
+        M = fmaxf(M, __ldcg(sg + rr));
     }
     M = warp_max(M);
     float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -385,11 +385,12 @@ __global__ void __launch_bounds__(128) prefix_merge_kernel(const mono_prefix_att
         float4 v[B];
 #pragma unroll
         for (int j = 0; j < B; ++j) {  // unconditional loads, all in flight together
-            int k;
-            const float* sg = seg_of(min(i0 + j * SPLIT, total - 1), &k);
-            m[j] = __ldcg(sg + row_in[k]);
-            l[j] = __ldcg(sg + tile_rows[k] + row_in[k]);
-            v[j] = ld_cg_f4_ordered(sg + 2 * tile_rows[k] + row_in[k] * kDim + lane * 4);
+            const float* sg;
+            int rows, rr;
+            part_of(min(i0 + j * SPLIT, total - 1), &sg, &rows, &rr);
+            m[j] = __ldcg(sg + rr);
+            l[j] = __ldcg(sg + rows + rr);
+            v[j] = ld_cg_f4_ordered(sg + 2 * rows + rr * kDim + lane * 4);
         }
 #pragma unroll
         for (int j = 0; j < B; ++j) {
@@ -430,14 +431,23 @@ static size_t narrow_segments(size_t tokens, size_t q_heads, size_t kv_heads, si
     const size_t tiles = (tokens * (q_heads / kv_heads)) / 16 + 1;
     return 2 * (size_t)sm_or_default() + kv_heads * (2 * tiles + seqs + groups);
 }
+// The wide kernel's entries have kWideRows rows at least, so there are at most 2 rows / kWideRows of them.
+static size_t wide_segments(size_t tokens, size_t q_heads, size_t kv_heads) {
+    const size_t rows = tokens * (q_heads / kv_heads);
+    if (rows < kWideRows) return 0;
+    return (size_t)sm_or_default() + kv_heads * 2 * (rows / Shape<true>::kTile + rows / kWideRows);
+}
+static size_t narrow_bytes(int tokens, int q_heads, int kv_heads, int seqs, int groups) {
+    return up256(narrow_segments(tokens, q_heads, kv_heads, seqs, groups) * Shape<false>::kSegFloats * sizeof(float));
+}
 
 }  // namespace prefix_attn
 
 extern "C" size_t mono_prefix_attn_scratch_bytes(int tokens, int q_heads, int kv_heads, int seqs, int groups) {
     using namespace prefix_attn;
     if (tokens < 1 || q_heads < 1 || kv_heads < 1 || seqs < 1 || groups < 0 || q_heads % kv_heads) return 0;
-    return 4 * up256((size_t)(seqs + groups + 1) * 4) +
-           up256(narrow_segments(tokens, q_heads, kv_heads, seqs, groups) * Shape<false>::kSegFloats * sizeof(float));
+    return 4 * up256((size_t)(seqs + groups + 1) * 4) + narrow_bytes(tokens, q_heads, kv_heads, seqs, groups) +
+           wide_segments(tokens, q_heads, kv_heads) * Shape<true>::kSegFloats * sizeof(float);
 }
 
 extern "C" int mono_prefix_attn_launch(const mono_prefix_attn_args* a, void* stream) {
@@ -458,7 +468,7 @@ extern "C" int mono_prefix_attn_launch(const mono_prefix_attn_args* a, void* str
         return MONO_E_ARG;
     }
     if (a->q_ld < (long)a->q_heads * kDim || (a->q_ld & 7) || ((reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->out)) & 15) ||
-        (reinterpret_cast<uintptr_t>(a->scratch) & 255) || !(a->k_scale > 0.f) || !(a->v_scale > 0.f)) {
+        (reinterpret_cast<uintptr_t>(a->scratch) & 255) || !(a->k_scale > 0.f) || !(a->v_scale > 0.f) || !(a->sm_scale > 0.f)) {
         mono_set_error("%s: q rows at least q_heads * 128 values apart (a multiple of 8) on 16-byte addresses, scratch on a 256-byte address and positive scales required", who);
         return MONO_E_ARG;
     }
@@ -490,7 +500,7 @@ extern "C" int mono_prefix_attn_launch(const mono_prefix_attn_args* a, void* str
         at += 2 * words;
     }
     p.s.seg[0] = reinterpret_cast<float*>(at);
-    p.s.seg[1] = nullptr;
+    p.s.seg[1] = reinterpret_cast<float*>(at + narrow_bytes(a->tokens, a->q_heads, a->kv_heads, a->seqs, a->groups));
     const cudaStream_t st = (cudaStream_t)stream;
     const size_t smem = 1024 + kStages * 2 * kTileBytes + kConsumers * 16 * kPitch * sizeof(float) + 2 * (size_t)(a->seqs + a->groups + 1) * 4;
     static std::atomic<uint64_t> attr_once{0};  // bit d: set on device d
@@ -504,13 +514,15 @@ extern "C" int mono_prefix_attn_launch(const mono_prefix_attn_args* a, void* str
         attr_done(attr_once);
     }
     const int narrow = 2 * sm_or_default();
-    cudaError_t e = launch_k(prefix_narrow_kernel, narrow, kThreads, smem, st, p);
+    const int wide = (long)a->tokens * (a->q_heads / a->kv_heads) >= kWideRows ? sm_or_default() : 0;  // no entry has more rows than the step
+    cudaError_t e = wide ? launch_wide(p, wide, st) : cudaSuccess;
+    if (e == cudaSuccess) e = launch_k(prefix_narrow_kernel, narrow, kThreads, smem, st, p);
     // Few rows: four warps share a row's segments (a long prefix leaves many of them); many rows: a warp each.
     if (e == cudaSuccess) {
         if ((long)a->tokens * a->q_heads < 2048)
-            e = launch_k(prefix_merge_kernel<4>, dim3(a->tokens, a->q_heads), 128, 0, st, *a, p.s, narrow, 0);
+            e = launch_k(prefix_merge_kernel<4>, dim3(a->tokens, a->q_heads), 128, 0, st, *a, p.s, narrow, wide);
         else
-            e = launch_k(prefix_merge_kernel<1>, dim3(a->tokens, (a->q_heads + 3) / 4), 128, 0, st, *a, p.s, narrow, 0);
+            e = launch_k(prefix_merge_kernel<1>, dim3(a->tokens, (a->q_heads + 3) / 4), 128, 0, st, *a, p.s, narrow, wide);
     }
     if (e != cudaSuccess) mono_set_error("%s: %s", who, cudaGetErrorString(e));
     return (int)e;

@@ -53,15 +53,18 @@ __device__ __forceinline__ int row_limit(const Entry& n, int row, int G) {
     return n.causal ? n.len - n.ntok + 1 + row / G : n.len;
 }
 
-// A kernel's view of the work: narrow (16-row tiles, 64-key units) or wide (128-row tiles, 128-key units).
+// A kernel's view of the work: narrow (16-row tiles, 64-key units) or wide (256-row tiles, 128-key units).
 template <bool WIDE>
 struct Shape {
-    static constexpr int kTile = WIDE ? 128 : 16;
+    static constexpr int kTile = WIDE ? 256 : 16;
     static constexpr int kKeys = WIDE ? 128 : 64;
     static constexpr int kSegFloats = 2 * kTile + kTile * kDim;  // max, sum, values
 };
 // rows of an entry from which the wide kernel takes it
-constexpr int kWideRows = 1 << 30;
+constexpr int kWideRows = 48;
+// A wide item of at most this many rows is computed twice over alternate units, by the two halves of its CTA: its
+// segments then hold two parts per row, at tile rows r and r + 128.
+constexpr int kWideHalf = 128;
 
 template <bool WIDE>
 __device__ __forceinline__ void entry_work(const mono_prefix_attn_args& a, const Entry& n, int* tiles, int* units) {
@@ -132,5 +135,14 @@ struct Scratch {
     uint32_t *off[2], *item[2];
     float* seg[2];
 };
+
+struct alignas(64) Params {
+    CUtensorMap kmap, vmap;
+    mono_prefix_attn_args a;
+    Scratch s;
+};
+
+// Runs the wide kernel (prefix_attn_tc.cu) on `ctas` CTAs.
+cudaError_t launch_wide(const Params& p, int ctas, cudaStream_t st);
 
 }  // namespace prefix_attn

@@ -186,7 +186,7 @@ class SharedPrefixAttnOp:
         self.dev = _device(device)
         self.q_heads, self.kv_heads = q_heads, kv_heads
         self.max_tokens, self.max_seqs, self.max_groups = max_tokens, max_seqs, max_groups
-        self.sm_scale = float(sm_scale) if sm_scale is not None else HEAD_DIM ** -0.5
+        self.sm_scale = _scale(sm_scale, "sm_scale") if sm_scale is not None else HEAD_DIM ** -0.5
         self.deadline_s = deadline_s
         with torch.cuda.device(self.dev):
             nbytes = L.load().mono_prefix_attn_scratch_bytes(max_tokens, q_heads, kv_heads, max_seqs, max_groups)

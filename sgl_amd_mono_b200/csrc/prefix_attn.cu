@@ -11,12 +11,14 @@
 extern void mono_set_error(const char* fmt, ...);
 
 namespace prefix_attn {
+MONO_TL_DECLARE(tl_narrow)
 
 constexpr int kConsumers = 4;                        // warps that compute; one more fetches
 constexpr int kThreads = (kConsumers + 1) * 32;
 constexpr int kStages = 4;
 constexpr int kTileBytes = kPage * kDim;             // one page of one kv head: 64 keys x 128 bytes
-constexpr int kPitch = kDim + 4;                     // floats of a combine row
+constexpr int kQBytes = 16 * kDim * 2;               // a tile's queries
+constexpr int kQuarter = 36, kPitch = 4 * kQuarter + 4;  // floats of a quarter and of a combine row: spread over the banks
 constexpr float kPBias = 14.f;                       // P is formed as 2^14 p, so that f16 keeps small weights
 
 // D(16x8,f32) += A(16x16,f16,row) * B(16x8,f16,col)
@@ -34,6 +36,11 @@ __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
 }
+__device__ __forceinline__ float ex2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
 // a maximum that keeps NaN: a row with a NaN score is a row of NaN
 __device__ __forceinline__ float max_nan(float a, float b) {
     float r;
@@ -46,19 +53,17 @@ __device__ __forceinline__ void consumer_sync() { asm volatile("bar.sync 1, 128;
 // as both operands share it, so thread (g, t) of a fragment takes dims 32 t .. 32 t + 31 of its rows: a key's 32 bytes
 // are then two 16-byte shared loads.  A row is scaled by a power of two so that its largest value lies in
 // [2^13, 2^14): f16 then holds every bf16 value down to 2^-28 of that exactly.
-__device__ __forceinline__ void load_q(const mono_prefix_attn_args& a, const Entry& n, int head, int row0, int G, uint32_t q[8][4], float qscale[2],
-                                       int lim[2]) {
+__device__ __forceinline__ void load_q(const mono_prefix_attn_args& a, const Entry& n, uint32_t rows /* shared: the tile's rows of 256 bytes */,
+                                       int row0, int G, uint32_t q[8][4], float qscale[2], int lim[2]) {
     const int g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
     uint4 raw[2][4];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const int row = row0 + g + 8 * i;
         const bool live = row < n.ntok * G;
-        const int r = live ? row : 0;
-        const __nv_bfloat16* src = reinterpret_cast<const __nv_bfloat16*>(a.q) + (size_t)(n.tok0 + r / G) * a.q_ld + (size_t)(head * G + r % G) * kDim + t * 32;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) raw[i][j] = live ? __ldg(reinterpret_cast<const uint4*>(src) + j) : make_uint4(0, 0, 0, 0);
-        lim[i] = live ? row_limit(n, row, G) : 0;
+        for (int j = 0; j < 4; ++j) raw[i][j] = live ? lds128(rows + (g + 8 * i) * (kDim * 2) + t * 64 + j * 16) : make_uint4(0, 0, 0, 0);
+        lim[i] = live ? row_limit(n, row, G) : INT32_MAX;  // a row that does not exist needs no mask
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -90,9 +95,10 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_narrow_kernel(const __grid
     float* comb = reinterpret_cast<float*>(ring + kStages * 2 * kTileBytes);  // [4 warps][16 rows][kPitch]
     const mono_prefix_attn_args& a = p.a;
     const int E = a.groups + a.seqs;
-    uint32_t* off = reinterpret_cast<uint32_t*>(comb + kConsumers * 16 * kPitch);
+    uint8_t* qbuf = reinterpret_cast<uint8_t*>(comb + kConsumers * 16 * kPitch);
+    uint32_t* off = reinterpret_cast<uint32_t*>(qbuf + 2 * kQBytes);
     uint32_t* item = off + E + 1;
-    __shared__ uint64_t full[kStages], empty[kStages];
+    __shared__ uint64_t full[kStages], empty[kStages], q_full[2], q_empty[2];
     __shared__ int page_ok[kStages];
     __shared__ uint32_t red[64];
     __shared__ float s_m[kConsumers][16], s_l[kConsumers][16];
@@ -105,41 +111,54 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_narrow_kernel(const __grid
             mbar_init(&full[i], 1);
             mbar_init(&empty[i], kConsumers);
         }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&q_full[i], 1);
+            mbar_init(&q_empty[i], kConsumers);
+        }
         mbar_fence_init();
         prefetch_tmap(&p.kmap);
         prefetch_tmap(&p.vmap);
     }
+    MONO_TL(tl_narrow, 0);
     pdl_launch_dependents();
     pdl_wait();
+    MONO_TL(tl_narrow, 1);
     if (tid == 0 && guard_failed(a.guard)) abort_flag = 1;
-    make_plan<false, kThreads>(a, off, item, red);
-    if (blockIdx.x == 0) {  // the merge reads it
-        for (int e = tid; e <= E; e += kThreads) {
-            p.s.off[0][e] = off[e];
-            p.s.item[0][e] = item[e];
-        }
-    }
-    const uint32_t U = off[E], n = min(gridDim.x, U);
+    make_plan<false, kThreads>(a, p.s, off, item, red);
+    MONO_TL(tl_narrow, 2);
+    const uint32_t U = off[E] * a.kv_heads, per = part_size(U, gridDim.x), u0 = min(blockIdx.x * per, U), u1 = min(u0 + per, U);
     const int G = a.q_heads / a.kv_heads;
     const uint64_t wait_ns = a.wait_ns ? a.wait_ns : kWaitLimitNs;
-    if (blockIdx.x < n) {
-        const uint32_t u0 = cut(U, blockIdx.x, n), u1 = cut(U, blockIdx.x + 1, n);
+    if (u0 < u1) {
         if (warp == kConsumers) {
             // ---- fetch: 32 units' pages at a time are looked up by the lanes, then requested in order
-            int it = 0;
+            int it = 0, nth = 0;
             for (uint32_t base = u0; base < u1 && !*abortp; base += 32) {
                 const uint32_t u = min(base + lane, u1 - 1);
-                const int e = find_entry(off, E, u);
-                const Entry en = entry_of(a, e);
-                int tiles, units;
-                entry_work<false>(a, en, &tiles, &units);
-                const uint32_t local = u - off[e];
-                const int head = (int)(local / units) / tiles;
-                const int page = en.table[local % units];
+                const Place at = place_of(off, E, u);
+                const Entry en = entry_of(a, at.e);
+                const Work w = entry_work<false>(a, en);
+                const int head = at.head, tile = (int)(at.local / w.units), unit = (int)(at.local - (uint32_t)tile * w.units);
+                const int page = en.table[unit];
                 const bool ok = page >= 0 && page < a.n_pages;
+                const bool first = u == u0 || unit == 0;  // of a segment: its queries come along
+                const int row0 = tile * 16, rows = min(16, en.ntok * G - row0);
                 const int cnt = (int)min(32u, u1 - base);
                 for (int j = 0; j < cnt; ++j, ++it) {
                     const int pj = __shfl_sync(0xffffffffu, page, j), hj = __shfl_sync(0xffffffffu, head, j), okj = __shfl_sync(0xffffffffu, (int)ok, j);
+                    if (__shfl_sync(0xffffffffu, (int)first, j)) {
+                        // rows r0 .. of kv head hj: a lane fetches what they have of one token, heads side by side
+                        const int r0 = __shfl_sync(0xffffffffu, row0, j), n = __shfl_sync(0xffffffffu, rows, j), t0 = __shfl_sync(0xffffffffu, en.tok0, j), qs = nth & 1;
+                        if (lane == 0 && !*abortp && (nth < 2 || mbar_wait(&q_empty[qs], ((nth >> 1) - 1) & 1, abortp, wait_ns)))
+                            mbar_expect_tx(&q_full[qs], (uint32_t)n * kDim * 2);
+                        __syncwarp();
+                        const int tok = r0 / G + lane, from = max(tok * G, r0), to = min(tok * G + G, r0 + n);
+                        if (!*abortp && from < to)
+                            bulk_load(qbuf + qs * kQBytes + (from - r0) * kDim * 2,
+                                      reinterpret_cast<const __nv_bfloat16*>(a.q) + (size_t)(t0 + tok) * a.q_ld + (size_t)(hj * G + from - tok * G) * kDim,
+                                      (uint32_t)(to - from) * kDim * 2, &q_full[qs]);
+                        ++nth;
+                    }
                     if (lane == 0) {
                         const int st = it % kStages;
                         if (*abortp || (it >= kStages && !mbar_wait(&empty[st], ((it / kStages) - 1) & 1, abortp, wait_ns))) {
@@ -161,19 +180,22 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_narrow_kernel(const __grid
             }
         } else {
             const int g = lane >> 2, t = lane & 3;
-            int it = 0, e = find_entry(off, E, u0);
-            for (uint32_t u = u0; u < u1;) {
-                while (off[e + 1] <= u) ++e;
-                const Entry en = entry_of(a, e);
-                int tiles, units;
-                entry_work<false>(a, en, &tiles, &units);
-                const uint32_t local = u - off[e], it_in = local / units;
-                const int head = (int)it_in / tiles, tile = (int)it_in % tiles;
-                const int p0 = (int)(local % units), cnt = (int)min((uint32_t)(units - p0), u1 - u);
+            int it = 0, nth = 0;
+            for (uint32_t u = u0; u < u1; ++nth) {
+                const Place at = place_of(off, E, u);
+                const Entry en = entry_of(a, at.e);
+                const Work wk = entry_work<false>(a, en);
+                const int tile = (int)(at.local / wk.units);
+                const int p0 = (int)(at.local - (uint32_t)tile * wk.units), cnt = (int)min((uint32_t)(wk.units - p0), u1 - u);
                 uint32_t q[8][4];
                 float qs[2], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
                 int lim[2];
-                load_q(a, en, head, tile * 16, G, q, qs, lim);
+                mbar_wait(&q_full[nth & 1], (nth >> 1) & 1, abortp, wait_ns);  // given up: the pages are too, and all warps meet below
+                load_q(a, en, smem_u32(qbuf + (nth & 1) * kQBytes), tile * 16, G, q, qs, lim);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&q_empty[nth & 1]);
+                const int lim_all = min(en.len, __reduce_min_sync(0xffffffffu, min(lim[0], lim[1])));  // keys below it are seen by every row
+                MONO_TL(tl_narrow, 3 + 4 * nth);  // the first three items
                 float o[16][4];
 #pragma unroll
                 for (int j = 0; j < 16; ++j)
@@ -182,6 +204,7 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_narrow_kernel(const __grid
                 for (int i = 0; i < cnt; ++i, ++it) {
                     const int st = it % kStages;
                     if (!mbar_wait(&full[st], (it / kStages) & 1, abortp, wait_ns)) break;
+                    if (i == 0) MONO_TL(tl_narrow, 4 + 4 * nth);
                     const uint32_t kb = smem_u32(ring + st * 2 * kTileBytes), vb = kb + kTileBytes;
                     const int key0 = (p0 + i) * kPage + warp * 16;  // this warp's first key
                     if (page_ok[st] && key0 < en.len) {
@@ -196,25 +219,26 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_narrow_kernel(const __grid
 #pragma unroll
                             for (int j = 0; j < 8; ++j) mma_f16(s[nt], q[j], e4m3x2_to_f16x2(w[j]), e4m3x2_to_f16x2(w[j] >> 16));
                         }
-                        float mx[2] = {-INFINITY, -INFINITY};
+                        // scores stay in the units of the product: qs > 0, so their maximum is the scaled scores'
+                        if (key0 + 16 > lim_all) {
 #pragma unroll
-                        for (int nt = 0; nt < 2; ++nt)
+                            for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                const int r = j >> 1, key = key0 + nt * 8 + 2 * t + (j & 1);
-                                s[nt][j] = key < lim[r] ? s[nt][j] * qs[r] : -INFINITY;
-                                mx[r] = max_nan(mx[r], s[nt][j]);
-                            }
-                        float mn[2], alpha[2];
+                                for (int j = 0; j < 4; ++j)
+                                    if (key0 + nt * 8 + 2 * t + (j & 1) >= min(lim[j >> 1], en.len)) s[nt][j] = -INFINITY;
+                        }
+                        float base[2], alpha[2];
 #pragma unroll
                         for (int r = 0; r < 2; ++r) {
-                            mx[r] = max_nan(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
-                            mx[r] = max_nan(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
-                            mn[r] = max_nan(m[r], mx[r]);
+                            float mx = max_nan(max_nan(s[0][2 * r], s[0][2 * r + 1]), max_nan(s[1][2 * r], s[1][2 * r + 1]));
+                            mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                            mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+                            const float mn = max_nan(m[r], mx * qs[r]), z = mn == -INFINITY ? 0.f : mn;
                             // a row that has seen no key yet keeps max = -inf, and weights of 0
-                            alpha[r] = mn[r] == -INFINITY ? 1.f : exp2f(m[r] - mn[r]);
-                            m[r] = mn[r];
+                            alpha[r] = ex2(m[r] - z);
+                            m[r] = mn;
                             l[r] *= alpha[r];
+                            base[r] = kPBias - z;
                         }
                         uint32_t pa[4];
                         float pv[2][4];
@@ -223,7 +247,7 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_narrow_kernel(const __grid
 #pragma unroll
                             for (int j = 0; j < 4; ++j) {
                                 const int r = j >> 1;
-                                pv[nt][j] = s[nt][j] == -INFINITY ? 0.f : exp2f(s[nt][j] - mn[r] + kPBias);
+                                pv[nt][j] = ex2(fmaf(s[nt][j], qs[r], base[r]));
                                 l[r] += pv[nt][j];
                             }
                         pa[0] = pack_f16(pv[0][0], pv[0][1]);
@@ -245,8 +269,12 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_narrow_kernel(const __grid
                         for (int i4 = 0; i4 < 4; ++i4) {
                             const int kr = 2 * t + (i4 & 1) + (i4 >> 1) * 8;
                             const uint4 v = lds128(vb + (warp * 16 + kr) * 128 + ((g ^ (kr & 7)) << 4));
-                            const bool live = key0 + kr < en.len;
-                            vw[i4][0] = live ? v.x : 0u; vw[i4][1] = live ? v.y : 0u; vw[i4][2] = live ? v.z : 0u; vw[i4][3] = live ? v.w : 0u;
+                            vw[i4][0] = v.x; vw[i4][1] = v.y; vw[i4][2] = v.z; vw[i4][3] = v.w;
+                        }
+                        if (key0 + 16 > en.len) {
+#pragma unroll
+                            for (int i4 = 0; i4 < 4; ++i4)
+                                if (key0 + 2 * t + (i4 & 1) + (i4 >> 1) * 8 >= en.len) vw[i4][0] = vw[i4][1] = vw[i4][2] = vw[i4][3] = 0;
                         }
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
@@ -261,6 +289,7 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_narrow_kernel(const __grid
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&empty[st]);
                 }
+                MONO_TL(tl_narrow, 5 + 4 * nth);
                 // ---- the segment's rows: the four warps' parts, brought to one maximum
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
@@ -276,8 +305,8 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_narrow_kernel(const __grid
                 for (int r = 0; r < 2; ++r) {
                     const int row = g + 8 * r;
                     const float M = fmaxf(fmaxf(s_m[0][row], s_m[1][row]), fmaxf(s_m[2][row], s_m[3][row]));
-                    const float f = m[r] == -INFINITY ? 0.f : exp2f(m[r] - M);
-                    float* dst = comb + (warp * 16 + row) * kPitch + t * 32;
+                    const float f = m[r] == -INFINITY ? 0.f : ex2(m[r] - M);
+                    float* dst = comb + (warp * 16 + row) * kPitch + t * kQuarter;
 #pragma unroll
                     for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -286,7 +315,7 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_narrow_kernel(const __grid
                 }
                 consumer_sync();
                 {
-                    float* seg = p.s.seg[0] + (size_t)(blockIdx.x + item[e] + it_in) * Shape<false>::kSegFloats;
+                    float* seg = p.s.seg[0] + (size_t)(blockIdx.x + at.head * item[E] + item[at.e] + tile) * Shape<false>::kSegFloats;
                     const int rows = min(16, en.ntok * G - tile * 16);
                     if (tid < rows) {
                         const float M = fmaxf(fmaxf(s_m[0][tid], s_m[1][tid]), fmaxf(s_m[2][tid], s_m[3][tid]));
@@ -299,16 +328,18 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_narrow_kernel(const __grid
                     for (int r = 0; r < rows; ++r) {
                         float sum = 0.f;
 #pragma unroll
-                        for (int w = 0; w < kConsumers; ++w) sum += comb[(w * 16 + r) * kPitch + tid];
+                        for (int w = 0; w < kConsumers; ++w) sum += comb[(w * 16 + r) * kPitch + (tid >> 5) * kQuarter + (tid & 31)];
                         seg[32 + r * kDim + tid] = sum;
                     }
                 }
                 consumer_sync();
+                MONO_TL(tl_narrow, 6 + 4 * nth);
                 u += cnt;
             }
         }
     }
     __syncthreads();
+    MONO_TL(tl_narrow, 15);
     if (*abortp) {
         for (int i = 0; i < 64; ++i) __nanosleep(1000);  // copies in flight land before the CTA's memory goes
         if (tid == 0 && !guard_failed(a.guard)) guard_fail(a.guard, MONO_ERR_DEADLINE, kSiteWait);
@@ -316,108 +347,129 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_narrow_kernel(const __grid
 }
 
 // ------------------------------------------------------------------ merge
-// One CTA of four warps per (token, 4 / SPLIT heads): SPLIT warps share a row's segments.  A lane holds four dims.
+// The parts of one row that one kernel left for one entry: `count` segments `stride` floats apart.
+struct Parts {
+    const float *m, *v;  // the first part's maximum (its sum lies `rows` floats behind) and the first of this lane's values
+    int rows, count, step;  // step: floats from the lane's first four values to the next four
+    size_t stride;
+};
+__device__ __forceinline__ Parts parts_of(const mono_prefix_attn_args& a, const Scratch& s, const Record& n, int token, int head, int G, int narrow_ctas,
+                                          int wide_ctas, int sub) {
+    Parts r = {nullptr, nullptr, 0, 0, 0, 0};
+    const int wide = n.wide;
+    const uint32_t per_head = s.total[wide][0], items = s.total[wide][1];
+    if (n.tiles == 0 || per_head == 0) return r;  // no keys, or refused tables
+    const int kh = head / G, row = (token - n.tok0) * G + head - kh * G;
+    r.rows = wide ? Shape<true>::kTile : Shape<false>::kTile;
+    r.stride = wide ? Shape<true>::kSegFloats : Shape<false>::kSegFloats;
+    const int tile = row / r.rows, at = row - tile * r.rows;
+    const uint32_t per = part_size(per_head * a.kv_heads, wide ? wide_ctas : narrow_ctas);
+    const uint32_t first = kh * per_head + n.off + (uint32_t)tile * n.units;
+    const uint32_t c0 = first / per, c1 = (first + (tile == n.tiles - 1 ? n.last : n.units) - 1) / per;
+    const float* seg = s.seg[wide] + (size_t)(c0 + kh * items + n.item + tile) * r.stride;
+    r.m = seg + at;
+    // narrow: rows of 128 values; wide: four dims of all rows, then the next four (as a thread per row writes them)
+    r.v = seg + 2 * r.rows + (wide ? (sub * 2 * Shape<true>::kTile + at) * 4 : at * kDim + sub * 8);
+    r.step = wide ? Shape<true>::kTile * 4 : 4;
+    r.count = (int)(c1 - c0) + 1;
+    return r;
+}
+
+// Half a warp per (token, head): a lane holds eight dims, and the rows of neighbouring heads, which lie side by side in a
+// wide segment, are read together.  SPLIT warps of a CTA share a pair of heads' parts; a batch of parts is requested at
+// once and added to a running maximum, so a row of few parts costs one round trip.
 template <int SPLIT>
 __global__ void __launch_bounds__(128) prefix_merge_kernel(const mono_prefix_attn_args a, const Scratch s, int narrow_ctas, int wide_ctas) {
     pdl_prologue();
-    __shared__ int s_seq, s_grp;
-    __shared__ float4 s_num[4][32];
-    __shared__ float s_den[4];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int token = blockIdx.x, head = blockIdx.y * (4 / SPLIT) + warp / SPLIT, part = warp % SPLIT;
-    if (tid == 0) { s_seq = INT32_MAX; s_grp = INT32_MAX; }
-    __syncthreads();
-    for (int e = tid; e < a.groups + a.seqs; e += 128) {
-        const Entry n = entry_of(a, e);
-        if (token >= n.tok0 && token < n.tok0 + n.ntok) atomicMin(e < a.groups ? &s_grp : &s_seq, e);
-    }
-    __syncthreads();
-    if (s_seq == INT32_MAX) return;  // behind the last sequence: the row stays as it was
-    const bool on = head < a.q_heads;
-    const int G = a.q_heads / a.kv_heads, E = a.groups + a.seqs;
-    // the segments of the row's two items: `count` segments `stride` floats apart
-    const float* base[2] = {nullptr, nullptr};
-    int count[2] = {0, 0}, stride[2] = {0, 0}, tile_rows[2] = {0, 0}, row_in[2] = {0, 0}, twice[2] = {0, 0};
+    __shared__ float s_num[4][8][32], s_m[4][2], s_den[4][2];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, half = lane >> 4, sub = lane & 15;
+    const int token = blockIdx.x, head = (blockIdx.y * (4 / SPLIT) + warp / SPLIT) * 2 + half, part = warp % SPLIT;
+    // The token's group and sequence.  Nobody clears the list between launches: what it says counts if the entry has the
+    // token.
+    const int E = a.groups + a.seqs;
+    const int e[2] = {a.groups ? s.entry[0][token] : -1, s.entry[1][token]};
+    Record rec[2];
+    bool in[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-        const int e = k ? s_seq : s_grp;
-        if (e == INT32_MAX || !on) continue;
-        const Entry n = entry_of(a, e);
-        const int w = n.ntok * G >= kWideRows;
-        const int tr = w ? Shape<true>::kTile : Shape<false>::kTile;
-        int tiles, units;
-        if (w) entry_work<true>(a, n, &tiles, &units); else entry_work<false>(a, n, &tiles, &units);
-        if (units == 0) continue;
-        const uint32_t* off = s.off[w];
-        const uint32_t U = off[E], ctas = min((uint32_t)(w ? wide_ctas : narrow_ctas), U);
-        if (U == 0) continue;  // refused tables
-        const int row = (token - n.tok0) * G + head % G, it_in = (head / G) * tiles + row / tr;
-        const uint32_t first = off[e] + (uint32_t)it_in * units;
-        const uint32_t c0 = owner(U, first, ctas), c1 = owner(U, first + units - 1, ctas);
-        stride[k] = w ? Shape<true>::kSegFloats : Shape<false>::kSegFloats;
-        base[k] = s.seg[w] + (size_t)(c0 + s.item[w][e] + it_in) * stride[k];
-        tile_rows[k] = tr;
-        row_in[k] = row % tr;
-        twice[k] = w && n.ntok * G - (row / tr) * tr <= kWideHalf;
-        count[k] = ((int)(c1 - c0) + 1) << twice[k];
+        in[k] = k ? e[k] >= a.groups && e[k] < E : e[k] >= 0 && e[k] < a.groups;
+        if (in[k]) rec[k] = s.rec[e[k]];
+        in[k] = in[k] && token >= rec[k].tok0 && token < rec[k].tok0 + rec[k].ntok;
     }
-    const int total = count[0] + count[1];
-    // part i of the row: where its segment lies, and the row in that segment
-    auto part_of = [&](int i, const float** sg, int* rows, int* r) {
-        const int k = i >= count[0], j = i - (k ? count[0] : 0);
-        *sg = base[k] + (size_t)(j >> twice[k]) * stride[k];
-        *rows = tile_rows[k];
-        *r = row_in[k] + (twice[k] ? (j & 1) * kWideHalf : 0);
-    };
-    float M = -INFINITY;
-    for (int i = lane; i < total; i += 32) {
-        const float* sg;
-        int rows, rr;
-        part_of(i, &sg, &rows, &rr);
-        M = fmaxf(M, __ldcg(sg + rr));
-    }
-    M = warp_max(M);
-    float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
-    float den = 0.f;
-    constexpr int B = 4;
-    for (int i0 = part; i0 < total; i0 += SPLIT * B) {
-        float m[B], l[B];
-        float4 v[B];
+    if (!in[1]) return;  // a token of no sequence: the row stays as it was
+    const int G = a.q_heads / a.kv_heads;
+    float M = -INFINITY, den = 0.f, num[8] = {};
+    if (head < a.q_heads) {
+#pragma unroll 1
+        for (int k = 0; k < 2; ++k) {
+            if (!(k ? in[1] : in[0])) continue;
+            const Parts ps = parts_of(a, s, k ? rec[1] : rec[0], token, head, G, narrow_ctas, wide_ctas, sub);
+            constexpr int B = 4;
+#pragma unroll 1
+            for (int i0 = part; i0 < ps.count; i0 += SPLIT * B) {
+                float m[B], l[B], top = M;
+                float4 v[B][2];
 #pragma unroll
-        for (int j = 0; j < B; ++j) {  // unconditional loads, all in flight together
-            const float* sg;
-            int rows, rr;
-            part_of(min(i0 + j * SPLIT, total - 1), &sg, &rows, &rr);
-            m[j] = __ldcg(sg + rr);
-            l[j] = __ldcg(sg + rows + rr);
-            v[j] = ld_cg_f4_ordered(sg + 2 * rows + rr * kDim + lane * 4);
-        }
+                for (int j = 0; j < B; ++j) {  // unconditional loads, all in flight together
+                    const size_t o = (size_t)min(i0 + j * SPLIT, ps.count - 1) * ps.stride;
+                    m[j] = ps.m[o];
+                    l[j] = ps.m[ps.rows + o];
+                    v[j][0] = *reinterpret_cast<const float4*>(ps.v + o);
+                    v[j][1] = *reinterpret_cast<const float4*>(ps.v + ps.step + o);
+                }
 #pragma unroll
-        for (int j = 0; j < B; ++j) {
-            const bool live = i0 + j * SPLIT < total && m[j] != -INFINITY;
-            const float w = live ? exp2f(m[j] - M) : 0.f;
-            den += live ? l[j] * w : 0.f;
-            num.x += live ? v[j].x * w : 0.f; num.y += live ? v[j].y * w : 0.f;
-            num.z += live ? v[j].z * w : 0.f; num.w += live ? v[j].w * w : 0.f;
+                for (int j = 0; j < B; ++j) {
+                    if (i0 + j * SPLIT >= ps.count) m[j] = -INFINITY;
+                    top = fmaxf(top, m[j]);
+                }
+                const float old = M == -INFINITY ? 0.f : exp2f(M - top);
+                den *= old;
+#pragma unroll
+                for (int q = 0; q < 8; ++q) num[q] *= old;
+#pragma unroll
+                for (int j = 0; j < B; ++j) {
+                    const bool live = m[j] != -INFINITY;  // also NaN: a row of NaN
+                    const float w = live ? exp2f(m[j] - top) : 0.f;
+                    den += live ? l[j] * w : 0.f;
+                    const float vv[8] = {v[j][0].x, v[j][0].y, v[j][0].z, v[j][0].w, v[j][1].x, v[j][1].y, v[j][1].z, v[j][1].w};
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) num[q] += live ? vv[q] * w : 0.f;
+                }
+                M = top;
+            }
         }
     }
     if (SPLIT > 1) {
-        s_num[warp][lane] = num;
-        if (lane == 0) s_den[warp] = den;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) s_num[warp][q][lane] = num[q];
+        if (sub == 0) { s_m[warp][half] = M; s_den[warp][half] = den; }
         __syncthreads();
         if (part != 0) return;
+        float top = M;
 #pragma unroll
-        for (int w = 1; w < SPLIT; ++w) {
-            const float4 x = s_num[warp + w][lane];
-            num.x += x.x; num.y += x.y; num.z += x.z; num.w += x.w;
-            den += s_den[warp + w];
+        for (int w = 1; w < SPLIT; ++w) top = fmaxf(top, s_m[warp + w][half]);
+        den = 0.f;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) num[q] = 0.f;
+#pragma unroll
+        for (int w = 0; w < SPLIT; ++w) {
+            const float d = s_den[warp + w][half], mw = s_m[warp + w][half];
+            // (a part of NaN alone has no maximum, and NaN sums)
+            const float f = mw != -INFINITY ? exp2f(mw - top) : d != d ? 1.f : 0.f;
+            den += d * f;
+#pragma unroll
+            for (int q = 0; q < 8; ++q) num[q] += s_num[warp + w][q][lane] * f;
         }
     }
-    if (!on) return;
+    if (head >= a.q_heads) return;
     const float f = den == 0.f ? 0.f : a.v_scale / den;  // a row that sees no key gives zeros
-    const __nv_bfloat162 lo = __floats2bfloat162_rn(num.x * f, num.y * f), hi = __floats2bfloat162_rn(num.z * f, num.w * f);
-    reinterpret_cast<uint2*>(a.out)[((size_t)token * a.q_heads + head) * (kDim / 4) + lane] =
-        make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+    uint32_t o[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const __nv_bfloat162 b = __floats2bfloat162_rn(num[2 * q] * f, num[2 * q + 1] * f);
+        o[q] = *reinterpret_cast<const uint32_t*>(&b);
+    }
+    reinterpret_cast<uint4*>(a.out)[((size_t)token * a.q_heads + head) * (kDim / 8) + sub] = make_uint4(o[0], o[1], o[2], o[3]);
 }
 
 // ------------------------------------------------------------------ host
@@ -446,7 +498,7 @@ static size_t narrow_bytes(int tokens, int q_heads, int kv_heads, int seqs, int 
 extern "C" size_t mono_prefix_attn_scratch_bytes(int tokens, int q_heads, int kv_heads, int seqs, int groups) {
     using namespace prefix_attn;
     if (tokens < 1 || q_heads < 1 || kv_heads < 1 || seqs < 1 || groups < 0 || q_heads % kv_heads) return 0;
-    return 4 * up256((size_t)(seqs + groups + 1) * 4) + narrow_bytes(tokens, q_heads, kv_heads, seqs, groups) +
+    return up256((size_t)(seqs + groups) * sizeof(Record)) + 256 + 2 * up256((size_t)tokens * 4) + narrow_bytes(tokens, q_heads, kv_heads, seqs, groups) +
            wide_segments(tokens, q_heads, kv_heads) * Shape<true>::kSegFloats * sizeof(float);
 }
 
@@ -493,19 +545,22 @@ extern "C" int mono_prefix_attn_launch(const mono_prefix_attn_args* a, void* str
     if (int rc = mono_tmap_encode_box(reinterpret_cast<mono_tmap_t*>(&p.vmap), a->v_cache, inner, rows, 1, inner, inner * rows, kPage)) return rc;
     p.a = *a;
     uint8_t* at = reinterpret_cast<uint8_t*>(a->scratch);
-    const size_t words = up256((size_t)(a->seqs + a->groups + 1) * 4);
+    p.s.rec = reinterpret_cast<Record*>(at);
+    at += up256((size_t)(a->seqs + a->groups) * sizeof(Record));
+    for (int w = 0; w < 2; ++w) p.s.total[w] = reinterpret_cast<uint32_t*>(at) + 2 * w;
+    at += 256;
     for (int w = 0; w < 2; ++w) {
-        p.s.off[w] = reinterpret_cast<uint32_t*>(at);
-        p.s.item[w] = reinterpret_cast<uint32_t*>(at + words);
-        at += 2 * words;
+        p.s.entry[w] = reinterpret_cast<int*>(at);
+        at += up256((size_t)a->tokens * 4);
     }
     p.s.seg[0] = reinterpret_cast<float*>(at);
     p.s.seg[1] = reinterpret_cast<float*>(at + narrow_bytes(a->tokens, a->q_heads, a->kv_heads, a->seqs, a->groups));
     const cudaStream_t st = (cudaStream_t)stream;
-    const size_t smem = 1024 + kStages * 2 * kTileBytes + kConsumers * 16 * kPitch * sizeof(float) + 2 * (size_t)(a->seqs + a->groups + 1) * 4;
+    constexpr size_t fixed = 1024 + kStages * 2 * kTileBytes + kConsumers * 16 * kPitch * sizeof(float) + 2 * kQBytes;
+    const size_t smem = fixed + 2 * (size_t)(a->seqs + a->groups + 1) * 4;
     static std::atomic<uint64_t> attr_once{0};  // bit d: set on device d
     if (attr_needed(attr_once)) {
-        const size_t most = 1024 + kStages * 2 * kTileBytes + kConsumers * 16 * kPitch * sizeof(float) + 2 * (size_t)(kMaxEntries + 1) * 4;
+        const size_t most = fixed + 2 * (size_t)(kMaxEntries + 1) * 4;
         const cudaError_t e = cudaFuncSetAttribute(prefix_narrow_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
         if (e != cudaSuccess) {
             mono_set_error("%s: %s", who, cudaGetErrorString(e));
@@ -517,13 +572,22 @@ extern "C" int mono_prefix_attn_launch(const mono_prefix_attn_args* a, void* str
     const int wide = (long)a->tokens * (a->q_heads / a->kv_heads) >= kWideRows ? sm_or_default() : 0;  // no entry has more rows than the step
     cudaError_t e = wide ? launch_wide(p, wide, st) : cudaSuccess;
     if (e == cudaSuccess) e = launch_k(prefix_narrow_kernel, narrow, kThreads, smem, st, p);
-    // Few rows: four warps share a row's segments (a long prefix leaves many of them); many rows: a warp each.
+    // Few rows: four warps share two heads' segments (a long prefix leaves many of them); many rows: a warp each.
     if (e == cudaSuccess) {
         if ((long)a->tokens * a->q_heads < 2048)
-            e = launch_k(prefix_merge_kernel<4>, dim3(a->tokens, a->q_heads), 128, 0, st, *a, p.s, narrow, wide);
+            e = launch_k(prefix_merge_kernel<4>, dim3(a->tokens, (a->q_heads + 1) / 2), 128, 0, st, *a, p.s, narrow, wide);
         else
-            e = launch_k(prefix_merge_kernel<1>, dim3(a->tokens, (a->q_heads + 3) / 4), 128, 0, st, *a, p.s, narrow, wide);
+            e = launch_k(prefix_merge_kernel<1>, dim3(a->tokens, (a->q_heads + 7) / 8), 128, 0, st, *a, p.s, narrow, wide);
     }
     if (e != cudaSuccess) mono_set_error("%s: %s", who, cudaGetErrorString(e));
     return (int)e;
 }
+
+#ifdef MONO_TIMELINE
+// Copies the narrow kernel's stamps of the last launch to `out` (MONO_TL_CTAS x MONO_TL_POINTS); blocks the host.
+extern "C" int mono_timeline_read_prefix_narrow(unsigned long long* out, int* ctas, int* points) {
+    *ctas = MONO_TL_CTAS;
+    *points = MONO_TL_POINTS;
+    return (int)cudaMemcpyFromSymbol(out, prefix_attn::tl_narrow, sizeof(unsigned long long) * MONO_TL_CTAS * MONO_TL_POINTS);
+}
+#endif

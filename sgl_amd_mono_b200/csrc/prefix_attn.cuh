@@ -53,30 +53,55 @@ __device__ __forceinline__ int row_limit(const Entry& n, int row, int G) {
     return n.causal ? n.len - n.ntok + 1 + row / G : n.len;
 }
 
-// A kernel's view of the work: narrow (16-row tiles, 64-key units) or wide (256-row tiles, 128-key units).
+// A kernel's view of the work: narrow (16-row tiles, units of 64 keys) or wide (256-row tiles, units of 128 keys).
+// A wide item of at most kWideHalf rows gives its CTA's two halves the same rows and alternate blocks of 128 keys, so
+// that its units are 256 keys and cost what the others' do.
 template <bool WIDE>
 struct Shape {
     static constexpr int kTile = WIDE ? 256 : 16;
     static constexpr int kKeys = WIDE ? 128 : 64;
     static constexpr int kSegFloats = 2 * kTile + kTile * kDim;  // max, sum, values
 };
+constexpr int kWideHalf = 128;
 // rows of an entry from which the wide kernel takes it
 constexpr int kWideRows = 48;
-// A wide item of at most this many rows is computed twice over alternate units, by the two halves of its CTA: its
-// segments then hold two parts per row, at tile rows r and r + 128.
-constexpr int kWideHalf = 128;
 
+struct Work {
+    int tiles, units, last;  // row tiles; units of a tile, and of the last one
+    __device__ __forceinline__ int per_head() const { return (tiles - 1) * units + last; }
+};
 template <bool WIDE>
-__device__ __forceinline__ void entry_work(const mono_prefix_attn_args& a, const Entry& n, int* tiles, int* units) {
+__device__ __forceinline__ Work entry_work(const mono_prefix_attn_args& a, const Entry& n) {
     const int rows = n.ntok * (a.q_heads / a.kv_heads);
-    const bool mine = (rows >= kWideRows) == WIDE && rows > 0 && n.len > 0;
-    *tiles = mine ? (rows + Shape<WIDE>::kTile - 1) / Shape<WIDE>::kTile : 0;
-    *units = mine ? (n.len + Shape<WIDE>::kKeys - 1) / Shape<WIDE>::kKeys : 0;
+    Work w = {0, 0, 0};
+    if ((rows >= kWideRows) != WIDE || rows <= 0 || n.len <= 0) return w;
+    w.tiles = (rows + Shape<WIDE>::kTile - 1) / Shape<WIDE>::kTile;
+    w.units = w.last = (n.len + Shape<WIDE>::kKeys - 1) / Shape<WIDE>::kKeys;
+    if (WIDE && rows - (w.tiles - 1) * Shape<WIDE>::kTile <= kWideHalf) w.last = (w.units + 1) / 2;
+    return w;
 }
 
-// off[0..E]: units before entry e (off[E]: all); item[0..E]: items before entry e.  Called by all threads of a block.
+// What the merge has to know of an entry, from the kernel that has the entry.
+struct alignas(16) Record {
+    int tok0, ntok;
+    uint32_t off, item;  // the entry's first unit and item of kv head 0
+    int tiles, units, last, wide;
+};
+// Where things lie in the scratch.  CTA c's segment of item i is number c + i: both grow along the list of units, so no
+// two segments share a number.  `entry`: per token its group (or what an earlier launch left) and its sequence.
+struct Scratch {
+    Record* rec;           // [entries]
+    uint32_t* total[2];    // units and items of one kv head
+    int* entry[2];         // [tokens]
+    float* seg[2];
+};
+
+// off[0..E]: units of one kv head before entry e (off[E]: all of them); item[0..E]: items likewise.  The list of units
+// runs through all entries for kv head 0, then for kv head 1, ...: CTAs of different heads walk the same pages at the
+// same time, and a page's rows, which lie head beside head, are fetched from HBM together.  Called by all threads of a
+// block; the blocks together leave the merge's records.
 template <bool WIDE, int THREADS>
-__device__ __forceinline__ void make_plan(const mono_prefix_attn_args& a, uint32_t* off, uint32_t* item, uint32_t* red /* [2 * 32] */) {
+__device__ __forceinline__ void make_plan(const mono_prefix_attn_args& a, const Scratch& s, uint32_t* off, uint32_t* item, uint32_t* red /* [2 * 32] */) {
     const int E = a.groups + a.seqs, per = (E + THREADS - 1) / THREADS;
     const int e0 = min((int)threadIdx.x * per, E), e1 = min(e0 + per, E);
     uint32_t su = 0, si = 0;
@@ -86,12 +111,16 @@ __device__ __forceinline__ void make_plan(const mono_prefix_attn_args& a, uint32
     for (int e = e0; e < e1; ++e) {
         const int32_t* st = e < a.groups ? a.group_start + e : a.q_start + (e - a.groups);
         bad |= st[0] < 0 || st[1] < st[0] || st[1] > (e < a.groups ? a.seqs : a.tokens);
-        int tiles, units;
-        entry_work<WIDE>(a, entry_of(a, e), &tiles, &units);
+        const Entry n = entry_of(a, e);
+        const Work w = entry_work<WIDE>(a, n);
         off[e] = su;
         item[e] = si;
-        su += (uint32_t)tiles * a.kv_heads * units;
-        si += (uint32_t)tiles * a.kv_heads;
+        if (w.tiles) su += (uint32_t)w.per_head();
+        si += (uint32_t)w.tiles;
+        if (!WIDE) {  // this block's share of the tokens
+            int t = n.tok0 + (int)((blockIdx.x + gridDim.x - (uint32_t)n.tok0 % gridDim.x) % gridDim.x);
+            for (; t < n.tok0 + n.ntok; t += gridDim.x) s.entry[e >= a.groups][t] = e;
+        }
     }
     // the sums of the threads before this one
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -102,39 +131,52 @@ __device__ __forceinline__ void make_plan(const mono_prefix_attn_args& a, uint32
         if (lane >= o) { pu += u; pi += i; }
     }
     if (lane == 31) { red[warp] = pu; red[32 + warp] = pi; }
-    __syncthreads();
+    bad = __syncthreads_or(bad);
     uint32_t bu = 0, bi = 0;
     for (int w = 0; w < warp; ++w) { bu += red[w]; bi += red[32 + w]; }
     bu += pu - su;
     bi += pi - si;
     for (int e = e0; e < e1; ++e) { off[e] += bu; item[e] += bi; }
-    if (threadIdx.x == THREADS - 1) { off[E] = bu + su; item[E] = bi + si; }
-    bad = __syncthreads_or(bad);
-    if (bad && threadIdx.x == 0) {
-        off[E] = 0;  // nobody has work
-        if (blockIdx.x == 0) guard_fail(a.guard, MONO_ERR_ARG, kSiteTables);
+    if (threadIdx.x == THREADS - 1) {
+        off[E] = bad ? 0 : bu + su;  // refused: nobody has work
+        item[E] = bi + si;
+        if (blockIdx.x == 0) {
+            s.total[WIDE][0] = off[E];
+            s.total[WIDE][1] = item[E];
+            if (bad) guard_fail(a.guard, MONO_ERR_ARG, kSiteTables);
+        }
+    }
+    if (blockIdx.x == 0) {
+        for (int e = e0; e < e1; ++e) {
+            const Entry n = entry_of(a, e);
+            const bool wide = n.ntok * (a.q_heads / a.kv_heads) >= kWideRows;
+            if (wide != WIDE) continue;
+            const Work w = entry_work<WIDE>(a, n);
+            s.rec[e] = Record{n.tok0, n.ntok, off[e], item[e], w.tiles, w.units, w.last, wide};
+        }
     }
     __syncthreads();
 }
-// the entry that holds unit u: the last e with off[e] <= u (entries without units share an offset with the next)
-__device__ __forceinline__ int find_entry(const uint32_t* off, int E, uint32_t u) {
-    int lo = 0, hi = E - 1;
+// A place in the list: kv head, entry, unit of the entry.
+struct Place {
+    int head, e;
+    uint32_t local;
+};
+__device__ __forceinline__ Place place_of(const uint32_t* off, int E, uint32_t u) {
+    Place p;
+    p.head = (int)(u / off[E]);
+    u -= (uint32_t)p.head * off[E];
+    int lo = 0, hi = E - 1;  // the last entry that starts at or before u (entries without units share a start with the next)
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
         if (off[mid] <= u) lo = mid; else hi = mid - 1;
     }
-    return lo;
+    p.e = lo;
+    p.local = u - off[lo];
+    return p;
 }
-// CTA c of n takes units [cut(c), cut(c + 1)) of U; n is at most U, so nobody's part is empty.
-__device__ __forceinline__ uint32_t cut(uint32_t U, uint32_t c, uint32_t n) { return (uint32_t)((uint64_t)U * c / n); }
-__device__ __forceinline__ uint32_t owner(uint32_t U, uint32_t u, uint32_t n) { return (uint32_t)((((uint64_t)u + 1) * n - 1) / U); }
-
-// Where things lie in the scratch: per kernel its plan (off, item: E + 1 words each) and its segments.  CTA c's segment
-// of item i is number c + i: both grow along the list of units, so no two segments share a number.
-struct Scratch {
-    uint32_t *off[2], *item[2];
-    float* seg[2];
-};
+// Every CTA takes `part_size` units, the last of them what is left: no part in use is empty.
+__device__ __forceinline__ uint32_t part_size(uint32_t U, uint32_t ctas) { return max((U + ctas - 1) / ctas, 1u); }
 
 struct alignas(64) Params {
     CUtensorMap kmap, vmap;

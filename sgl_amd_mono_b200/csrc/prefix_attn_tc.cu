@@ -19,11 +19,15 @@
 
 namespace prefix_attn {
 namespace {
+MONO_TL_DECLARE(tl_wide)
 
 constexpr int kKeys = 128;
-constexpr int kSoftmaxThreads = 256;  // warps 0..3: stream 0, 4..7: stream 1
+// warps 0..3: softmax of stream 0, 4..7: of stream 1
 constexpr int kConvWarp0 = 8, kTmaWarp = 12, kMmaWarp = 13;
-constexpr int kThreadsWide = 14 * 32;
+constexpr int kThreadsWide = 16 * 32;  // warps 14 and 15 only fill the fetching warps' warpgroup
+// Registers per thread: 128 at launch, moved from the warpgroups that need few to the two softmax ones, which hold a
+// X.
+constexpr int kRegsSoftmax = 168, kRegsConv = 72, kRegsFetch = 104;
 constexpr int kKStages = 3, kVStages = 2, kWStages = 2;  // K bytes, V bytes, widened V
 constexpr int kQPlane = 128 * 128;                       // [128 rows][128 B]
 constexpr int kKTile = kKeys * 128, kVTile = kKeys * 128, kWTile = 2 * kKeys * 128;
@@ -32,6 +36,30 @@ constexpr int kSmemFixed = 1024 + 2 * 2 * kQPlane + kKStages * kKTile + kVStages
 constexpr int kTmemCols = 512;  // S of stream 0 and 1 (P over their first half), O of stream 0 and 1
 constexpr float kBias = 7.f, kLazy = 8.f;
 
+template <int N> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+// The roles share the instruction caches, and the issuing warp pays for every line the others push out (it took 0.5 us
+// to issue eight products beside softmax loops unrolled over a whole block): waits are short code, and the loops below are
+// rolled over quarters of a block.
+__device__ __forceinline__ bool wait_on(uint64_t* bar, uint32_t parity, volatile int* abort_flag, uint64_t limit_ns) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const uint64_t t0 = globaltimer_ns();
+#pragma unroll 1
+    while (!mbar_try_wait(bar, parity)) {  // (each try sleeps for a while)
+        if (*abort_flag) return false;
+        if (globaltimer_ns() - t0 > limit_ns) {
+            *abort_flag = 1;
+            return false;
+        }
+    }
+    return true;
+}
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
@@ -49,6 +77,11 @@ __device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t bdes
         "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
         "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
         ::"r"(d), "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t r[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(taddr) : "memory");
 }
 #define PA_REGS32(r) "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
 // 32 columns of this thread's lane, requested; wait_ld() before they are used
@@ -87,85 +120,149 @@ __device__ __forceinline__ uint32_t widen2(uint32_t lo16) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// The CTA's current item, as every role walks it.
-struct Item {
-    Entry en;
-    int head, row0, rows;  // first row, rows of the item (at most 256)
-    int p0, units;         // first unit, units to compute (those no row sees are left out)
-    bool split;            // both streams have the same rows and take alternate units
-    uint32_t seg, span;    // segment number; units of the list that this covers
-    // stream st takes units first(st), first(st) + step, ...
-    __device__ __forceinline__ int first(int st) const { return split ? st : 0; }
-    __device__ __forceinline__ int step() const { return split ? 2 : 1; }
-    __device__ __forceinline__ int count(int st) const { return split ? (units - st + 1) / 2 : units; }
-};
-__device__ __forceinline__ Item item_at(const mono_prefix_attn_args& a, const uint32_t* off, const uint32_t* item, uint32_t u, uint32_t u1, int* e) {
-    Item it;
-    const int E = a.groups + a.seqs, G = a.q_heads / a.kv_heads;
-    if (*e < 0) *e = find_entry(off, E, u);
-    while (off[*e + 1] <= u) ++*e;
-    it.en = entry_of(a, *e);
-    int tiles, units;
-    entry_work<true>(a, it.en, &tiles, &units);
-    const uint32_t local = u - off[*e], in = local / units;
-    it.head = (int)in / tiles;
-    it.row0 = ((int)in % tiles) * Shape<true>::kTile;
-    it.rows = min(Shape<true>::kTile, it.en.ntok * G - it.row0);
-    it.split = it.rows <= kWideHalf;
-    it.p0 = (int)(local % units);
-    it.span = min((uint32_t)(units - it.p0), u1 - u);
-    const int seen = max(row_limit(it.en, it.row0 + it.rows - 1, G), 0);
-    it.units = max(0, min((int)it.span, (seen + kKeys - 1) / kKeys - it.p0));
-    it.seg = blockIdx.x + item[*e] + in;
-    return it;
-}
-
-// A unit's scores: weights into P, their sum into l.  `vis`: how many of the unit's keys this row sees; `ok`: which of
-// its two pages exist.
+// A block's scores, in two passes over tensor memory (a quarter is requested while the one before is worked on): their
+// maximum, then the weights into P, over columns of S that have been read, and the weights' sum.  `vis`: how many of the
+// block's keys this row sees; `ok`: which of its two pages exist.
 template <bool MASK>
-__device__ __forceinline__ float unit_max(uint32_t s_addr, int vis, int ok) {
-    float mx = -INFINITY;
-#pragma unroll 1
-    for (int c = 0; c < 4; ++c) {
-        uint32_t r[32];
-        tmem_ld32(s_addr + c * 32, r);
-        wait_ld();
-        const bool page = ok >> (c >> 1) & 1;
-        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+__device__ __forceinline__ float quarter_max(const uint32_t r[32], int c, int vis, int ok, float mx) {
+    const int n = MASK ? (ok >> (c >> 1) & 1 ? vis - c * 32 : 0) : 32;
+    float m4[4] = {mx, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-            float v = __uint_as_float(r[i]);
-            if (MASK) v = page && c * 32 + i < vis ? v : -INFINITY;
-            m4[i & 3] = fmaxf(m4[i & 3], v);
-        }
-        mx = fmaxf(mx, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
+    for (int i = 0; i < 32; ++i) m4[i & 3] = fmaxf(m4[i & 3], !MASK || i < n ? __uint_as_float(r[i]) : -INFINITY);
+    return fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+}
+template <bool MASK>
+__device__ __forceinline__ float block_max(uint32_t s_addr, int vis, int ok) {
+    uint32_t a[32], b[32];
+    float mx = -INFINITY;
+    tmem_ld32(s_addr, a);
+    wait_ld();
+#pragma unroll 1
+    for (int c = 0; c < 4; c += 2) {
+        tmem_ld32(s_addr + (c + 1) * 32, b);
+        mx = quarter_max<MASK>(a, c, vis, ok, mx);
+        wait_ld();
+        tmem_ld32(s_addr + ((c + 2) & 3) * 32, a);
+        mx = quarter_max<MASK>(b, c + 1, vis, ok, mx);
+        wait_ld();
     }
     return mx;
 }
 template <bool MASK>
-__device__ __forceinline__ float unit_weights(uint32_t s_addr, int vis, int ok, float scale, float shift) {
-    float l4[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 1
-    for (int c = 0; c < 4; ++c) {
-        uint32_t r[32], w[16];
-        tmem_ld32(s_addr + c * 32, r);
-        wait_ld();
-        const bool page = ok >> (c >> 1) & 1;
+__device__ __forceinline__ void quarter_weights(const uint32_t r[32], uint32_t s_addr, int c, int vis, int ok, float scale, float shift, float l4[4]) {
+    const int n = MASK ? (ok >> (c >> 1) & 1 ? vis - c * 32 : 0) : 32;
+    uint32_t w[16];
 #pragma unroll
-        for (int i = 0; i < 32; i += 2) {
-            float x0 = fmaf(__uint_as_float(r[i]), scale, shift), x1 = fmaf(__uint_as_float(r[i + 1]), scale, shift);
-            if (MASK) {
-                x0 = page && c * 32 + i < vis ? x0 : -INFINITY;
-                x1 = page && c * 32 + i + 1 < vis ? x1 : -INFINITY;
-            }
-            const float p0 = ex2(x0), p1 = ex2(x1);
-            l4[i & 2] += p0;
-            l4[(i & 2) + 1] += p1;
-            w[i >> 1] = pack_half(p0, p1);
+    for (int i = 0; i < 32; i += 2) {
+        float p0 = ex2(fmaf(__uint_as_float(r[i]), scale, shift)), p1 = ex2(fmaf(__uint_as_float(r[i + 1]), scale, shift));
+        if (MASK) {
+            p0 = i < n ? p0 : 0.f;
+            p1 = i + 1 < n ? p1 : 0.f;
         }
-        tmem_st16(s_addr + c * 16, w);  // over columns of S that have been read
+        l4[i & 2] += p0;
+        l4[(i & 2) + 1] += p1;
+        w[i >> 1] = pack_half(p0, p1);
+    }
+    tmem_st16(s_addr + c * 16, w);
+}
+template <bool MASK>
+__device__ __forceinline__ float block_weights(uint32_t s_addr, int vis, int ok, float scale, float shift) {
+    uint32_t a[32], b[32];
+    float l4[4] = {0.f, 0.f, 0.f, 0.f};
+    tmem_ld32(s_addr, a);
+    wait_ld();
+#pragma unroll 1
+    for (int c = 0; c < 4; c += 2) {
+        tmem_ld32(s_addr + (c + 1) * 32, b);
+        quarter_weights<MASK>(a, s_addr, c, vis, ok, scale, shift, l4);
+        wait_ld();
+        if (c == 0) tmem_ld32(s_addr + 64, a);
+        quarter_weights<MASK>(b, s_addr, c + 1, vis, ok, scale, shift, l4);
+        wait_ld();
     }
     return (l4[0] + l4[1]) + (l4[2] + l4[3]);
+}
+
+// The queries of a warp's 32 rows (row0 ..; those from `rows` on are zeros) as two planes of E4M3 in the layout of a
+// K-major operand at `dst` (rows of 128 bytes, 16-byte pieces swizzled by the row's low three bits), each row scaled by
+// the power of two that brings its largest value into [128, 256) (E4M3 ends at 448).  Half a warp loads a row (lines are
+// read whole: many CTAs want the same queries at the same time).  Returns what undoes the scale of row0 + lane.
+__device__ __forceinline__ float write_queries(const mono_prefix_attn_args& a, const Entry& en, int head, int G, int row0, int rows, uint8_t* dst) {
+    const int lane = threadIdx.x & 31, half = lane >> 4, sub = lane & 15;
+    const __nv_bfloat16* q = reinterpret_cast<const __nv_bfloat16*>(a.q) + (size_t)en.tok0 * a.q_ld + (size_t)head * G * kDim + sub * 8;
+    float mine = 1.f;
+    constexpr int B = 8;
+#pragma unroll 1
+    for (int r0 = 0; r0 < 32; r0 += 2 * B) {
+        uint4 v[B];
+#pragma unroll
+        for (int j = 0; j < B; ++j) {
+            const int row = row0 + r0 + 2 * j + half, r = row < rows ? row : 0, tok = r / G;
+            v[j] = __ldg(reinterpret_cast<const uint4*>(q + (size_t)tok * a.q_ld + (size_t)(r - tok * G) * kDim));
+        }
+#pragma unroll
+        for (int j = 0; j < B; ++j) {
+            const int at = r0 + 2 * j + half;
+            const uint32_t w[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+            uint32_t top = 0;  // the exponent of the largest |value|: NaN and infinity have the largest
+#pragma unroll
+            for (int i = 0; i < 4; ++i) top = max(top, max((w[i] << 16) & 0x7F800000u, w[i] & 0x7F800000u));
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+            const int ex = clamp_int((int)(top >> 23), 30, 254);
+            const float up = row0 + at < rows ? __uint_as_float((uint32_t)(261 - ex) << 23) : 0.f;  // 2^(134 - ex)
+            uint32_t hi[2] = {0, 0}, lo[2] = {0, 0};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float f0 = __uint_as_float(w[i] << 16) * up, f1 = __uint_as_float(w[i] & 0xFFFF0000u) * up;
+                const __nv_fp8x2_storage_t hb = __nv_cvt_float2_to_fp8x2(make_float2(f0, f1), __NV_SATFINITE, __NV_E4M3);
+                const __half2_raw hr = __nv_cvt_fp8x2_to_halfraw2(hb, __NV_E4M3);
+                const float2 hf = __half22float2(*reinterpret_cast<const __half2*>(&hr));
+                const __nv_fp8x2_storage_t lb = __nv_cvt_float2_to_fp8x2(make_float2(f0 - hf.x, f1 - hf.y), __NV_SATFINITE, __NV_E4M3);
+                hi[i >> 1] |= (uint32_t)hb << (16 * (i & 1));
+                lo[i >> 1] |= (uint32_t)lb << (16 * (i & 1));
+            }
+            uint8_t* d = dst + at * 128 + (((sub >> 1) ^ (at & 7)) << 4) + (sub & 1) * 8;
+            *reinterpret_cast<uint2*>(d) = make_uint2(hi[0], hi[1]);
+            *reinterpret_cast<uint2*>(d + kQPlane) = make_uint2(lo[0], lo[1]);
+            // infinite or NaN: saturation would hide it; a row of NaN
+            float back = top == 0x7F800000u ? __uint_as_float(0x7FC00000u) : __uint_as_float((uint32_t)(ex - 7) << 23);
+            back = __shfl_sync(0xffffffffu, back, (lane & 1) * 16);
+            if (lane >> 1 == (r0 >> 1) + j) mine = back;
+        }
+    }
+    return mine;
+}
+
+// The CTA's current item, as every role walks it.
+struct Item {
+    Entry en;
+    int head, row0, rows;  // first row, rows of the item (at most 256)
+    int b0, blocks;        // first block of 128 keys, blocks to compute (those no row sees are left out)
+    bool split;            // both streams have the same rows and take alternate blocks
+    uint32_t seg, span;    // segment number; units of the list that this covers
+    // stream st takes blocks first(st), first(st) + step, ...
+    __device__ __forceinline__ int first(int st) const { return split ? st : 0; }
+    __device__ __forceinline__ int step() const { return split ? 2 : 1; }
+    __device__ __forceinline__ int count(int st) const { return split ? (blocks - st + 1) / 2 : blocks; }
+};
+__device__ __forceinline__ Item item_at(const mono_prefix_attn_args& a, const uint32_t* off, const uint32_t* item, uint32_t u, uint32_t u1) {
+    Item it;
+    const int E = a.groups + a.seqs, G = a.q_heads / a.kv_heads;
+    const Place at = place_of(off, E, u);
+    it.en = entry_of(a, at.e);
+    it.head = at.head;
+    const Work w = entry_work<true>(a, it.en);
+    const int tile = min((int)at.local / w.units, w.tiles - 1), unit = (int)at.local - tile * w.units;
+    it.row0 = tile * Shape<true>::kTile;
+    it.rows = min(Shape<true>::kTile, it.en.ntok * G - it.row0);
+    it.split = it.rows <= kWideHalf;
+    it.span = min((uint32_t)((tile == w.tiles - 1 ? w.last : w.units) - unit), u1 - u);
+    it.b0 = it.split ? 2 * unit : unit;
+    const int seen = max(row_limit(it.en, it.row0 + it.rows - 1, G), 0);
+    it.blocks = max(0, min((int)it.span * it.step(), (seen + kKeys - 1) / kKeys - it.b0));
+    it.seg = blockIdx.x + it.head * item[E] + item[at.e] + tile;
+    return it;
 }
 
 __global__ void __launch_bounds__(kThreadsWide, 1) prefix_wide_kernel(const __grid_constant__ Params p) {
@@ -179,7 +276,8 @@ __global__ void __launch_bounds__(kThreadsWide, 1) prefix_wide_kernel(const __gr
     uint32_t* off = reinterpret_cast<uint32_t*>(wbuf + kWStages * kWTile);
     uint32_t* item = off + E + 1;
     __shared__ uint64_t k_full[kKStages], k_empty[kKStages], v_full[kVStages], v_empty[kVStages], w_full[kWStages], w_empty[kWStages];
-    __shared__ uint64_t q_full[2], s_full[2], p_full[2], o_full[2];
+    __shared__ uint64_t q_full[2], s_full[2], p_full[2], o_full[2], j_free, j_full, j_done;
+    __shared__ float s_join[2][128];  // stream 1's maxima and sums
     __shared__ int page_ok[kOkRing];
     __shared__ uint32_t red[64], tmem_base_s;
     __shared__ int abort_flag;
@@ -191,6 +289,9 @@ __global__ void __launch_bounds__(kThreadsWide, 1) prefix_wide_kernel(const __gr
         for (int i = 0; i < kVStages; ++i) { mbar_init(&v_full[i], 1); mbar_init(&v_empty[i], 4); }
         for (int i = 0; i < kWStages; ++i) { mbar_init(&w_full[i], 128); mbar_init(&w_empty[i], 1); }
         for (int i = 0; i < 2; ++i) { mbar_init(&q_full[i], 128); mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 128); mbar_init(&o_full[i], 1); }
+        mbar_init(&j_free, 128);
+        mbar_init(&j_full, 128);
+        mbar_init(&j_done, 128);
         mbar_fence_init();
         prefetch_tmap(&p.kmap);
         prefetch_tmap(&p.vmap);
@@ -203,47 +304,43 @@ __global__ void __launch_bounds__(kThreadsWide, 1) prefix_wide_kernel(const __gr
     __syncthreads();
     fence_after();
     const uint32_t tmem = tmem_base_s;
+    MONO_TL(tl_wide, 0);
     pdl_launch_dependents();
     pdl_wait();
     if (tid == 0 && guard_failed(a.guard)) abort_flag = 1;
-    make_plan<true, kThreadsWide>(a, off, item, red);
-    if (blockIdx.x == 0) {  // the merge reads it
-        for (int e = tid; e <= E; e += kThreadsWide) {
-            p.s.off[1][e] = off[e];
-            p.s.item[1][e] = item[e];
-        }
-    }
-    const uint32_t U = off[E], n = min(gridDim.x, U);
+    MONO_TL(tl_wide, 1);
+    make_plan<true, kThreadsWide>(a, p.s, off, item, red);
+    MONO_TL(tl_wide, 2);
+    const uint32_t U = off[E] * a.kv_heads, per = part_size(U, gridDim.x), u0 = min(blockIdx.x * per, U), u1 = min(u0 + per, U);
     const uint64_t wait_ns = a.wait_ns ? a.wait_ns : kWaitLimitNs;
-    if (blockIdx.x < n) {
-        const uint32_t u0 = cut(U, blockIdx.x, n), u1 = cut(U, blockIdx.x + 1, n);
-        int e = -1;
-        if (warp == kTmaWarp) {
-            // ---- fetch: lane l looks up the two pages of a batch's unit l; lane 0 requests them in order
+    if (warp >= kTmaWarp) {
+        regs_down<kRegsFetch>();
+        if (u0 < u1 && warp == kTmaWarp) {
+            // ---- fetch: lane l looks up the two pages of a batch's block l; lane 0 requests them in order
             int it = 0;
             for (uint32_t u = u0; u < u1 && !*abortp;) {
-                const Item x = item_at(a, off, item, u, u1, &e);
+                const Item x = item_at(a, off, item, u, u1);
                 const int pages = (x.en.len + kPage - 1) / kPage;
-                for (int b = 0; b < x.units && !*abortp; b += 32) {
+                for (int b = 0; b < x.blocks && !*abortp; b += 32) {
                     int pg[2] = {-1, -1};
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const int at = (x.p0 + min(b + lane, x.units - 1)) * 2 + h;
+                        const int at = (x.b0 + min(b + lane, x.blocks - 1)) * 2 + h;
                         if (at < pages) pg[h] = x.en.table[at];
                         if (pg[h] >= a.n_pages) pg[h] = -1;
                     }
-                    const int cnt = min(32, x.units - b);
+                    const int cnt = min(32, x.blocks - b);
                     for (int j = 0; j < cnt; ++j, ++it) {
                         const int g0 = __shfl_sync(0xffffffffu, pg[0], j), g1 = __shfl_sync(0xffffffffu, pg[1], j);
                         if (lane == 0 && !*abortp) {
                             const int ks = it % kKStages, vs = it % kVStages;
                             const uint32_t bytes = (g0 >= 0 ? kPage * 128 : 0) + (g1 >= 0 ? kPage * 128 : 0);
-                            if (it < kKStages || mbar_wait(&k_empty[ks], ((it / kKStages) - 1) & 1, abortp, wait_ns)) {
+                            if (it < kKStages || wait_on(&k_empty[ks], ((it / kKStages) - 1) & 1, abortp, wait_ns)) {
                                 page_ok[it % kOkRing] = (g0 >= 0 ? 1 : 0) | (g1 >= 0 ? 2 : 0);
                                 mbar_expect_tx(&k_full[ks], bytes);
                                 if (g0 >= 0) tma_load_3d(kbuf + ks * kKTile, &p.kmap, x.head * kDim, g0 * kPage, 0, &k_full[ks]);
                                 if (g1 >= 0) tma_load_3d(kbuf + ks * kKTile + kPage * 128, &p.kmap, x.head * kDim, g1 * kPage, 0, &k_full[ks]);
-                                if (it < kVStages || mbar_wait(&v_empty[vs], ((it / kVStages) - 1) & 1, abortp, wait_ns)) {
+                                if (it < kVStages || wait_on(&v_empty[vs], ((it / kVStages) - 1) & 1, abortp, wait_ns)) {
                                     mbar_expect_tx(&v_full[vs], bytes);
                                     if (g0 >= 0) tma_load_3d(vbuf + vs * kVTile, &p.vmap, x.head * kDim, g0 * kPage, 0, &v_full[vs]);
                                     if (g1 >= 0) tma_load_3d(vbuf + vs * kVTile + kPage * 128, &p.vmap, x.head * kDim, g1 * kPage, 0, &v_full[vs]);
@@ -255,46 +352,49 @@ __global__ void __launch_bounds__(kThreadsWide, 1) prefix_wide_kernel(const __gr
                 }
                 u += x.span;
             }
-        } else if (warp == kMmaWarp) {
-            // ---- the products: one thread issues; per stream S, (softmax), O, in the order that lets the streams alternate
-            if (lane == 0) {
-                int it0 = 0;                                    // units before this item, over the CTA's life
+        } else if (u0 < u1 && warp == kMmaWarp) {
+            // ---- the products: per stream S, (softmax), O, in the order that lets the streams alternate.  The warp walks
+            // together and one elected lane issues, so that descriptors stay in uniform registers.
+            {
+                int it0 = 0;  // blocks before this item, over the CTA's life
                 uint32_t qph[2] = {0, 0}, pph[2] = {0, 0};
                 bool live = true;
                 for (uint32_t u = u0; u < u1 && live;) {
-                    const Item x = item_at(a, off, item, u, u1, &e);
+                    const Item x = item_at(a, off, item, u, u1);
                     auto scores = [&](int st, int t) -> bool {  // S of the stream's t-th unit
                         const int i = it0 + x.first(st) + t * x.step(), ks = i % kKStages;
                         if (t == 0) {
-                            if (!mbar_wait(&q_full[st], qph[st], abortp, wait_ns)) return false;
+                            if (!wait_on(&q_full[st], qph[st], abortp, wait_ns)) return false;
                             qph[st] ^= 1;
                         }
-                        if (!mbar_wait(&k_full[ks], (i / kKStages) & 1, abortp, wait_ns)) return false;
+                        if (!wait_on(&k_full[ks], (i / kKStages) & 1, abortp, wait_ns)) return false;
                         fence_after();
                         const uint32_t q = smem_u32(qbuf + st * 2 * kQPlane), k = smem_u32(kbuf + ks * kKTile);
-                        const uint64_t kd = desc_sw128(k, 0, 1024);
+                        const uint64_t kd = desc_sw128(k, 0, 1024), qd = desc_sw128(q, 0, 1024);
+                        if (elect_one()) {
 #pragma unroll
-                        for (int pl = 0; pl < 2; ++pl) {
-                            const uint64_t qd = desc_sw128(q + pl * kQPlane, 0, 1024);
-#pragma unroll
-                            for (int s = 0; s < 4; ++s) mma_f8(tmem + st * 128, qd + 2 * s, kd + 2 * s, kIdescS, pl + s > 0);
+                            for (int s = 0; s < 8; ++s) mma_f8(tmem + st * 128, qd + (s >> 2) * (kQPlane / 16) + 2 * (s & 3), kd + 2 * (s & 3), kIdescS, s > 0);
+                            mma_commit(&s_full[st]);
+                            if (x.split || st == 1) mma_commit(&k_empty[ks]);
                         }
-                        mma_commit(&s_full[st]);
-                        if (x.split || st == 1) mma_commit(&k_empty[ks]);
+                        __syncwarp();
                         return true;
                     };
                     auto values = [&](int st, int t) -> bool {  // O += P V of the stream's t-th unit
                         const int i = it0 + x.first(st) + t * x.step(), ws = i % kWStages;
-                        if (!mbar_wait(&w_full[ws], (i / kWStages) & 1, abortp, wait_ns)) return false;
-                        if (!mbar_wait(&p_full[st], pph[st], abortp, wait_ns)) return false;
+                        if (!wait_on(&w_full[ws], (i / kWStages) & 1, abortp, wait_ns)) return false;
+                        if (!wait_on(&p_full[st], pph[st], abortp, wait_ns)) return false;
                         pph[st] ^= 1;
                         fence_after();
-                        const uint32_t w = smem_u32(wbuf + ws * kWTile);
+                        const uint64_t wd = desc_sw128(smem_u32(wbuf + ws * kWTile), kKeys * 128, 1024);
+                        if (elect_one()) {
 #pragma unroll
-                        for (int s = 0; s < 8; ++s)
-                            mma_f16_ts(tmem + 256 + st * 128, tmem + st * 128 + s * 8, desc_sw128(w + s * 16 * 128, kKeys * 128, 1024), kIdescO, t > 0 || s > 0);
-                        if (x.split || st == 1) mma_commit(&w_empty[ws]);
-                        if (t == x.count(st) - 1) mma_commit(&o_full[st]);
+                            for (int s = 0; s < 8; ++s)
+                                mma_f16_ts(tmem + 256 + st * 128, tmem + st * 128 + s * 8, wd + s * (16 * 128 / 16), kIdescO, s > 0 || t > 0);
+                            if (x.split || st == 1) mma_commit(&w_empty[ws]);
+                            if (t == x.count(st) - 1) mma_commit(&o_full[st]);
+                        }
+                        __syncwarp();
                         return true;
                     };
                     for (int st = 0; st < 2 && live; ++st)
@@ -305,27 +405,29 @@ __global__ void __launch_bounds__(kThreadsWide, 1) prefix_wide_kernel(const __gr
                             live = values(st, t);
                             if (live && t + 1 < x.count(st)) live = scores(st, t + 1);
                         }
-                    it0 += x.units;
+                    it0 += x.blocks;
                     u += x.span;
                 }
             }
-            __syncwarp();
-        } else if (warp >= kConvWarp0) {
+        }
+    } else if (warp >= kConvWarp0) {
+        regs_down<kRegsConv>();
+        if (u0 < u1) {
             // ---- widen V: bytes [key][dim], as TMA left them, to f16 in the layout of an MN-major operand.  Keys behind
             // the entry's last and pages that do not exist become zeros: 0 x NaN would be NaN.
             const int ct = tid - kConvWarp0 * 32;
             int it = 0;
             bool live = true;
             for (uint32_t u = u0; u < u1 && live;) {
-                const Item x = item_at(a, off, item, u, u1, &e);
-                for (int i = 0; i < x.units && live; ++i, ++it) {
+                const Item x = item_at(a, off, item, u, u1);
+                for (int i = 0; i < x.blocks && live; ++i, ++it) {
                     const int vs = it % kVStages, ws = it % kWStages;
-                    live = mbar_wait(&v_full[vs], (it / kVStages) & 1, abortp, wait_ns) &&
-                           (it < kWStages || mbar_wait(&w_empty[ws], ((it / kWStages) - 1) & 1, abortp, wait_ns));
+                    live = wait_on(&v_full[vs], (it / kVStages) & 1, abortp, wait_ns) &&
+                           (it < kWStages || wait_on(&w_empty[ws], ((it / kWStages) - 1) & 1, abortp, wait_ns));
                     if (!live) break;
                     const uint32_t src = smem_u32(vbuf + vs * kVTile), dst = smem_u32(wbuf + ws * kWTile);
-                    const int have = x.en.len - (x.p0 + i) * kKeys, ok = page_ok[it % kOkRing];
-#pragma unroll
+                    const int have = x.en.len - (x.b0 + i) * kKeys, ok = page_ok[it % kOkRing];
+#pragma unroll 2
                     for (int j = 0; j < 8; ++j) {
                         const int key = (ct & 7) + 8 * j + 64 * (ct >> 6), c16 = (ct >> 3) & 7;  // eight lanes: eight keys, no bank twice
                         uint4 v = lds128(src + key * 128 + ((c16 ^ (key & 7)) << 4));
@@ -341,75 +443,45 @@ __global__ void __launch_bounds__(kThreadsWide, 1) prefix_wide_kernel(const __gr
                 }
                 u += x.span;
             }
-        } else {
+        }
+    } else {
+        regs_up<kRegsSoftmax>();
+        if (u0 < u1) {
             // ---- softmax: thread = row
             const int st = warp >> 2, row_in = tid & 127;
             const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
             const uint32_t s_addr = tmem + lanes + st * 128, o_addr = tmem + lanes + 256 + st * 128;
+            float* joint = reinterpret_cast<float*>(qbuf);  // [32 x 4 dims][128 rows] of stream 1, once a split item's queries are done with
             int it0 = 0;
-            uint32_t sph = 0, oph = 0;
+            uint32_t sph = 0, oph = 0, jph = 0;
             bool live = true;
             for (uint32_t u = u0; u < u1 && live;) {
-                const Item x = item_at(a, off, item, u, u1, &e);
+                const Item x = item_at(a, off, item, u, u1);
                 const int row = x.row0 + (x.split ? row_in : st * 128 + row_in);
                 const bool mine = row < x.row0 + x.rows;
                 const int count = x.count(st);
+                const bool join = x.split && x.count(1) > 0;  // stream 0 takes stream 1's part into its own
                 float m = -INFINITY, l = 0.f;
                 if (count > 0) {
-                    // ---- the row's query, as two planes of E4M3 in the layout of a K-major operand
-                    float qs;
-                    {
-                        const int r = mine ? row : x.row0;
-                        const __nv_bfloat16* src = reinterpret_cast<const __nv_bfloat16*>(a.q) + (size_t)(x.en.tok0 + r / G) * a.q_ld + (size_t)(x.head * G + r % G) * kDim;
-                        float amax = 0.f;
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) {
-                            const uint4 v = __ldg(reinterpret_cast<const uint4*>(src) + j);
-                            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                            for (int q = 0; q < 4; ++q) amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(w[q] << 16)), fabsf(__uint_as_float(w[q] & 0xFFFF0000u))));
-                        }
-                        // the power of two that brings the largest value into [128, 256): E4M3 ends at 448
-                        const int ex = clamp_int((int)(__float_as_uint(amax) >> 23), 30, 254);
-                        const float up = mine ? __uint_as_float((uint32_t)(261 - ex) << 23) : 0.f;  // 2^(134 - ex)
-                        qs = __uint_as_float((uint32_t)(ex - 7) << 23) * (a.sm_scale * a.k_scale * 1.4426950408889634f);
-                        uint8_t* dst = qbuf + st * 2 * kQPlane + row_in * 128;
-#pragma unroll
-                        for (int c = 0; c < 8; ++c) {
-                            uint32_t hi[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0};
-#pragma unroll
-                            for (int h = 0; h < 2; ++h) {
-                                const uint4 v = __ldg(reinterpret_cast<const uint4*>(src) + 2 * c + h);
-                                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                                for (int q = 0; q < 4; ++q) {
-                                    const float f0 = __uint_as_float(w[q] << 16) * up, f1 = __uint_as_float(w[q] & 0xFFFF0000u) * up;
-                                    const __nv_fp8x2_storage_t hb = __nv_cvt_float2_to_fp8x2(make_float2(f0, f1), __NV_SATFINITE, __NV_E4M3);
-                                    const __half2_raw hr = __nv_cvt_fp8x2_to_halfraw2(hb, __NV_E4M3);
-                                    const float2 hf = __half22float2(*reinterpret_cast<const __half2*>(&hr));
-                                    const __nv_fp8x2_storage_t lb = __nv_cvt_float2_to_fp8x2(make_float2(f0 - hf.x, f1 - hf.y), __NV_SATFINITE, __NV_E4M3);
-                                    hi[h * 2 + (q >> 1)] |= (uint32_t)hb << (16 * (q & 1));
-                                    lo[h * 2 + (q >> 1)] |= (uint32_t)lb << (16 * (q & 1));
-                                }
-                            }
-                            uint8_t* d = dst + ((c ^ (row_in & 7)) << 4);
-                            *reinterpret_cast<uint4*>(d) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                            *reinterpret_cast<uint4*>(d + kQPlane) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-                        }
-                        if (!(amax <= 3.0e38f)) qs = __uint_as_float(0x7FC00000u);  // a query of infinities or NaN: a row of NaN
-                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                        mbar_arrive(&q_full[st]);
-                    }
+                    const int w0 = (warp & 3) * 32;  // this warp's rows
+                    const float qs = write_queries(a, x.en, x.head, G, x.row0 + (x.split ? 0 : st * 128) + w0, x.row0 + x.rows, qbuf + st * 2 * kQPlane + w0 * 128) *
+                                     (a.sm_scale * a.k_scale * 1.4426950408889634f);
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    mbar_arrive(&q_full[st]);
+                    MONO_TL(tl_wide, 3);
                     const int lim = mine ? row_limit(x.en, row, G) : 0;
                     for (int t = 0; t < count; ++t) {
                         const int i = x.first(st) + t * x.step();
-                        live = mbar_wait(&s_full[st], sph, abortp, wait_ns);
+                        live = wait_on(&s_full[st], sph, abortp, wait_ns);
                         if (!live) break;
                         sph ^= 1;
                         fence_after();
-                        const int vis = lim - (x.p0 + i) * kKeys, ok = page_ok[(it0 + i) % kOkRing];
-                        const bool plain = __all_sync(0xffffffffu, vis >= kKeys) && ok == 3;
-                        const float mx = (plain ? unit_max<false>(s_addr, vis, ok) : unit_max<true>(s_addr, vis, ok)) * qs;
+                        MONO_TL(tl_wide, 4 + 3 * t);  // the first three blocks
+                        // keys of the block that this row sees, of the pages that exist
+                        const int vis = lim - (x.b0 + i) * kKeys, ok = page_ok[(it0 + i) % kOkRing];
+                        const bool masked = !__all_sync(0xffffffffu, vis >= kKeys) || ok != 3;
+                        const float mx = (masked ? block_max<true>(s_addr, vis, ok) : block_max<false>(s_addr, vis, ok)) * qs;
+                        MONO_TL(tl_wide, 5 + 3 * t);
                         // raise the reference where it must be, and O with it
                         float up = 1.f;
                         if (mx > m + kLazy || (m == -INFINITY && mx > m)) {
@@ -419,59 +491,108 @@ __global__ void __launch_bounds__(kThreadsWide, 1) prefix_wide_kernel(const __gr
                         if (t > 0 && __any_sync(0xffffffffu, up != 1.f)) {
                             l *= up;
 #pragma unroll 1
-                            for (int c = 0; c < 4; ++c) {
-                                uint32_t r[32];
-                                tmem_ld32(o_addr + c * 32, r);
+                            for (int c = 0; c < 8; ++c) {
+                                uint32_t r16[16];
+                                tmem_ld16(o_addr + c * 16, r16);
                                 wait_ld();
 #pragma unroll
-                                for (int q = 0; q < 32; ++q) r[q] = __float_as_uint(__uint_as_float(r[q]) * up);
-                                tmem_st16(o_addr + c * 32, r);
-                                tmem_st16(o_addr + c * 32 + 16, r + 16);
+                                for (int q = 0; q < 16; ++q) r16[q] = __float_as_uint(__uint_as_float(r16[q]) * up);
+                                tmem_st16(o_addr + c * 16, r16);
                             }
                         }
                         const float shift = kBias - (m == -INFINITY ? 0.f : m);
-                        l += plain ? unit_weights<false>(s_addr, vis, ok, qs, shift) : unit_weights<true>(s_addr, vis, ok, qs, shift);
+                        l += masked ? block_weights<true>(s_addr, vis, ok, qs, shift) : block_weights<false>(s_addr, vis, ok, qs, shift);
                         wait_st();
                         fence_before();
                         mbar_arrive(&p_full[st]);
+                        MONO_TL(tl_wide, 6 + 3 * t);
                     }
                     if (!live) break;
-                    live = mbar_wait(&o_full[st], oph, abortp, wait_ns);
+                    live = wait_on(&o_full[st], oph, abortp, wait_ns);
+                    MONO_TL(tl_wide, 13);
                     if (!live) break;
                     oph ^= 1;
                     fence_after();
                 }
-                // ---- the segment's row; a stream without units leaves an empty part
-                float* seg = p.s.seg[1] + (size_t)x.seg * Shape<true>::kSegFloats;
-                const int at = st * 128 + row_in;
-                if (mine) {
-                    seg[at] = l != l ? l : m - kBias;
-                    seg[Shape<true>::kTile + at] = l;
-                }
-                if (count > 0) {
-                    float* dst = seg + 2 * Shape<true>::kTile + at * kDim;
+                // ---- the segment's row; an item without blocks leaves an empty part
+                float f0 = 1.f, f1 = 0.f;
+                if (join) {
+                    if (st == 1) {
+                        // the other stream's queries are done with too: its last scores come before its part is asked for
+                        live = wait_on(&j_free, jph, abortp, wait_ns);
+                        if (!live) break;
+                        s_join[0][row_in] = m;
+                        s_join[1][row_in] = l;
 #pragma unroll 1
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t r[32];
-                        tmem_ld32(o_addr + c * 32, r);
-                        wait_ld();
+                        for (int c = 0; c < 8; ++c) {
+                            uint32_t r16[16];
+                            tmem_ld16(o_addr + c * 16, r16);
+                            wait_ld();
+#pragma unroll
+                            for (int q = 0; q < 16; q += 4)
+                                *reinterpret_cast<uint4*>(joint + ((c * 4 + q / 4) * 128 + row_in) * 4) = make_uint4(r16[q], r16[q + 1], r16[q + 2], r16[q + 3]);
+                        }
+                        mbar_arrive(&j_full);
+                    } else {
+                        mbar_arrive(&j_free);
+                        live = wait_on(&j_full, jph, abortp, wait_ns);
+                        if (!live) break;
+                        const float m1 = s_join[0][row_in], l1 = s_join[1][row_in], top = fmaxf(m, m1);
+                        f0 = m == -INFINITY ? 0.f : ex2(m - top);
+                        f1 = m1 == -INFINITY ? 0.f : ex2(m1 - top);
+                        l = (l != l || l1 != l1) ? __uint_as_float(0x7FC00000u) : l * f0 + l1 * f1;
+                        m = top;
+                    }
+                }
+                if (!(x.split && st == 1)) {
+                    float* seg = p.s.seg[1] + (size_t)x.seg * Shape<true>::kSegFloats;
+                    const int at = st * 128 + row_in;
+                    if (mine) {
+                        seg[at] = l != l ? l : m - kBias;
+                        seg[Shape<true>::kTile + at] = l;
+                    }
+                    float* dst = seg + 2 * Shape<true>::kTile + at * 4;  // [32 x 4 dims][256 rows][4]
+#pragma unroll 1
+                    for (int c = 0; c < 8; ++c) {
+                        uint32_t r16[16];
+                        if (count > 0) {
+                            tmem_ld16(o_addr + c * 16, r16);
+                            wait_ld();
+                        } else {
+#pragma unroll
+                            for (int q = 0; q < 16; ++q) r16[q] = 0;
+                        }
+                        if (join) {
+#pragma unroll
+                            for (int q = 0; q < 16; q += 4) {
+                                const float4 o = *reinterpret_cast<const float4*>(joint + ((c * 4 + q / 4) * 128 + row_in) * 4);
+                                const float ov[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) r16[q + k] = __float_as_uint(__uint_as_float(r16[q + k]) * f0 + ov[k] * f1);
+                            }
+                        }
                         if (mine) {
 #pragma unroll
-                            for (int q = 0; q < 32; q += 4)
-                                *reinterpret_cast<uint4*>(dst + c * 32 + q) = make_uint4(r[q], r[q + 1], r[q + 2], r[q + 3]);
+                            for (int q = 0; q < 16; q += 4)
+                                *reinterpret_cast<uint4*>(dst + (c * 4 + q / 4) * (Shape<true>::kTile * 4)) = make_uint4(r16[q], r16[q + 1], r16[q + 2], r16[q + 3]);
                         }
                     }
-                    fence_before();
-                } else if (mine) {
-                    for (int q = 0; q < kDim; q += 4) *reinterpret_cast<uint4*>(seg + 2 * Shape<true>::kTile + at * kDim + q) = make_uint4(0, 0, 0, 0);
                 }
-                it0 += x.units;
+                fence_before();
+                if (join) {  // the next item's queries overwrite what stream 0 reads here
+                    if (st == 0) mbar_arrive(&j_done);
+                    live = wait_on(&j_done, jph, abortp, wait_ns);
+                    jph ^= 1;
+                }
+                MONO_TL(tl_wide, 14);
+                it0 += x.blocks;
                 u += x.span;
             }
         }
     }
     fence_before();
     __syncthreads();
+    MONO_TL(tl_wide, 15);
     if (*abortp) {
         for (int i = 0; i < 64; ++i) __nanosleep(1000);  // copies and products in flight end before the CTA's memory goes
         if (tid == 0 && !guard_failed(a.guard)) guard_fail(a.guard, MONO_ERR_DEADLINE, kSiteWait);
@@ -495,3 +616,12 @@ cudaError_t launch_wide(const Params& p, int ctas, cudaStream_t st) {
 }
 
 }  // namespace prefix_attn
+
+#ifdef MONO_TIMELINE
+// Copies the wide kernel's stamps of the last launch to `out` (MONO_TL_CTAS x MONO_TL_POINTS); blocks the host.
+extern "C" int mono_timeline_read_prefix_wide(unsigned long long* out, int* ctas, int* points) {
+    *ctas = MONO_TL_CTAS;
+    *points = MONO_TL_POINTS;
+    return (int)cudaMemcpyFromSymbol(out, prefix_attn::tl_wide, sizeof(unsigned long long) * MONO_TL_CTAS * MONO_TL_POINTS);
+}
+#endif

@@ -18,152 +18,214 @@ using namespace mono;
 constexpr int kDim = 128;
 constexpr int kThreads = 256;
 
-__device__ __forceinline__ void unpack8(const uint4 w, float v[8]) {
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        v[2 * j] = __uint_as_float(u[j] << 16);
-        v[2 * j + 1] = __uint_as_float(u[j] & 0xFFFF0000u);
-    }
+typedef unsigned long long f32x2;  // two f32 that one instruction works on
+__device__ __forceinline__ f32x2 pair(float lo, float hi) {
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
 }
-__device__ __forceinline__ uint4 pack8(const float v[8]) {
-    uint32_t u[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
-        u[j] = *reinterpret_cast<const uint32_t*>(&b);
-    }
-    return make_uint4(u[0], u[1], u[2], u[3]);
+__device__ __forceinline__ float2 halves(f32x2 v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
 }
-// n table entries from entry i of a row (n = 4 or 8, i a multiple of n)
-template <int N>
-__device__ __forceinline__ void load_table(const void* table, int is_f32, size_t at, float v[N]) {
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ f32x2 swapped(f32x2 v) {
+    const float2 h = halves(v);
+    return pair(h.y, h.x);
+}
+__device__ __forceinline__ f32x2 unpack2(uint32_t w) { return pair(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u)); }
+__device__ __forceinline__ void unpack8(const uint4 w, f32x2 v[4]) {
+    v[0] = unpack2(w.x); v[1] = unpack2(w.y); v[2] = unpack2(w.z); v[3] = unpack2(w.w);
+}
+__device__ __forceinline__ uint32_t pack2(f32x2 v) {
+    const float2 h = halves(v);
+    const __nv_bfloat162 b = __floats2bfloat162_rn(h.x, h.y);
+    return *reinterpret_cast<const uint32_t*>(&b);
+}
+// two table entries from entry `at` on (at even)
+__device__ __forceinline__ f32x2 load2(const void* table, int is_f32, size_t at) {
     if (is_f32) {
-        const float4* p = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(table) + at);
+        const float2 f = __ldg(reinterpret_cast<const float2*>(reinterpret_cast<const float*>(table) + at));
+        return pair(f.x, f.y);
+    }
+    return unpack2(__ldg(reinterpret_cast<const uint32_t*>(reinterpret_cast<const __nv_bfloat16*>(table) + at)));
+}
+
+// What a lane multiplies its eight dims of a q or k head by: out = f (x A + other B), other being the dims' partners.
+// Norm and rotation are linear in the head up to the factor f = 1 / rms, so A = (1 + g) cos and B = -+(1 + g of the
+// partner) sin serve all heads of a token and kind.
+struct Coef {
+    f32x2 a[4], b[4];
+};
+template <bool INTERLEAVED>
+__device__ __forceinline__ void make_coef(const mono_qkv_append_args& args, const void* gain, size_t row, int sub, int psub, bool turned, bool low, Coef& c) {
+    const f32x2 one = pair(1.f, 1.f);
+    f32x2 g[4] = {one, one, one, one}, o[4] = {one, one, one, one};
+    if (gain) {
+        unpack8(__ldg(reinterpret_cast<const uint4*>(gain) + sub), g);
+        unpack8(__ldg(reinterpret_cast<const uint4*>(gain) + psub), o);
 #pragma unroll
-        for (int j = 0; j < N / 4; ++j) {
-            const float4 f = __ldg(p + j);
-            v[4 * j] = f.x; v[4 * j + 1] = f.y; v[4 * j + 2] = f.z; v[4 * j + 3] = f.w;
-        }
-    } else {
-        const uint2* p = reinterpret_cast<const uint2*>(reinterpret_cast<const __nv_bfloat16*>(table) + at);
+        for (int j = 0; j < 4; ++j) { g[j] = fma2(one, one, g[j]); o[j] = fma2(one, one, o[j]); }
+    }
 #pragma unroll
-        for (int j = 0; j < N / 4; ++j) {
-            const uint2 w = __ldg(p + j);
-            v[4 * j] = __uint_as_float(w.x << 16); v[4 * j + 1] = __uint_as_float(w.x & 0xFFFF0000u);
-            v[4 * j + 2] = __uint_as_float(w.y << 16); v[4 * j + 3] = __uint_as_float(w.y & 0xFFFF0000u);
+    for (int j = 0; j < 4; ++j) {
+        c.a[j] = g[j];
+        c.b[j] = pair(0.f, 0.f);
+        if (!turned) continue;
+        if (INTERLEAVED) {  // two dims share an angle: (x0, x1) -> (x0 c - x1 s, x1 c + x0 s)
+            const size_t at = row + sub * 4 + (j & 2);
+            const float2 cs = halves(load2(args.cos, args.table_f32, at)), sn = halves(load2(args.sin, args.table_f32, at));
+            const float cj = j & 1 ? cs.y : cs.x, sj = j & 1 ? sn.y : sn.x;
+            c.a[j] = mul2(g[j], pair(cj, cj));
+            c.b[j] = mul2(swapped(g[j]), pair(-sj, sj));
+        } else {  // this lane holds the first or the second dims of eight pairs
+            const size_t at = row + (low ? sub : psub) * 8 + 2 * j;
+            const float2 sn = halves(load2(args.sin, args.table_f32, at));
+            c.a[j] = mul2(g[j], load2(args.cos, args.table_f32, at));
+            c.b[j] = mul2(o[j], low ? pair(-sn.x, -sn.y) : pair(sn.x, sn.y));
         }
     }
 }
 
-// A warp takes PAIRS pairs of heads of one token; lanes 0..15 hold the even head of a pair, 16..31 the odd one.
-template <int PAIRS, bool F32SRC>
-__global__ void __launch_bounds__(kThreads) qkv_append_kernel(const mono_qkv_append_args a, int chunks) {
+// Per warp: where it reads and writes.
+struct Lane {
+    int sub, half, psub;  // piece of the head, head of the pair, piece that holds the partners
+    bool turned, low;     // its dims are rotated; they are the first of their pairs
+    size_t row;           // of the tables
+};
+
+// The pairs of heads p0 .. p1 - 1 of one kind (0 q, 1 k, 2 v); kBatch of them are in flight.
+template <int KIND, bool INTERLEAVED, bool F32SRC>
+__device__ __forceinline__ void do_heads(const mono_qkv_append_args& a, const Lane& n, int token, int p0, int p1, uint8_t* to) {
+    if (p0 >= p1) return;
+    constexpr int kBatch = F32SRC ? 1 : 4;
+    const int count = KIND == 0 ? a.q_heads : a.kv_heads, first = KIND == 0 ? 0 : KIND == 1 ? a.q_heads : a.q_heads + a.kv_heads;
+    const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(a.src_bf16) + (size_t)token * a.src_ld) + first * (kDim / 8) + n.sub;
+    const void* gain = KIND == 0 ? a.g_q : a.g_k;
+    Coef cf;
+    const float scale = KIND == 0 ? 1.f : 1.f / (KIND == 1 ? a.k_scale : a.v_scale);
+    uint4 raw[kBatch];
+    if (!F32SRC) {
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) raw[j] = __ldg(src + min(2 * (p0 + j) + n.half, count - 1) * (kDim / 8));
+    }
+    if (KIND != 2) make_coef<INTERLEAVED>(a, gain, n.row, n.sub, n.psub, n.turned, n.low, cf);
+    for (int p = p0; p < p1; p += kBatch) {
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+            if (p + j >= p1) break;
+            const int h = 2 * (p + j) + n.half;
+            f32x2 x[4], other[4];
+            if (F32SRC) {
+                const float* f = a.src_f32 + (size_t)token * a.src_ld + (size_t)(first + min(h, count - 1)) * kDim + n.sub * 8;
+                const float4 lo = sum_partials4<4>(f, (size_t)a.sum_stride, a.nsum), hi = sum_partials4<4>(f + 4, (size_t)a.sum_stride, a.nsum);
+                x[0] = pair(lo.x, lo.y); x[1] = pair(lo.z, lo.w);
+                x[2] = pair(hi.x, hi.y); x[3] = pair(hi.z, hi.w);
+                if (KIND != 2) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) other[i] = INTERLEAVED ? swapped(x[i]) : __shfl_sync(0xffffffffu, x[i], n.half * 16 + n.psub);
+                }
+            } else {
+                const uint4 w = raw[j];
+                unpack8(w, x);
+                if (KIND != 2 && INTERLEAVED) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) other[i] = swapped(x[i]);
+                } else if (KIND != 2) {
+                    const int from = n.half * 16 + n.psub;
+                    unpack8(make_uint4(__shfl_sync(0xffffffffu, w.x, from), __shfl_sync(0xffffffffu, w.y, from), __shfl_sync(0xffffffffu, w.z, from),
+                                       __shfl_sync(0xffffffffu, w.w, from)), other);
+                }
+                raw[j] = __ldg(src + min(h + 2 * kBatch, count - 1) * (kDim / 8));
+            }
+            float f = scale;
+            if (KIND != 2) {
+                if (gain) {
+                    f32x2 sq = mul2(x[0], x[0]);
+#pragma unroll
+                    for (int i = 1; i < 4; ++i) sq = fma2(x[i], x[i], sq);
+                    const float2 sh = halves(sq);
+                    float ssq = sh.x + sh.y;
+#pragma unroll
+                    for (int o = 8; o > 0; o >>= 1) ssq += __shfl_xor_sync(0xffffffffu, ssq, o);
+                    f *= rsqrtf(ssq * (1.f / kDim) + a.eps);
+                }
+                // dims that are not turned keep no trace of others, infinite or not
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[i] = n.turned ? fma2(other[i], cf.b[i], mul2(x[i], cf.a[i])) : mul2(x[i], cf.a[i]);
+            }
+            const f32x2 ff = pair(f, f);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = mul2(x[i], ff);
+            if (h < count && to) {
+                if (KIND == 0) {
+                    *reinterpret_cast<uint4*>(to + h * kDim * 2) = make_uint4(pack2(x[0]), pack2(x[1]), pack2(x[2]), pack2(x[3]));
+                } else {
+                    uint32_t b[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) b[i] = __nv_cvt_float2_to_fp8x2(halves(x[i]), __NV_SATFINITE, __NV_E4M3);
+                    *reinterpret_cast<uint2*>(to + h * kDim) = make_uint2(b[0] | b[1] << 16, b[2] | b[3] << 16);
+                }
+            }
+        }
+    }
+}
+
+// A warp takes `pairs` pairs of heads of one token (q pairs, then k, then v); lanes 0..15 hold the even head of a pair,
+// 16..31 the odd one.
+template <bool INTERLEAVED, bool F32SRC>
+__global__ void __launch_bounds__(kThreads, 4) qkv_append_kernel(const __grid_constant__ mono_qkv_append_args a, int chunks, int pairs) {
     pdl_prologue();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane & 15, half = lane >> 4;
-    const long long work = (long long)blockIdx.x * (kThreads / 32) + warp;
-    const long long token = work / chunks;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const unsigned work = blockIdx.x * (kThreads / 32) + warp;
+    const int token = (int)(work / (unsigned)chunks);
     if (token >= a.tokens) return;  // whole warps leave together
-    const int chunk = (int)(work - token * chunks);
-    const int heads = a.q_heads + 2 * a.kv_heads;
-    const int head0 = chunk * PAIRS * 2 + half;
-    float x[PAIRS][8];
-    if (F32SRC) {
-#pragma unroll
-        for (int p = 0; p < PAIRS; ++p) {
-            const int h = min(head0 + 2 * p, heads - 1);
-            const float* src = a.src_f32 + (size_t)token * a.src_ld + (size_t)h * kDim + sub * 8;
-            const float4 lo = sum_partials4<4>(src, (size_t)a.sum_stride, a.nsum);
-            const float4 hi = sum_partials4<4>(src + 4, (size_t)a.sum_stride, a.nsum);
-            x[p][0] = lo.x; x[p][1] = lo.y; x[p][2] = lo.z; x[p][3] = lo.w;
-            x[p][4] = hi.x; x[p][5] = hi.y; x[p][6] = hi.z; x[p][7] = hi.w;
-        }
-    } else {
-        const __nv_bfloat16* src = reinterpret_cast<const __nv_bfloat16*>(a.src_bf16) + (size_t)token * a.src_ld + sub * 8;
-        uint4 raw[PAIRS];  // every load is issued before the first is used
-#pragma unroll
-        for (int p = 0; p < PAIRS; ++p) raw[p] = __ldg(reinterpret_cast<const uint4*>(src + (size_t)min(head0 + 2 * p, heads - 1) * kDim));
-#pragma unroll
-        for (int p = 0; p < PAIRS; ++p) unpack8(raw[p], x[p]);
-    }
-    // the token's angles: this lane's eight dims are one side of eight pairs (half layout) or four whole pairs
-    const int lanes_half = a.rot_dim >> 4;  // lanes that hold the first half of the rotated dims
-    const bool turned = sub < 2 * lanes_half;
-    int partner = lane;
-    float c[8], s[8];
-    {
-        int64_t pos = a.positions[token];
-        pos = pos < 0 ? 0 : pos >= a.table_rows ? a.table_rows - 1 : pos;
-        const size_t row = (size_t)pos * (a.rot_dim >> 1);
-        if (turned && !a.interleaved) {
-            partner = sub < lanes_half ? lane + lanes_half : lane - lanes_half;
-            const int i = (sub < lanes_half ? sub : sub - lanes_half) * 8;
-            load_table<8>(a.cos, a.table_f32, row + i, c);
-            load_table<8>(a.sin, a.table_f32, row + i, s);
-        } else if (turned) {
-            load_table<4>(a.cos, a.table_f32, row + sub * 4, c);
-            load_table<4>(a.sin, a.table_f32, row + sub * 4, s);
-        }
-    }
+    const int p0 = (int)(work - (unsigned)token * chunks) * pairs, p1 = p0 + pairs;
     const int64_t slot = a.slots ? a.slots[token] : -1;
     const bool insert = slot >= 0 && slot < a.n_pages * kPage;
-#pragma unroll
-    for (int p = 0; p < PAIRS; ++p) {
-        const int h = head0 + 2 * p;
-        const int kind = h < a.q_heads ? 0 : h < a.q_heads + a.kv_heads ? 1 : 2;
-        const void* gp = kind == 0 ? a.g_q : kind == 1 ? a.g_k : nullptr;
-        float ssq = 0.f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) ssq += x[p][j] * x[p][j];
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) ssq += __shfl_xor_sync(0xffffffffu, ssq, o);
-        if (gp) {
-            const float rstd = rsqrtf(ssq * (1.f / kDim) + a.eps);
-            float g[8];
-            unpack8(__ldg(reinterpret_cast<const uint4*>(gp) + sub), g);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[p][j] = x[p][j] * rstd * (1.f + g[j]);
-        }
-        if (!a.interleaved) {
-            const float sign = sub < lanes_half ? -1.f : 1.f;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float other = __shfl_sync(0xffffffffu, x[p][j], partner);
-                if (turned && kind != 2) x[p][j] = x[p][j] * c[j] + sign * other * s[j];
-            }
-        } else if (turned && kind != 2) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float lo = x[p][2 * j], hi = x[p][2 * j + 1];
-                x[p][2 * j] = lo * c[j] - hi * s[j];
-                x[p][2 * j + 1] = hi * c[j] + lo * s[j];
-            }
-        }
-        if (h >= heads) continue;
-        if (kind == 0) {
-            reinterpret_cast<uint4*>(a.q_out)[((size_t)token * a.q_heads + h) * (kDim / 8) + sub] = pack8(x[p]);
-        } else if (insert) {
-            const float sc = kind == 1 ? a.k_scale : a.v_scale;
-            uint8_t* cache = kind == 1 ? a.k_cache : a.v_cache;
-            const int kh = h - a.q_heads - (kind == 1 ? 0 : a.kv_heads);
-            uint32_t w[2] = {0, 0};
-#pragma unroll
-            for (int j = 0; j < 8; j += 2)
-                w[j >> 2] |= (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(__fdiv_rn(x[p][j], sc), __fdiv_rn(x[p][j + 1], sc)), __NV_SATFINITE, __NV_E4M3)
-                             << (8 * (j & 3));
-            *reinterpret_cast<uint2*>(cache + ((size_t)slot * a.kv_heads + kh) * kDim + sub * 8) = make_uint2(w[0], w[1]);
-        }
-    }
+    Lane n;
+    n.sub = lane & 15;
+    n.half = lane >> 4;
+    const int lanes_half = a.rot_dim >> 4;  // lanes that hold the first half of the rotated dims
+    n.turned = n.sub < 2 * lanes_half;
+    n.low = n.sub < lanes_half;
+    n.psub = INTERLEAVED || !n.turned ? n.sub : n.low ? n.sub + lanes_half : n.sub - lanes_half;
+    int64_t pos = a.positions[token];
+    pos = pos < 0 ? 0 : pos >= a.table_rows ? a.table_rows - 1 : pos;
+    n.row = (size_t)pos * (a.rot_dim >> 1);
+    const int pq = (a.q_heads + 1) >> 1, pk = (a.kv_heads + 1) >> 1;
+    uint8_t* q_to = reinterpret_cast<uint8_t*>(a.q_out) + (size_t)token * a.q_heads * kDim * 2 + n.sub * 16;
+    const size_t kv_at = (size_t)(insert ? slot : 0) * a.kv_heads * kDim + n.sub * 8;
+    do_heads<0, INTERLEAVED, F32SRC>(a, n, token, p0, min(p1, pq), q_to);
+    if (!insert) return;
+    do_heads<1, INTERLEAVED, F32SRC>(a, n, token, max(p0 - pq, 0), min(p1 - pq, pk), a.k_cache + kv_at);
+    do_heads<2, INTERLEAVED, F32SRC>(a, n, token, max(p0 - pq - pk, 0), min(p1 - pq - pk, pk), a.v_cache + kv_at);
 }
 
-template <int PAIRS>
+template <bool INTERLEAVED>
 static cudaError_t launch(const mono_qkv_append_args* a, cudaStream_t st) {
-    const int pairs = (a->q_heads + 2 * a->kv_heads + 1) / 2;
-    const int chunks = (pairs + PAIRS - 1) / PAIRS;
+    const int pairs = (a->q_heads + 1) / 2 + 2 * ((a->kv_heads + 1) / 2);
+    // A token's angles are read once per warp and kind of head, so a warp takes as many of its heads as leave every SM
+    // 64 warps; a small step is spread over more warps.
+    const int sms = mono_sm_count() > 0 ? mono_sm_count() : 148;
+    const long long want = ((long long)sms * 64 + a->tokens - 1) / a->tokens;
+    int chunks = (int)(want < 1 ? 1 : want > pairs ? pairs : want);
+    const int per = (pairs + chunks - 1) / chunks;
+    chunks = (pairs + per - 1) / per;
     const long long warps = (long long)a->tokens * chunks;
     const unsigned grid = (unsigned)((warps + kThreads / 32 - 1) / (kThreads / 32));
-    return a->src_f32 ? launch_k(qkv_append_kernel<PAIRS, true>, grid, kThreads, 0, st, *a, chunks)
-                      : launch_k(qkv_append_kernel<PAIRS, false>, grid, kThreads, 0, st, *a, chunks);
+    return a->src_f32 ? launch_k(qkv_append_kernel<INTERLEAVED, true>, grid, kThreads, 0, st, *a, chunks, per)
+                      : launch_k(qkv_append_kernel<INTERLEAVED, false>, grid, kThreads, 0, st, *a, chunks, per);
 }
 
 }  // namespace qkv_append
@@ -195,12 +257,7 @@ extern "C" int mono_qkv_append_launch(const mono_qkv_append_args* a, void* strea
         mono_set_error("%s: rope tables, positions, q output and caches with positive scales required, 16-byte aligned", who);
         return MONO_E_ARG;
     }
-    // A warp that takes four pairs has four row loads in flight and reads its angles once for eight heads; a small
-    // step is spread over more warps instead.
-    const long long pairs = (long long)a->tokens * ((a->q_heads + 2 * a->kv_heads + 1) / 2);
-    const int sms = mono_sm_count();
-    const cudaError_t e = pairs >= (long long)(sms > 0 ? sms : 148) * 64 ? qkv_append::launch<4>(a, (cudaStream_t)stream)
-                                                                         : qkv_append::launch<1>(a, (cudaStream_t)stream);
+    const cudaError_t e = a->interleaved ? qkv_append::launch<true>(a, (cudaStream_t)stream) : qkv_append::launch<false>(a, (cudaStream_t)stream);
     if (e != cudaSuccess) mono_set_error("%s: %s", who, cudaGetErrorString(e));
     return (int)e;
 }

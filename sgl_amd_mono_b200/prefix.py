@@ -47,26 +47,40 @@ def _scale(x: float, name: str) -> float:
     return x
 
 
-def _on(t: torch.Tensor, name: str, dev: torch.device, dtype=None, shape=None) -> torch.Tensor:
-    ops.require(t, name, dtype, shape)
-    if t.device != dev:
+def _on(t: torch.Tensor, name: str, dev: torch.device, dtype=None, shape=None) -> int:
+    """The address of a tensor that is what it has to be (a step makes some thirty of these checks: the common case is
+    four comparisons)."""
+    if not (isinstance(t, torch.Tensor) and t.device == dev and (dtype is None or t.dtype is dtype) and (shape is None or t.shape == shape)
+            and t.is_contiguous()):
+        ops.require(t, name, dtype, shape)
         raise ValueError(f"{name}: on {t.device}, the op was built for {dev}")
-    return t
+    return t.data_ptr()
 
 
-def _aligned(t: torch.Tensor, name: str) -> torch.Tensor:
-    if t.data_ptr() % 16:
+def _aligned(address: int, name: str) -> int:
+    if address % 16:
         raise ValueError(f"{name}: must start on a 16-byte address")
-    return t
+    return address
 
 
-def _caches(k_cache, v_cache, kv_heads: int, dev) -> None:
-    for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
-        _aligned(_on(t, name, dev, torch.uint8), name)
-        if t.dim() != 4 or tuple(t.shape[1:]) != (PAGE, kv_heads, HEAD_DIM) or t.shape[0] < 1:
-            raise ValueError(f"{name}: shape {tuple(t.shape)}, needs [pages, {PAGE}, {kv_heads}, {HEAD_DIM}]")
-    if k_cache.shape != v_cache.shape:
-        raise ValueError(f"v_cache: {v_cache.shape[0]} pages, k_cache has {k_cache.shape[0]}")
+def _caches(a, k_cache, v_cache, kv_heads: int, dev) -> None:
+    a.k_cache = _aligned(_on(k_cache, "k_cache", dev, torch.uint8), "k_cache")
+    shape = k_cache.shape
+    if len(shape) != 4 or shape[0] < 1 or shape[1:] != (PAGE, kv_heads, HEAD_DIM):
+        raise ValueError(f"k_cache: shape {tuple(shape)}, needs [pages, {PAGE}, {kv_heads}, {HEAD_DIM}]")
+    a.v_cache = _aligned(_on(v_cache, "v_cache", dev, torch.uint8, shape), "v_cache")
+    a.n_pages = shape[0]
+
+
+def _launch(fn, a, index: int, what: str) -> None:
+    """Enqueues on the current stream of device ``index``, whichever device is current."""
+    if torch.cuda.current_device() == index:
+        rc = fn(C.byref(a), torch.cuda.current_stream(index).cuda_stream)
+    else:
+        with torch.cuda.device(index):
+            rc = fn(C.byref(a), torch.cuda.current_stream(index).cuda_stream)
+    if rc:
+        L.check(rc, what)
 
 
 class QkvAppendOp:
@@ -91,6 +105,11 @@ class QkvAppendOp:
         self.q_heads, self.kv_heads, self.max_tokens = q_heads, kv_heads, max_tokens
         self.rot_dim, self.interleaved, self.eps = rot_dim, bool(interleaved), float(eps)
         self.q = torch.zeros(max_tokens, q_heads, HEAD_DIM, dtype=torch.bfloat16, device=self.dev)
+        self.width = (q_heads + 2 * kv_heads) * HEAD_DIM
+        self._fn = L.load().mono_qkv_append_launch
+        self._fixed = f = L.QkvAppendArgs()  # what no call changes
+        f.q_heads, f.kv_heads, f.rot_dim, f.interleaved, f.eps = q_heads, kv_heads, rot_dim, int(self.interleaved), self.eps
+        f.k_scale, f.v_scale, f.q_out = self.k_scale, self.v_scale, self.q.data_ptr()
 
     def __call__(self, qkv: torch.Tensor, g_q, g_k, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor, slots,
                  k_cache: torch.Tensor, v_cache: torch.Tensor, tokens: int | None = None) -> torch.Tensor:
@@ -100,54 +119,51 @@ class QkvAppendOp:
         ``positions``, ``slots``: int64 ``[tokens]``; a position outside the table is taken to its nearest row, a slot
         (page * 64 + offset) outside the cache inserts nothing, and the slots inside it must differ.
         Returns q ``[tokens, q_heads, 128]`` (the op's own buffer)."""
-        width = (self.q_heads + 2 * self.kv_heads) * HEAD_DIM
+        width, dev = self.width, self.dev
         a = L.QkvAppendArgs()
-        if not isinstance(qkv, torch.Tensor) or not qkv.is_cuda or qkv.device != self.dev:
-            raise ValueError(f"qkv: must be a tensor on {self.dev} (there is no CPU path)")
-        if qkv.dtype == torch.bfloat16:
-            if qkv.dim() != 2 or qkv.shape[1] != width or qkv.stride(1) != 1 or (qkv.shape[0] > 1 and qkv.stride(0) < width):
-                raise ValueError(f"qkv: shape {tuple(qkv.shape)} strides {qkv.stride()}, needs [tokens, {width}] with contiguous rows")
-            if tokens is not None and tokens != qkv.shape[0]:
-                raise ValueError(f"qkv: {qkv.shape[0]} rows, tokens says {tokens}")
-            n = qkv.shape[0]
-            a.src_bf16, a.src_ld = qkv.data_ptr(), qkv.stride(0) if n > 1 else width
-        elif qkv.dtype == torch.float32:
-            if qkv.dim() != 3 or not qkv.is_contiguous() or qkv.shape[2] != width:
-                raise ValueError(f"qkv: shape {tuple(qkv.shape)}, needs contiguous f32 partial sums [nsum, rows, {width}]")
-            if tokens is None or not 1 <= tokens <= min(L.MAX_ROWS, qkv.shape[1]):
-                raise ValueError(f"tokens: {tokens}, partial sums of {qkv.shape[1]} rows serve 1..{min(L.MAX_ROWS, qkv.shape[1])}")
+        C.memmove(C.byref(a), C.byref(self._fixed), C.sizeof(a))
+        if not isinstance(qkv, torch.Tensor) or qkv.device != dev:
+            raise ValueError(f"qkv: must be a tensor on {dev} (there is no CPU path)")
+        shape = qkv.shape
+        if qkv.dtype is torch.bfloat16:
+            if len(shape) != 2 or shape[1] != width or qkv.stride(1) != 1 or (shape[0] > 1 and qkv.stride(0) < width):
+                raise ValueError(f"qkv: shape {tuple(shape)} strides {qkv.stride()}, needs [tokens, {width}] with contiguous rows")
+            n = shape[0]
+            if tokens is not None and tokens != n:
+                raise ValueError(f"qkv: {n} rows, tokens says {tokens}")
+            ld = qkv.stride(0) if n > 1 else width
+            if ld % 8:
+                raise ValueError(f"qkv: rows {ld} values apart, needs a multiple of 8")
+            a.src_bf16, a.src_ld = _aligned(qkv.data_ptr(), "qkv"), ld
+        elif qkv.dtype is torch.float32:
+            if len(shape) != 3 or not qkv.is_contiguous() or shape[2] != width:
+                raise ValueError(f"qkv: shape {tuple(shape)}, needs contiguous f32 partial sums [nsum, rows, {width}]")
+            if tokens is None or not 1 <= tokens <= min(L.MAX_ROWS, shape[1]):
+                raise ValueError(f"tokens: {tokens}, partial sums of {shape[1]} rows serve 1..{min(L.MAX_ROWS, shape[1])}")
             n = tokens
-            a.src_f32, a.nsum, a.src_ld, a.sum_stride = qkv.data_ptr(), qkv.shape[0], width, qkv.shape[1] * width
+            a.src_f32, a.nsum, a.src_ld, a.sum_stride = _aligned(qkv.data_ptr(), "qkv"), shape[0], width, shape[1] * width
         else:
             raise ValueError(f"qkv: dtype {qkv.dtype}, needs bfloat16 rows or float32 partial sums")
         if not 1 <= n <= self.max_tokens:
             raise ValueError(f"qkv: {n} tokens, the op was built for 1..{self.max_tokens}")
-        if a.src_ld % 8:
-            raise ValueError(f"qkv: rows {a.src_ld} values apart, needs a multiple of 8")
-        _aligned(qkv, "qkv")
-        for g, name in ((g_q, "g_q"), (g_k, "g_k")):
-            if g is not None:
-                _aligned(_on(g, name, self.dev, torch.bfloat16, (HEAD_DIM,)), name)
+        if g_q is not None:
+            a.g_q = _aligned(_on(g_q, "g_q", dev, torch.bfloat16, (HEAD_DIM,)), "g_q")
+        if g_k is not None:
+            a.g_k = _aligned(_on(g_k, "g_k", dev, torch.bfloat16, (HEAD_DIM,)), "g_k")
         if not isinstance(cos, torch.Tensor) or cos.dtype not in (torch.bfloat16, torch.float32):
             raise ValueError("cos: needs a bfloat16 or float32 tensor")
-        for t, name in ((cos, "cos"), (sin, "sin")):
-            _aligned(_on(t, name, self.dev, cos.dtype), name)
-            if t.dim() != 2 or t.shape[0] < 1 or t.shape[1] != self.rot_dim // 2 or t.shape != cos.shape:
-                raise ValueError(f"{name}: shape {tuple(t.shape)}, needs [positions, {self.rot_dim // 2}]")
-        _on(positions, "positions", self.dev, torch.int64, (n,))
+        table = cos.shape
+        a.cos = _aligned(_on(cos, "cos", dev), "cos")
+        if len(table) != 2 or table[0] < 1 or table[1] != self.rot_dim // 2:
+            raise ValueError(f"cos: shape {tuple(table)}, needs [positions, {self.rot_dim // 2}]")
+        a.sin = _aligned(_on(sin, "sin", dev, cos.dtype, table), "sin")
+        a.table_f32, a.table_rows = cos.dtype is torch.float32, table[0]
+        a.positions = _on(positions, "positions", dev, torch.int64, (n,))
         if slots is not None:
-            _on(slots, "slots", self.dev, torch.int64, (n,))
-        _caches(k_cache, v_cache, self.kv_heads, self.dev)
-        a.tokens, a.q_heads, a.kv_heads = n, self.q_heads, self.kv_heads
-        a.rot_dim, a.interleaved = self.rot_dim, int(self.interleaved)
-        a.g_q, a.g_k, a.eps = ops._p(g_q), ops._p(g_k), self.eps
-        a.cos, a.sin, a.table_f32, a.table_rows = cos.data_ptr(), sin.data_ptr(), int(cos.dtype == torch.float32), cos.shape[0]
-        a.positions, a.slots = positions.data_ptr(), ops._p(slots)
-        a.k_scale, a.v_scale = self.k_scale, self.v_scale
-        a.k_cache, a.v_cache, a.n_pages = k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0]
-        a.q_out = self.q.data_ptr()
-        with torch.cuda.device(self.dev):
-            L.check(L.load().mono_qkv_append_launch(C.byref(a), ops._stream()), "mono_qkv_append_launch")
+            a.slots = _on(slots, "slots", dev, torch.int64, (n,))
+        _caches(a, k_cache, v_cache, self.kv_heads, dev)
+        a.tokens = n
+        _launch(self._fn, a, dev.index, "mono_qkv_append_launch")
         return self.q[:n]
 
 
@@ -187,69 +203,66 @@ class SharedPrefixAttnOp:
         self.q_heads, self.kv_heads = q_heads, kv_heads
         self.max_tokens, self.max_seqs, self.max_groups = max_tokens, max_seqs, max_groups
         self.sm_scale = _scale(sm_scale, "sm_scale") if sm_scale is not None else HEAD_DIM ** -0.5
-        self.deadline_s = deadline_s
         with torch.cuda.device(self.dev):
             nbytes = L.load().mono_prefix_attn_scratch_bytes(max_tokens, q_heads, kv_heads, max_seqs, max_groups)
         self.scratch = torch.zeros(nbytes, dtype=torch.uint8, device=self.dev)
         self.out = torch.zeros(max_tokens, q_heads, HEAD_DIM, dtype=torch.bfloat16, device=self.dev)
         self.guard = guard if guard is not None else torch.zeros(L.GUARD_WORDS, dtype=torch.int32, device=self.dev)
+        self._fn = L.load().mono_prefix_attn_launch
+        self._fixed = f = L.PrefixAttnArgs()  # what no call changes
+        f.q_heads, f.kv_heads, f.k_scale, f.v_scale, f.sm_scale = q_heads, kv_heads, self.k_scale, self.v_scale, self.sm_scale
+        f.scratch, f.scratch_bytes, f.out = self.scratch.data_ptr(), nbytes, self.out.data_ptr()
+        f.guard, f.wait_ns = self.guard.data_ptr(), int(deadline_s * 1e9)
 
-    def _table(self, t, name: str, rows: int) -> torch.Tensor:
-        _on(t, name, self.dev, torch.int32)
+    def _table(self, t, name: str, rows: int) -> tuple[int, int]:
+        address = _on(t, name, self.dev, torch.int32)
         if t.dim() != 2 or t.shape[0] != rows or t.shape[1] < 1:
             raise ValueError(f"{name}: shape {tuple(t.shape)}, needs [{rows}, at least 1]")
-        return t
+        return address, t.shape[1]
 
     def __call__(self, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, t: PrefixTables,
                  out: torch.Tensor | None = None) -> torch.Tensor:
         """``q``: bf16 ``[tokens, q_heads, 128]`` (token rows may lie further apart).  Returns ``out`` (default: the
         op's own buffer), bf16 ``[tokens, q_heads, 128]``."""
-        if not isinstance(q, torch.Tensor) or q.device != self.dev:
-            raise ValueError(f"q: must be a tensor on {self.dev} (there is no CPU path)")
-        if q.dtype != torch.bfloat16:
+        dev = self.dev
+        if not isinstance(q, torch.Tensor) or q.device != dev:
+            raise ValueError(f"q: must be a tensor on {dev} (there is no CPU path)")
+        if q.dtype is not torch.bfloat16:
             raise ValueError(f"q: dtype {q.dtype}, needs torch.bfloat16")
-        if q.dim() != 3 or tuple(q.shape[1:]) != (self.q_heads, HEAD_DIM):
-            raise ValueError(f"q: shape {tuple(q.shape)}, needs [tokens, {self.q_heads}, {HEAD_DIM}]")
-        n = q.shape[0]
+        shape, strides = q.shape, q.stride()
+        if len(shape) != 3 or shape[1] != self.q_heads or shape[2] != HEAD_DIM:
+            raise ValueError(f"q: shape {tuple(shape)}, needs [tokens, {self.q_heads}, {HEAD_DIM}]")
+        n = shape[0]
         if not 1 <= n <= self.max_tokens:
             raise ValueError(f"q: {n} tokens, the op was built for 1..{self.max_tokens}")
         width = self.q_heads * HEAD_DIM
-        ld = q.stride(0) if n > 1 else width
-        if q.stride(2) != 1 or (self.q_heads > 1 and q.stride(1) != HEAD_DIM) or ld < width or ld % 8:
-            raise ValueError(f"q: strides {q.stride()}, needs contiguous heads and token rows a multiple of 8 values apart")
-        _aligned(q, "q")
-        _caches(k_cache, v_cache, self.kv_heads, self.dev)
-        _on(t.lens, "lens", self.dev, torch.int32)
-        seqs = t.lens.numel()
-        if t.lens.dim() != 1 or not 1 <= seqs <= self.max_seqs:
+        ld = strides[0] if n > 1 else width
+        if strides[2] != 1 or (self.q_heads > 1 and strides[1] != HEAD_DIM) or ld < width or ld % 8:
+            raise ValueError(f"q: strides {strides}, needs contiguous heads and token rows a multiple of 8 values apart")
+        a = L.PrefixAttnArgs()
+        C.memmove(C.byref(a), C.byref(self._fixed), C.sizeof(a))
+        a.tokens, a.q, a.q_ld = n, _aligned(q.data_ptr(), "q"), ld
+        _caches(a, k_cache, v_cache, self.kv_heads, dev)
+        a.lens = _on(t.lens, "lens", dev, torch.int32)
+        seqs = t.lens.shape[0] if t.lens.dim() == 1 else 0
+        if not 1 <= seqs <= self.max_seqs:
             raise ValueError(f"lens: shape {tuple(t.lens.shape)}, the op was built for 1..{self.max_seqs} sequences")
-        _on(t.q_start, "q_start", self.dev, torch.int32, (seqs + 1,))
-        self._table(t.page_table, "page_table", seqs)
-        groups = 0
+        a.seqs = seqs
+        a.q_start = _on(t.q_start, "q_start", dev, torch.int32, (seqs + 1,))
+        a.page_table, a.pt_ld = self._table(t.page_table, "page_table", seqs)
         if t.prefix_lens is not None:
-            _on(t.prefix_lens, "prefix_lens", self.dev, torch.int32)
-            groups = t.prefix_lens.numel()
-            if t.prefix_lens.dim() != 1 or not 1 <= groups <= self.max_groups:
+            a.prefix_lens = _on(t.prefix_lens, "prefix_lens", dev, torch.int32)
+            groups = t.prefix_lens.shape[0] if t.prefix_lens.dim() == 1 else 0
+            if not 1 <= groups <= self.max_groups:
                 raise ValueError(f"prefix_lens: shape {tuple(t.prefix_lens.shape)}, the op was built for up to {self.max_groups} groups")
-            _on(t.group_start, "group_start", self.dev, torch.int32, (groups + 1,))
-            self._table(t.prefix_table, "prefix_table", groups)
+            a.groups = groups
+            a.group_start = _on(t.group_start, "group_start", dev, torch.int32, (groups + 1,))
+            a.prefix_table, a.prefix_ld = self._table(t.prefix_table, "prefix_table", groups)
         elif t.group_start is not None or t.prefix_table is not None:
             raise ValueError("prefix_lens: missing beside group_start / prefix_table")
         if out is None:
             out = self.out[:n]
         else:
-            _aligned(_on(out, "out", self.dev, torch.bfloat16, (n, self.q_heads, HEAD_DIM)), "out")
-        a = L.PrefixAttnArgs()
-        a.tokens, a.q_heads, a.kv_heads, a.seqs, a.groups = n, self.q_heads, self.kv_heads, seqs, groups
-        a.q, a.q_ld = q.data_ptr(), ld
-        a.k_cache, a.v_cache, a.n_pages = k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0]
-        a.q_start, a.page_table, a.pt_ld, a.lens = t.q_start.data_ptr(), t.page_table.data_ptr(), t.page_table.shape[1], t.lens.data_ptr()
-        if groups:
-            a.group_start, a.prefix_lens = t.group_start.data_ptr(), t.prefix_lens.data_ptr()
-            a.prefix_table, a.prefix_ld = t.prefix_table.data_ptr(), t.prefix_table.shape[1]
-        a.k_scale, a.v_scale, a.sm_scale = self.k_scale, self.v_scale, self.sm_scale
-        a.scratch, a.scratch_bytes = self.scratch.data_ptr(), self.scratch.numel()
-        a.out, a.guard, a.wait_ns = out.data_ptr(), self.guard.data_ptr(), int(self.deadline_s * 1e9)
-        with torch.cuda.device(self.dev):
-            L.check(L.load().mono_prefix_attn_launch(C.byref(a), ops._stream()), "mono_prefix_attn_launch")
+            a.out = _aligned(_on(out, "out", dev, torch.bfloat16, (n, self.q_heads, HEAD_DIM)), "out")
+        _launch(self._fn, a, dev.index, "mono_prefix_attn_launch")
         return out

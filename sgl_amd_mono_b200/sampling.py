@@ -16,8 +16,7 @@ import ctypes as C
 import torch
 
 from . import _lib as L
-from . import ops
-from .prefix import _device, _on
+from .prefix import _device, _launch, _on
 
 
 class SampleOp:
@@ -31,6 +30,7 @@ class SampleOp:
         self.vocab, self.max_rows = vocab, max_rows
         self.tokens = torch.zeros(max_rows, dtype=torch.int64, device=self.dev)
         self.logprobs = torch.zeros(max_rows, dtype=torch.float32, device=self.dev)
+        self._fn, self._out = L.load().mono_sample_launch, (self.tokens.data_ptr(), self.logprobs.data_ptr())
 
     def __call__(self, logits: torch.Tensor, u: torch.Tensor, temperature=None, top_k=None, top_p=None, min_p=None):
         """``logits``: f32 or bf16 ``[rows, vocab]`` (rows may lie further apart); ``u``: f32 ``[rows]`` in [0, 1);
@@ -38,27 +38,30 @@ class SampleOp:
         Temperature 0 or below takes the best token.  Returns (tokens int64 ``[rows]``, logprobs f32 ``[rows]``): the
         drawn token's log probability at the row's temperature before any filter (at temperature 1 for greedy rows).  A
         row whose logits are all -inf or NaN gives token -1."""
-        if not isinstance(logits, torch.Tensor) or logits.device != self.dev:
-            raise ValueError(f"logits: must be a tensor on {self.dev} (there is no CPU path)")
+        dev = self.dev
+        if not isinstance(logits, torch.Tensor) or logits.device != dev:
+            raise ValueError(f"logits: must be a tensor on {dev} (there is no CPU path)")
         if logits.dtype not in (torch.float32, torch.bfloat16):
             raise ValueError(f"logits: dtype {logits.dtype}, needs float32 or bfloat16")
-        if logits.dim() != 2 or logits.shape[1] != self.vocab or not 1 <= logits.shape[0] <= self.max_rows:
-            raise ValueError(f"logits: shape {tuple(logits.shape)}, needs [1..{self.max_rows}, {self.vocab}]")
-        rows = logits.shape[0]
+        shape = logits.shape
+        if len(shape) != 2 or shape[1] != self.vocab or not 1 <= shape[0] <= self.max_rows:
+            raise ValueError(f"logits: shape {tuple(shape)}, needs [1..{self.max_rows}, {self.vocab}]")
+        rows = shape[0]
         ld = logits.stride(0) if rows > 1 else self.vocab
         if (self.vocab > 1 and logits.stride(1) != 1) or ld < self.vocab:
             raise ValueError(f"logits: strides {logits.stride()}, needs contiguous rows")
-        _on(u, "u", self.dev, torch.float32, (rows,))
-        for t, name, dt in ((temperature, "temperature", torch.float32), (top_k, "top_k", torch.int32),
-                            (top_p, "top_p", torch.float32), (min_p, "min_p", torch.float32)):
-            if t is not None:
-                _on(t, name, self.dev, dt, (rows,))
         a = L.SampleArgs()
-        a.rows, a.vocab, a.logits, a.ld = rows, self.vocab, logits.data_ptr(), ld
-        a.logits_bf16 = int(logits.dtype == torch.bfloat16)
-        a.u, a.temperature, a.top_k = u.data_ptr(), ops._p(temperature), ops._p(top_k)
-        a.top_p, a.min_p = ops._p(top_p), ops._p(min_p)
-        a.tokens, a.logprobs = self.tokens.data_ptr(), self.logprobs.data_ptr()
-        with torch.cuda.device(self.dev):
-            L.check(L.load().mono_sample_launch(C.byref(a), ops._stream()), "mono_sample_launch")
+        a.rows, a.vocab, a.logits, a.ld, a.logits_bf16 = rows, self.vocab, logits.data_ptr(), ld, logits.dtype is torch.bfloat16
+        n = (rows,)
+        a.u = _on(u, "u", dev, torch.float32, n)
+        if temperature is not None:
+            a.temperature = _on(temperature, "temperature", dev, torch.float32, n)
+        if top_k is not None:
+            a.top_k = _on(top_k, "top_k", dev, torch.int32, n)
+        if top_p is not None:
+            a.top_p = _on(top_p, "top_p", dev, torch.float32, n)
+        if min_p is not None:
+            a.min_p = _on(min_p, "min_p", dev, torch.float32, n)
+        a.tokens, a.logprobs = self._out
+        _launch(self._fn, a, dev.index, "mono_sample_launch")
         return self.tokens[:rows], self.logprobs[:rows]

@@ -489,6 +489,10 @@ static size_t wide_segments(size_t tokens, size_t q_heads, size_t kv_heads) {
     if (rows < kWideRows) return 0;
     return (size_t)sm_or_default() + kv_heads * 2 * (rows / Shape<true>::kTile + rows / kWideRows);
 }
+// The wide kernel's queries (two planes of 128 bytes a row) and their scales; none where no entry can have so many rows.
+static size_t image_bytes(size_t tokens, size_t q_heads, size_t kv_heads) {
+    return tokens * (q_heads / kv_heads) < kWideRows ? 0 : up256(tokens * q_heads * 256) + up256(tokens * q_heads * 4);
+}
 static size_t narrow_bytes(int tokens, int q_heads, int kv_heads, int seqs, int groups) {
     return up256(narrow_segments(tokens, q_heads, kv_heads, seqs, groups) * Shape<false>::kSegFloats * sizeof(float));
 }
@@ -498,7 +502,7 @@ static size_t narrow_bytes(int tokens, int q_heads, int kv_heads, int seqs, int 
 extern "C" size_t mono_prefix_attn_scratch_bytes(int tokens, int q_heads, int kv_heads, int seqs, int groups) {
     using namespace prefix_attn;
     if (tokens < 1 || q_heads < 1 || kv_heads < 1 || seqs < 1 || groups < 0 || q_heads % kv_heads) return 0;
-    return up256((size_t)(seqs + groups) * sizeof(Record)) + 256 + 2 * up256((size_t)tokens * 4) + narrow_bytes(tokens, q_heads, kv_heads, seqs, groups) +
+    return up256((size_t)(seqs + groups) * sizeof(Record)) + 256 + 2 * up256((size_t)tokens * 4) + image_bytes(tokens, q_heads, kv_heads) + narrow_bytes(tokens, q_heads, kv_heads, seqs, groups) +
            wide_segments(tokens, q_heads, kv_heads) * Shape<true>::kSegFloats * sizeof(float);
 }
 
@@ -553,6 +557,9 @@ extern "C" int mono_prefix_attn_launch(const mono_prefix_attn_args* a, void* str
         p.s.entry[w] = reinterpret_cast<int*>(at);
         at += up256((size_t)a->tokens * 4);
     }
+    p.s.q_image = at;
+    p.s.q_scale = reinterpret_cast<float*>(at + up256((size_t)a->tokens * a->q_heads * 256));
+    at += image_bytes(a->tokens, a->q_heads, a->kv_heads);
     p.s.seg[0] = reinterpret_cast<float*>(at);
     p.s.seg[1] = reinterpret_cast<float*>(at + narrow_bytes(a->tokens, a->q_heads, a->kv_heads, a->seqs, a->groups));
     const cudaStream_t st = (cudaStream_t)stream;
@@ -570,6 +577,9 @@ extern "C" int mono_prefix_attn_launch(const mono_prefix_attn_args* a, void* str
     }
     const int narrow = 2 * sm_or_default();
     const int wide = (long)a->tokens * (a->q_heads / a->kv_heads) >= kWideRows ? sm_or_default() : 0;  // no entry has more rows than the step
+    const uint64_t q_rows = (uint64_t)a->tokens * a->q_heads;
+    if (wide)
+        if (int rc = mono_tmap_encode_box(reinterpret_cast<mono_tmap_t*>(&p.qmap), p.s.q_image, 128, q_rows, 2, 128, q_rows * 128, 128)) return rc;
     cudaError_t e = wide ? launch_wide(p, wide, st) : cudaSuccess;
     if (e == cudaSuccess) e = launch_k(prefix_narrow_kernel, narrow, kThreads, smem, st, p);
     // Few rows: four warps share two heads' segments (a long prefix leaves many of them); many rows: a warp each.

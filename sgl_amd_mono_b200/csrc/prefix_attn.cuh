@@ -53,13 +53,12 @@ __device__ __forceinline__ int row_limit(const Entry& n, int row, int G) {
     return n.causal ? n.len - n.ntok + 1 + row / G : n.len;
 }
 
-// A kernel's view of the work: narrow (16-row tiles, units of 64 keys) or wide (256-row tiles, units of 128 keys).
-// A wide item of at most kWideHalf rows gives its CTA's two halves the same rows and alternate blocks of 128 keys, so
-// that its units are 256 keys and cost what the others' do.
+// A kernel's view of the work: narrow (16-row tiles) or wide (256-row tiles), in units of one page of keys.  A wide item
+// of at most kWideHalf rows gives its CTA's two halves the same rows and alternate pages, so that its units are two pages
+// and cost what the others' do.
 template <bool WIDE>
 struct Shape {
     static constexpr int kTile = WIDE ? 256 : 16;
-    static constexpr int kKeys = WIDE ? 128 : 64;
     static constexpr int kSegFloats = 2 * kTile + kTile * kDim;  // max, sum, values
 };
 constexpr int kWideHalf = 128;
@@ -76,7 +75,7 @@ __device__ __forceinline__ Work entry_work(const mono_prefix_attn_args& a, const
     Work w = {0, 0, 0};
     if ((rows >= kWideRows) != WIDE || rows <= 0 || n.len <= 0) return w;
     w.tiles = (rows + Shape<WIDE>::kTile - 1) / Shape<WIDE>::kTile;
-    w.units = w.last = (n.len + Shape<WIDE>::kKeys - 1) / Shape<WIDE>::kKeys;
+    w.units = w.last = (n.len + kPage - 1) / kPage;
     if (WIDE && rows - (w.tiles - 1) * Shape<WIDE>::kTile <= kWideHalf) w.last = (w.units + 1) / 2;
     return w;
 }
@@ -94,6 +93,8 @@ struct Scratch {
     uint32_t* total[2];    // units and items of one kv head
     int* entry[2];         // [tokens]
     float* seg[2];
+    uint8_t* q_image;      // the wide kernel's queries: [2][kv heads][tokens][q heads per kv head][128], and per row
+    float* q_scale;        // what undoes their scale
 };
 
 // off[0..E]: units of one kv head before entry e (off[E]: all of them); item[0..E]: items likewise.  The list of units
@@ -179,12 +180,12 @@ __device__ __forceinline__ Place place_of(const uint32_t* off, int E, uint32_t u
 __device__ __forceinline__ uint32_t part_size(uint32_t U, uint32_t ctas) { return max((U + ctas - 1) / ctas, 1u); }
 
 struct alignas(64) Params {
-    CUtensorMap kmap, vmap;
+    CUtensorMap kmap, vmap, qmap;
     mono_prefix_attn_args a;
     Scratch s;
 };
 
-// Runs the wide kernel (prefix_attn_tc.cu) on `ctas` CTAs.
+// Makes the query image and runs the wide kernel on `ctas` CTAs (prefix_attn_tc.cu).
 cudaError_t launch_wide(const Params& p, int ctas, cudaStream_t st);
 
 }  // namespace prefix_attn

@@ -1,39 +1,39 @@
 // Shared-prefix attention for many rows on 5th-generation tensor cores (prefix_attn.cuh: how the work is cut).
 //
-// A unit is 128 keys of one kv head for up to 256 rows, which two streams of 128 rows (the TMEM lanes) work on:
-//   S[row][key] = sum_d Q[row][d] K[key][d]   kind::f8f6f4, M 128, N 128, K 128, twice: the bf16 queries as two E4M3 planes
-//   O[row][dim] += sum_k P[row][k] V[k][dim]  kind::f16, M 128, N 128, K 128, P in tensor memory
+// A block is one page (64 keys) of one kv head for up to 256 rows, which two streams of 128 rows (the TMEM lanes) work on:
+//   S[row][key] = sum_d Q[row][d] K[key][d]   kind::f8f6f4, M 128, N 64, K 128, twice: the bf16 queries as two E4M3 planes
+//   O[row][dim] += sum_k P[row][k] V[k][dim]  kind::f16, M 128, N 128, K 64, P in tensor memory
 // K is used as the bytes that lie in the cache: a query row, scaled by a power of two, is split into hi + lo E4M3 values,
 // exactly for values within 2^12 of the row's largest.  P is f16 (11 bits, and with the bias below weights down to 2^-31 of
 // the largest: two E4M3 planes would drop weights below 2^-18, which a long tail of small weights adds up), so four
-// warps widen V to f16 in shared memory, which is exact.  Each stream has a warpgroup of softmax threads, one row each,
-// and while it works on its scores the tensor core works for the other stream.  An item of at most 128 rows gives both
-// streams the same rows and alternate units.
+// warps widen V to f16 in shared memory, which is exact.  Each stream has a warpgroup of softmax threads, one row each.
+// The softmax takes a block's scores to registers at once, so the next block's are made while it works; P has two buffers,
+// so it does not wait for the second product either.  An item of at most 128 rows gives both streams
+// the same rows and alternate pages, and their two parts are joined in shared memory at its end.
 //
 // The running maximum is lazy: values are scaled to a reference that is raised (and O rescaled in tensor memory) only
 // when a score passes it by 2^8, which f16 P has room for.
 //
-// Bound: the two products are 4 x 128 x 128 x 128 multiply-adds a unit and stream pair, 2048 tensor cycles, against 2048
-// cycles of exponentials (16 a cycle); from HBM a unit is 32 KB, read once for all 256 rows.
+// Bound: per block and stream pair shared memory moves 168 KB (the queries are read again for every block: 6 KB for 32
+// tensor cycles of the first product), 1312 cycles, the products take 1024 cycles and the exponentials 1024 (16 a cycle).
 #include "prefix_attn.cuh"
 
 namespace prefix_attn {
 namespace {
 MONO_TL_DECLARE(tl_wide)
 
-constexpr int kKeys = 128;
 // warps 0..3: softmax of stream 0, 4..7: of stream 1
-constexpr int kConvWarp0 = 8, kTmaWarp = 12, kMmaWarp = 13;
-constexpr int kThreadsWide = 16 * 32;  // warps 14 and 15 only fill the fetching warps' warpgroup
+constexpr int kConvWarp0 = 8, kTmaWarp = 12, kMmaWarp = 13;  // 13 and 14: the products of stream 0 and 1
+constexpr int kThreadsWide = 16 * 32;                         // (warp 15 only fills the warpgroup)
 // Registers per thread: 128 at launch, moved from the warpgroups that need few to the two softmax ones, which hold a
-// X.
-constexpr int kRegsSoftmax = 168, kRegsConv = 72, kRegsFetch = 104;
-constexpr int kKStages = 3, kVStages = 2, kWStages = 2;  // K bytes, V bytes, widened V
+// block's 64 scores: 2 x 152 + 88 + 120 = 4 x 128.
+constexpr int kRegsSoftmax = 152, kRegsConv = 88, kRegsFetch = 120;
+constexpr int kKStages = 6, kVStages = 4, kWStages = 4;  // K bytes, V bytes, widened V
 constexpr int kQPlane = 128 * 128;                       // [128 rows][128 B]
-constexpr int kKTile = kKeys * 128, kVTile = kKeys * 128, kWTile = 2 * kKeys * 128;
-constexpr int kOkRing = 8;  // page flags outlive their K stage until the softmax of their unit
+constexpr int kKTile = kPage * 128, kVTile = kPage * 128, kWTile = 2 * kPage * 128;
+constexpr int kOkRing = 16;  // page flags outlive their K stage until the softmax of their block (eleven blocks at most)
 constexpr int kSmemFixed = 1024 + 2 * 2 * kQPlane + kKStages * kKTile + kVStages * kVTile + kWStages * kWTile;
-constexpr int kTmemCols = 512;  // S of stream 0 and 1 (P over their first half), O of stream 0 and 1
+constexpr int kTmemCols = 512;  // per stream S (64 columns) and two buffers of P (32 each), then O of stream 0 and 1
 constexpr float kBias = 7.f, kLazy = 8.f;
 
 template <int N> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
@@ -44,11 +44,14 @@ template <int N> __device__ __forceinline__ void regs_down() { asm volatile("set
 // rolled over quarters of a block.
 __device__ __forceinline__ bool wait_on(uint64_t* bar, uint32_t parity, volatile int* abort_flag, uint64_t limit_ns) {
     if (mbar_try_wait(bar, parity)) return true;
-    const uint64_t t0 = globaltimer_ns();
+    uint64_t t0 = 0;
 #pragma unroll 1
-    while (!mbar_try_wait(bar, parity)) {  // (each try sleeps for a while)
+    for (uint32_t i = 1; !mbar_try_wait(bar, parity); ++i) {  // (each try sleeps for a while)
+        if (i & 31) continue;  // the global timer is slow to read: only once a wait is clearly long
+        const uint64_t now = globaltimer_ns();
+        if (t0 == 0) t0 = now;
         if (*abort_flag) return false;
-        if (globaltimer_ns() - t0 > limit_ns) {
+        if (now - t0 > limit_ns) {
             *abort_flag = 1;
             return false;
         }
@@ -103,12 +106,17 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t r[16]) 
 __device__ __forceinline__ uint64_t desc_sw128(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
     return (uint64_t)((saddr & 0x3FFFF) >> 4) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(sbo >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
-constexpr uint32_t kIdescS = (1u << 4) | ((128u >> 3) << 17) | ((128u >> 4) << 24);               // E4M3 x E4M3 -> f32, both K-major
+constexpr uint32_t kIdescS = (1u << 4) | ((64u >> 3) << 17) | ((128u >> 4) << 24);               // E4M3 x E4M3 -> f32, both K-major
 constexpr uint32_t kIdescO = (1u << 4) | (1u << 16) | ((128u >> 3) << 17) | ((128u >> 4) << 24);  // f16 x f16 -> f32, B MN-major
 
 __device__ __forceinline__ float ex2(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
 __device__ __forceinline__ uint32_t pack_half(float a, float b) {
@@ -120,131 +128,74 @@ __device__ __forceinline__ uint32_t widen2(uint32_t lo16) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// A block's scores, in two passes over tensor memory (a quarter is requested while the one before is worked on): their
-// maximum, then the weights into P, over columns of S that have been read, and the weights' sum.  `vis`: how many of the
-// block's keys this row sees; `ok`: which of its two pages exist.
-template <bool MASK>
-__device__ __forceinline__ float quarter_max(const uint32_t r[32], int c, int vis, int ok, float mx) {
-    const int n = MASK ? (ok >> (c >> 1) & 1 ? vis - c * 32 : 0) : 32;
-    float m4[4] = {mx, -INFINITY, -INFINITY, -INFINITY};
+// ------------------------------------------------------------------ queries
+// Every query row as two planes of E4M3, scaled by the power of two that brings its largest value into [128, 256) (E4M3
+// ends at 448), and what undoes the scale.  Image: [plane][kv head][token][head of the kv head][128 bytes].  Half a warp
+// per row.  (The rows are wanted by every CTA that has a part of their prefix: made by each of them, on its own rows, at
+// its start, they cost 4 to 7 us of it.)
+__global__ void __launch_bounds__(256) prefix_split_kernel(const mono_prefix_attn_args a, uint8_t* image, float* back_scale) {
+    pdl_prologue();
+    const int lane = threadIdx.x & 31, sub = lane & 15;
+    const unsigned G = a.q_heads / a.kv_heads, rows = (unsigned)a.tokens * a.q_heads;
+    const unsigned r = (blockIdx.x * 8 + (threadIdx.x >> 5)) * 2 + (lane >> 4);  // row of the image
+    const unsigned k = min(r, rows - 1), per = (unsigned)a.tokens * G, kh = k / per, tok = (k - kh * per) / G, g = k - kh * per - tok * G;
+    const uint4 v = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(a.q) + (size_t)tok * a.q_ld + (size_t)(kh * G + g) * kDim) + sub);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    uint32_t top = 0;  // the exponent of the largest |value|: NaN and infinity have the largest
 #pragma unroll
-    for (int i = 0; i < 32; ++i) m4[i & 3] = fmaxf(m4[i & 3], !MASK || i < n ? __uint_as_float(r[i]) : -INFINITY);
-    return fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-}
-template <bool MASK>
-__device__ __forceinline__ float block_max(uint32_t s_addr, int vis, int ok) {
-    uint32_t a[32], b[32];
-    float mx = -INFINITY;
-    tmem_ld32(s_addr, a);
-    wait_ld();
-#pragma unroll 1
-    for (int c = 0; c < 4; c += 2) {
-        tmem_ld32(s_addr + (c + 1) * 32, b);
-        mx = quarter_max<MASK>(a, c, vis, ok, mx);
-        wait_ld();
-        tmem_ld32(s_addr + ((c + 2) & 3) * 32, a);
-        mx = quarter_max<MASK>(b, c + 1, vis, ok, mx);
-        wait_ld();
-    }
-    return mx;
-}
-template <bool MASK>
-__device__ __forceinline__ void quarter_weights(const uint32_t r[32], uint32_t s_addr, int c, int vis, int ok, float scale, float shift, float l4[4]) {
-    const int n = MASK ? (ok >> (c >> 1) & 1 ? vis - c * 32 : 0) : 32;
-    uint32_t w[16];
+    for (int i = 0; i < 4; ++i) top = max(top, max((w[i] << 16) & 0x7F800000u, w[i] & 0x7F800000u));
 #pragma unroll
-    for (int i = 0; i < 32; i += 2) {
-        float p0 = ex2(fmaf(__uint_as_float(r[i]), scale, shift)), p1 = ex2(fmaf(__uint_as_float(r[i + 1]), scale, shift));
-        if (MASK) {
-            p0 = i < n ? p0 : 0.f;
-            p1 = i + 1 < n ? p1 : 0.f;
-        }
-        l4[i & 2] += p0;
-        l4[(i & 2) + 1] += p1;
-        w[i >> 1] = pack_half(p0, p1);
+    for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const int ex = clamp_int((int)(top >> 23), 30, 254);
+    const float up = __uint_as_float((uint32_t)(261 - ex) << 23);  // 2^(134 - ex)
+    uint32_t hi[2] = {0, 0}, lo[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float f0 = __uint_as_float(w[i] << 16) * up, f1 = __uint_as_float(w[i] & 0xFFFF0000u) * up;
+        const __nv_fp8x2_storage_t hb = __nv_cvt_float2_to_fp8x2(make_float2(f0, f1), __NV_SATFINITE, __NV_E4M3);
+        const __half2_raw hr = __nv_cvt_fp8x2_to_halfraw2(hb, __NV_E4M3);
+        const float2 hf = __half22float2(*reinterpret_cast<const __half2*>(&hr));
+        const __nv_fp8x2_storage_t lb = __nv_cvt_float2_to_fp8x2(make_float2(f0 - hf.x, f1 - hf.y), __NV_SATFINITE, __NV_E4M3);
+        hi[i >> 1] |= (uint32_t)hb << (16 * (i & 1));
+        lo[i >> 1] |= (uint32_t)lb << (16 * (i & 1));
     }
-    tmem_st16(s_addr + c * 16, w);
-}
-template <bool MASK>
-__device__ __forceinline__ float block_weights(uint32_t s_addr, int vis, int ok, float scale, float shift) {
-    uint32_t a[32], b[32];
-    float l4[4] = {0.f, 0.f, 0.f, 0.f};
-    tmem_ld32(s_addr, a);
-    wait_ld();
-#pragma unroll 1
-    for (int c = 0; c < 4; c += 2) {
-        tmem_ld32(s_addr + (c + 1) * 32, b);
-        quarter_weights<MASK>(a, s_addr, c, vis, ok, scale, shift, l4);
-        wait_ld();
-        if (c == 0) tmem_ld32(s_addr + 64, a);
-        quarter_weights<MASK>(b, s_addr, c + 1, vis, ok, scale, shift, l4);
-        wait_ld();
-    }
-    return (l4[0] + l4[1]) + (l4[2] + l4[3]);
+    if (r >= rows) return;
+    *reinterpret_cast<uint2*>(image + (size_t)r * 128 + sub * 8) = make_uint2(hi[0], hi[1]);
+    *reinterpret_cast<uint2*>(image + ((size_t)rows + r) * 128 + sub * 8) = make_uint2(lo[0], lo[1]);
+    // infinite or NaN: saturation would hide it; a row of NaN
+    if (sub == 0) back_scale[r] = top == 0x7F800000u ? __uint_as_float(0x7FC00000u) : __uint_as_float((uint32_t)(ex - 7) << 23);
 }
 
-// The queries of a warp's 32 rows (row0 ..; those from `rows` on are zeros) as two planes of E4M3 in the layout of a
-// K-major operand at `dst` (rows of 128 bytes, 16-byte pieces swizzled by the row's low three bits), each row scaled by
-// the power of two that brings its largest value into [128, 256) (E4M3 ends at 448).  Half a warp loads a row (lines are
-// read whole: many CTAs want the same queries at the same time).  Returns what undoes the scale of row0 + lane.
-__device__ __forceinline__ float write_queries(const mono_prefix_attn_args& a, const Entry& en, int head, int G, int row0, int rows, uint8_t* dst) {
-    const int lane = threadIdx.x & 31, half = lane >> 4, sub = lane & 15;
-    const __nv_bfloat16* q = reinterpret_cast<const __nv_bfloat16*>(a.q) + (size_t)en.tok0 * a.q_ld + (size_t)head * G * kDim + sub * 8;
-    float mine = 1.f;
-    constexpr int B = 8;
-#pragma unroll 1
-    for (int r0 = 0; r0 < 32; r0 += 2 * B) {
-        uint4 v[B];
+// ------------------------------------------------------------------ attention
+// f16 weights 2^(s scale + shift) of a block's scores, pairwise, their f32 sum and the scores' maximum.
+__device__ __forceinline__ float weights(const uint32_t s[64], float scale, float shift, uint32_t w[32], float* mx) {
+    float l4[4] = {0.f, 0.f, 0.f, 0.f}, m2[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-        for (int j = 0; j < B; ++j) {
-            const int row = row0 + r0 + 2 * j + half, r = row < rows ? row : 0, tok = r / G;
-            v[j] = __ldg(reinterpret_cast<const uint4*>(q + (size_t)tok * a.q_ld + (size_t)(r - tok * G) * kDim));
-        }
-#pragma unroll
-        for (int j = 0; j < B; ++j) {
-            const int at = r0 + 2 * j + half;
-            const uint32_t w[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
-            uint32_t top = 0;  // the exponent of the largest |value|: NaN and infinity have the largest
-#pragma unroll
-            for (int i = 0; i < 4; ++i) top = max(top, max((w[i] << 16) & 0x7F800000u, w[i] & 0x7F800000u));
-#pragma unroll
-            for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-            const int ex = clamp_int((int)(top >> 23), 30, 254);
-            const float up = row0 + at < rows ? __uint_as_float((uint32_t)(261 - ex) << 23) : 0.f;  // 2^(134 - ex)
-            uint32_t hi[2] = {0, 0}, lo[2] = {0, 0};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float f0 = __uint_as_float(w[i] << 16) * up, f1 = __uint_as_float(w[i] & 0xFFFF0000u) * up;
-                const __nv_fp8x2_storage_t hb = __nv_cvt_float2_to_fp8x2(make_float2(f0, f1), __NV_SATFINITE, __NV_E4M3);
-                const __half2_raw hr = __nv_cvt_fp8x2_to_halfraw2(hb, __NV_E4M3);
-                const float2 hf = __half22float2(*reinterpret_cast<const __half2*>(&hr));
-                const __nv_fp8x2_storage_t lb = __nv_cvt_float2_to_fp8x2(make_float2(f0 - hf.x, f1 - hf.y), __NV_SATFINITE, __NV_E4M3);
-                hi[i >> 1] |= (uint32_t)hb << (16 * (i & 1));
-                lo[i >> 1] |= (uint32_t)lb << (16 * (i & 1));
-            }
-            uint8_t* d = dst + at * 128 + (((sub >> 1) ^ (at & 7)) << 4) + (sub & 1) * 8;
-            *reinterpret_cast<uint2*>(d) = make_uint2(hi[0], hi[1]);
-            *reinterpret_cast<uint2*>(d + kQPlane) = make_uint2(lo[0], lo[1]);
-            // infinite or NaN: saturation would hide it; a row of NaN
-            float back = top == 0x7F800000u ? __uint_as_float(0x7FC00000u) : __uint_as_float((uint32_t)(ex - 7) << 23);
-            back = __shfl_sync(0xffffffffu, back, (lane & 1) * 16);
-            if (lane >> 1 == (r0 >> 1) + j) mine = back;
-        }
+    for (int k = 0; k < 64; k += 2) {
+        const float a = __uint_as_float(s[k]), b = __uint_as_float(s[k + 1]);
+        const float p0 = ex2(fmaf(a, scale, shift)), p1 = ex2(fmaf(b, scale, shift));
+        m2[(k >> 1) & 1] = max3(m2[(k >> 1) & 1], a, b);
+        l4[k & 2] += p0;
+        l4[(k & 2) + 1] += p1;
+        w[k >> 1] = pack_half(p0, p1);
     }
-    return mine;
+    *mx = fmaxf(m2[0], m2[1]);
+    return (l4[0] + l4[1]) + (l4[2] + l4[3]);
 }
 
 // The CTA's current item, as every role walks it.
 struct Item {
     Entry en;
     int head, row0, rows;  // first row, rows of the item (at most 256)
-    int b0, blocks;        // first block of 128 keys, blocks to compute (those no row sees are left out)
-    bool split;            // both streams have the same rows and take alternate blocks
+    int b0, blocks;        // first page, pages to compute (those no row sees are left out)
+    bool split;            // both streams have the same rows and take alternate pages
     uint32_t seg, span;    // segment number; units of the list that this covers
+    int image;             // its first row in the query image
     // stream st takes blocks first(st), first(st) + step, ...
     __device__ __forceinline__ int first(int st) const { return split ? st : 0; }
     __device__ __forceinline__ int step() const { return split ? 2 : 1; }
     __device__ __forceinline__ int count(int st) const { return split ? (blocks - st + 1) / 2 : blocks; }
+    __device__ __forceinline__ bool join() const { return split && blocks > 1; }  // both streams have a part of the same rows
 };
 __device__ __forceinline__ Item item_at(const mono_prefix_attn_args& a, const uint32_t* off, const uint32_t* item, uint32_t u, uint32_t u1) {
     Item it;
@@ -260,8 +211,9 @@ __device__ __forceinline__ Item item_at(const mono_prefix_attn_args& a, const ui
     it.span = min((uint32_t)((tile == w.tiles - 1 ? w.last : w.units) - unit), u1 - u);
     it.b0 = it.split ? 2 * unit : unit;
     const int seen = max(row_limit(it.en, it.row0 + it.rows - 1, G), 0);
-    it.blocks = max(0, min((int)it.span * it.step(), (seen + kKeys - 1) / kKeys - it.b0));
+    it.blocks = max(0, min((int)it.span * it.step(), (seen + kPage - 1) / kPage - it.b0));
     it.seg = blockIdx.x + it.head * item[E] + item[at.e] + tile;
+    it.image = (it.head * a.tokens + it.en.tok0) * G + it.row0;
     return it;
 }
 
@@ -276,7 +228,7 @@ __global__ void __launch_bounds__(kThreadsWide, 1) prefix_wide_kernel(const __gr
     uint32_t* off = reinterpret_cast<uint32_t*>(wbuf + kWStages * kWTile);
     uint32_t* item = off + E + 1;
     __shared__ uint64_t k_full[kKStages], k_empty[kKStages], v_full[kVStages], v_empty[kVStages], w_full[kWStages], w_empty[kWStages];
-    __shared__ uint64_t q_full[2], s_full[2], p_full[2], o_full[2], j_free, j_full, j_done;
+    __shared__ uint64_t q_full[2], q_free[2], s_full[2], s_free[2], p_full[2][2], o_done[2], j_free, j_full, j_done;
     __shared__ float s_join[2][128];  // stream 1's maxima and sums
     __shared__ int page_ok[kOkRing];
     __shared__ uint32_t red[64], tmem_base_s;
@@ -285,16 +237,17 @@ __global__ void __launch_bounds__(kThreadsWide, 1) prefix_wide_kernel(const __gr
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
         abort_flag = 0;
-        for (int i = 0; i < kKStages; ++i) { mbar_init(&k_full[i], 1); mbar_init(&k_empty[i], 1); }
+        for (int i = 0; i < kKStages; ++i) { mbar_init(&k_full[i], 1); mbar_init(&k_empty[i], 2); }
         for (int i = 0; i < kVStages; ++i) { mbar_init(&v_full[i], 1); mbar_init(&v_empty[i], 4); }
-        for (int i = 0; i < kWStages; ++i) { mbar_init(&w_full[i], 128); mbar_init(&w_empty[i], 1); }
-        for (int i = 0; i < 2; ++i) { mbar_init(&q_full[i], 128); mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 128); mbar_init(&o_full[i], 1); }
+        for (int i = 0; i < kWStages; ++i) { mbar_init(&w_full[i], 128); mbar_init(&w_empty[i], 2); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&q_full[i], 1); mbar_init(&q_free[i], 1); mbar_init(&s_full[i], 1); mbar_init(&s_free[i], 4); mbar_init(&p_full[0][i], 4); mbar_init(&p_full[1][i], 4); mbar_init(&o_done[i], 1); }
         mbar_init(&j_free, 128);
         mbar_init(&j_full, 128);
         mbar_init(&j_done, 128);
         mbar_fence_init();
         prefetch_tmap(&p.kmap);
         prefetch_tmap(&p.vmap);
+        prefetch_tmap(&p.qmap);
     }
     if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_s)), "r"(kTmemCols) : "memory");
@@ -316,34 +269,48 @@ __global__ void __launch_bounds__(kThreadsWide, 1) prefix_wide_kernel(const __gr
     if (warp >= kTmaWarp) {
         regs_down<kRegsFetch>();
         if (u0 < u1 && warp == kTmaWarp) {
-            // ---- fetch: lane l looks up the two pages of a batch's block l; lane 0 requests them in order
+            // ---- fetch: lane l looks up the page of a batch's block l; lane 0 requests them in order
             int it = 0;
+            uint32_t fph[2] = {0, 0}, jph = 0;
+            bool joined = false, used[2] = {false, false};  // how the item before used the query buffers
             for (uint32_t u = u0; u < u1 && !*abortp;) {
                 const Item x = item_at(a, off, item, u, u1);
-                const int pages = (x.en.len + kPage - 1) / kPage;
-                for (int b = 0; b < x.blocks && !*abortp; b += 32) {
-                    int pg[2] = {-1, -1};
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const int at = (x.b0 + min(b + lane, x.blocks - 1)) * 2 + h;
-                        if (at < pages) pg[h] = x.en.table[at];
-                        if (pg[h] >= a.n_pages) pg[h] = -1;
+                if (lane == 0) {
+                    // the streams' queries, once the last item's scores are made, or its parts joined in the same place
+                    if (joined) {
+                        wait_on(&j_done, jph, abortp, wait_ns);
+                        jph ^= 1;
                     }
+                    for (int st = 0; st < 2; ++st) {
+                        if (used[st]) {
+                            wait_on(&q_free[st], fph[st], abortp, wait_ns);
+                            fph[st] ^= 1;
+                        }
+                        used[st] = x.count(st) > 0;
+                        if (!used[st] || *abortp) continue;
+                        mbar_expect_tx(&q_full[st], 2 * kQPlane);
+                        for (int pl = 0; pl < 2; ++pl)
+                            tma_load_3d(qbuf + (st * 2 + pl) * kQPlane, &p.qmap, 0, x.image + (x.split ? 0 : st * 128), pl, &q_full[st]);
+                    }
+                    joined = x.join();
+                }
+                __syncwarp();
+                for (int b = 0; b < x.blocks && !*abortp; b += 32) {
+                    int page = x.en.table[x.b0 + min(b + lane, x.blocks - 1)];
+                    if (page >= a.n_pages) page = -1;
                     const int cnt = min(32, x.blocks - b);
                     for (int j = 0; j < cnt; ++j, ++it) {
-                        const int g0 = __shfl_sync(0xffffffffu, pg[0], j), g1 = __shfl_sync(0xffffffffu, pg[1], j);
+                        const int g = __shfl_sync(0xffffffffu, page, j);
                         if (lane == 0 && !*abortp) {
                             const int ks = it % kKStages, vs = it % kVStages;
-                            const uint32_t bytes = (g0 >= 0 ? kPage * 128 : 0) + (g1 >= 0 ? kPage * 128 : 0);
+                            const uint32_t bytes = g >= 0 ? kPage * 128 : 0;
                             if (it < kKStages || wait_on(&k_empty[ks], ((it / kKStages) - 1) & 1, abortp, wait_ns)) {
-                                page_ok[it % kOkRing] = (g0 >= 0 ? 1 : 0) | (g1 >= 0 ? 2 : 0);
+                                page_ok[it % kOkRing] = g >= 0;
                                 mbar_expect_tx(&k_full[ks], bytes);
-                                if (g0 >= 0) tma_load_3d(kbuf + ks * kKTile, &p.kmap, x.head * kDim, g0 * kPage, 0, &k_full[ks]);
-                                if (g1 >= 0) tma_load_3d(kbuf + ks * kKTile + kPage * 128, &p.kmap, x.head * kDim, g1 * kPage, 0, &k_full[ks]);
+                                if (g >= 0) tma_load_3d(kbuf + ks * kKTile, &p.kmap, x.head * kDim, g * kPage, 0, &k_full[ks]);
                                 if (it < kVStages || wait_on(&v_empty[vs], ((it / kVStages) - 1) & 1, abortp, wait_ns)) {
                                     mbar_expect_tx(&v_full[vs], bytes);
-                                    if (g0 >= 0) tma_load_3d(vbuf + vs * kVTile, &p.vmap, x.head * kDim, g0 * kPage, 0, &v_full[vs]);
-                                    if (g1 >= 0) tma_load_3d(vbuf + vs * kVTile + kPage * 128, &p.vmap, x.head * kDim, g1 * kPage, 0, &v_full[vs]);
+                                    if (g >= 0) tma_load_3d(vbuf + vs * kVTile, &p.vmap, x.head * kDim, g * kPage, 0, &v_full[vs]);
                                 }
                             }
                         }
@@ -352,62 +319,62 @@ __global__ void __launch_bounds__(kThreadsWide, 1) prefix_wide_kernel(const __gr
                 }
                 u += x.span;
             }
-        } else if (u0 < u1 && warp == kMmaWarp) {
-            // ---- the products: per stream S, (softmax), O, in the order that lets the streams alternate.  The warp walks
-            // together and one elected lane issues, so that descriptors stay in uniform registers.
-            {
-                int it0 = 0;  // blocks before this item, over the CTA's life
-                uint32_t qph[2] = {0, 0}, pph[2] = {0, 0};
-                bool live = true;
-                for (uint32_t u = u0; u < u1 && live;) {
-                    const Item x = item_at(a, off, item, u, u1);
-                    auto scores = [&](int st, int t) -> bool {  // S of the stream's t-th unit
-                        const int i = it0 + x.first(st) + t * x.step(), ks = i % kKStages;
-                        if (t == 0) {
-                            if (!wait_on(&q_full[st], qph[st], abortp, wait_ns)) return false;
-                            qph[st] ^= 1;
+        } else if (u0 < u1 && warp < kMmaWarp + 2) {
+            // ---- the products of one stream.  The warp walks together and one elected lane issues, so that descriptors
+            // stay in uniform registers.  (Waits, commits and issue cost a warp some 0.6 us a block: one warp for both streams
+            // needed 1.5 us where the tensor core needs 0.7.)
+            const int st = warp - kMmaWarp;
+            int it0 = 0, g0 = 0;  // blocks before this item over the CTA's life, and of them this stream's
+            uint32_t qph = 0;
+            bool live = true;
+            const uint64_t qd = desc_sw128(smem_u32(qbuf + st * 2 * kQPlane), 0, 1024);
+            const uint32_t s_at = tmem + st * 128, o_at = tmem + 256 + st * 128;
+            for (uint32_t u = u0; u < u1 && live;) {
+                const Item x = item_at(a, off, item, u, u1);
+                const int count = x.count(st), step = x.step();
+                // A block's scores are asked for as soon as the softmax has the scores before in registers, ahead of that
+                // block's values.  One thread's products are done in order: when S of block t + 2 is there, P of block t
+                // has been used.
+                for (int t = -1; t < count && live; ++t) {
+                    if (t + 1 < count) {  // S = Q K^T of block t + 1
+                        const int i = it0 + x.first(st) + (t + 1) * step, ks = i % kKStages, g = g0 + t + 1;
+                        if (t < 0) {
+                            live = wait_on(&q_full[st], qph, abortp, wait_ns);
+                            qph ^= 1;
                         }
-                        if (!wait_on(&k_full[ks], (i / kKStages) & 1, abortp, wait_ns)) return false;
+                        live = live && wait_on(&k_full[ks], (i / kKStages) & 1, abortp, wait_ns) && (g == 0 || wait_on(&s_free[st], (g - 1) & 1, abortp, wait_ns));
+                        if (!live) break;
                         fence_after();
-                        const uint32_t q = smem_u32(qbuf + st * 2 * kQPlane), k = smem_u32(kbuf + ks * kKTile);
-                        const uint64_t kd = desc_sw128(k, 0, 1024), qd = desc_sw128(q, 0, 1024);
+                        const uint64_t kd = desc_sw128(smem_u32(kbuf + ks * kKTile), 0, 1024);
                         if (elect_one()) {
 #pragma unroll
-                            for (int s = 0; s < 8; ++s) mma_f8(tmem + st * 128, qd + (s >> 2) * (kQPlane / 16) + 2 * (s & 3), kd + 2 * (s & 3), kIdescS, s > 0);
+                            for (int s = 0; s < 8; ++s) mma_f8(s_at, qd + (s >> 2) * (kQPlane / 16) + 2 * (s & 3), kd + 2 * (s & 3), kIdescS, s > 0);
                             mma_commit(&s_full[st]);
-                            if (x.split || st == 1) mma_commit(&k_empty[ks]);
+                            mma_commit(&k_empty[ks]);  // two arrivals free a stage: one per stream, or both from the only stream that uses it
+                            if (x.split) mma_commit(&k_empty[ks]);
+                            if (t + 1 == count - 1) mma_commit(&q_free[st]);
                         }
                         __syncwarp();
-                        return true;
-                    };
-                    auto values = [&](int st, int t) -> bool {  // O += P V of the stream's t-th unit
-                        const int i = it0 + x.first(st) + t * x.step(), ws = i % kWStages;
-                        if (!wait_on(&w_full[ws], (i / kWStages) & 1, abortp, wait_ns)) return false;
-                        if (!wait_on(&p_full[st], pph[st], abortp, wait_ns)) return false;
-                        pph[st] ^= 1;
+                    }
+                    if (t >= 0) {  // O += P V of block t
+                        const int i = it0 + x.first(st) + t * step, ws = i % kWStages, g = g0 + t;
+                        live = wait_on(&w_full[ws], (i / kWStages) & 1, abortp, wait_ns) && wait_on(&p_full[st][g & 1], (g >> 1) & 1, abortp, wait_ns);
+                        if (!live) break;
                         fence_after();
-                        const uint64_t wd = desc_sw128(smem_u32(wbuf + ws * kWTile), kKeys * 128, 1024);
+                        const uint64_t wd = desc_sw128(smem_u32(wbuf + ws * kWTile), kPage * 128, 1024);
                         if (elect_one()) {
 #pragma unroll
-                            for (int s = 0; s < 8; ++s)
-                                mma_f16_ts(tmem + 256 + st * 128, tmem + st * 128 + s * 8, wd + s * (16 * 128 / 16), kIdescO, s > 0 || t > 0);
-                            if (x.split || st == 1) mma_commit(&w_empty[ws]);
-                            if (t == x.count(st) - 1) mma_commit(&o_full[st]);
+                            for (int s = 0; s < 4; ++s) mma_f16_ts(o_at, s_at + 64 + (g & 1) * 32 + s * 8, wd + s * (16 * 128 / 16), kIdescO, s > 0 || t > 0);
+                            mma_commit(&o_done[st]);
+                            mma_commit(&w_empty[ws]);
+                            if (x.split) mma_commit(&w_empty[ws]);
                         }
                         __syncwarp();
-                        return true;
-                    };
-                    for (int st = 0; st < 2 && live; ++st)
-                        if (x.count(st) > 0) live = scores(st, 0);
-                    for (int t = 0; t < x.count(0) && live; ++t)
-                        for (int st = 0; st < 2 && live; ++st) {
-                            if (t >= x.count(st)) continue;
-                            live = values(st, t);
-                            if (live && t + 1 < x.count(st)) live = scores(st, t + 1);
-                        }
-                    it0 += x.blocks;
-                    u += x.span;
+                    }
                 }
+                g0 += count;
+                it0 += x.blocks;
+                u += x.span;
             }
         }
     } else if (warp >= kConvWarp0) {
@@ -426,15 +393,24 @@ __global__ void __launch_bounds__(kThreadsWide, 1) prefix_wide_kernel(const __gr
                            (it < kWStages || wait_on(&w_empty[ws], ((it / kWStages) - 1) & 1, abortp, wait_ns));
                     if (!live) break;
                     const uint32_t src = smem_u32(vbuf + vs * kVTile), dst = smem_u32(wbuf + ws * kWTile);
-                    const int have = x.en.len - (x.b0 + i) * kKeys, ok = page_ok[it % kOkRing];
-#pragma unroll 2
-                    for (int j = 0; j < 8; ++j) {
-                        const int key = (ct & 7) + 8 * j + 64 * (ct >> 6), c16 = (ct >> 3) & 7;  // eight lanes: eight keys, no bank twice
-                        uint4 v = lds128(src + key * 128 + ((c16 ^ (key & 7)) << 4));
-                        if (key >= have || !(ok >> (key >> 6) & 1)) v = make_uint4(0, 0, 0, 0);
-                        const uint32_t at = dst + (c16 >> 2) * (kKeys * 128) + key * 128, c = (c16 & 3) * 2;
-                        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at + ((c ^ (key & 7)) << 4)), "r"(widen2(v.x)), "r"(widen2(v.x >> 16)), "r"(widen2(v.y)), "r"(widen2(v.y >> 16)) : "memory");
-                        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at + (((c + 1) ^ (key & 7)) << 4)), "r"(widen2(v.z)), "r"(widen2(v.z >> 16)), "r"(widen2(v.w)), "r"(widen2(v.w >> 16)) : "memory");
+                    const int have = page_ok[it % kOkRing] ? x.en.len - (x.b0 + i) * kPage : 0;
+                    uint4 v[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {  // eight lanes: eight keys, no bank twice
+                        const int key = (ct & 7) + 8 * j + 32 * (ct >> 6), c16 = (ct >> 3) & 7;
+                        v[j] = lds128(src + key * 128 + ((c16 ^ (key & 7)) << 4));
+                    }
+                    if (have < kPage) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            if ((ct & 7) + 8 * j + 32 * (ct >> 6) >= have) v[j] = make_uint4(0, 0, 0, 0);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int key = (ct & 7) + 8 * j + 32 * (ct >> 6), c16 = (ct >> 3) & 7;
+                        const uint32_t at = dst + (c16 >> 2) * (kPage * 128) + key * 128, c = (c16 & 3) * 2;
+                        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at + ((c ^ (key & 7)) << 4)), "r"(widen2(v[j].x)), "r"(widen2(v[j].x >> 16)), "r"(widen2(v[j].y)), "r"(widen2(v[j].y >> 16)) : "memory");
+                        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at + (((c + 1) ^ (key & 7)) << 4)), "r"(widen2(v[j].z)), "r"(widen2(v[j].z >> 16)), "r"(widen2(v[j].w)), "r"(widen2(v[j].w >> 16)) : "memory");
                     }
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     mbar_arrive(&w_full[ws]);
@@ -452,86 +428,104 @@ __global__ void __launch_bounds__(kThreadsWide, 1) prefix_wide_kernel(const __gr
             const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
             const uint32_t s_addr = tmem + lanes + st * 128, o_addr = tmem + lanes + 256 + st * 128;
             float* joint = reinterpret_cast<float*>(qbuf);  // [32 x 4 dims][128 rows] of stream 1, once a split item's queries are done with
-            int it0 = 0;
-            uint32_t sph = 0, oph = 0, jph = 0;
+            int it0 = 0, g0 = 0;  // blocks before this item over the CTA's life, and of them this stream's
+            uint32_t jph = 0;
             bool live = true;
             for (uint32_t u = u0; u < u1 && live;) {
                 const Item x = item_at(a, off, item, u, u1);
                 const int row = x.row0 + (x.split ? row_in : st * 128 + row_in);
                 const bool mine = row < x.row0 + x.rows;
                 const int count = x.count(st);
-                const bool join = x.split && x.count(1) > 0;  // stream 0 takes stream 1's part into its own
+                const bool join = x.join();  // stream 0 takes stream 1's part into its own
                 float m = -INFINITY, l = 0.f;
                 if (count > 0) {
-                    const int w0 = (warp & 3) * 32;  // this warp's rows
-                    const float qs = write_queries(a, x.en, x.head, G, x.row0 + (x.split ? 0 : st * 128) + w0, x.row0 + x.rows, qbuf + st * 2 * kQPlane + w0 * 128) *
-                                     (a.sm_scale * a.k_scale * 1.4426950408889634f);
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    mbar_arrive(&q_full[st]);
-                    MONO_TL(tl_wide, 3);
+                    const float qs = mine ? __ldg(p.s.q_scale + x.image + row - x.row0) * (a.sm_scale * a.k_scale * 1.4426950408889634f) : 1.f;
                     const int lim = mine ? row_limit(x.en, row, G) : 0;
                     for (int t = 0; t < count; ++t) {
-                        const int i = x.first(st) + t * x.step();
-                        live = wait_on(&s_full[st], sph, abortp, wait_ns);
+                        const int i = x.first(st) + t * x.step(), g = g0 + t;
+                        live = wait_on(&s_full[st], g & 1, abortp, wait_ns);
                         if (!live) break;
-                        sph ^= 1;
                         fence_after();
                         MONO_TL(tl_wide, 4 + 3 * t);  // the first three blocks
-                        // keys of the block that this row sees, of the pages that exist
-                        const int vis = lim - (x.b0 + i) * kKeys, ok = page_ok[(it0 + i) % kOkRing];
-                        const bool masked = !__all_sync(0xffffffffu, vis >= kKeys) || ok != 3;
-                        const float mx = (masked ? block_max<true>(s_addr, vis, ok) : block_max<false>(s_addr, vis, ok)) * qs;
-                        MONO_TL(tl_wide, 5 + 3 * t);
-                        // raise the reference where it must be, and O with it
+                        // how many of the block's keys this row sees
+                        const int vis = page_ok[(it0 + i) % kOkRing] ? lim - (x.b0 + i) * kPage : 0;
+                        uint32_t s[64];
+                        tmem_ld32(s_addr, s);
+                        tmem_ld32(s_addr + 32, s + 32);
+                        wait_ld();
+                        fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&s_free[st]);
+                        if (!__all_sync(0xffffffffu, vis >= kPage)) {
+#pragma unroll
+                            for (int k = 0; k < 64; ++k)
+                                if (k >= vis) s[k] = 0xFF800000u;
+                        }
+                        // Weights by the reference as it is, and beside them the block's maximum (which so costs no time of
+                        // its own); where it passes the reference too far, the reference is raised, O with it, and the
+                        // weights are made again.
+                        uint32_t w[32];
+                        float mx, sum = weights(s, qs, kBias - (m == -INFINITY ? 0.f : m), w, &mx);
+                        mx *= qs;
                         float up = 1.f;
                         if (mx > m + kLazy || (m == -INFINITY && mx > m)) {
                             up = m == -INFINITY ? 0.f : ex2(m - mx);
                             m = mx;
                         }
-                        if (t > 0 && __any_sync(0xffffffffu, up != 1.f)) {
+                        MONO_TL(tl_wide, 5 + 3 * t);
+                        if (__any_sync(0xffffffffu, up != 1.f)) {
                             l *= up;
+                            if (t > 0) {
+                                live = wait_on(&o_done[st], (g - 1) & 1, abortp, wait_ns);  // the block before is in O
+                                if (!live) break;
+                                fence_after();
 #pragma unroll 1
-                            for (int c = 0; c < 8; ++c) {
-                                uint32_t r16[16];
-                                tmem_ld16(o_addr + c * 16, r16);
-                                wait_ld();
+                                for (int c = 0; c < 8; ++c) {
+                                    uint32_t r16[16];
+                                    tmem_ld16(o_addr + c * 16, r16);
+                                    wait_ld();
 #pragma unroll
-                                for (int q = 0; q < 16; ++q) r16[q] = __float_as_uint(__uint_as_float(r16[q]) * up);
-                                tmem_st16(o_addr + c * 16, r16);
+                                    for (int q = 0; q < 16; ++q) r16[q] = __float_as_uint(__uint_as_float(r16[q]) * up);
+                                    tmem_st16(o_addr + c * 16, r16);
+                                }
                             }
+                            sum = weights(s, qs, kBias - (m == -INFINITY ? 0.f : m), w, &mx);
                         }
-                        const float shift = kBias - (m == -INFINITY ? 0.f : m);
-                        l += masked ? block_weights<true>(s_addr, vis, ok, qs, shift) : block_weights<false>(s_addr, vis, ok, qs, shift);
+                        tmem_st16(s_addr + 64 + (g & 1) * 32, w);
+                        tmem_st16(s_addr + 64 + (g & 1) * 32 + 16, w + 16);
+                        l += sum;
                         wait_st();
                         fence_before();
-                        mbar_arrive(&p_full[st]);
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&p_full[st][g & 1]);
                         MONO_TL(tl_wide, 6 + 3 * t);
                     }
                     if (!live) break;
-                    live = wait_on(&o_full[st], oph, abortp, wait_ns);
+                    g0 += count;
+                    live = wait_on(&o_done[st], (g0 - 1) & 1, abortp, wait_ns);
                     MONO_TL(tl_wide, 13);
                     if (!live) break;
-                    oph ^= 1;
                     fence_after();
                 }
                 // ---- the segment's row; an item without blocks leaves an empty part
                 float f0 = 1.f, f1 = 0.f;
                 if (join) {
                     if (st == 1) {
-                        // the other stream's queries are done with too: its last scores come before its part is asked for
+                        // the other stream's queries are done with too, and no thread of it still reads the item before's
                         live = wait_on(&j_free, jph, abortp, wait_ns);
                         if (!live) break;
                         s_join[0][row_in] = m;
                         s_join[1][row_in] = l;
 #pragma unroll 1
-                        for (int c = 0; c < 8; ++c) {
-                            uint32_t r16[16];
-                            tmem_ld16(o_addr + c * 16, r16);
+                        for (int c = 0; c < 4; ++c) {
+                            uint32_t r32[32];
+                            tmem_ld32(o_addr + c * 32, r32);
                             wait_ld();
 #pragma unroll
-                            for (int q = 0; q < 16; q += 4)
-                                *reinterpret_cast<uint4*>(joint + ((c * 4 + q / 4) * 128 + row_in) * 4) = make_uint4(r16[q], r16[q + 1], r16[q + 2], r16[q + 3]);
+                            for (int q = 0; q < 32; q += 4)
+                                *reinterpret_cast<uint4*>(joint + ((c * 8 + q / 4) * 128 + row_in) * 4) = make_uint4(r32[q], r32[q + 1], r32[q + 2], r32[q + 3]);
                         }
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // queries come here again
                         mbar_arrive(&j_full);
                     } else {
                         mbar_arrive(&j_free);
@@ -553,35 +547,34 @@ __global__ void __launch_bounds__(kThreadsWide, 1) prefix_wide_kernel(const __gr
                     }
                     float* dst = seg + 2 * Shape<true>::kTile + at * 4;  // [32 x 4 dims][256 rows][4]
 #pragma unroll 1
-                    for (int c = 0; c < 8; ++c) {
-                        uint32_t r16[16];
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t r32[32];
                         if (count > 0) {
-                            tmem_ld16(o_addr + c * 16, r16);
+                            tmem_ld32(o_addr + c * 32, r32);
                             wait_ld();
                         } else {
 #pragma unroll
-                            for (int q = 0; q < 16; ++q) r16[q] = 0;
+                            for (int q = 0; q < 32; ++q) r32[q] = 0;
                         }
                         if (join) {
 #pragma unroll
-                            for (int q = 0; q < 16; q += 4) {
-                                const float4 o = *reinterpret_cast<const float4*>(joint + ((c * 4 + q / 4) * 128 + row_in) * 4);
+                            for (int q = 0; q < 32; q += 4) {
+                                const float4 o = *reinterpret_cast<const float4*>(joint + ((c * 8 + q / 4) * 128 + row_in) * 4);
                                 const float ov[4] = {o.x, o.y, o.z, o.w};
 #pragma unroll
-                                for (int k = 0; k < 4; ++k) r16[q + k] = __float_as_uint(__uint_as_float(r16[q + k]) * f0 + ov[k] * f1);
+                                for (int k = 0; k < 4; ++k) r32[q + k] = __float_as_uint(__uint_as_float(r32[q + k]) * f0 + ov[k] * f1);
                             }
                         }
                         if (mine) {
 #pragma unroll
-                            for (int q = 0; q < 16; q += 4)
-                                *reinterpret_cast<uint4*>(dst + (c * 4 + q / 4) * (Shape<true>::kTile * 4)) = make_uint4(r16[q], r16[q + 1], r16[q + 2], r16[q + 3]);
+                            for (int q = 0; q < 32; q += 4)
+                                *reinterpret_cast<uint4*>(dst + (c * 8 + q / 4) * (Shape<true>::kTile * 4)) = make_uint4(r32[q], r32[q + 1], r32[q + 2], r32[q + 3]);
                         }
                     }
                 }
                 fence_before();
-                if (join) {  // the next item's queries overwrite what stream 0 reads here
+                if (join) {  // the next item's queries overwrite what stream 0 has read here
                     if (st == 0) mbar_arrive(&j_done);
-                    live = wait_on(&j_done, jph, abortp, wait_ns);
                     jph ^= 1;
                 }
                 MONO_TL(tl_wide, 14);
@@ -612,6 +605,9 @@ cudaError_t launch_wide(const Params& p, int ctas, cudaStream_t st) {
         if (e != cudaSuccess) return e;
         attr_done(attr_once);
     }
+    const unsigned rows = (unsigned)p.a.tokens * p.a.q_heads;
+    const cudaError_t e = launch_k(prefix_split_kernel, (rows + 15) / 16, 256, 0, st, p.a, p.s.q_image, p.s.q_scale);
+    if (e != cudaSuccess) return e;
     return launch_k(prefix_wide_kernel, ctas, kThreadsWide, kSmemFixed + 2 * (size_t)(p.a.seqs + p.a.groups + 1) * 4, st, p);
 }
 

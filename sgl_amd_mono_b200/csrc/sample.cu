@@ -37,6 +37,7 @@ constexpr int kPerThread = kBins / kThreads;
 constexpr double kOne = 17592186044416.0;  // 2^44
 constexpr float kSteps = kBins / 44.001f;  // histogram steps per factor of two: weights down to 2^-44
 typedef unsigned long long u64;
+MONO_TL_DECLARE(tl_sample)
 
 // Order-preserving image of a logit (NaN has been taken to -inf).
 __device__ __forceinline__ uint32_t key_of(float x) {
@@ -44,15 +45,20 @@ __device__ __forceinline__ uint32_t key_of(float x) {
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float logit_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7FFFFFFFu : ~key); }
+// The logit f for which x <= f says key_of(x) <= key.  One key has no logit, that of -0, and -0 compares as 0 does.
+__device__ __forceinline__ float below_or_at(uint32_t key) { return logit_of(key == 0x7FFFFFFFu ? key - 1 : key); }
 constexpr uint32_t kKeyNegInf = 0x007FFFFFu;
 
+constexpr int kTable = 256;
+constexpr double kTwo52 = 4503599627370496.0;
+
 struct Row {
-    float mx;          // largest logit
-    float c;           // log2(e) / T, f32: for histogram steps only
-    double c64;        // the same
-    u64 k;             // rank below this
-    u64 floor_w;       // weight at least this
-    const double* tab; // 2^(i / 16)
+    float mx;           // largest logit
+    float c;            // log2(e) / T, f32: for histogram steps only
+    double mx64, c64;   // the same, f64
+    u64 k;              // rank below this
+    u64 floor_w;        // weight at least this
+    const double* tab;  // 2^(i / 256)
 };
 
 // f32 -> f64 by bits (conversions between the two run at a quarter of the rate of the arithmetic): normal numbers; a
@@ -62,31 +68,27 @@ __device__ __forceinline__ double widen(float x) {
     return __hiloint2double((int)((b & 0x80000000u) | (((b & 0x7FFFFFFFu) >> 3) + 0x38000000u)), (int)(b << 29));
 }
 
-// round(2^44 exp((x - mx) / T)).  y = (x - mx) log2(e) / T = n + i / 16 + r, 0 <= i < 16, |r| <= 1/32:
-// 2^y = 2^n 2^(i/16) exp(r ln 2), the last by its Taylor series (r ln 2 <= 0.0217: the seventh power's term is below
-// 2^-51), all in f64; then the mantissa is shifted to its place.
-__device__ __forceinline__ u64 weight_of(float x, const Row& r) {
-    if (x == r.mx) return (u64)kOne;
-    const double y = (widen(x) - widen(r.mx)) * r.c64;
-    if (!(y > -45.0) || x == -INFINITY) return 0;
-    const double shifted = y * 16.0 + 6755399441055744.0;  // 2^52 + 2^51: the low word holds round(16 y)
+// round(2^44 exp((x - mx) / T)), an f64 whole number.  y = (x - mx) log2(e) / T = n + i / 256 + r, 0 <= i < 256, |r| <= 1/512:
+// 2^y = 2^n 2^(i/256) 2^r, the last by its series in r ln 2 (at most 0.00136: the fifth power's term is below 2^-54).
+__device__ __forceinline__ double weight_f64(float x, const Row& r) {
+    const double y = (widen(x) - r.mx64) * r.c64;
+    const double shifted = fma(y, 256.0, 6755399441055744.0);  // + 2^52 + 2^51: the low word holds round(256 y)
     const int q = __double2loint(shifted);
-    const double t = fma(shifted - 6755399441055744.0, -0.0625, y) * 0.69314718055994530942;
-    double e = fma(t, 1.0 / 720, 1.0 / 120);
-    e = fma(t, e, 1.0 / 24);
-    e = fma(t, e, 1.0 / 6);
-    e = fma(t, e, 0.5);
+    const double t = fma(shifted - 6755399441055744.0, -1.0 / 256, y);
+    constexpr double L = 0.69314718055994530942;
+    double e = fma(t, L * L * L * L / 24, L * L * L / 6);
+    e = fma(t, e, L * L / 2);
+    e = fma(t, e, L);
     e = fma(t, e, 1.0);
-    e = fma(t, e, 1.0);
-    e *= r.tab[q & 15];                       // in (0.97, 2.0)
-    const double v = e + 1.0;                 // exponent 0 or 1: e + 1 in (1.97, 3.0); 51 bits below the point at least
-    const u64 m = (u64)__double_as_longlong(v);
-    // v = (2^52 + frac) 2^(E - 52), so 2^52 e = ((2^52 + frac) << E) - 2^52
-    const int E = (int)(m >> 52) - 1023;
-    const u64 fix = (((m & 0xFFFFFFFFFFFFFull) | 0x10000000000000ull) << E) - 0x10000000000000ull;
-    const int sh = 8 - (q >> 4);  // 2^52 e 2^n / 2^8
-    return sh > 62 ? 0 : (fix + (1ull << (sh - 1))) >> sh;
+    e *= r.tab[q & 255];
+    e = __hiloint2double(__double2hiint(e) + ((q >> 8) + 44) * (1 << 20), __double2loint(e));  // times 2^(n + 44)
+    e = (e + kTwo52) - kTwo52;                                                                  // to a whole number
+    // weights below 2^-45 are 0 (there the exponent above may have left its range), and so is that of -inf
+    e = y > -45.0 && x != -INFINITY ? e : 0.0;
+    return x == r.mx ? kOne : e;
 }
+__device__ __forceinline__ u64 whole(double w) { return (u64)__double_as_longlong(w + kTwo52) & 0xFFFFFFFFFFFFFull; }  // below 2^52
+__device__ __forceinline__ u64 weight_of(float x, const Row& r) { return whole(weight_f64(x, r)); }
 // floor(u W) for 0 <= u < 1
 __device__ __forceinline__ u64 share_of(float u, u64 W) {
     const int e = (int)((__float_as_uint(u) >> 23) & 0xFF);
@@ -104,6 +106,15 @@ __device__ __forceinline__ u64 warp_sum_u64(u64 v) {
     return v;
 }
 
+// two words of CTA `rank`'s shared memory, at the place of `p` in this one's
+__device__ __forceinline__ uint2 ld_peer(const uint32_t* p, int rank) {
+    uint2 v;
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
+    return v;
+}
+
 struct Hist {
     uint32_t n[2][kBins], lo[2][kBins], hi[2][kBins];  // counts, and masses in two words; two sets, used in turn
 };
@@ -116,6 +127,12 @@ __device__ __forceinline__ void hist_add(Hist& h, int set, int bin, uint32_t n, 
 }
 
 // Sums of the threads before this one (exclusive), and all threads' bins are in thread order.
+// (step_of: the histogram step of a weight above 0.  Rounding to the nearest whole number by adding 2^23 + 2^22 keeps the
+// order of the logits and is within 2^-22 of the true step.)
+__device__ __forceinline__ int step_of(float x, const Row& r) {
+    const float at = x == r.mx ? 0.f : fmaf((r.mx - x) * r.c, kSteps, -0.5f);
+    return min(max(__float_as_int(fminf(at, 2000.f) + 12582912.f) - 0x4B400000, 0), kBins - 1);
+}
 template <typename A>
 __device__ __forceinline__ A block_before(A v, A* red) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -141,14 +158,16 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 2) sam
     __shared__ uint32_t s_wties[kWarps], red32[kWarps], s_key[kCtas], s_num[kCtas], s_cnt[2];
     __shared__ float redf[2][kWarps];
     __shared__ int s_bin[2];
-    __shared__ double s_tab[16];
+    __shared__ double s_tab[kTable];
     cg::cluster_group cluster = cg::this_cluster();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, row = blockIdx.x / kCtas, V = a.vocab;
     const int rank = (int)cluster.block_rank();
-    if (tid < 16) s_tab[tid] = exp2(tid / 16.0);
+    if (tid < kTable) s_tab[tid] = exp2(tid / (double)kTable);
     for (int i = tid; i < kBins; i += kThreads) h.n[0][i] = 0;
     if (tid == 0) { s_bin[0] = kBins; s_bin[1] = kBins; }
+    MONO_TL(tl_sample, 0);
     pdl_prologue();
+    MONO_TL(tl_sample, 1);
     const int first = min(rank * slice, V), count = min(slice, V - first);  // this CTA's tokens
     const T* x = reinterpret_cast<const T*>(a.logits) + (size_t)row * a.ld + first;
     const float temp = a.temperature ? a.temperature[row] : 1.f;
@@ -188,6 +207,7 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 2) sam
         }
         for (int i = vecs * N + tid; i < slice; i += kThreads) put(i, i < count ? (float)x[i] : -INFINITY);
     }
+    MONO_TL(tl_sample, 2);
     kmax = __reduce_max_sync(0xffffffffu, kmax);
     if (lane == 0) red32[warp] = kmax;
     __syncthreads();
@@ -196,6 +216,7 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 2) sam
         *cluster.map_shared_rank(&s_key[rank], tid) = kmax;
     }
     cluster.sync();
+    MONO_TL(tl_sample, 3);
     kmax = 0;
     for (int i = 0; i < kCtas; ++i) kmax = max(kmax, s_key[i]);
     if (kmax <= kKeyNegInf) {  // no logit above -inf: all CTAs of the row leave
@@ -212,6 +233,7 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 2) sam
     // temperatures below 2^-100 tell no more logits apart than 2^-100 does; beside an infinite logit nothing has weight
     r.c64 = r.mx == INFINITY ? 1e30 : greedy ? 1.4426950408889634 : 1.4426950408889634 / fmax((double)temp, 7.888609052210118e-31);
     r.c = (float)r.c64;
+    r.mx64 = widen(r.mx);
     r.k = greedy ? 1ull : tk < 1 || tk > V ? (u64)V : (u64)tk;
     const double p = !greedy && tp < 1.f ? fmax((double)tp, 0.0) : 1.0;
     r.floor_w = !greedy && mp > 0.f ? (u64)ceil((double)fminf(mp, 1.f) * kOne) : 0ull;
@@ -219,30 +241,31 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 2) sam
     // ---- Z, and the histogram of counts over steps of log2 w
     const int i0 = min(warp * run, slice), i1 = min(i0 + run, slice);
     {
-        u64 z = 0;
+        // whole numbers up to 2^44 add exactly in f64 to 2^53: a thread has at most 96
+        double zd = 0.0;
         for (int i = i0 + lane * 4; i < i1; i += 128) {
             const float4 v4 = *reinterpret_cast<const float4*>(xs + i);
             const float v[4] = {v4.x, v4.y, v4.z, v4.w};
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const u64 w = weight_of(v[j], r);
-                z += w;
-                if (filtered && w) {
-                    const float y = v[j] == r.mx ? 0.f : (r.mx - v[j]) * r.c;
-                    atomicAdd(&h.n[0][min((int)(y * kSteps), kBins - 1)], 1u);
-                }
+                const double w = weight_f64(v[j], r);
+                zd += w;
+                if (filtered && w > 0.0) atomicAdd(&h.n[0][step_of(v[j], r)], 1u);
             }
         }
+        u64 z = whole(zd);
         z = warp_sum_u64(z);
         if (lane == 0) s_wsum[warp] = z;
     }
     __syncthreads();
+    MONO_TL(tl_sample, 4);
     if (tid < kCtas) {
         u64 z = 0;
         for (int i = 0; i < kWarps; ++i) z += s_wsum[i];
         *cluster.map_shared_rank(&s_z[rank], tid) = z;
     }
     cluster.sync();
+    MONO_TL(tl_sample, 5);
     u64 Z = 0;
     for (int i = 0; i < kCtas; ++i) Z += s_z[i];
     // kept: keys above khi; of the keys klo .. khi (one key, or one token) the first `ties` of `tied`
@@ -255,11 +278,11 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 2) sam
         // ---- bounds of the border among the steps
         {
             uint32_t n[kPerThread] = {};
-            for (int c = 0; c < kCtas; ++c) {
-                const uint2 v = *reinterpret_cast<const uint2*>(cluster.map_shared_rank(&h.n[0][tid * kPerThread], c));
-                n[0] += v.x;
-                n[1] += v.y;
-            }
+            uint2 v[kCtas];
+#pragma unroll
+            for (int c = 0; c < kCtas; ++c) v[c] = ld_peer(&h.n[0][tid * kPerThread], c);  // all in flight
+#pragma unroll
+            for (int c = 0; c < kCtas; ++c) { n[0] += v[c].x; n[1] += v[c].y; }
             static_assert(kPerThread == 2, "two bins per thread");
             // a step's weights lie in (2^-((b + 1) / kSteps), 2^-(b / kSteps)], in units of the largest
             float top[kPerThread + 1];
@@ -298,6 +321,7 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 2) sam
             klo = b1 < kBins - 1 && key_of(xl) > kKeyNegInf + 2u ? key_of(xl) - 2u : kKeyNegInf + 1u;
             u64 above = 0;
             uint32_t n_above = 0;
+            MONO_TL(tl_sample, 6);
             for (int level = 1;; ++level) {
                 const int set = level & 1;
                 const uint32_t width = khi - klo;
@@ -307,23 +331,24 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 2) sam
                 __syncthreads();
                 u64 m_ab = 0;
                 uint32_t n_ab = 0;
+                const float fhi = below_or_at(khi), flo = logit_of(klo);  // order as the keys do, and cost nothing to compare
                 for (int b = i0; b < i1; b += 128) {  // whole warps: the lanes vote
                     const int i = b + lane * 4;
                     const float4 v4 = i < i1 ? *reinterpret_cast<const float4*>(xs + i) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
                     const float v[4] = {v4.x, v4.y, v4.z, v4.w};
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const uint32_t k = key_of(v[j]);
-                        u64 w = 0;
-                        if (k >= klo && (k <= khi || level == 1)) w = weight_of(v[j], r);
-                        if (level == 1 && k > khi) {
+                        const bool some_here = v[j] >= flo && (v[j] <= fhi || level == 1);
+                        if (!__any_sync(0xffffffffu, some_here)) continue;
+                        u64 w = some_here ? weight_of(v[j], r) : 0;
+                        if (v[j] > fhi) {  // (on the first level) surely kept
                             m_ab += w;
                             n_ab += w != 0;
                             w = 0;
                         }
                         const unsigned in = __ballot_sync(0xffffffffu, w != 0);
                         if (in == 0) continue;
-                        const int bin = (int)((khi - k) >> sh), lead = __ffs(in) - 1;
+                        const int bin = (int)((khi - key_of(v[j])) >> sh), lead = __ffs(in) - 1;
                         const int lb = __shfl_sync(0xffffffffu, bin, lead);
                         if (__popc(in) > 4 && __all_sync(0xffffffffu, w == 0 || bin == lb)) {  // many equal logits: one addition for all
                             const u64 sum = warp_sum_u64(w);
@@ -348,18 +373,26 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 2) sam
                     *cluster.map_shared_rank(&s_num[rank], tid) = n;
                 }
                 cluster.sync();
+                MONO_TL(tl_sample, 5 + 2 * level);
                 if (level == 1)
                     for (int i = 0; i < kCtas; ++i) { above += s_part[i]; n_above += s_num[i]; }
                 uint32_t n[kPerThread] = {};
                 u64 m[kPerThread] = {};
-                for (int c = 0; c < kCtas; ++c) {
-                    const uint2 vn = *reinterpret_cast<const uint2*>(cluster.map_shared_rank(&h.n[set][tid * kPerThread], c));
-                    const uint2 vl = *reinterpret_cast<const uint2*>(cluster.map_shared_rank(&h.lo[set][tid * kPerThread], c));
-                    const uint2 vh = *reinterpret_cast<const uint2*>(cluster.map_shared_rank(&h.hi[set][tid * kPerThread], c));
-                    n[0] += vn.x;
-                    n[1] += vn.y;
-                    m[0] += ((u64)vh.x << 32) + vl.x;
-                    m[1] += ((u64)vh.y << 32) + vl.y;
+                {
+                    uint2 vn[kCtas], vl[kCtas], vh[kCtas];
+#pragma unroll
+                    for (int c = 0; c < kCtas; ++c) {  // all in flight
+                        vn[c] = ld_peer(&h.n[set][tid * kPerThread], c);
+                        vl[c] = ld_peer(&h.lo[set][tid * kPerThread], c);
+                        vh[c] = ld_peer(&h.hi[set][tid * kPerThread], c);
+                    }
+#pragma unroll
+                    for (int c = 0; c < kCtas; ++c) {
+                        n[0] += vn[c].x;
+                        n[1] += vn[c].y;
+                        m[0] += ((u64)vh[c].x << 32) + vl[c].x;
+                        m[1] += ((u64)vh[c].y << 32) + vl[c].y;
+                    }
                 }
                 uint32_t c = n_above + block_before<uint32_t>(n[0] + n[1], red32);
                 u64 mass = above + block_before<u64>(m[0] + m[1], red64);
@@ -378,6 +411,7 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 2) sam
                     const uint32_t low = top - klo < (1u << sh) ? klo : top - ((1u << sh) - 1);
                     if (c > r.k || mass >= limit || weight_of(logit_of(low), r) < r.floor_w) mine = j;
                 }
+                MONO_TL(tl_sample, 6 + 2 * level);
                 if (mine >= 0) atomicMin(&s_bin[set], tid * kPerThread + mine);
                 __syncthreads();
                 const int b = s_bin[set];
@@ -418,24 +452,26 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 2) sam
             }
         }
     }
+    MONO_TL(tl_sample, 13);
     if (!(u > 0.f)) u = 0.f;
     const u64 target = u >= 1.f ? kept - 1 : share_of(u, kept);
     // ---- the draw: every warp's run of kept mass; where only some of the tied tokens are kept, their number apart
     const bool some = !all && ties > 0 && ties < tied;
     if (!all && !some && ties == tied) khi = klo - 1;  // all of the tied are kept: so is every key from klo on
     if (!all) {
-        u64 m = 0;
+        double md = 0.0;
         uint32_t t = 0;
+        const float fhi = below_or_at(khi), flo = logit_of(klo);
         for (int i = i0 + lane * 4; i < i1; i += 128) {
             const float4 v4 = *reinterpret_cast<const float4*>(xs + i);
             const float v[4] = {v4.x, v4.y, v4.z, v4.w};
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const uint32_t k = key_of(v[j]);
-                if (k > khi) m += weight_of(v[j], r);
-                else if (some && k >= klo) ++t;
+                if (v[j] > fhi) md += weight_f64(v[j], r);
+                else if (some && v[j] >= flo) ++t;
             }
         }
+        u64 m = whole(md);
         m = warp_sum_u64(m);
         t = __reduce_add_sync(0xffffffffu, t);
         if (lane == 0) { s_wsum[warp] = m; s_wties[warp] = t; }
@@ -449,6 +485,7 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 2) sam
         }
         cluster.sync();
     }
+    MONO_TL(tl_sample, 14);
     // from here on a CTA reads only what is its own
     u64 before = 0;
     uint32_t t_before = 0;
@@ -511,6 +548,7 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 2) sam
             before += __shfl_sync(0xffffffffu, s, 31);
         }
     }
+    MONO_TL(tl_sample, 15);
 }
 
 template <typename T>
@@ -549,3 +587,12 @@ extern "C" int mono_sample_launch(const mono_sample_args* a, void* stream) {
     if (e != cudaSuccess) mono_set_error("%s: %s", who, cudaGetErrorString(e));
     return (int)e;
 }
+
+#ifdef MONO_TIMELINE
+// Copies the kernel's stamps of the last launch to `out` (MONO_TL_CTAS x MONO_TL_POINTS); blocks the host.
+extern "C" int mono_timeline_read_sample(unsigned long long* out, int* ctas, int* points) {
+    *ctas = MONO_TL_CTAS;
+    *points = MONO_TL_POINTS;
+    return (int)cudaMemcpyFromSymbol(out, sampling::tl_sample, sizeof(unsigned long long) * MONO_TL_CTAS * MONO_TL_POINTS);
+}
+#endif

@@ -104,6 +104,23 @@ def test_equal_logits_keep_the_lowest_indices():
     _check(x, u, top_p=torch.full((rows,), 0.37))
 
 
+def test_borders_at_zero_and_among_the_smallest_numbers():
+    """Ties at 0 and -0 (equal), the filter's border there, and subnormal logits on both sides of it."""
+    rows, vocab = 12, 900
+    x = torch.full((rows, vocab), -1.0)
+    x[:, ::3] = 0.0
+    x[:, 1::3] = -0.0
+    x[:, 5] = 2.0
+    x[:, 2] = -(2.0**-149)
+    x[:, 8] = 2.0**-149
+    u = _u(rows, 13)
+    for k in (1, 2, 3, 300, 601, 602, 603):
+        _check(x, u, top_k=torch.full((rows,), k, dtype=torch.int32))
+    _check(x, u, top_p=torch.full((rows,), 0.5))
+    _check(x, u, min_p=torch.full((rows,), 0.1353))
+    _check(x, u, min_p=torch.full((rows,), 0.1354))
+
+
 def test_infinities_nan_and_empty_rows():
     rows, vocab = 8, 1300
     x = _logits(rows, vocab, 4)

@@ -14,8 +14,9 @@
 // passes run on that.  The border is found in steps that all eight CTAs decide alike from merged histograms (read over
 // distributed shared memory; one cluster barrier a step):
 //   1. the largest logit;
-//   2. Z, and a histogram of token counts over 1024 equal steps of log2 w.  The weights of a step differ by 3 %, so the
-//      counts bound the masses, and the border lies in a few neighbouring steps;
+//   2. Z, and a histogram over 1024 equal steps of log2 w of the tokens' number and of how far into its step each lies;
+//      the weights of a step differ by 3 % and these two sums give its mass to 2^-11, so the border lies in one step as a
+//      rule;
 //   3. those steps' range of keys (the order-preserving image of the f32 bits) by 1024 bins with counts and masses,
 //      again on the bin that holds the border, until one key or one token is left (two rounds as a rule).
 // Then each warp's run of kept mass says which warp walks to the token.
@@ -47,45 +48,39 @@ __device__ __forceinline__ uint32_t key_of(float x) {
 __device__ __forceinline__ float logit_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7FFFFFFFu : ~key); }
 // The logit f for which x <= f says key_of(x) <= key.  One key has no logit, that of -0, and -0 compares as 0 does.
 __device__ __forceinline__ float below_or_at(uint32_t key) { return logit_of(key == 0x7FFFFFFFu ? key - 1 : key); }
-constexpr uint32_t kKeyNegInf = 0x007FFFFFu;
+constexpr uint32_t kKeyNegInf = 0x007FFFFFu, kKeyInf = 0xFF800000u;
 
-constexpr int kTable = 256;
+constexpr int kTable = 32, kCopies = 16;  // a copy of the table per pair of banks: looked up by all lanes, it has no conflicts
 constexpr double kTwo52 = 4503599627370496.0;
 
 struct Row {
-    float mx;           // largest logit
+    float mx;           // largest logit (finite)
     float c;            // log2(e) / T, f32: for histogram steps only
     double mx64, c64;   // the same, f64
     u64 k;              // rank below this
     u64 floor_w;        // weight at least this
-    const double* tab;  // 2^(i / 256)
+    const double* tab;  // 2^(44 + i / 32), this lane's copy
 };
 
-// f32 -> f64 by bits (conversions between the two run at a quarter of the rate of the arithmetic): normal numbers; a
-// subnormal f32 gives another number below 2^-126, which no difference of logits notices
-__device__ __forceinline__ double widen(float x) {
-    const uint32_t b = __float_as_uint(x);
-    return __hiloint2double((int)((b & 0x80000000u) | (((b & 0x7FFFFFFFu) >> 3) + 0x38000000u)), (int)(b << 29));
-}
-
-// round(2^44 exp((x - mx) / T)), an f64 whole number.  y = (x - mx) log2(e) / T = n + i / 256 + r, 0 <= i < 256, |r| <= 1/512:
-// 2^y = 2^n 2^(i/256) 2^r, the last by its series in r ln 2 (at most 0.00136: the fifth power's term is below 2^-54).
+// round(2^44 exp((x - mx) / T)), an f64 whole number.  y = (x - mx) log2(e) / T = n + i / 32 + r, 0 <= i < 32, |r| <= 1/64:
+// 2^y = 2^n 2^(i/32) 2^r, the last by its series in r ln 2 (at most 0.0109: the sixth power's term is below 2^-48).
 __device__ __forceinline__ double weight_f64(float x, const Row& r) {
-    const double y = (widen(x) - r.mx64) * r.c64;
-    const double shifted = fma(y, 256.0, 6755399441055744.0);  // + 2^52 + 2^51: the low word holds round(256 y)
+    const double y = ((double)x - r.mx64) * r.c64;
+    const double shifted = fma(y, (double)kTable, 6755399441055744.0);  // + 2^52 + 2^51: the low word holds round(32 y)
     const int q = __double2loint(shifted);
-    const double t = fma(shifted - 6755399441055744.0, -1.0 / 256, y);
+    const double t = fma(shifted - 6755399441055744.0, -1.0 / kTable, y);
     constexpr double L = 0.69314718055994530942;
-    double e = fma(t, L * L * L * L / 24, L * L * L / 6);
+    double e = fma(t, L * L * L * L * L / 120, L * L * L * L / 24);
+    e = fma(t, e, L * L * L / 6);
     e = fma(t, e, L * L / 2);
     e = fma(t, e, L);
     e = fma(t, e, 1.0);
-    e *= r.tab[q & 255];
-    e = __hiloint2double(__double2hiint(e) + ((q >> 8) + 44) * (1 << 20), __double2loint(e));  // times 2^(n + 44)
-    e = (e + kTwo52) - kTwo52;                                                                  // to a whole number
-    // weights below 2^-45 are 0 (there the exponent above may have left its range), and so is that of -inf
-    e = y > -45.0 && x != -INFINITY ? e : 0.0;
-    return x == r.mx ? kOne : e;
+    e *= r.tab[(q & (kTable - 1)) * kCopies];
+    // times 2^n, by the exponent.  Below 2^-45 (and for -inf) the exponent may leave its range: a high word of 0 leaves a
+    // number next to 0.
+    const int hi = __double2hiint(e) + ((q & ~(kTable - 1)) << 15);
+    e = __hiloint2double(y > -45.0 ? hi : 0, __double2loint(e));
+    return (e + kTwo52) - kTwo52;  // to a whole number
 }
 __device__ __forceinline__ u64 whole(double w) { return (u64)__double_as_longlong(w + kTwo52) & 0xFFFFFFFFFFFFFull; }  // below 2^52
 __device__ __forceinline__ u64 weight_of(float x, const Row& r) { return whole(weight_f64(x, r)); }
@@ -106,15 +101,6 @@ __device__ __forceinline__ u64 warp_sum_u64(u64 v) {
     return v;
 }
 
-// two words of CTA `rank`'s shared memory, at the place of `p` in this one's
-__device__ __forceinline__ uint2 ld_peer(const uint32_t* p, int rank) {
-    uint2 v;
-    uint32_t a;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
-    asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
-    return v;
-}
-
 struct Hist {
     uint32_t n[2][kBins], lo[2][kBins], hi[2][kBins];  // counts, and masses in two words; two sets, used in turn
 };
@@ -126,12 +112,57 @@ __device__ __forceinline__ void hist_add(Hist& h, int set, int bin, uint32_t n, 
     if (wh) atomicAdd(&h.hi[set][bin], wh);
 }
 
+__device__ __forceinline__ uint32_t peer_address(const void* p, int rank) {
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+    return a;
+}
+__device__ __forceinline__ uint32_t ld_peer(const uint32_t* p, int rank) {
+    uint32_t v;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(peer_address(p, rank)) : "memory");
+    return v;
+}
+__device__ __forceinline__ void st_peer(uint32_t* p, int rank, uint32_t v) {
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(peer_address(p, rank)), "r"(v) : "memory");
+}
+// The eight CTAs' histograms of set `set`, added into set `set ^ 1` of all of them: each CTA adds an eighth of the bins and
+// writes it to every CTA.  (Shared memory of other CTAs is read at some 8 bytes a cycle: with every CTA reading all
+// bins of all others a level took 3 us.)  Barriers before and after.
+__device__ __forceinline__ void hist_merge(Hist& h, int set, int rank, cg::cluster_group& cluster) {
+    constexpr int kShare = kBins / kCtas;
+    static_assert(2 * kShare <= kThreads, "a thread per bin and kind");
+    cluster.sync();
+    const int b = rank * kShare + (threadIdx.x & (kShare - 1)), what = threadIdx.x / kShare;
+    if (what == 0) {
+        uint32_t v[kCtas], n = 0;
+#pragma unroll
+        for (int c = 0; c < kCtas; ++c) v[c] = ld_peer(&h.n[set][b], c);
+#pragma unroll
+        for (int c = 0; c < kCtas; ++c) n += v[c];
+#pragma unroll
+        for (int c = 0; c < kCtas; ++c) st_peer(&h.n[set ^ 1][b], c, n);
+    } else if (what == 1) {
+        uint32_t lo[kCtas], hi[kCtas];
+        u64 m = 0;
+#pragma unroll
+        for (int c = 0; c < kCtas; ++c) { lo[c] = ld_peer(&h.lo[set][b], c); hi[c] = ld_peer(&h.hi[set][b], c); }
+#pragma unroll
+        for (int c = 0; c < kCtas; ++c) m += ((u64)hi[c] << 32) + lo[c];
+#pragma unroll
+        for (int c = 0; c < kCtas; ++c) { st_peer(&h.lo[set ^ 1][b], c, (uint32_t)m); st_peer(&h.hi[set ^ 1][b], c, (uint32_t)(m >> 32)); }
+    }
+    cluster.sync();
+}
+
 // Sums of the threads before this one (exclusive), and all threads' bins are in thread order.
-// (step_of: the histogram step of a weight above 0.  Rounding to the nearest whole number by adding 2^23 + 2^22 keeps the
-// order of the logits and is within 2^-22 of the true step.)
-__device__ __forceinline__ int step_of(float x, const Row& r) {
-    const float at = x == r.mx ? 0.f : fmaf((r.mx - x) * r.c, kSteps, -0.5f);
-    return min(max(__float_as_int(fminf(at, 2000.f) + 12582912.f) - 0x4B400000, 0), kBins - 1);
+// The histogram step of a weight above 0, and how far into the step it lies, in 2^-16 (clamped to the step).  Rounding to
+// the nearest whole number by adding 2^23 + 2^22 keeps the order of the logits; f32 places a logit within 2^-12 of its
+// true step number.
+__device__ __forceinline__ int step_of(float x, const Row& r, uint32_t* within) {
+    const float at = x == r.mx ? 0.f : fminf((r.mx - x) * r.c * kSteps, 2000.f);
+    const int b = min(max(__float_as_int(at - 0.5f + 12582912.f) - 0x4B400000, 0), kBins - 1);
+    *within = (uint32_t)(__float_as_int(fminf(fmaxf(at - (float)b, 0.f), 1.f) * 65535.f + 12582912.f) - 0x4B400000);
+    return b;
 }
 template <typename A>
 __device__ __forceinline__ A block_before(A v, A* red) {
@@ -158,12 +189,12 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 2) sam
     __shared__ uint32_t s_wties[kWarps], red32[kWarps], s_key[kCtas], s_num[kCtas], s_cnt[2];
     __shared__ float redf[2][kWarps];
     __shared__ int s_bin[2];
-    __shared__ double s_tab[kTable];
+    __shared__ double s_tab[kTable * kCopies];
     cg::cluster_group cluster = cg::this_cluster();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, row = blockIdx.x / kCtas, V = a.vocab;
     const int rank = (int)cluster.block_rank();
-    if (tid < kTable) s_tab[tid] = exp2(tid / (double)kTable);
-    for (int i = tid; i < kBins; i += kThreads) h.n[0][i] = 0;
+    if (tid < kTable * kCopies) s_tab[tid] = exp2((tid / kCopies) / (double)kTable) * kOne;
+    for (int i = tid; i < kBins; i += kThreads) { h.n[0][i] = 0; h.lo[0][i] = 0; h.hi[0][i] = 0; }
     if (tid == 0) { s_bin[0] = kBins; s_bin[1] = kBins; }
     MONO_TL(tl_sample, 0);
     pdl_prologue();
@@ -175,38 +206,43 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 2) sam
     const float tp = a.top_p ? a.top_p[row] : 1.f, mp = a.min_p ? a.min_p[row] : 0.f;
     float u = a.u[row];
     // ---- the slice into shared memory, and its largest logit; places behind the vocabulary hold -inf
-    uint32_t kmax = 0;
+    float top = -INFINITY;
     {
         constexpr int N = sizeof(T) == 4 ? 4 : 8;  // logits of a 16-byte load
-        auto put = [&](int i, float v) {
-            v = v == v ? v : -INFINITY;
-            kmax = max(kmax, key_of(v));
-            xs[i] = v;
+        auto clean = [&](float v) {  // fmaxf takes the number beside NaN
+            v = fmaxf(v, -INFINITY);
+            top = fmaxf(top, v);
+            return v;
         };
         const int vecs = (reinterpret_cast<uintptr_t>(x) & 15) ? 0 : count / N;
-        constexpr int B = 4;
-        for (int i0 = tid; i0 < vecs; i0 += kThreads * B) {
+        constexpr int B = 8;
+        for (int v0 = tid; v0 < vecs; v0 += kThreads * B) {
             uint4 w[B];
 #pragma unroll
-            for (int j = 0; j < B; ++j) w[j] = __ldg(reinterpret_cast<const uint4*>(x) + min(i0 + j * kThreads, vecs - 1));
+            for (int j = 0; j < B; ++j) w[j] = __ldg(reinterpret_cast<const uint4*>(x) + min(v0 + j * kThreads, vecs - 1));
 #pragma unroll
             for (int j = 0; j < B; ++j) {
-                const int i = i0 + j * kThreads;
+                const int i = v0 + j * kThreads;
                 if (i >= vecs) break;
-                const uint32_t ws[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
+                if (sizeof(T) == 4) {
+                    reinterpret_cast<float4*>(xs)[i] = make_float4(clean(__uint_as_float(w[j].x)), clean(__uint_as_float(w[j].y)), clean(__uint_as_float(w[j].z)),
+                                                                   clean(__uint_as_float(w[j].w)));
+                } else {
+                    const uint32_t ws[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
+                    float f[8];
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    if (sizeof(T) == 4) {
-                        put(i * 4 + q, __uint_as_float(ws[q]));
-                    } else {
-                        put(i * 8 + 2 * q, __uint_as_float(ws[q] << 16));
-                        put(i * 8 + 2 * q + 1, __uint_as_float(ws[q] & 0xFFFF0000u));
+                    for (int q = 0; q < 4; ++q) {
+                        f[2 * q] = clean(__uint_as_float(ws[q] << 16));
+                        f[2 * q + 1] = clean(__uint_as_float(ws[q] & 0xFFFF0000u));
                     }
+                    reinterpret_cast<float4*>(xs)[2 * i] = make_float4(f[0], f[1], f[2], f[3]);
+                    reinterpret_cast<float4*>(xs)[2 * i + 1] = make_float4(f[4], f[5], f[6], f[7]);
                 }
             }
         }
-        for (int i = vecs * N + tid; i < slice; i += kThreads) put(i, i < count ? (float)x[i] : -INFINITY);
+        for (int i = vecs * N + tid; i < slice; i += kThreads) xs[i] = clean(i < count ? (float)x[i] : -INFINITY);
     }
+    uint32_t kmax = key_of(top);
     MONO_TL(tl_sample, 2);
     kmax = __reduce_max_sync(0xffffffffu, kmax);
     if (lane == 0) red32[warp] = kmax;
@@ -226,14 +262,19 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 2) sam
         }
         return;
     }
+    if (kmax == kKeyInf) {  // beside an infinite logit nothing has weight: its likes become 0, the others -inf
+        for (int i = tid; i < slice; i += kThreads) xs[i] = xs[i] == INFINITY ? 0.f : -INFINITY;
+        kmax = key_of(0.f);
+        __syncthreads();
+    }
     Row r;
-    r.tab = s_tab;
+    r.tab = s_tab + (lane & (kCopies - 1));
     r.mx = logit_of(kmax);
     const bool greedy = !(temp > 0.f);
-    // temperatures below 2^-100 tell no more logits apart than 2^-100 does; beside an infinite logit nothing has weight
-    r.c64 = r.mx == INFINITY ? 1e30 : greedy ? 1.4426950408889634 : 1.4426950408889634 / fmax((double)temp, 7.888609052210118e-31);
+    // Temperatures beyond 2^-100 and 2^100 weigh no logits otherwise than those do, short of logits of 2^-93 or 2^55.
+    r.c64 = greedy ? 1.4426950408889634 : 1.4426950408889634 / fmin(fmax((double)temp, 7.888609052210118e-31), 1.2676506002282294e30);
     r.c = (float)r.c64;
-    r.mx64 = widen(r.mx);
+    r.mx64 = (double)r.mx;
     r.k = greedy ? 1ull : tk < 1 || tk > V ? (u64)V : (u64)tk;
     const double p = !greedy && tp < 1.f ? fmax((double)tp, 0.0) : 1.0;
     r.floor_w = !greedy && mp > 0.f ? (u64)ceil((double)fminf(mp, 1.f) * kOne) : 0ull;
@@ -243,14 +284,22 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 2) sam
     {
         // whole numbers up to 2^44 add exactly in f64 to 2^53: a thread has at most 96
         double zd = 0.0;
-        for (int i = i0 + lane * 4; i < i1; i += 128) {
-            const float4 v4 = *reinterpret_cast<const float4*>(xs + i);
-            const float v[4] = {v4.x, v4.y, v4.z, v4.w};
+        for (int i = i0 + lane * 4; i < i1; i += 256) {  // eight weights at a time: f64 arithmetic answers late
+            const bool second = i + 128 < i1;
+            const float4 a4 = *reinterpret_cast<const float4*>(xs + i), b4 = second ? *reinterpret_cast<const float4*>(xs + i + 128) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+            const float v[8] = {a4.x, a4.y, a4.z, a4.w, b4.x, b4.y, b4.z, b4.w};
+            double w[8];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const double w = weight_f64(v[j], r);
-                zd += w;
-                if (filtered && w > 0.0) atomicAdd(&h.n[0][step_of(v[j], r)], 1u);
+            for (int j = 0; j < 8; ++j) w[j] = weight_f64(v[j], r);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                zd += w[j];
+                if (filtered && w[j] > 0.0) {
+                    uint32_t within;
+                    const int b = step_of(v[j], r, &within);
+                    atomicAdd(&h.n[0][b], 1u);
+                    atomicAdd(&h.lo[0][b], within);  // at most 49152 x 65535: below 2^32
+                }
             }
         }
         u64 z = whole(zd);
@@ -264,7 +313,7 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 2) sam
         for (int i = 0; i < kWarps; ++i) z += s_wsum[i];
         *cluster.map_shared_rank(&s_z[rank], tid) = z;
     }
-    cluster.sync();
+    if (filtered) hist_merge(h, 0, rank, cluster); else cluster.sync();
     MONO_TL(tl_sample, 5);
     u64 Z = 0;
     for (int i = 0; i < kCtas; ++i) Z += s_z[i];
@@ -272,35 +321,42 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 2) sam
     uint32_t khi = 0, klo = 1, tied = 0, ties = 0;
     u64 kept = Z, tie_w = 0;
     bool all = !filtered;
+    u64 run_above = 0;       // of this warp's run: the mass above the range that the keys were first searched in,
+    float first_hi = 0.f;    // which ends here
     if (filtered) {
         // "mass before < p Z", for masses in whole units
         const u64 limit = p < 1.0 ? max((u64)ceil(p * (double)Z), 1ull) : ~0ull;
         // ---- bounds of the border among the steps
         {
-            uint32_t n[kPerThread] = {};
-            uint2 v[kCtas];
-#pragma unroll
-            for (int c = 0; c < kCtas; ++c) v[c] = ld_peer(&h.n[0][tid * kPerThread], c);  // all in flight
-#pragma unroll
-            for (int c = 0; c < kCtas; ++c) { n[0] += v[c].x; n[1] += v[c].y; }
+            const uint2 n2 = *reinterpret_cast<const uint2*>(&h.n[1][tid * kPerThread]);
+            const uint32_t n[kPerThread] = {n2.x, n2.y};
             static_assert(kPerThread == 2, "two bins per thread");
-            // a step's weights lie in (2^-((b + 1) / kSteps), 2^-(b / kSteps)], in units of the largest
-            float top[kPerThread + 1];
+            const uint2 l2 = *reinterpret_cast<const uint2*>(&h.lo[1][tid * kPerThread]), h2 = *reinterpret_cast<const uint2*>(&h.hi[1][tid * kPerThread]);
+            const float f[kPerThread] = {((float)h2.x * 65536.f + (float)l2.x * (1.f / 65536.f)), ((float)h2.y * 65536.f + (float)l2.y * (1.f / 65536.f))};
+            // A weight f steps into a step is 2^(-f / kSteps) of the step's first: 1 - a f, plus at most (a f)^2 / 2 <= a^2 / 2 f.
+            constexpr float a = 0.69314718f / kSteps, a2 = a * a * 0.5f;
+            float top[kPerThread + 1], m_lo[kPerThread], m_hi[kPerThread];
 #pragma unroll
             for (int j = 0; j <= kPerThread; ++j) top[j] = exp2f(-(float)(tid * kPerThread + j) / kSteps);
-            const float m_hi = n[0] * top[0] + n[1] * top[1], m_lo = n[0] * top[1] + n[1] * top[2];
+#pragma unroll
+            for (int j = 0; j < kPerThread; ++j) {
+                m_lo[j] = fmaxf(top[j] * ((float)n[j] - a * f[j]), 0.f);
+                m_hi[j] = top[j] * ((float)n[j] - a * f[j] + a2 * f[j]);
+            }
             uint32_t c = block_before<uint32_t>(n[0] + n[1], red32);
-            float hi = block_before<float>(m_hi, redf[0]), lo = block_before<float>(m_lo, redf[1]);
-            // f32 sums of at most 1024 terms, and steps that f32 places to a few 2^-24 of their number: 0.1 % covers both
+            float hi = block_before<float>(m_hi[0] + m_hi[1], redf[0]), lo = block_before<float>(m_lo[0] + m_lo[1], redf[1]);
+            // f32 sums of at most 1024 terms (2^-14 at worst), the places' 2^-12 of a step (2^-17 of a weight) and their
+            // rounding: 2^-12 covers them.  The last step also holds weights below it, 2^-44 of the largest each.
+            constexpr float up = 1.f + 0x1p-12f, down = 1.f - 0x1p-12f;
             const float lim = limit == ~0ull ? INFINITY : (float)((double)limit / kOne), fl = (float)((double)r.floor_w / kOne);
 #pragma unroll
             for (int j = 0; j < kPerThread; ++j) {
                 c += n[j];
-                hi += n[j] * top[j];
-                lo += n[j] * top[j + 1];
+                hi += m_hi[j];
+                lo += m_lo[j];
                 const int b = tid * kPerThread + j;
-                if (c > r.k || hi * 1.001f >= lim || top[j + 1] * 0.999f < fl) atomicMin(&s_bin[0], b);  // may not be kept whole
-                if (c > r.k || lo * 0.999f >= lim || top[j] * 1.001f < fl) atomicMin(&s_bin[1], b);      // the border is not behind it
+                if (c > r.k || hi * up >= lim || top[j + 1] * down < fl) atomicMin(&s_bin[0], b);  // may not be kept whole
+                if (c > r.k || lo * down >= lim || top[j] * up < fl) atomicMin(&s_bin[1], b);      // the border is not behind it
             }
         }
         __syncthreads();
@@ -308,12 +364,11 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 2) sam
         __syncthreads();
         if (b0 >= kBins) {
             all = true;
-            cluster.sync();  // no CTA leaves while another reads its histogram
         } else {
             // the steps' range of logits, with room for the rounding of the step's number
             const double per = 1.0 / ((double)r.c * (double)kSteps);
-            float xh = b0 == 0 ? r.mx : (float)((double)r.mx - (double)b0 * per * (1.0 - 4e-6));
-            float xl = (float)((double)r.mx - (double)(b1 + 1) * per * (1.0 + 4e-6));
+            float xh = b0 == 0 ? r.mx : (float)((double)r.mx - ((double)b0 - 0x1p-10) * per);
+            float xl = (float)((double)r.mx - ((double)(b1 + 1) + 0x1p-10) * per);
             if (!(xh <= r.mx)) xh = r.mx;
             if (!(xl <= xh)) xl = -INFINITY;  // no number: infinite temperature, infinite logits
             khi = min(key_of(xh) + 2u, kmax);
@@ -323,46 +378,61 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 2) sam
             uint32_t n_above = 0;
             MONO_TL(tl_sample, 6);
             for (int level = 1;; ++level) {
-                const int set = level & 1;
+                const int set = (level & 1) ^ 1;  // the one that does not hold the sums of the step before
                 const uint32_t width = khi - klo;
                 const int sh = width < kBins ? 0 : 22 - __clz(width);
                 for (int i = tid; i < kBins; i += kThreads) { h.n[set][i] = 0; h.lo[set][i] = 0; h.hi[set][i] = 0; }
                 if (tid == 0) s_bin[set] = kBins;  // not the one that slower threads may still read
                 __syncthreads();
-                u64 m_ab = 0;
                 uint32_t n_ab = 0;
                 const float fhi = below_or_at(khi), flo = logit_of(klo);  // order as the keys do, and cost nothing to compare
+                double above_d = 0.0;
                 for (int b = i0; b < i1; b += 128) {  // whole warps: the lanes vote
                     const int i = b + lane * 4;
                     const float4 v4 = i < i1 ? *reinterpret_cast<const float4*>(xs + i) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
                     const float v[4] = {v4.x, v4.y, v4.z, v4.w};
+                    bool wanted = false;  // the first level also weighs what is above the range
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) wanted = wanted || (v[j] >= flo && (level == 1 || v[j] <= fhi));
+                    if (!__any_sync(0xffffffffu, wanted)) continue;
+                    double w[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) w[j] = weight_f64(v[j], r);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const bool some_here = v[j] >= flo && (v[j] <= fhi || level == 1);
-                        if (!__any_sync(0xffffffffu, some_here)) continue;
-                        u64 w = some_here ? weight_of(v[j], r) : 0;
-                        if (v[j] > fhi) {  // (on the first level) surely kept
-                            m_ab += w;
-                            n_ab += w != 0;
-                            w = 0;
+                        if (level == 1 && v[j] > fhi) {  // surely kept
+                            above_d += w[j];
+                            n_ab += w[j] > 0.0;
                         }
-                        const unsigned in = __ballot_sync(0xffffffffu, w != 0);
+                    }
+                    bool near = false;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) near = near || (v[j] >= flo && v[j] <= fhi);
+                    if (!__any_sync(0xffffffffu, near)) continue;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const bool here = v[j] >= flo && v[j] <= fhi && w[j] > 0.0;
+                        const unsigned in = __ballot_sync(0xffffffffu, here);
                         if (in == 0) continue;
                         const int bin = (int)((khi - key_of(v[j])) >> sh), lead = __ffs(in) - 1;
                         const int lb = __shfl_sync(0xffffffffu, bin, lead);
-                        if (__popc(in) > 4 && __all_sync(0xffffffffu, w == 0 || bin == lb)) {  // many equal logits: one addition for all
-                            const u64 sum = warp_sum_u64(w);
+                        const u64 wi = here ? whole(w[j]) : 0;
+                        if (__popc(in) > 4 && __all_sync(0xffffffffu, !here || bin == lb)) {  // many equal logits: one addition for all
+                            const u64 sum = warp_sum_u64(wi);
                             if (lane == lead) hist_add(h, set, bin, __popc(in), sum);
-                        } else if (w) {
-                            hist_add(h, set, bin, 1, w);
+                        } else if (here) {
+                            hist_add(h, set, bin, 1, wi);
                         }
                         __syncwarp();
                     }
                 }
+                u64 m_ab = whole(above_d);
                 if (level == 1) {
                     m_ab = warp_sum_u64(m_ab);
                     n_ab = __reduce_add_sync(0xffffffffu, n_ab);
                     if (lane == 0) { red64[warp] = m_ab; red32[warp] = n_ab; }
+                    run_above = m_ab;
+                    first_hi = fhi;
                 }
                 __syncthreads();
                 if (level == 1 && tid < kCtas) {
@@ -372,28 +442,14 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 2) sam
                     *cluster.map_shared_rank(&s_part[rank], tid) = m;
                     *cluster.map_shared_rank(&s_num[rank], tid) = n;
                 }
-                cluster.sync();
+                hist_merge(h, set, rank, cluster);
                 MONO_TL(tl_sample, 5 + 2 * level);
                 if (level == 1)
                     for (int i = 0; i < kCtas; ++i) { above += s_part[i]; n_above += s_num[i]; }
-                uint32_t n[kPerThread] = {};
-                u64 m[kPerThread] = {};
-                {
-                    uint2 vn[kCtas], vl[kCtas], vh[kCtas];
-#pragma unroll
-                    for (int c = 0; c < kCtas; ++c) {  // all in flight
-                        vn[c] = ld_peer(&h.n[set][tid * kPerThread], c);
-                        vl[c] = ld_peer(&h.lo[set][tid * kPerThread], c);
-                        vh[c] = ld_peer(&h.hi[set][tid * kPerThread], c);
-                    }
-#pragma unroll
-                    for (int c = 0; c < kCtas; ++c) {
-                        n[0] += vn[c].x;
-                        n[1] += vn[c].y;
-                        m[0] += ((u64)vh[c].x << 32) + vl[c].x;
-                        m[1] += ((u64)vh[c].y << 32) + vl[c].y;
-                    }
-                }
+                const uint2 n2 = *reinterpret_cast<const uint2*>(&h.n[set ^ 1][tid * kPerThread]), l2 = *reinterpret_cast<const uint2*>(&h.lo[set ^ 1][tid * kPerThread]),
+                            h2 = *reinterpret_cast<const uint2*>(&h.hi[set ^ 1][tid * kPerThread]);
+                const uint32_t n[kPerThread] = {n2.x, n2.y};
+                const u64 m[kPerThread] = {((u64)h2.x << 32) + l2.x, ((u64)h2.y << 32) + l2.y};
                 uint32_t c = n_above + block_before<uint32_t>(n[0] + n[1], red32);
                 u64 mass = above + block_before<u64>(m[0] + m[1], red64);
                 uint32_t c_at[kPerThread];
@@ -465,14 +521,22 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 2) sam
         for (int i = i0 + lane * 4; i < i1; i += 128) {
             const float4 v4 = *reinterpret_cast<const float4*>(xs + i);
             const float v[4] = {v4.x, v4.y, v4.z, v4.w};
+            // what lies above the first range has been added up
+            bool wanted = false;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) wanted = wanted || (v[j] <= first_hi && v[j] >= (some ? flo : fhi));
+            if (!wanted) continue;
+            double w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = weight_f64(v[j], r);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                if (v[j] > fhi) md += weight_f64(v[j], r);
+                if (v[j] > fhi) md += v[j] <= first_hi ? w[j] : 0.0;
                 else if (some && v[j] >= flo) ++t;
             }
         }
         u64 m = whole(md);
-        m = warp_sum_u64(m);
+        m = warp_sum_u64(m) + run_above;
         t = __reduce_add_sync(0xffffffffu, t);
         if (lane == 0) { s_wsum[warp] = m; s_wties[warp] = t; }
         __syncthreads();

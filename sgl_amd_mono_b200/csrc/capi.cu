@@ -91,10 +91,20 @@ extern "C" int mono_tmap_encode(mono_tmap_t* out, const void* base, uint64_t inn
     return mono_tmap_encode_box(out, base, inner_bytes, rows, outer, row_stride_bytes, outer_stride_bytes, 128);
 }
 
+int mono_tmap_encode_box3(mono_tmap_t* out, const void* base, uint64_t inner_bytes, uint64_t rows, uint64_t outer, uint64_t row_stride_bytes,
+                          uint64_t outer_stride_bytes, uint32_t box_rows, uint32_t box_outer);
+
 extern "C" int mono_tmap_encode_box(mono_tmap_t* out, const void* base, uint64_t inner_bytes, uint64_t rows,
                                     uint64_t outer, uint64_t row_stride_bytes, uint64_t outer_stride_bytes, uint32_t box_rows) {
+    return mono_tmap_encode_box3(out, base, inner_bytes, rows, outer, row_stride_bytes, outer_stride_bytes, box_rows, 1);
+}
+
+// The same with boxes of `box_outer` matrices; their distance may be smaller than the rows' (heads that lie side by side
+// in a token's row come out one after the other).
+int mono_tmap_encode_box3(mono_tmap_t* out, const void* base, uint64_t inner_bytes, uint64_t rows, uint64_t outer, uint64_t row_stride_bytes,
+                          uint64_t outer_stride_bytes, uint32_t box_rows, uint32_t box_outer) {
     static_assert(sizeof(CUtensorMap) == sizeof(mono_tmap_t), "descriptor size");
-    if (!out || !base || inner_bytes == 0 || rows == 0 || outer == 0 || box_rows == 0 || box_rows > 256) {
+    if (!out || !base || inner_bytes == 0 || rows == 0 || outer == 0 || box_rows == 0 || box_rows > 256 || box_outer == 0 || box_outer > 256) {
         mono_set_error("mono_tmap_encode: null or empty tensor, or box rows outside 1..256");
         return MONO_E_ARG;
     }
@@ -111,7 +121,7 @@ extern "C" int mono_tmap_encode_box(mono_tmap_t* out, const void* base, uint64_t
     }
     cuuint64_t dims[3] = {inner_bytes, rows, outer};
     cuuint64_t strides[2] = {row_stride_bytes, outer > 1 ? outer_stride_bytes : row_stride_bytes * rows};
-    cuuint32_t box[3] = {128, box_rows, 1};
+    cuuint32_t box[3] = {128, box_rows, box_outer};
     cuuint32_t estr[3] = {1, 1, 1};
     CUresult r = fn(reinterpret_cast<CUtensorMap*>(out), CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims,
                     strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,

@@ -9,15 +9,16 @@
 #include "prefix_attn.cuh"
 
 extern void mono_set_error(const char* fmt, ...);
+extern int mono_tmap_encode_box3(mono_tmap_t* out, const void* base, uint64_t inner_bytes, uint64_t rows, uint64_t outer, uint64_t row_stride_bytes,
+                                 uint64_t outer_stride_bytes, uint32_t box_rows, uint32_t box_outer);
 
 namespace prefix_attn {
 MONO_TL_DECLARE(tl_narrow)
 
-constexpr int kConsumers = 4;                        // warps that compute; one more fetches
+constexpr int kConsumers = 8;                        // warps that compute; one more fetches
 constexpr int kThreads = (kConsumers + 1) * 32;
-constexpr int kStages = 4;
-constexpr int kTileBytes = kPage * kDim;             // one page of one kv head: 64 keys x 128 bytes
-constexpr int kQBytes = 16 * kDim * 2;               // a tile's queries
+constexpr int kStages = 5;
+constexpr int kTileBytes = 128 * kDim;               // 128 rows of K (or V): 128 / heads keys of each head of the group
 constexpr int kQuarter = 36, kPitch = 4 * kQuarter + 4;  // floats of a quarter and of a combine row: spread over the banks
 constexpr float kPBias = 14.f;                       // P is formed as 2^14 p, so that f16 keeps small weights
 
@@ -47,22 +48,23 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
-__device__ __forceinline__ void consumer_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+__device__ __forceinline__ void consumer_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
 // The queries of one tile in the layout of the A fragments, and their scales.  The contraction's order is free as long
 // as both operands share it, so thread (g, t) of a fragment takes dims 32 t .. 32 t + 31 of its rows: a key's 32 bytes
 // are then two 16-byte shared loads.  A row is scaled by a power of two so that its largest value lies in
 // [2^13, 2^14): f16 then holds every bf16 value down to 2^-28 of that exactly.
-__device__ __forceinline__ void load_q(const mono_prefix_attn_args& a, const Entry& n, uint32_t rows /* shared: the tile's rows of 256 bytes */,
-                                       int row0, int G, uint32_t q[8][4], float qscale[2], int lim[2]) {
+__device__ __forceinline__ void load_q(const mono_prefix_attn_args& a, const Entry& n, int head, int row0, int G, uint32_t q[8][4], float qscale[2], int lim[2]) {
     const int g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
     uint4 raw[2][4];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const int row = row0 + g + 8 * i;
         const bool live = row < n.ntok * G;
+        const int r = live ? row : 0;
+        const __nv_bfloat16* src = reinterpret_cast<const __nv_bfloat16*>(a.q) + (size_t)(n.tok0 + r / G) * a.q_ld + (size_t)(head * G + r % G) * kDim + t * 32;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) raw[i][j] = live ? lds128(rows + (g + 8 * i) * (kDim * 2) + t * 64 + j * 16) : make_uint4(0, 0, 0, 0);
+        for (int j = 0; j < 4; ++j) raw[i][j] = live ? __ldg(reinterpret_cast<const uint4*>(src) + j) : make_uint4(0, 0, 0, 0);
         lim[i] = live ? row_limit(n, row, G) : INT32_MAX;  // a row that does not exist needs no mask
     }
 #pragma unroll
@@ -85,21 +87,21 @@ __device__ __forceinline__ void load_q(const mono_prefix_attn_args& a, const Ent
     }
 }
 
-// Up to 16 rows per tile.  Four warps take 16 of a page's 64 keys each, for all rows of the tile, with a running
-// maximum and sum of their own; the fifth warp keeps a ring of pages in flight by TMA (128-byte swizzle, which makes
-// the 16-byte shared loads below free of bank conflicts).  Bound: HBM; K and V stay bytes until a warp has them in
-// registers, where they become f16 exactly.
-__global__ void __launch_bounds__(kThreads, 2) prefix_narrow_kernel(const __grid_constant__ Params p) {
+// Up to 16 rows per tile, of every head of a group.  A unit's 128 rows of K and V arrive by one TMA box each, head after
+// head (128-byte swizzle, which makes the 16-byte shared loads below free of bank conflicts); each of the eight warps
+// takes 16 keys of one head, with a running maximum and sum of its own.  Where a head has several warps they join their
+// parts at the segment's end.  The ninth warp keeps the ring of units full.  Bound: HBM; K and V stay bytes until a warp
+// has them in registers, where they become f16 exactly.
+__global__ void __launch_bounds__(kThreads, 1) prefix_narrow_kernel(const __grid_constant__ Params p) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     float* comb = reinterpret_cast<float*>(ring + kStages * 2 * kTileBytes);  // [4 warps][16 rows][kPitch]
     const mono_prefix_attn_args& a = p.a;
     const int E = a.groups + a.seqs;
-    uint8_t* qbuf = reinterpret_cast<uint8_t*>(comb + kConsumers * 16 * kPitch);
-    uint32_t* off = reinterpret_cast<uint32_t*>(qbuf + 2 * kQBytes);
+    uint32_t* off = reinterpret_cast<uint32_t*>(comb + 4 * 16 * kPitch);
     uint32_t* item = off + E + 1;
-    __shared__ uint64_t full[kStages], empty[kStages], q_full[2], q_empty[2];
-    __shared__ int page_ok[kStages];
+    __shared__ uint64_t full[kStages], empty[kStages];
+    __shared__ int page_ok[kStages];  // bit i: page i of the unit (a unit of one head has two)
     __shared__ uint32_t red[64];
     __shared__ float s_m[kConsumers][16], s_l[kConsumers][16];
     __shared__ int abort_flag;
@@ -110,10 +112,6 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_narrow_kernel(const __grid
         for (int i = 0; i < kStages; ++i) {
             mbar_init(&full[i], 1);
             mbar_init(&empty[i], kConsumers);
-        }
-        for (int i = 0; i < 2; ++i) {
-            mbar_init(&q_full[i], 1);
-            mbar_init(&q_empty[i], kConsumers);
         }
         mbar_fence_init();
         prefetch_tmap(&p.kmap);
@@ -126,52 +124,46 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_narrow_kernel(const __grid
     if (tid == 0 && guard_failed(a.guard)) abort_flag = 1;
     make_plan<false, kThreads>(a, p.s, off, item, red);
     MONO_TL(tl_narrow, 2);
-    const uint32_t U = off[E] * a.kv_heads, per = part_size(U, gridDim.x), u0 = min(blockIdx.x * per, U), u1 = min(u0 + per, U);
-    const int G = a.q_heads / a.kv_heads;
+    const int G = a.q_heads / a.kv_heads, hg = group_heads(a.kv_heads), keys = unit_keys(a.kv_heads);
+    const uint32_t U = off[E] * head_groups(a.kv_heads), per = part_size(U, gridDim.x), u0 = min(blockIdx.x * per, U), u1 = min(u0 + per, U);
     const uint64_t wait_ns = a.wait_ns ? a.wait_ns : kWaitLimitNs;
     if (u0 < u1) {
         if (warp == kConsumers) {
             // ---- fetch: 32 units' pages at a time are looked up by the lanes, then requested in order
-            int it = 0, nth = 0;
+            const int span = min(keys, kPage);  // keys of a box
+            const int n_box = keys / span;
+            int it = 0;
             for (uint32_t base = u0; base < u1 && !*abortp; base += 32) {
                 const uint32_t u = min(base + lane, u1 - 1);
                 const Place at = place_of(off, E, u);
                 const Entry en = entry_of(a, at.e);
                 const Work w = entry_work<false>(a, en);
-                const int head = at.head, tile = (int)(at.local / w.units), unit = (int)(at.local - (uint32_t)tile * w.units);
-                const int page = en.table[unit];
-                const bool ok = page >= 0 && page < a.n_pages;
-                const bool first = u == u0 || unit == 0;  // of a segment: its queries come along
-                const int row0 = tile * 16, rows = min(16, en.ntok * G - row0);
+                const int key = (int)(at.local % (uint32_t)w.units) * keys;
+                int row[2];  // of the cache, where the boxes start; -1: no such page
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int k = key + i * span, page = i < n_box && k < en.len ? en.table[k / kPage] : -1;
+                    row[i] = page >= 0 && page < a.n_pages ? page * kPage + k % kPage : -1;
+                }
                 const int cnt = (int)min(32u, u1 - base);
                 for (int j = 0; j < cnt; ++j, ++it) {
-                    const int pj = __shfl_sync(0xffffffffu, page, j), hj = __shfl_sync(0xffffffffu, head, j), okj = __shfl_sync(0xffffffffu, (int)ok, j);
-                    if (__shfl_sync(0xffffffffu, (int)first, j)) {
-                        // rows r0 .. of kv head hj: a lane fetches what they have of one token, heads side by side
-                        const int r0 = __shfl_sync(0xffffffffu, row0, j), n = __shfl_sync(0xffffffffu, rows, j), t0 = __shfl_sync(0xffffffffu, en.tok0, j), qs = nth & 1;
-                        if (lane == 0 && !*abortp && (nth < 2 || mbar_wait(&q_empty[qs], ((nth >> 1) - 1) & 1, abortp, wait_ns)))
-                            mbar_expect_tx(&q_full[qs], (uint32_t)n * kDim * 2);
-                        __syncwarp();
-                        const int tok = r0 / G + lane, from = max(tok * G, r0), to = min(tok * G + G, r0 + n);
-                        if (!*abortp && from < to)
-                            bulk_load(qbuf + qs * kQBytes + (from - r0) * kDim * 2,
-                                      reinterpret_cast<const __nv_bfloat16*>(a.q) + (size_t)(t0 + tok) * a.q_ld + (size_t)(hj * G + from - tok * G) * kDim,
-                                      (uint32_t)(to - from) * kDim * 2, &q_full[qs]);
-                        ++nth;
-                    }
+                    const int r0 = __shfl_sync(0xffffffffu, row[0], j), r1 = __shfl_sync(0xffffffffu, row[1], j), hj = __shfl_sync(0xffffffffu, at.head, j) * hg;
                     if (lane == 0) {
                         const int st = it % kStages;
                         if (*abortp || (it >= kStages && !mbar_wait(&empty[st], ((it / kStages) - 1) & 1, abortp, wait_ns))) {
                             // given up: the consumers' waits see the flag
                         } else {
-                            page_ok[st] = okj;
-                            if (okj) {
-                                uint8_t* dst = ring + st * 2 * kTileBytes;
-                                mbar_expect_tx(&full[st], 2 * kTileBytes);
-                                tma_load_3d(dst, &p.kmap, hj * kDim, pj * kPage, 0, &full[st]);
-                                tma_load_3d(dst + kTileBytes, &p.vmap, hj * kDim, pj * kPage, 0, &full[st]);
-                            } else {
-                                mbar_arrive(&full[st]);
+                            page_ok[st] = (r0 >= 0 ? 1 : 0) | (r1 >= 0 ? 2 : 0);
+                            const uint32_t box = (uint32_t)span * hg * kDim;
+                            uint8_t* dst = ring + st * 2 * kTileBytes;
+                            mbar_expect_tx(&full[st], ((r0 >= 0 ? 2 : 0) + (r1 >= 0 ? 2 : 0)) * box);
+                            if (r0 >= 0) {
+                                tma_load_3d(dst, &p.kmap, 0, r0, hj, &full[st]);
+                                tma_load_3d(dst + kTileBytes, &p.vmap, 0, r0, hj, &full[st]);
+                            }
+                            if (r1 >= 0) {
+                                tma_load_3d(dst + box, &p.kmap, 0, r1, hj, &full[st]);
+                                tma_load_3d(dst + kTileBytes + box, &p.vmap, 0, r1, hj, &full[st]);
                             }
                         }
                     }
@@ -180,20 +172,22 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_narrow_kernel(const __grid
             }
         } else {
             const int g = lane >> 2, t = lane & 3;
+            const int h = warp & (hg - 1), slot = warp / hg, slots = kConsumers / hg;  // head of the group; which 16 of its keys
+            const int rows_at = h * keys + slot * 16;                                  // in a unit's tile
+            const int ok_bit = slot * 16 / kPage;
             int it = 0, nth = 0;
             for (uint32_t u = u0; u < u1; ++nth) {
                 const Place at = place_of(off, E, u);
                 const Entry en = entry_of(a, at.e);
                 const Work wk = entry_work<false>(a, en);
+                const int head = at.head * hg + h;
+                const bool mine = head < a.kv_heads;
                 const int tile = (int)(at.local / wk.units);
                 const int p0 = (int)(at.local - (uint32_t)tile * wk.units), cnt = (int)min((uint32_t)(wk.units - p0), u1 - u);
                 uint32_t q[8][4];
                 float qs[2], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
                 int lim[2];
-                mbar_wait(&q_full[nth & 1], (nth >> 1) & 1, abortp, wait_ns);  // given up: the pages are too, and all warps meet below
-                load_q(a, en, smem_u32(qbuf + (nth & 1) * kQBytes), tile * 16, G, q, qs, lim);
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&q_empty[nth & 1]);
+                load_q(a, en, mine ? head : 0, tile * 16, G, q, qs, lim);
                 const int lim_all = min(en.len, __reduce_min_sync(0xffffffffu, min(lim[0], lim[1])));  // keys below it are seen by every row
                 MONO_TL(tl_narrow, 3 + 4 * nth);  // the first three items
                 float o[16][4];
@@ -201,59 +195,85 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_narrow_kernel(const __grid
                 for (int j = 0; j < 16; ++j)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) o[j][i] = 0.f;
-                for (int i = 0; i < cnt; ++i, ++it) {
-                    const int st = it % kStages;
-                    if (!mbar_wait(&full[st], (it / kStages) & 1, abortp, wait_ns)) break;
+                // Two units a turn where there are two: a warp's chain of loads, products, shuffles and exponentials is long, and
+                // the second unit's runs beside the first's.
+                for (int i = 0; i < cnt; i += 2) {
+                    const int np = min(2, cnt - i);
+                    uint32_t kb[2];
+                    bool on[2];
+                    int key0[2];  // this warp's first key of each unit
+                    bool have = true;
+#pragma unroll
+                    for (int z = 0; z < 2; ++z) {
+                        const int st = (it + z) % kStages;
+                        if (z < np) have = have && mbar_wait(&full[st], ((it + z) / kStages) & 1, abortp, wait_ns);
+                        kb[z] = smem_u32(ring + st * 2 * kTileBytes) + rows_at * 128;
+                        key0[z] = (p0 + i + z) * keys + slot * 16;
+                        on[z] = z < np && have && mine && (page_ok[st] >> ok_bit & 1) && key0[z] < en.len;
+                    }
+                    if (!have) break;
                     if (i == 0) MONO_TL(tl_narrow, 4 + 4 * nth);
-                    const uint32_t kb = smem_u32(ring + st * 2 * kTileBytes), vb = kb + kTileBytes;
-                    const int key0 = (p0 + i) * kPage + warp * 16;  // this warp's first key
-                    if (page_ok[st] && key0 < en.len) {
-                        float s[2][4];
+                    if (on[0] || on[1]) {
+                        float s[2][2][4];
 #pragma unroll
-                        for (int nt = 0; nt < 2; ++nt) {
-                            const uint32_t rowa = kb + (warp * 16 + nt * 8 + g) * 128;
-                            const uint4 k0 = lds128(rowa + (((2 * t) ^ g) << 4)), k1 = lds128(rowa + (((2 * t + 1) ^ g) << 4));
-                            const uint32_t w[8] = {k0.x, k0.y, k0.z, k0.w, k1.x, k1.y, k1.z, k1.w};
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) s[nt][j] = 0.f;
-#pragma unroll
-                            for (int j = 0; j < 8; ++j) mma_f16(s[nt], q[j], e4m3x2_to_f16x2(w[j]), e4m3x2_to_f16x2(w[j] >> 16));
-                        }
-                        // scores stay in the units of the product: qs > 0, so their maximum is the scaled scores'
-                        if (key0 + 16 > lim_all) {
+                        for (int z = 0; z < 2; ++z)
 #pragma unroll
                             for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
-                                for (int j = 0; j < 4; ++j)
-                                    if (key0 + nt * 8 + 2 * t + (j & 1) >= min(lim[j >> 1], en.len)) s[nt][j] = -INFINITY;
+                                for (int j = 0; j < 4; ++j) s[z][nt][j] = on[z] ? 0.f : -INFINITY;
+#pragma unroll
+                        for (int z = 0; z < 2; ++z) {
+                            if (!on[z]) continue;
+#pragma unroll
+                            for (int nt = 0; nt < 2; ++nt) {
+                                const uint32_t rowa = kb[z] + (nt * 8 + g) * 128;
+                                const uint4 k0 = lds128(rowa + (((2 * t) ^ g) << 4)), k1 = lds128(rowa + (((2 * t + 1) ^ g) << 4));
+                                const uint32_t w[8] = {k0.x, k0.y, k0.z, k0.w, k1.x, k1.y, k1.z, k1.w};
+#pragma unroll
+                                for (int j = 0; j < 8; ++j) mma_f16(s[z][nt], q[j], e4m3x2_to_f16x2(w[j]), e4m3x2_to_f16x2(w[j] >> 16));
+                            }
                         }
+                        // scores stay in the units of the product: qs > 0, so their maximum is the scaled scores'
+#pragma unroll
+                        for (int z = 0; z < 2; ++z)
+                            if (on[z] && key0[z] + 16 > lim_all) {
+#pragma unroll
+                                for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                                    for (int j = 0; j < 4; ++j)
+                                        if (key0[z] + nt * 8 + 2 * t + (j & 1) >= min(lim[j >> 1], en.len)) s[z][nt][j] = -INFINITY;
+                            }
                         float base[2], alpha[2];
 #pragma unroll
                         for (int r = 0; r < 2; ++r) {
-                            float mx = max_nan(max_nan(s[0][2 * r], s[0][2 * r + 1]), max_nan(s[1][2 * r], s[1][2 * r + 1]));
+                            float mx = -INFINITY;
+#pragma unroll
+                            for (int z = 0; z < 2; ++z) mx = max_nan(mx, max_nan(max_nan(s[z][0][2 * r], s[z][0][2 * r + 1]), max_nan(s[z][1][2 * r], s[z][1][2 * r + 1])));
                             mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
                             mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                            const float mn = max_nan(m[r], mx * qs[r]), z = mn == -INFINITY ? 0.f : mn;
+                            const float mn = max_nan(m[r], mx * qs[r]), zero = mn == -INFINITY ? 0.f : mn;
                             // a row that has seen no key yet keeps max = -inf, and weights of 0
-                            alpha[r] = ex2(m[r] - z);
+                            alpha[r] = ex2(m[r] - zero);
                             m[r] = mn;
                             l[r] *= alpha[r];
-                            base[r] = kPBias - z;
+                            base[r] = kPBias - zero;
                         }
-                        uint32_t pa[4];
-                        float pv[2][4];
+                        uint32_t pa[2][4];
 #pragma unroll
-                        for (int nt = 0; nt < 2; ++nt)
+                        for (int z = 0; z < 2; ++z) {
+                            float pv[2][4];
 #pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                const int r = j >> 1;
-                                pv[nt][j] = ex2(fmaf(s[nt][j], qs[r], base[r]));
-                                l[r] += pv[nt][j];
-                            }
-                        pa[0] = pack_f16(pv[0][0], pv[0][1]);
-                        pa[1] = pack_f16(pv[0][2], pv[0][3]);
-                        pa[2] = pack_f16(pv[1][0], pv[1][1]);
-                        pa[3] = pack_f16(pv[1][2], pv[1][3]);
+                            for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) {
+                                    pv[nt][j] = ex2(fmaf(s[z][nt][j], qs[j >> 1], base[j >> 1]));
+                                    l[j >> 1] += pv[nt][j];
+                                }
+                            pa[z][0] = pack_f16(pv[0][0], pv[0][1]);
+                            pa[z][1] = pack_f16(pv[0][2], pv[0][3]);
+                            pa[z][2] = pack_f16(pv[1][0], pv[1][1]);
+                            pa[z][3] = pack_f16(pv[1][2], pv[1][3]);
+                        }
                         if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
 #pragma unroll
                             for (int j = 0; j < 16; ++j) {
@@ -261,78 +281,121 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_narrow_kernel(const __grid
                                 o[j][2] *= alpha[1]; o[j][3] *= alpha[1];
                             }
                         }
-                        // V: thread (g, t) takes dims 16 g .. 16 g + 15 of keys 2t, 2t + 1, 2t + 8, 2t + 9; output
-                        // column g of product j is dim 16 g + j.  Keys behind the entry's last hold anything, NaN among
-                        // it, and 0 x NaN is NaN, so their bytes become zeros.
-                        uint32_t vw[4][4];
+                        // V: thread (g, t) takes dims 16 g .. 16 g + 15 of keys 2t, 2t + 1, 2t + 8, 2t + 9; output column g of
+                        // product j is dim 16 g + j.  Keys behind the entry's last hold anything, NaN among it, and 0 x NaN is
+                        // NaN, so their bytes become zeros.
 #pragma unroll
-                        for (int i4 = 0; i4 < 4; ++i4) {
-                            const int kr = 2 * t + (i4 & 1) + (i4 >> 1) * 8;
-                            const uint4 v = lds128(vb + (warp * 16 + kr) * 128 + ((g ^ (kr & 7)) << 4));
-                            vw[i4][0] = v.x; vw[i4][1] = v.y; vw[i4][2] = v.z; vw[i4][3] = v.w;
-                        }
-                        if (key0 + 16 > en.len) {
+                        for (int z = 0; z < 2; ++z) {
+                            if (!on[z]) continue;
+                            const uint32_t vb = kb[z] + kTileBytes;
+                            uint32_t vw[4][4];
 #pragma unroll
-                            for (int i4 = 0; i4 < 4; ++i4)
-                                if (key0 + 2 * t + (i4 & 1) + (i4 >> 1) * 8 >= en.len) vw[i4][0] = vw[i4][1] = vw[i4][2] = vw[i4][3] = 0;
-                        }
+                            for (int i4 = 0; i4 < 4; ++i4) {
+                                const int kr = 2 * t + (i4 & 1) + (i4 >> 1) * 8;
+                                const uint4 v = lds128(vb + kr * 128 + ((g ^ (kr & 7)) << 4));
+                                vw[i4][0] = v.x; vw[i4][1] = v.y; vw[i4][2] = v.z; vw[i4][3] = v.w;
+                            }
+                            if (key0[z] + 16 > en.len) {
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const uint32_t a01 = __byte_perm(vw[0][j], vw[1][j], 0x5140), a23 = __byte_perm(vw[0][j], vw[1][j], 0x7362);
-                            const uint32_t b01 = __byte_perm(vw[2][j], vw[3][j], 0x5140), b23 = __byte_perm(vw[2][j], vw[3][j], 0x7362);
-                            mma_f16(o[4 * j], pa, e4m3x2_to_f16x2(a01), e4m3x2_to_f16x2(b01));
-                            mma_f16(o[4 * j + 1], pa, e4m3x2_to_f16x2(a01 >> 16), e4m3x2_to_f16x2(b01 >> 16));
-                            mma_f16(o[4 * j + 2], pa, e4m3x2_to_f16x2(a23), e4m3x2_to_f16x2(b23));
-                            mma_f16(o[4 * j + 3], pa, e4m3x2_to_f16x2(a23 >> 16), e4m3x2_to_f16x2(b23 >> 16));
+                                for (int i4 = 0; i4 < 4; ++i4)
+                                    if (key0[z] + 2 * t + (i4 & 1) + (i4 >> 1) * 8 >= en.len) vw[i4][0] = vw[i4][1] = vw[i4][2] = vw[i4][3] = 0;
+                            }
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const uint32_t a01 = __byte_perm(vw[0][j], vw[1][j], 0x5140), a23 = __byte_perm(vw[0][j], vw[1][j], 0x7362);
+                                const uint32_t b01 = __byte_perm(vw[2][j], vw[3][j], 0x5140), b23 = __byte_perm(vw[2][j], vw[3][j], 0x7362);
+                                mma_f16(o[4 * j], pa[z], e4m3x2_to_f16x2(a01), e4m3x2_to_f16x2(b01));
+                                mma_f16(o[4 * j + 1], pa[z], e4m3x2_to_f16x2(a01 >> 16), e4m3x2_to_f16x2(b01 >> 16));
+                                mma_f16(o[4 * j + 2], pa[z], e4m3x2_to_f16x2(a23), e4m3x2_to_f16x2(b23));
+                                mma_f16(o[4 * j + 3], pa[z], e4m3x2_to_f16x2(a23 >> 16), e4m3x2_to_f16x2(b23 >> 16));
+                            }
                         }
                     }
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&empty[st]);
+                    if (lane == 0) {
+                        mbar_arrive(&empty[it % kStages]);
+                        if (np == 2) mbar_arrive(&empty[(it + 1) % kStages]);
+                    }
+                    it += np;
                 }
                 MONO_TL(tl_narrow, 5 + 4 * nth);
-                // ---- the segment's rows: the four warps' parts, brought to one maximum
+                // ---- the segment's rows of this head
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
                     l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
                     l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+                }
+                if (slots > 1) {  // the head's warps bring their parts to one maximum and add them up in halves
                     if (t == 0) {
-                        s_m[warp][g + 8 * r] = m[r];
-                        s_l[warp][g + 8 * r] = l[r];
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) {
+                            s_m[warp][g + 8 * r] = m[r];
+                            s_l[warp][g + 8 * r] = l[r];
+                        }
+                    }
+                    consumer_sync();
+                    float f[2];
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        float top = -INFINITY, sum = 0.f;
+                        for (int k = 0; k < slots; ++k) top = fmaxf(top, s_m[k * hg + h][g + 8 * r]);
+                        for (int k = 0; k < slots; ++k) {
+                            const float mk = s_m[k * hg + h][g + 8 * r];
+                            sum += mk == -INFINITY ? 0.f : s_l[k * hg + h][g + 8 * r] * ex2(mk - top);
+                        }
+                        f[r] = m[r] == -INFINITY ? 0.f : ex2(m[r] - top);
+                        m[r] = top;
+                        l[r] = sum;
+                    }
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        o[j][0] *= f[0]; o[j][1] *= f[0];
+                        o[j][2] *= f[1]; o[j][3] *= f[1];
+                    }
+                    for (int half = slots / 2; half >= 1; half /= 2) {
+                        float* at4 = comb + ((slot & (half - 1)) * hg + h) * 16 * kPitch + t * kQuarter;
+                        if (slot >= half && slot < 2 * half) {
+#pragma unroll
+                            for (int r = 0; r < 2; ++r)
+#pragma unroll
+                                for (int c = 0; c < 2; ++c)
+#pragma unroll
+                                    for (int j = 0; j < 16; j += 4)
+                                        *reinterpret_cast<float4*>(at4 + (g + 8 * r) * kPitch + c * 16 + j) = make_float4(o[j][2 * r + c], o[j + 1][2 * r + c], o[j + 2][2 * r + c], o[j + 3][2 * r + c]);
+                        }
+                        consumer_sync();
+                        if (slot < half) {
+#pragma unroll
+                            for (int r = 0; r < 2; ++r)
+#pragma unroll
+                                for (int c = 0; c < 2; ++c)
+#pragma unroll
+                                    for (int j = 0; j < 16; j += 4) {
+                                        const float4 v = *reinterpret_cast<const float4*>(at4 + (g + 8 * r) * kPitch + c * 16 + j);
+                                        o[j][2 * r + c] += v.x; o[j + 1][2 * r + c] += v.y; o[j + 2][2 * r + c] += v.z; o[j + 3][2 * r + c] += v.w;
+                                    }
+                        }
+                        consumer_sync();
                     }
                 }
-                consumer_sync();
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    const int row = g + 8 * r;
-                    const float M = fmaxf(fmaxf(s_m[0][row], s_m[1][row]), fmaxf(s_m[2][row], s_m[3][row]));
-                    const float f = m[r] == -INFINITY ? 0.f : ex2(m[r] - M);
-                    float* dst = comb + (warp * 16 + row) * kPitch + t * kQuarter;
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-#pragma unroll
-                        for (int j = 0; j < 16; j += 4)
-                            *reinterpret_cast<float4*>(dst + h * 16 + j) = make_float4(o[j][2 * r + h] * f, o[j + 1][2 * r + h] * f, o[j + 2][2 * r + h] * f, o[j + 3][2 * r + h] * f);
-                }
-                consumer_sync();
-                {
-                    float* seg = p.s.seg[0] + (size_t)(blockIdx.x + at.head * item[E] + item[at.e] + tile) * Shape<false>::kSegFloats;
+                if (slot == 0 && mine) {
+                    float* seg = p.s.seg[0] + ((size_t)(blockIdx.x + at.head * item[E] + item[at.e] + tile) * hg + h) * Shape<false>::kSegFloats;
                     const int rows = min(16, en.ntok * G - tile * 16);
-                    if (tid < rows) {
-                        const float M = fmaxf(fmaxf(s_m[0][tid], s_m[1][tid]), fmaxf(s_m[2][tid], s_m[3][tid]));
-                        float sum = 0.f;
 #pragma unroll
-                        for (int w = 0; w < kConsumers; ++w) sum += s_m[w][tid] == -INFINITY ? 0.f : s_l[w][tid] * exp2f(s_m[w][tid] - M);
-                        seg[tid] = M - kPBias;
-                        seg[16 + tid] = sum;
-                    }
-                    for (int r = 0; r < rows; ++r) {
-                        float sum = 0.f;
+                    for (int r = 0; r < 2; ++r) {
+                        const int row = g + 8 * r;
+                        if (row >= rows) continue;
+                        if (t == 0) {
+                            seg[row] = l[r] != l[r] ? l[r] : m[r] - kPBias;  // a row of NaN stays one
+                            seg[16 + row] = l[r];
+                        }
 #pragma unroll
-                        for (int w = 0; w < kConsumers; ++w) sum += comb[(w * 16 + r) * kPitch + (tid >> 5) * kQuarter + (tid & 31)];
-                        seg[32 + r * kDim + tid] = sum;
+                        for (int c = 0; c < 2; ++c)
+#pragma unroll
+                            for (int j = 0; j < 16; j += 4)
+                                *reinterpret_cast<float4*>(seg + 32 + row * kDim + t * 32 + c * 16 + j) = make_float4(o[j][2 * r + c], o[j + 1][2 * r + c], o[j + 2][2 * r + c], o[j + 3][2 * r + c]);
                     }
                 }
-                consumer_sync();
                 MONO_TL(tl_narrow, 6 + 4 * nth);
                 u += cnt;
             }
@@ -361,12 +424,13 @@ __device__ __forceinline__ Parts parts_of(const mono_prefix_attn_args& a, const 
     if (n.tiles == 0 || per_head == 0) return r;  // no keys, or refused tables
     const int kh = head / G, row = (token - n.tok0) * G + head - kh * G;
     r.rows = wide ? Shape<true>::kTile : Shape<false>::kTile;
-    r.stride = wide ? Shape<true>::kSegFloats : Shape<false>::kSegFloats;
     const int tile = row / r.rows, at = row - tile * r.rows;
-    const uint32_t per = part_size(per_head * a.kv_heads, wide ? wide_ctas : narrow_ctas);
-    const uint32_t first = kh * per_head + n.off + (uint32_t)tile * n.units;
+    const int hg = wide ? 1 : group_heads(a.kv_heads), list = kh / hg, lists = wide ? a.kv_heads : head_groups(a.kv_heads);
+    const uint32_t per = part_size(per_head * lists, wide ? wide_ctas : narrow_ctas);
+    const uint32_t first = list * per_head + n.off + (uint32_t)tile * n.units;
     const uint32_t c0 = first / per, c1 = (first + (tile == n.tiles - 1 ? n.last : n.units) - 1) / per;
-    const float* seg = s.seg[wide] + (size_t)(c0 + kh * items + n.item + tile) * r.stride;
+    r.stride = wide ? Shape<true>::kSegFloats : hg * Shape<false>::kSegFloats;
+    const float* seg = s.seg[wide] + (size_t)(c0 + list * items + n.item + tile) * r.stride + (kh - list * hg) * Shape<false>::kSegFloats;
     r.m = seg + at;
     // narrow: rows of 128 values; wide: four dims of all rows, then the next four (as a thread per row writes them)
     r.v = seg + 2 * r.rows + (wide ? (sub * 2 * Shape<true>::kTile + at) * 4 : at * kDim + sub * 8);
@@ -478,10 +542,10 @@ static int sm_or_default() {
     return n > 0 ? n : 148;
 }
 static size_t up256(size_t v) { return (v + 255) & ~size_t(255); }
-// Segments a launch may leave: one per CTA and one per item.
+// Segments a launch may leave: one per CTA and one per item, for each head of a group.
 static size_t narrow_segments(size_t tokens, size_t q_heads, size_t kv_heads, size_t seqs, size_t groups) {
     const size_t tiles = (tokens * (q_heads / kv_heads)) / 16 + 1;
-    return 2 * (size_t)sm_or_default() + kv_heads * (2 * tiles + seqs + groups);
+    return group_heads((int)kv_heads) * ((size_t)sm_or_default() + head_groups((int)kv_heads) * (2 * tiles + seqs + groups));
 }
 // The wide kernel's entries have kWideRows rows at least, so there are at most 2 rows / kWideRows of them.
 static size_t wide_segments(size_t tokens, size_t q_heads, size_t kv_heads) {
@@ -534,7 +598,7 @@ extern "C" int mono_prefix_attn_launch(const mono_prefix_attn_args* a, void* str
     }
     // units are counted in 32 bits: 16-row tiles x pages, for the sequences' own keys and once more for the prefixes
     const double tiles = (double)a->tokens * (a->q_heads / a->kv_heads) / 16 + a->seqs + a->groups;
-    if (tiles * a->kv_heads * ((double)a->pt_ld + a->prefix_ld) >= 4.0e9) {
+    if (tiles * (a->kv_heads + 3) * ((double)a->pt_ld + a->prefix_ld) >= 4.0e9) {
         mono_set_error("%s: too much work for one launch (tiles x kv heads x table width above 4e9): split the tokens", who);
         return MONO_E_ARG;
     }
@@ -545,8 +609,12 @@ extern "C" int mono_prefix_attn_launch(const mono_prefix_attn_args* a, void* str
     }
     Params p;
     const uint64_t inner = (uint64_t)a->kv_heads * kDim, rows = (uint64_t)a->n_pages * kPage;
-    if (int rc = mono_tmap_encode_box(reinterpret_cast<mono_tmap_t*>(&p.kmap), a->k_cache, inner, rows, 1, inner, inner * rows, kPage)) return rc;
-    if (int rc = mono_tmap_encode_box(reinterpret_cast<mono_tmap_t*>(&p.vmap), a->v_cache, inner, rows, 1, inner, inner * rows, kPage)) return rc;
+    const int hg = group_heads(a->kv_heads), span = unit_keys(a->kv_heads) < kPage ? unit_keys(a->kv_heads) : kPage;
+    for (int v = 0; v < 2; ++v) {  // boxes of the narrow kernel (the group's heads) and of the wide one (a head of a page)
+        const uint8_t* cache = v ? a->v_cache : a->k_cache;
+        if (int rc = mono_tmap_encode_box3(reinterpret_cast<mono_tmap_t*>(v ? &p.vmap : &p.kmap), cache, kDim, rows, a->kv_heads, inner, kDim, span, hg)) return rc;
+        if (int rc = mono_tmap_encode_box3(reinterpret_cast<mono_tmap_t*>(v ? &p.vmap1 : &p.kmap1), cache, kDim, rows, a->kv_heads, inner, kDim, kPage, 1)) return rc;
+    }
     p.a = *a;
     uint8_t* at = reinterpret_cast<uint8_t*>(a->scratch);
     p.s.rec = reinterpret_cast<Record*>(at);
@@ -563,7 +631,7 @@ extern "C" int mono_prefix_attn_launch(const mono_prefix_attn_args* a, void* str
     p.s.seg[0] = reinterpret_cast<float*>(at);
     p.s.seg[1] = reinterpret_cast<float*>(at + narrow_bytes(a->tokens, a->q_heads, a->kv_heads, a->seqs, a->groups));
     const cudaStream_t st = (cudaStream_t)stream;
-    constexpr size_t fixed = 1024 + kStages * 2 * kTileBytes + kConsumers * 16 * kPitch * sizeof(float) + 2 * kQBytes;
+    constexpr size_t fixed = 1024 + kStages * 2 * kTileBytes + 4 * 16 * kPitch * sizeof(float);
     const size_t smem = fixed + 2 * (size_t)(a->seqs + a->groups + 1) * 4;
     static std::atomic<uint64_t> attr_once{0};  // bit d: set on device d
     if (attr_needed(attr_once)) {
@@ -575,7 +643,7 @@ extern "C" int mono_prefix_attn_launch(const mono_prefix_attn_args* a, void* str
         }
         attr_done(attr_once);
     }
-    const int narrow = 2 * sm_or_default();
+    const int narrow = sm_or_default();
     const int wide = (long)a->tokens * (a->q_heads / a->kv_heads) >= kWideRows ? sm_or_default() : 0;  // no entry has more rows than the step
     const uint64_t q_rows = (uint64_t)a->tokens * a->q_heads;
     if (wide)

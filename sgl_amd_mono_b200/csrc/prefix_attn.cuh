@@ -53,15 +53,21 @@ __device__ __forceinline__ int row_limit(const Entry& n, int row, int G) {
     return n.causal ? n.len - n.ntok + 1 + row / G : n.len;
 }
 
-// A kernel's view of the work: narrow (16-row tiles) or wide (256-row tiles), in units of one page of keys.  A wide item
-// of at most kWideHalf rows gives its CTA's two halves the same rows and alternate pages, so that its units are two pages
-// and cost what the others' do.
+// A kernel's view of the work: narrow (16-row tiles, for a group of up to 8 kv heads at once) or wide (256-row tiles, one kv
+// head).  A narrow unit is 128 rows of K and V, (keys x heads of the group): a token's heads lie side by side in the
+// cache, and read together they come from HBM at its full rate, which they do not head by head.  A wide unit is one page;
+// a wide item of at most kWideHalf rows gives its CTA's two halves the same rows and alternate pages, so that its units
+// are two pages and cost what the others' do.
 template <bool WIDE>
 struct Shape {
     static constexpr int kTile = WIDE ? 256 : 16;
     static constexpr int kSegFloats = 2 * kTile + kTile * kDim;  // max, sum, values
 };
 constexpr int kWideHalf = 128;
+// kv heads of a narrow group (the last group of a step may have fewer): a power of two
+__host__ __device__ __forceinline__ int group_heads(int kv_heads) { return kv_heads >= 8 ? 8 : kv_heads >= 4 ? 4 : kv_heads >= 2 ? 2 : 1; }
+__host__ __device__ __forceinline__ int head_groups(int kv_heads) { return (kv_heads + group_heads(kv_heads) - 1) / group_heads(kv_heads); }
+__host__ __device__ __forceinline__ int unit_keys(int kv_heads) { return 128 / group_heads(kv_heads); }
 // rows of an entry from which the wide kernel takes it
 constexpr int kWideRows = 48;
 
@@ -75,7 +81,8 @@ __device__ __forceinline__ Work entry_work(const mono_prefix_attn_args& a, const
     Work w = {0, 0, 0};
     if ((rows >= kWideRows) != WIDE || rows <= 0 || n.len <= 0) return w;
     w.tiles = (rows + Shape<WIDE>::kTile - 1) / Shape<WIDE>::kTile;
-    w.units = w.last = (n.len + kPage - 1) / kPage;
+    const int keys = WIDE ? kPage : unit_keys(a.kv_heads);
+    w.units = w.last = (n.len + keys - 1) / keys;
     if (WIDE && rows - (w.tiles - 1) * Shape<WIDE>::kTile <= kWideHalf) w.last = (w.units + 1) / 2;
     return w;
 }
@@ -83,7 +90,7 @@ __device__ __forceinline__ Work entry_work(const mono_prefix_attn_args& a, const
 // What the merge has to know of an entry, from the kernel that has the entry.
 struct alignas(16) Record {
     int tok0, ntok;
-    uint32_t off, item;  // the entry's first unit and item of kv head 0
+    uint32_t off, item;  // the entry's first unit and item of kv head (narrow: head group) 0
     int tiles, units, last, wide;
 };
 // Where things lie in the scratch.  CTA c's segment of item i is number c + i: both grow along the list of units, so no
@@ -97,10 +104,9 @@ struct Scratch {
     float* q_scale;        // what undoes their scale
 };
 
-// off[0..E]: units of one kv head before entry e (off[E]: all of them); item[0..E]: items likewise.  The list of units
-// runs through all entries for kv head 0, then for kv head 1, ...: CTAs of different heads walk the same pages at the
-// same time, and a page's rows, which lie head beside head, are fetched from HBM together.  Called by all threads of a
-// block; the blocks together leave the merge's records.
+// off[0..E]: units of one kv head (narrow: head group) before entry e (off[E]: all of them); item[0..E]: items likewise.  The
+// list of units runs through all entries for kv head 0, then for kv head 1, ...  Called by all threads of a block; the
+// blocks together leave the merge's records.
 template <bool WIDE, int THREADS>
 __device__ __forceinline__ void make_plan(const mono_prefix_attn_args& a, const Scratch& s, uint32_t* off, uint32_t* item, uint32_t* red /* [2 * 32] */) {
     const int E = a.groups + a.seqs, per = (E + THREADS - 1) / THREADS;
@@ -158,7 +164,7 @@ __device__ __forceinline__ void make_plan(const mono_prefix_attn_args& a, const 
     }
     __syncthreads();
 }
-// A place in the list: kv head, entry, unit of the entry.
+// A place in the list: kv head (narrow: head group), entry, unit of the entry.
 struct Place {
     int head, e;
     uint32_t local;
@@ -180,7 +186,7 @@ __device__ __forceinline__ Place place_of(const uint32_t* off, int E, uint32_t u
 __device__ __forceinline__ uint32_t part_size(uint32_t U, uint32_t ctas) { return max((U + ctas - 1) / ctas, 1u); }
 
 struct alignas(64) Params {
-    CUtensorMap kmap, vmap, qmap;
+    CUtensorMap kmap, vmap, kmap1, vmap1, qmap;  // boxes of a head group, of one head's page, of 128 query rows
     mono_prefix_attn_args a;
     Scratch s;
 };

@@ -245,8 +245,8 @@ __global__ void __launch_bounds__(kThreadsWide, 1) prefix_wide_kernel(const __gr
         mbar_init(&j_full, 128);
         mbar_init(&j_done, 128);
         mbar_fence_init();
-        prefetch_tmap(&p.kmap);
-        prefetch_tmap(&p.vmap);
+        prefetch_tmap(&p.kmap1);
+        prefetch_tmap(&p.vmap1);
         prefetch_tmap(&p.qmap);
     }
     if (warp == kMmaWarp) {
@@ -307,10 +307,10 @@ __global__ void __launch_bounds__(kThreadsWide, 1) prefix_wide_kernel(const __gr
                             if (it < kKStages || wait_on(&k_empty[ks], ((it / kKStages) - 1) & 1, abortp, wait_ns)) {
                                 page_ok[it % kOkRing] = g >= 0;
                                 mbar_expect_tx(&k_full[ks], bytes);
-                                if (g >= 0) tma_load_3d(kbuf + ks * kKTile, &p.kmap, x.head * kDim, g * kPage, 0, &k_full[ks]);
+                                if (g >= 0) tma_load_3d(kbuf + ks * kKTile, &p.kmap1, 0, g * kPage, x.head, &k_full[ks]);
                                 if (it < kVStages || wait_on(&v_empty[vs], ((it / kVStages) - 1) & 1, abortp, wait_ns)) {
                                     mbar_expect_tx(&v_full[vs], bytes);
-                                    if (g >= 0) tma_load_3d(vbuf + vs * kVTile, &p.vmap, x.head * kDim, g * kPage, 0, &v_full[vs]);
+                                    if (g >= 0) tma_load_3d(vbuf + vs * kVTile, &p.vmap1, 0, g * kPage, x.head, &v_full[vs]);
                                 }
                             }
                         }

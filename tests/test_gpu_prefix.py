@@ -212,7 +212,14 @@ def _attend(hq, hk, ntok, own, starts, prefix, seed=0, columns=0, qmul=2.0, **kw
     (12, 2, [3, 1, 5, 2], [40, 1, 5, 130], [0, 4], [500]),           # several query tokens, causal
     (6, 1, [1] * 40, [1 + 7 * i for i in range(40)], [0, 40], [190]),   # more rows than one tile of the prefix
     (6, 3, [70, 1, 200], [70, 65, 333], [0, 2, 3], [77, 130]),       # prompt chunks
-    (24, 2, [1] * 33, [9] * 33, [0, 33], [1111])])
+    (24, 2, [1] * 33, [9] * 33, [0, 33], [1111]),
+    # kv heads that do not fill a group of heads, and more than one group
+    (6, 3, [1, 2], [130, 70], [0, 2], [200]),
+    (5, 5, [1, 1], [65, 3], [0, 2], [129]),
+    (14, 7, [2, 1], [40, 300], [0, 1, 2], [10, 64]),
+    (12, 12, [1] * 3, [63, 64, 1000], [0, 3], [65]),
+    (16, 16, [1] * 2, [17, 200], [], []),
+    (32, 2, [1] * 7, [500, 1, 16, 17, 31, 48, 49], [0, 7], [2000])])
 def test_attend(hq, hk, ntok, own, starts, prefix):
     _attend(hq, hk, ntok, own, starts, prefix, columns=2)
 

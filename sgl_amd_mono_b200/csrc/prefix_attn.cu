@@ -19,7 +19,7 @@ constexpr int kConsumers = 8;                        // warps that compute; one 
 constexpr int kThreads = (kConsumers + 1) * 32;
 constexpr int kStages = 5;
 constexpr int kTileBytes = 128 * kDim;               // 128 rows of K (or V): 128 / heads keys of each head of the group
-constexpr int kQuarter = 36, kPitch = 4 * kQuarter + 4;  // floats of a quarter and of a combine row: spread over the banks
+constexpr int kPitch = kDim + 4;                     // floats of a joint row: rows two apart start eight banks apart
 constexpr float kPBias = 14.f;                       // P is formed as 2^14 p, so that f16 keeps small weights
 
 // D(16x8,f32) += A(16x16,f16,row) * B(16x8,f16,col)
@@ -50,55 +50,60 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 }
 __device__ __forceinline__ void consumer_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
-// The queries of one tile in the layout of the A fragments, and their scales.  The contraction's order is free as long
-// as both operands share it, so thread (g, t) of a fragment takes dims 32 t .. 32 t + 31 of its rows: a key's 32 bytes
-// are then two 16-byte shared loads.  A row is scaled by a power of two so that its largest value lies in
-// [2^13, 2^14): f16 then holds every bf16 value down to 2^-28 of that exactly.
-__device__ __forceinline__ void load_q(const mono_prefix_attn_args& a, const Entry& n, int head, int row0, int G, uint32_t q[8][4], float qscale[2], int lim[2]) {
-    const int g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
-    uint4 raw[2][4];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int row = row0 + g + 8 * i;
-        const bool live = row < n.ntok * G;
-        const int r = live ? row : 0;
-        const __nv_bfloat16* src = reinterpret_cast<const __nv_bfloat16*>(a.q) + (size_t)(n.tok0 + r / G) * a.q_ld + (size_t)(head * G + r % G) * kDim + t * 32;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) raw[i][j] = live ? __ldg(reinterpret_cast<const uint4*>(src) + j) : make_uint4(0, 0, 0, 0);
-        lim[i] = live ? row_limit(n, row, G) : INT32_MAX;  // a row that does not exist needs no mask
-    }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const uint32_t* w = reinterpret_cast<const uint32_t*>(raw[i]);
-        float amax = 0.f;
-#pragma unroll
-        for (int j = 0; j < 16; ++j) amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(w[j] << 16)), fabsf(__uint_as_float(w[j] & 0xFFFF0000u))));
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-        // exponent field of the largest value, kept where 2^(13 - e) and its inverse are normal numbers
-        const int e = clamp_int((int)(__float_as_uint(amax) >> 23), 30, 254);
-        const float up = __uint_as_float((uint32_t)(267 - e) << 23);  // 2^(13 - (e - 127))
-        qscale[i] = __uint_as_float((uint32_t)(e - 13) << 23) * (a.sm_scale * a.k_scale * 1.4426950408889634f);
-#pragma unroll
-        for (int s = 0; s < 8; ++s) {
-            q[s][i] = pack_f16(__uint_as_float(w[2 * s] << 16) * up, __uint_as_float(w[2 * s] & 0xFFFF0000u) * up);
-            q[s][2 + i] = pack_f16(__uint_as_float(w[2 * s + 1] << 16) * up, __uint_as_float(w[2 * s + 1] & 0xFFFF0000u) * up);
-        }
-    }
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {  // of a matrix of f16: lane (g, t) has row g, columns 2t, 2t + 1
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
+    return r;
 }
 
-// Up to 16 rows per tile, of every head of a group.  A unit's 128 rows of K and V arrive by one TMA box each, head after
+// The queries of eight rows in the layout of the B fragments of S^T = K Q^T, and their scales.  The contraction's order
+// is free as long as both operands share it, so thread (g, t) of a fragment takes dims 32 t .. 32 t + 31 of row g: a key's
+// 32 bytes are then two 16-byte shared loads.  A row is scaled by a power of two so that its largest value lies in
+// [2^13, 2^14): f16 then holds every bf16 value down to 2^-28 of that exactly.  scale: of rows 2t and 2t + 1.
+__device__ __forceinline__ void load_q(const mono_prefix_attn_args& a, const Entry& n, int head, int row0, int G, uint32_t q[8][2], float scale[2]) {
+    const int g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3, row = row0 + g;
+    const bool live = row < n.ntok * G;
+    const int r = live ? row : 0;
+    const __nv_bfloat16* src = reinterpret_cast<const __nv_bfloat16*>(a.q) + (size_t)(n.tok0 + r / G) * a.q_ld + (size_t)(head * G + r % G) * kDim + t * 32;
+    uint4 raw[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) raw[j] = live ? __ldg(reinterpret_cast<const uint4*>(src) + j) : make_uint4(0, 0, 0, 0);
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(raw);
+    float amax = 0.f;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(w[j] << 16)), fabsf(__uint_as_float(w[j] & 0xFFFF0000u))));
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+    // exponent field of the largest value, kept where 2^(13 - e) and its inverse are normal numbers
+    const int e = clamp_int((int)(__float_as_uint(amax) >> 23), 30, 254);
+    const float up = __uint_as_float((uint32_t)(267 - e) << 23);  // 2^(13 - (e - 127))
+    const float back = __uint_as_float((uint32_t)(e - 13) << 23) * (a.sm_scale * a.k_scale * 1.4426950408889634f);
+#pragma unroll
+    for (int s = 0; s < 8; ++s)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) q[s][i] = pack_f16(__uint_as_float(w[2 * s + i] << 16) * up, __uint_as_float(w[2 * s + i] & 0xFFFF0000u) * up);
+    scale[0] = __shfl_sync(0xffffffffu, back, 8 * t);
+    scale[1] = __shfl_sync(0xffffffffu, back, 8 * t + 4);
+}
+
+// Up to 8 NT rows per tile, of every head of a group.  A unit's 128 rows of K and V arrive by one TMA box each, head after
 // head (128-byte swizzle, which makes the 16-byte shared loads below free of bank conflicts); each of the eight warps
 // takes 16 keys of one head, with a running maximum and sum of its own.  Where a head has several warps they join their
 // parts at the segment's end.  The ninth warp keeps the ring of units full.  Bound: HBM; K and V stay bytes until a warp
 // has them in registers, where they become f16 exactly.
+//
+// Both products are formed transposed: S^T[key][row] = K Q^T and O^T[dim][row] += V^T P^T, with keys and dims as the 16
+// rows of the fragments and NT times 8 query rows as their columns: one token's heads are at most eight as a rule, and as
+// the 16 rows they left most of the work empty.  P^T is turned from result to operand by two 8 x 8 transpositions.
+template <int NT>
 __global__ void __launch_bounds__(kThreads, 1) prefix_narrow_kernel(const __grid_constant__ Params p) {
+    constexpr int kTile = 8 * NT;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    float* comb = reinterpret_cast<float*>(ring + kStages * 2 * kTileBytes);  // [4 warps][16 rows][kPitch]
+    float* comb = reinterpret_cast<float*>(ring + kStages * 2 * kTileBytes);  // [4 warps][kNarrowTile rows][kPitch]
     const mono_prefix_attn_args& a = p.a;
     const int E = a.groups + a.seqs;
-    uint32_t* off = reinterpret_cast<uint32_t*>(comb + 4 * 16 * kPitch);
+    uint32_t* off = reinterpret_cast<uint32_t*>(comb + 4 * kNarrowTile * kPitch);
     uint32_t* item = off + E + 1;
     __shared__ uint64_t full[kStages], empty[kStages];
     __shared__ int page_ok[kStages];  // bit i: page i of the unit (a unit of one head has two)
@@ -184,17 +189,31 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_narrow_kernel(const __grid
                 const bool mine = head < a.kv_heads;
                 const int tile = (int)(at.local / wk.units);
                 const int p0 = (int)(at.local - (uint32_t)tile * wk.units), cnt = (int)min((uint32_t)(wk.units - p0), u1 - u);
-                uint32_t q[8][4];
-                float qs[2], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-                int lim[2];
-                load_q(a, en, mine ? head : 0, tile * 16, G, q, qs, lim);
-                const int lim_all = min(en.len, __reduce_min_sync(0xffffffffu, min(lim[0], lim[1])));  // keys below it are seen by every row
+                const int rows = en.ntok * G - tile * kTile;
+                uint32_t q[NT][8][2];
+                float qs[NT][2], m[NT][2], l[NT][2];
+                int lim[NT][2], lim_all = en.len;  // keys below lim_all are seen by every row
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    load_q(a, en, mine ? head : 0, tile * kTile + n * 8, G, q[n], qs[n]);
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        const int row = n * 8 + 2 * t + c;
+                        lim[n][c] = row < rows ? min(row_limit(en, tile * kTile + row, G), en.len) : en.len;
+                        lim_all = min(lim_all, lim[n][c]);
+                        m[n][c] = -INFINITY;
+                        l[n][c] = 0.f;
+                    }
+                }
+                lim_all = __reduce_min_sync(0xffffffffu, lim_all);
                 MONO_TL(tl_narrow, 3 + 4 * nth);  // the first three items
-                float o[16][4];
+                float o[8][NT][4];  // dims 16 g + 2 j, 16 g + 2 j + 1 of rows 8 n + 2 t, 8 n + 2 t + 1
 #pragma unroll
-                for (int j = 0; j < 16; ++j)
+                for (int j = 0; j < 8; ++j)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) o[j][i] = 0.f;
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) o[j][n][i] = 0.f;
                 // Two units a turn where there are two: a warp's chain of loads, products, shuffles and exponentials is long, and
                 // the second unit's runs beside the first's.
                 for (int i = 0; i < cnt; i += 2) {
@@ -214,23 +233,25 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_narrow_kernel(const __grid
                     if (!have) break;
                     if (i == 0) MONO_TL(tl_narrow, 4 + 4 * nth);
                     if (on[0] || on[1]) {
-                        float s[2][2][4];
+                        float s[2][NT][4];  // keys g and g + 8, rows 2t and 2t + 1
 #pragma unroll
                         for (int z = 0; z < 2; ++z)
 #pragma unroll
-                            for (int nt = 0; nt < 2; ++nt)
+                            for (int n = 0; n < NT; ++n)
 #pragma unroll
-                                for (int j = 0; j < 4; ++j) s[z][nt][j] = on[z] ? 0.f : -INFINITY;
+                                for (int j = 0; j < 4; ++j) s[z][n][j] = on[z] ? 0.f : -INFINITY;
 #pragma unroll
                         for (int z = 0; z < 2; ++z) {
                             if (!on[z]) continue;
+                            const uint32_t rowa = kb[z] + g * 128, c0 = ((2 * t) ^ g) << 4, c1 = ((2 * t + 1) ^ g) << 4;
+                            const uint4 k00 = lds128(rowa + c0), k01 = lds128(rowa + c1), k10 = lds128(rowa + 1024 + c0), k11 = lds128(rowa + 1024 + c1);
+                            const uint32_t wa[8] = {k00.x, k00.y, k00.z, k00.w, k01.x, k01.y, k01.z, k01.w};
+                            const uint32_t wb[8] = {k10.x, k10.y, k10.z, k10.w, k11.x, k11.y, k11.z, k11.w};
 #pragma unroll
-                            for (int nt = 0; nt < 2; ++nt) {
-                                const uint32_t rowa = kb[z] + (nt * 8 + g) * 128;
-                                const uint4 k0 = lds128(rowa + (((2 * t) ^ g) << 4)), k1 = lds128(rowa + (((2 * t + 1) ^ g) << 4));
-                                const uint32_t w[8] = {k0.x, k0.y, k0.z, k0.w, k1.x, k1.y, k1.z, k1.w};
+                            for (int j = 0; j < 8; ++j) {
+                                const uint32_t fa[4] = {e4m3x2_to_f16x2(wa[j]), e4m3x2_to_f16x2(wb[j]), e4m3x2_to_f16x2(wa[j] >> 16), e4m3x2_to_f16x2(wb[j] >> 16)};
 #pragma unroll
-                                for (int j = 0; j < 8; ++j) mma_f16(s[z][nt], q[j], e4m3x2_to_f16x2(w[j]), e4m3x2_to_f16x2(w[j] >> 16));
+                                for (int n = 0; n < NT; ++n) mma_f16(s[z][n], fa, q[n][j][0], q[n][j][1]);
                             }
                         }
                         // scores stay in the units of the product: qs > 0, so their maximum is the scaled scores'
@@ -238,52 +259,53 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_narrow_kernel(const __grid
                         for (int z = 0; z < 2; ++z)
                             if (on[z] && key0[z] + 16 > lim_all) {
 #pragma unroll
-                                for (int nt = 0; nt < 2; ++nt)
+                                for (int n = 0; n < NT; ++n)
 #pragma unroll
                                     for (int j = 0; j < 4; ++j)
-                                        if (key0[z] + nt * 8 + 2 * t + (j & 1) >= min(lim[j >> 1], en.len)) s[z][nt][j] = -INFINITY;
+                                        if (key0[z] + g + 8 * (j >> 1) >= lim[n][j & 1]) s[z][n][j] = -INFINITY;
                             }
-                        float base[2], alpha[2];
+                        bool moved = false;
+                        float alpha[NT][2];
+                        uint32_t pb[2][NT][2];
 #pragma unroll
-                        for (int r = 0; r < 2; ++r) {
-                            float mx = -INFINITY;
+                        for (int n = 0; n < NT; ++n) {
+                            float base[2];
 #pragma unroll
-                            for (int z = 0; z < 2; ++z) mx = max_nan(mx, max_nan(max_nan(s[z][0][2 * r], s[z][0][2 * r + 1]), max_nan(s[z][1][2 * r], s[z][1][2 * r + 1])));
-                            mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-                            mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                            const float mn = max_nan(m[r], mx * qs[r]), zero = mn == -INFINITY ? 0.f : mn;
-                            // a row that has seen no key yet keeps max = -inf, and weights of 0
-                            alpha[r] = ex2(m[r] - zero);
-                            m[r] = mn;
-                            l[r] *= alpha[r];
-                            base[r] = kPBias - zero;
-                        }
-                        uint32_t pa[2][4];
+                            for (int c = 0; c < 2; ++c) {
+                                float mx = max_nan(max_nan(s[0][n][c], s[0][n][c + 2]), max_nan(s[1][n][c], s[1][n][c + 2]));
 #pragma unroll
-                        for (int z = 0; z < 2; ++z) {
-                            float pv[2][4];
+                                for (int x = 4; x < 32; x *= 2) mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+                                const float mn = max_nan(m[n][c], mx * qs[n][c]), zero = mn == -INFINITY ? 0.f : mn;
+                                // a row that has seen no key yet keeps max = -inf, and weights of 0
+                                alpha[n][c] = ex2(m[n][c] - zero);
+                                moved = moved || alpha[n][c] != 1.f;
+                                m[n][c] = mn;
+                                l[n][c] *= alpha[n][c];
+                                base[c] = kPBias - zero;
+                            }
 #pragma unroll
-                            for (int nt = 0; nt < 2; ++nt)
+                            for (int z = 0; z < 2; ++z) {
+                                float pv[4];
 #pragma unroll
                                 for (int j = 0; j < 4; ++j) {
-                                    pv[nt][j] = ex2(fmaf(s[z][nt][j], qs[j >> 1], base[j >> 1]));
-                                    l[j >> 1] += pv[nt][j];
+                                    pv[j] = ex2(fmaf(s[z][n][j], qs[n][j & 1], base[j & 1]));
+                                    l[n][j & 1] += pv[j];
                                 }
-                            pa[z][0] = pack_f16(pv[0][0], pv[0][1]);
-                            pa[z][1] = pack_f16(pv[0][2], pv[0][3]);
-                            pa[z][2] = pack_f16(pv[1][0], pv[1][1]);
-                            pa[z][3] = pack_f16(pv[1][2], pv[1][3]);
-                        }
-                        if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
-#pragma unroll
-                            for (int j = 0; j < 16; ++j) {
-                                o[j][0] *= alpha[0]; o[j][1] *= alpha[0];
-                                o[j][2] *= alpha[1]; o[j][3] *= alpha[1];
+                                pb[z][n][0] = transpose8x8(pack_f16(pv[0], pv[1]));
+                                pb[z][n][1] = transpose8x8(pack_f16(pv[2], pv[3]));
                             }
                         }
-                        // V: thread (g, t) takes dims 16 g .. 16 g + 15 of keys 2t, 2t + 1, 2t + 8, 2t + 9; output column g of
-                        // product j is dim 16 g + j.  Keys behind the entry's last hold anything, NaN among it, and 0 x NaN is
-                        // NaN, so their bytes become zeros.
+                        if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+                            for (int j = 0; j < 8; ++j)
+#pragma unroll
+                                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                                    for (int i = 0; i < 4; ++i) o[j][n][i] *= alpha[n][i & 1];
+                        }
+                        // V: thread (g, t) takes dims 16 g .. 16 g + 15 of keys 2t, 2t + 1, 2t + 8, 2t + 9; rows g and g + 8 of
+                        // product j are dims 16 g + 2 j and 16 g + 2 j + 1.  Keys behind the entry's last hold anything, NaN
+                        // among it, and 0 x NaN is NaN, so their bytes become zeros.
 #pragma unroll
                         for (int z = 0; z < 2; ++z) {
                             if (!on[z]) continue;
@@ -304,10 +326,13 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_narrow_kernel(const __grid
                             for (int j = 0; j < 4; ++j) {
                                 const uint32_t a01 = __byte_perm(vw[0][j], vw[1][j], 0x5140), a23 = __byte_perm(vw[0][j], vw[1][j], 0x7362);
                                 const uint32_t b01 = __byte_perm(vw[2][j], vw[3][j], 0x5140), b23 = __byte_perm(vw[2][j], vw[3][j], 0x7362);
-                                mma_f16(o[4 * j], pa[z], e4m3x2_to_f16x2(a01), e4m3x2_to_f16x2(b01));
-                                mma_f16(o[4 * j + 1], pa[z], e4m3x2_to_f16x2(a01 >> 16), e4m3x2_to_f16x2(b01 >> 16));
-                                mma_f16(o[4 * j + 2], pa[z], e4m3x2_to_f16x2(a23), e4m3x2_to_f16x2(b23));
-                                mma_f16(o[4 * j + 3], pa[z], e4m3x2_to_f16x2(a23 >> 16), e4m3x2_to_f16x2(b23 >> 16));
+                                const uint32_t f01[4] = {e4m3x2_to_f16x2(a01), e4m3x2_to_f16x2(a01 >> 16), e4m3x2_to_f16x2(b01), e4m3x2_to_f16x2(b01 >> 16)};
+                                const uint32_t f23[4] = {e4m3x2_to_f16x2(a23), e4m3x2_to_f16x2(a23 >> 16), e4m3x2_to_f16x2(b23), e4m3x2_to_f16x2(b23 >> 16)};
+#pragma unroll
+                                for (int n = 0; n < NT; ++n) {
+                                    mma_f16(o[2 * j][n], f01, pb[z][n][0], pb[z][n][1]);
+                                    mma_f16(o[2 * j + 1][n], f23, pb[z][n][0], pb[z][n][1]);
+                                }
                             }
                         }
                     }
@@ -321,80 +346,85 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_narrow_kernel(const __grid
                 MONO_TL(tl_narrow, 5 + 4 * nth);
                 // ---- the segment's rows of this head
 #pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-                    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-                }
-                if (slots > 1) {  // the head's warps bring their parts to one maximum and add them up in halves
-                    if (t == 0) {
+                for (int n = 0; n < NT; ++n)
 #pragma unroll
-                        for (int r = 0; r < 2; ++r) {
-                            s_m[warp][g + 8 * r] = m[r];
-                            s_l[warp][g + 8 * r] = l[r];
-                        }
+                    for (int c = 0; c < 2; ++c)
+#pragma unroll
+                        for (int x = 4; x < 32; x *= 2) l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], x);
+                if (slots > 1) {  // the head's warps bring their parts to one maximum and add them up in halves
+                    if (g == 0) {
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int c = 0; c < 2; ++c) {
+                                s_m[warp][n * 8 + 2 * t + c] = m[n][c];
+                                s_l[warp][n * 8 + 2 * t + c] = l[n][c];
+                            }
                     }
                     consumer_sync();
-                    float f[2];
 #pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        float top = -INFINITY, sum = 0.f;
-                        for (int k = 0; k < slots; ++k) top = fmaxf(top, s_m[k * hg + h][g + 8 * r]);
-                        for (int k = 0; k < slots; ++k) {
-                            const float mk = s_m[k * hg + h][g + 8 * r];
-                            sum += mk == -INFINITY ? 0.f : s_l[k * hg + h][g + 8 * r] * ex2(mk - top);
+                    for (int n = 0; n < NT; ++n) {
+                        float f[2];
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            const int row = n * 8 + 2 * t + c;
+                            float top = -INFINITY, sum = 0.f;
+                            for (int k = 0; k < slots; ++k) top = fmaxf(top, s_m[k * hg + h][row]);
+                            for (int k = 0; k < slots; ++k) {
+                                const float mk = s_m[k * hg + h][row];
+                                sum += mk == -INFINITY ? 0.f : s_l[k * hg + h][row] * ex2(mk - top);
+                            }
+                            f[c] = m[n][c] == -INFINITY ? 0.f : ex2(m[n][c] - top);
+                            m[n][c] = top;
+                            l[n][c] = sum;
                         }
-                        f[r] = m[r] == -INFINITY ? 0.f : ex2(m[r] - top);
-                        m[r] = top;
-                        l[r] = sum;
-                    }
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        o[j][0] *= f[0]; o[j][1] *= f[0];
-                        o[j][2] *= f[1]; o[j][3] *= f[1];
+                        for (int j = 0; j < 8; ++j)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) o[j][n][i] *= f[i & 1];
                     }
                     for (int half = slots / 2; half >= 1; half /= 2) {
-                        float* at4 = comb + ((slot & (half - 1)) * hg + h) * 16 * kPitch + t * kQuarter;
+                        float* at4 = comb + ((slot & (half - 1)) * hg + h) * kTile * kPitch + g * 16;
                         if (slot >= half && slot < 2 * half) {
 #pragma unroll
-                            for (int r = 0; r < 2; ++r)
+                            for (int n = 0; n < NT; ++n)
 #pragma unroll
                                 for (int c = 0; c < 2; ++c)
 #pragma unroll
-                                    for (int j = 0; j < 16; j += 4)
-                                        *reinterpret_cast<float4*>(at4 + (g + 8 * r) * kPitch + c * 16 + j) = make_float4(o[j][2 * r + c], o[j + 1][2 * r + c], o[j + 2][2 * r + c], o[j + 3][2 * r + c]);
+                                    for (int j = 0; j < 8; j += 2)
+                                        *reinterpret_cast<float4*>(at4 + (n * 8 + 2 * t + c) * kPitch + 2 * j) = make_float4(o[j][n][c], o[j][n][c + 2], o[j + 1][n][c], o[j + 1][n][c + 2]);
                         }
                         consumer_sync();
                         if (slot < half) {
 #pragma unroll
-                            for (int r = 0; r < 2; ++r)
+                            for (int n = 0; n < NT; ++n)
 #pragma unroll
                                 for (int c = 0; c < 2; ++c)
 #pragma unroll
-                                    for (int j = 0; j < 16; j += 4) {
-                                        const float4 v = *reinterpret_cast<const float4*>(at4 + (g + 8 * r) * kPitch + c * 16 + j);
-                                        o[j][2 * r + c] += v.x; o[j + 1][2 * r + c] += v.y; o[j + 2][2 * r + c] += v.z; o[j + 3][2 * r + c] += v.w;
+                                    for (int j = 0; j < 8; j += 2) {
+                                        const float4 v = *reinterpret_cast<const float4*>(at4 + (n * 8 + 2 * t + c) * kPitch + 2 * j);
+                                        o[j][n][c] += v.x; o[j][n][c + 2] += v.y; o[j + 1][n][c] += v.z; o[j + 1][n][c + 2] += v.w;
                                     }
                         }
                         consumer_sync();
                     }
                 }
                 if (slot == 0 && mine) {
-                    float* seg = p.s.seg[0] + ((size_t)(blockIdx.x + at.head * item[E] + item[at.e] + tile) * hg + h) * Shape<false>::kSegFloats;
-                    const int rows = min(16, en.ntok * G - tile * 16);
+                    float* seg = p.s.seg[0] + ((size_t)(blockIdx.x + at.head * item[E] + item[at.e] + tile) * hg + h) * seg_floats(kTile);
 #pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        const int row = g + 8 * r;
-                        if (row >= rows) continue;
-                        if (t == 0) {
-                            seg[row] = l[r] != l[r] ? l[r] : m[r] - kPBias;  // a row of NaN stays one
-                            seg[16 + row] = l[r];
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            const int row = n * 8 + 2 * t + c;
+                            if (row >= rows) continue;
+                            if (g == 0) {
+                                seg[row] = l[n][c] != l[n][c] ? l[n][c] : m[n][c] - kPBias;  // a row of NaN stays one
+                                seg[kTile + row] = l[n][c];
+                            }
+#pragma unroll
+                            for (int j = 0; j < 8; j += 2)
+                                *reinterpret_cast<float4*>(seg + 2 * kTile + row * kDim + g * 16 + 2 * j) = make_float4(o[j][n][c], o[j][n][c + 2], o[j + 1][n][c], o[j + 1][n][c + 2]);
                         }
-#pragma unroll
-                        for (int c = 0; c < 2; ++c)
-#pragma unroll
-                            for (int j = 0; j < 16; j += 4)
-                                *reinterpret_cast<float4*>(seg + 32 + row * kDim + t * 32 + c * 16 + j) = make_float4(o[j][2 * r + c], o[j + 1][2 * r + c], o[j + 2][2 * r + c], o[j + 3][2 * r + c]);
-                    }
                 }
                 MONO_TL(tl_narrow, 6 + 4 * nth);
                 u += cnt;
@@ -423,18 +453,18 @@ __device__ __forceinline__ Parts parts_of(const mono_prefix_attn_args& a, const 
     const uint32_t per_head = s.total[wide][0], items = s.total[wide][1];
     if (n.tiles == 0 || per_head == 0) return r;  // no keys, or refused tables
     const int kh = head / G, row = (token - n.tok0) * G + head - kh * G;
-    r.rows = wide ? Shape<true>::kTile : Shape<false>::kTile;
+    r.rows = wide ? kWideTile : narrow_tile(a);
     const int tile = row / r.rows, at = row - tile * r.rows;
     const int hg = wide ? 1 : group_heads(a.kv_heads), list = kh / hg, lists = wide ? a.kv_heads : head_groups(a.kv_heads);
     const uint32_t per = part_size(per_head * lists, wide ? wide_ctas : narrow_ctas);
     const uint32_t first = list * per_head + n.off + (uint32_t)tile * n.units;
     const uint32_t c0 = first / per, c1 = (first + (tile == n.tiles - 1 ? n.last : n.units) - 1) / per;
-    r.stride = wide ? Shape<true>::kSegFloats : hg * Shape<false>::kSegFloats;
-    const float* seg = s.seg[wide] + (size_t)(c0 + list * items + n.item + tile) * r.stride + (kh - list * hg) * Shape<false>::kSegFloats;
+    r.stride = hg * seg_floats(r.rows);
+    const float* seg = s.seg[wide] + (size_t)(c0 + list * items + n.item + tile) * r.stride + (kh - list * hg) * seg_floats(r.rows);
     r.m = seg + at;
     // narrow: rows of 128 values; wide: four dims of all rows, then the next four (as a thread per row writes them)
-    r.v = seg + 2 * r.rows + (wide ? (sub * 2 * Shape<true>::kTile + at) * 4 : at * kDim + sub * 8);
-    r.step = wide ? Shape<true>::kTile * 4 : 4;
+    r.v = seg + 2 * r.rows + (wide ? (sub * 2 * kWideTile + at) * 4 : at * kDim + sub * 8);
+    r.step = wide ? kWideTile * 4 : 4;
     r.count = (int)(c1 - c0) + 1;
     return r;
 }
@@ -551,14 +581,14 @@ static size_t narrow_segments(size_t tokens, size_t q_heads, size_t kv_heads, si
 static size_t wide_segments(size_t tokens, size_t q_heads, size_t kv_heads) {
     const size_t rows = tokens * (q_heads / kv_heads);
     if (rows < kWideRows) return 0;
-    return (size_t)sm_or_default() + kv_heads * 2 * (rows / Shape<true>::kTile + rows / kWideRows);
+    return (size_t)sm_or_default() + kv_heads * 2 * (rows / kWideTile + rows / kWideRows);
 }
 // The wide kernel's queries (two planes of 128 bytes a row) and their scales; none where no entry can have so many rows.
 static size_t image_bytes(size_t tokens, size_t q_heads, size_t kv_heads) {
     return tokens * (q_heads / kv_heads) < kWideRows ? 0 : up256(tokens * q_heads * 256) + up256(tokens * q_heads * 4);
 }
 static size_t narrow_bytes(int tokens, int q_heads, int kv_heads, int seqs, int groups) {
-    return up256(narrow_segments(tokens, q_heads, kv_heads, seqs, groups) * Shape<false>::kSegFloats * sizeof(float));
+    return up256(narrow_segments(tokens, q_heads, kv_heads, seqs, groups) * seg_floats(kNarrowTile) * sizeof(float));
 }
 
 }  // namespace prefix_attn
@@ -567,7 +597,7 @@ extern "C" size_t mono_prefix_attn_scratch_bytes(int tokens, int q_heads, int kv
     using namespace prefix_attn;
     if (tokens < 1 || q_heads < 1 || kv_heads < 1 || seqs < 1 || groups < 0 || q_heads % kv_heads) return 0;
     return up256((size_t)(seqs + groups) * sizeof(Record)) + 256 + 2 * up256((size_t)tokens * 4) + image_bytes(tokens, q_heads, kv_heads) + narrow_bytes(tokens, q_heads, kv_heads, seqs, groups) +
-           wide_segments(tokens, q_heads, kv_heads) * Shape<true>::kSegFloats * sizeof(float);
+           wide_segments(tokens, q_heads, kv_heads) * seg_floats(kWideTile) * sizeof(float);
 }
 
 extern "C" int mono_prefix_attn_launch(const mono_prefix_attn_args* a, void* stream) {
@@ -631,12 +661,13 @@ extern "C" int mono_prefix_attn_launch(const mono_prefix_attn_args* a, void* str
     p.s.seg[0] = reinterpret_cast<float*>(at);
     p.s.seg[1] = reinterpret_cast<float*>(at + narrow_bytes(a->tokens, a->q_heads, a->kv_heads, a->seqs, a->groups));
     const cudaStream_t st = (cudaStream_t)stream;
-    constexpr size_t fixed = 1024 + kStages * 2 * kTileBytes + 4 * 16 * kPitch * sizeof(float);
+    constexpr size_t fixed = 1024 + kStages * 2 * kTileBytes + 4 * kNarrowTile * kPitch * sizeof(float);
     const size_t smem = fixed + 2 * (size_t)(a->seqs + a->groups + 1) * 4;
     static std::atomic<uint64_t> attr_once{0};  // bit d: set on device d
     if (attr_needed(attr_once)) {
         const size_t most = fixed + 2 * (size_t)(kMaxEntries + 1) * 4;
-        const cudaError_t e = cudaFuncSetAttribute(prefix_narrow_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
+        cudaError_t e = cudaFuncSetAttribute(prefix_narrow_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(prefix_narrow_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
         if (e != cudaSuccess) {
             mono_set_error("%s: %s", who, cudaGetErrorString(e));
             return (int)e;
@@ -649,7 +680,7 @@ extern "C" int mono_prefix_attn_launch(const mono_prefix_attn_args* a, void* str
     if (wide)
         if (int rc = mono_tmap_encode_box(reinterpret_cast<mono_tmap_t*>(&p.qmap), p.s.q_image, 128, q_rows, 2, 128, q_rows * 128, 128)) return rc;
     cudaError_t e = wide ? launch_wide(p, wide, st) : cudaSuccess;
-    if (e == cudaSuccess) e = launch_k(prefix_narrow_kernel, narrow, kThreads, smem, st, p);
+    if (e == cudaSuccess) e = launch_k(narrow_tile(*a) == 8 ? prefix_narrow_kernel<1> : prefix_narrow_kernel<2>, narrow, kThreads, smem, st, p);
     // Few rows: four warps share two heads' segments (a long prefix leaves many of them); many rows: a warp each.
     if (e == cudaSuccess) {
         if ((long)a->tokens * a->q_heads < 2048)

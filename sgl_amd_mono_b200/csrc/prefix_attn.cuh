@@ -53,16 +53,16 @@ __device__ __forceinline__ int row_limit(const Entry& n, int row, int G) {
     return n.causal ? n.len - n.ntok + 1 + row / G : n.len;
 }
 
-// A kernel's view of the work: narrow (16-row tiles, for a group of up to 8 kv heads at once) or wide (256-row tiles, one kv
+// A kernel's view of the work: narrow (8- or 16-row tiles, for a group of up to 8 kv heads at once) or wide (256-row tiles, one kv
 // head).  A narrow unit is 128 rows of K and V, (keys x heads of the group): a token's heads lie side by side in the
 // cache, and read together they come from HBM at its full rate, which they do not head by head.  A wide unit is one page;
 // a wide item of at most kWideHalf rows gives its CTA's two halves the same rows and alternate pages, so that its units
 // are two pages and cost what the others' do.
-template <bool WIDE>
-struct Shape {
-    static constexpr int kTile = WIDE ? 256 : 16;
-    static constexpr int kSegFloats = 2 * kTile + kTile * kDim;  // max, sum, values
-};
+constexpr int kWideTile = 256, kNarrowTile = 16;
+__host__ __device__ constexpr int seg_floats(int tile) { return 2 * tile + tile * kDim; }  // max, sum, values
+// Rows of a narrow tile.  With eight the products are as wide as the rows of one token of up to eight q heads; steps of
+// several tokens a sequence (or more heads) take sixteen, so as not to read their keys twice.
+__host__ __device__ __forceinline__ int narrow_tile(const mono_prefix_attn_args& a) { return a.q_heads / a.kv_heads <= 8 && a.tokens <= a.seqs ? 8 : kNarrowTile; }
 constexpr int kWideHalf = 128;
 // kv heads of a narrow group (the last group of a step may have fewer): a power of two
 __host__ __device__ __forceinline__ int group_heads(int kv_heads) { return kv_heads >= 8 ? 8 : kv_heads >= 4 ? 4 : kv_heads >= 2 ? 2 : 1; }
@@ -80,10 +80,11 @@ __device__ __forceinline__ Work entry_work(const mono_prefix_attn_args& a, const
     const int rows = n.ntok * (a.q_heads / a.kv_heads);
     Work w = {0, 0, 0};
     if ((rows >= kWideRows) != WIDE || rows <= 0 || n.len <= 0) return w;
-    w.tiles = (rows + Shape<WIDE>::kTile - 1) / Shape<WIDE>::kTile;
+    const int tile = WIDE ? kWideTile : narrow_tile(a);
+    w.tiles = (rows + tile - 1) / tile;
     const int keys = WIDE ? kPage : unit_keys(a.kv_heads);
     w.units = w.last = (n.len + keys - 1) / keys;
-    if (WIDE && rows - (w.tiles - 1) * Shape<WIDE>::kTile <= kWideHalf) w.last = (w.units + 1) / 2;
+    if (WIDE && rows - (w.tiles - 1) * kWideTile <= kWideHalf) w.last = (w.units + 1) / 2;
     return w;
 }
 

@@ -205,8 +205,8 @@ __device__ __forceinline__ Item item_at(const mono_prefix_attn_args& a, const ui
     it.head = at.head;
     const Work w = entry_work<true>(a, it.en);
     const int tile = min((int)at.local / w.units, w.tiles - 1), unit = (int)at.local - tile * w.units;
-    it.row0 = tile * Shape<true>::kTile;
-    it.rows = min(Shape<true>::kTile, it.en.ntok * G - it.row0);
+    it.row0 = tile * kWideTile;
+    it.rows = min(kWideTile, it.en.ntok * G - it.row0);
     it.split = it.rows <= kWideHalf;
     it.span = min((uint32_t)((tile == w.tiles - 1 ? w.last : w.units) - unit), u1 - u);
     it.b0 = it.split ? 2 * unit : unit;
@@ -539,13 +539,13 @@ __global__ void __launch_bounds__(kThreadsWide, 1) prefix_wide_kernel(const __gr
                     }
                 }
                 if (!(x.split && st == 1)) {
-                    float* seg = p.s.seg[1] + (size_t)x.seg * Shape<true>::kSegFloats;
+                    float* seg = p.s.seg[1] + (size_t)x.seg * seg_floats(kWideTile);
                     const int at = st * 128 + row_in;
                     if (mine) {
                         seg[at] = l != l ? l : m - kBias;
-                        seg[Shape<true>::kTile + at] = l;
+                        seg[kWideTile + at] = l;
                     }
-                    float* dst = seg + 2 * Shape<true>::kTile + at * 4;  // [32 x 4 dims][256 rows][4]
+                    float* dst = seg + 2 * kWideTile + at * 4;  // [32 x 4 dims][256 rows][4]
 #pragma unroll 1
                     for (int c = 0; c < 4; ++c) {
                         uint32_t r32[32];
@@ -568,7 +568,7 @@ __global__ void __launch_bounds__(kThreadsWide, 1) prefix_wide_kernel(const __gr
                         if (mine) {
 #pragma unroll
                             for (int q = 0; q < 32; q += 4)
-                                *reinterpret_cast<uint4*>(dst + (c * 8 + q / 4) * (Shape<true>::kTile * 4)) = make_uint4(r32[q], r32[q + 1], r32[q + 2], r32[q + 3]);
+                                *reinterpret_cast<uint4*>(dst + (c * 8 + q / 4) * (kWideTile * 4)) = make_uint4(r32[q], r32[q + 1], r32[q + 2], r32[q + 3]);
                         }
                     }
                 }

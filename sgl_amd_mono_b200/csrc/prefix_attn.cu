@@ -446,21 +446,26 @@ struct Parts {
     int rows, count, step;  // step: floats from the lane's first four values to the next four
     size_t stride;
 };
-__device__ __forceinline__ Parts parts_of(const mono_prefix_attn_args& a, const Scratch& s, const Record& n, int token, int head, int G, int narrow_ctas,
-                                          int wide_ctas, int sub) {
+__device__ __forceinline__ uint32_t over(uint32_t x, uint32_t per, uint32_t inverse) {  // x / per
+    uint32_t c = __umulhi(x, inverse);
+    if (c * per > x) --c;
+    if (x - c * per >= per) ++c;
+    return c;
+}
+__device__ __forceinline__ Parts parts_of(const mono_prefix_attn_args& a, const Scratch& s, const Record& n, int token, int kh, int in_group, int G, int sub) {
     Parts r = {nullptr, nullptr, 0, 0, 0, 0};
     const int wide = n.wide;
-    const uint32_t per_head = s.total[wide][0], items = s.total[wide][1];
-    if (n.tiles == 0 || per_head == 0) return r;  // no keys, or refused tables
-    const int kh = head / G, row = (token - n.tok0) * G + head - kh * G;
-    r.rows = wide ? kWideTile : narrow_tile(a);
-    const int tile = row / r.rows, at = row - tile * r.rows;
-    const int hg = wide ? 1 : group_heads(a.kv_heads), list = kh / hg, lists = wide ? a.kv_heads : head_groups(a.kv_heads);
-    const uint32_t per = part_size(per_head * lists, wide ? wide_ctas : narrow_ctas);
-    const uint32_t first = list * per_head + n.off + (uint32_t)tile * n.units;
-    const uint32_t c0 = first / per, c1 = (first + (tile == n.tiles - 1 ? n.last : n.units) - 1) / per;
+    const uint4 tot = *reinterpret_cast<const uint4*>(s.total[wide]);  // units and items of a list, units of a part, inverse
+    if (n.tiles == 0 || tot.x == 0) return r;  // no keys, or refused tables
+    const int row = (token - n.tok0) * G + in_group;
+    const int shift = wide ? 8 : narrow_tile(a) == 8 ? 3 : 4;  // rows of a tile
+    r.rows = 1 << shift;
+    const int tile = row >> shift, at = row & (r.rows - 1);
+    const int hg = wide ? 1 : group_heads(a.kv_heads), list = wide ? kh : kh / hg;
+    const uint32_t first = list * tot.x + n.off + (uint32_t)tile * n.units;
+    const uint32_t c0 = over(first, tot.z, tot.w), c1 = over(first + (tile == n.tiles - 1 ? n.last : n.units) - 1, tot.z, tot.w);
     r.stride = hg * seg_floats(r.rows);
-    const float* seg = s.seg[wide] + (size_t)(c0 + list * items + n.item + tile) * r.stride + (kh - list * hg) * seg_floats(r.rows);
+    const float* seg = s.seg[wide] + (size_t)(c0 + list * tot.y + n.item + tile) * r.stride + (kh - list * hg) * seg_floats(r.rows);
     r.m = seg + at;
     // narrow: rows of 128 values; wide: four dims of all rows, then the next four (as a thread per row writes them)
     r.v = seg + 2 * r.rows + (wide ? (sub * 2 * kWideTile + at) * 4 : at * kDim + sub * 8);
@@ -473,7 +478,7 @@ __device__ __forceinline__ Parts parts_of(const mono_prefix_attn_args& a, const 
 // wide segment, are read together.  SPLIT warps of a CTA share a pair of heads' parts; a batch of parts is requested at
 // once and added to a running maximum, so a row of few parts costs one round trip.
 template <int SPLIT>
-__global__ void __launch_bounds__(128) prefix_merge_kernel(const mono_prefix_attn_args a, const Scratch s, int narrow_ctas, int wide_ctas) {
+__global__ void __launch_bounds__(128) prefix_merge_kernel(const __grid_constant__ mono_prefix_attn_args a, const __grid_constant__ Scratch s) {
     pdl_prologue();
     __shared__ float s_num[4][8][32], s_m[4][2], s_den[4][2];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, half = lane >> 4, sub = lane & 15;
@@ -491,43 +496,46 @@ __global__ void __launch_bounds__(128) prefix_merge_kernel(const mono_prefix_att
         in[k] = in[k] && token >= rec[k].tok0 && token < rec[k].tok0 + rec[k].ntok;
     }
     if (!in[1]) return;  // a token of no sequence: the row stays as it was
-    const int G = a.q_heads / a.kv_heads;
+    const int G = a.q_heads / a.kv_heads, kh = head / G;
     float M = -INFINITY, den = 0.f, num[8] = {};
     if (head < a.q_heads) {
-#pragma unroll 1
+        const Parts both[2] = {in[0] ? parts_of(a, s, rec[0], token, kh, head - kh * G, G, sub) : Parts{nullptr, nullptr, 0, 0, 0, 0},
+                               parts_of(a, s, rec[1], token, kh, head - kh * G, G, sub)};
+#pragma unroll
         for (int k = 0; k < 2; ++k) {
-            if (!(k ? in[1] : in[0])) continue;
-            const Parts ps = parts_of(a, s, k ? rec[1] : rec[0], token, head, G, narrow_ctas, wide_ctas, sub);
+            const Parts ps = both[k];
             constexpr int B = 4;
 #pragma unroll 1
             for (int i0 = part; i0 < ps.count; i0 += SPLIT * B) {
                 float m[B], l[B], top = M;
                 float4 v[B][2];
 #pragma unroll
-                for (int j = 0; j < B; ++j) {  // unconditional loads, all in flight together
-                    const size_t o = (size_t)min(i0 + j * SPLIT, ps.count - 1) * ps.stride;
-                    m[j] = ps.m[o];
-                    l[j] = ps.m[ps.rows + o];
-                    v[j][0] = *reinterpret_cast<const float4*>(ps.v + o);
-                    v[j][1] = *reinterpret_cast<const float4*>(ps.v + ps.step + o);
+                for (int j = 0; j < B; ++j) {  // all in flight together
+                    m[j] = -INFINITY;
+                    l[j] = 0.f;
+                    v[j][0] = v[j][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (i0 + j * SPLIT < ps.count) {
+                        const size_t o = (size_t)(i0 + j * SPLIT) * ps.stride;
+                        m[j] = ps.m[o];
+                        l[j] = ps.m[ps.rows + o];
+                        v[j][0] = *reinterpret_cast<const float4*>(ps.v + o);
+                        v[j][1] = *reinterpret_cast<const float4*>(ps.v + ps.step + o);
+                    }
                 }
 #pragma unroll
-                for (int j = 0; j < B; ++j) {
-                    if (i0 + j * SPLIT >= ps.count) m[j] = -INFINITY;
-                    top = fmaxf(top, m[j]);
-                }
-                const float old = M == -INFINITY ? 0.f : exp2f(M - top);
+                for (int j = 0; j < B; ++j) top = fmaxf(top, m[j]);
+                // A part without keys (m = -inf) has sums of zeros, and so has its weight; without any, all stay zero.
+                const float base = top == -INFINITY ? 0.f : top, old = exp2f(M - base);
                 den *= old;
 #pragma unroll
                 for (int q = 0; q < 8; ++q) num[q] *= old;
 #pragma unroll
                 for (int j = 0; j < B; ++j) {
-                    const bool live = m[j] != -INFINITY;  // also NaN: a row of NaN
-                    const float w = live ? exp2f(m[j] - top) : 0.f;
-                    den += live ? l[j] * w : 0.f;
+                    const float w = exp2f(m[j] - base);  // NaN for a row of NaN
                     const float vv[8] = {v[j][0].x, v[j][0].y, v[j][0].z, v[j][0].w, v[j][1].x, v[j][1].y, v[j][1].z, v[j][1].w};
+                    den = fmaf(l[j], w, den);
 #pragma unroll
-                    for (int q = 0; q < 8; ++q) num[q] += live ? vv[q] * w : 0.f;
+                    for (int q = 0; q < 8; ++q) num[q] = fmaf(vv[q], w, num[q]);
                 }
                 M = top;
             }
@@ -639,17 +647,19 @@ extern "C" int mono_prefix_attn_launch(const mono_prefix_attn_args* a, void* str
     }
     Params p;
     const uint64_t inner = (uint64_t)a->kv_heads * kDim, rows = (uint64_t)a->n_pages * kPage;
+    const int wide = (long)a->tokens * (a->q_heads / a->kv_heads) >= kWideRows ? sm_or_default() : 0;  // no entry has more rows than the step
     const int hg = group_heads(a->kv_heads), span = unit_keys(a->kv_heads) < kPage ? unit_keys(a->kv_heads) : kPage;
     for (int v = 0; v < 2; ++v) {  // boxes of the narrow kernel (the group's heads) and of the wide one (a head of a page)
         const uint8_t* cache = v ? a->v_cache : a->k_cache;
         if (int rc = mono_tmap_encode_box3(reinterpret_cast<mono_tmap_t*>(v ? &p.vmap : &p.kmap), cache, kDim, rows, a->kv_heads, inner, kDim, span, hg)) return rc;
-        if (int rc = mono_tmap_encode_box3(reinterpret_cast<mono_tmap_t*>(v ? &p.vmap1 : &p.kmap1), cache, kDim, rows, a->kv_heads, inner, kDim, kPage, 1)) return rc;
+        if (wide)
+            if (int rc = mono_tmap_encode_box3(reinterpret_cast<mono_tmap_t*>(v ? &p.vmap1 : &p.kmap1), cache, kDim, rows, a->kv_heads, inner, kDim, kPage, 1)) return rc;
     }
     p.a = *a;
     uint8_t* at = reinterpret_cast<uint8_t*>(a->scratch);
     p.s.rec = reinterpret_cast<Record*>(at);
     at += up256((size_t)(a->seqs + a->groups) * sizeof(Record));
-    for (int w = 0; w < 2; ++w) p.s.total[w] = reinterpret_cast<uint32_t*>(at) + 2 * w;
+    for (int w = 0; w < 2; ++w) p.s.total[w] = reinterpret_cast<uint32_t*>(at) + 4 * w;
     at += 256;
     for (int w = 0; w < 2; ++w) {
         p.s.entry[w] = reinterpret_cast<int*>(at);
@@ -675,7 +685,6 @@ extern "C" int mono_prefix_attn_launch(const mono_prefix_attn_args* a, void* str
         attr_done(attr_once);
     }
     const int narrow = sm_or_default();
-    const int wide = (long)a->tokens * (a->q_heads / a->kv_heads) >= kWideRows ? sm_or_default() : 0;  // no entry has more rows than the step
     const uint64_t q_rows = (uint64_t)a->tokens * a->q_heads;
     if (wide)
         if (int rc = mono_tmap_encode_box(reinterpret_cast<mono_tmap_t*>(&p.qmap), p.s.q_image, 128, q_rows, 2, 128, q_rows * 128, 128)) return rc;
@@ -683,10 +692,10 @@ extern "C" int mono_prefix_attn_launch(const mono_prefix_attn_args* a, void* str
     if (e == cudaSuccess) e = launch_k(narrow_tile(*a) == 8 ? prefix_narrow_kernel<1> : prefix_narrow_kernel<2>, narrow, kThreads, smem, st, p);
     // Few rows: four warps share two heads' segments (a long prefix leaves many of them); many rows: a warp each.
     if (e == cudaSuccess) {
-        if ((long)a->tokens * a->q_heads < 2048)
-            e = launch_k(prefix_merge_kernel<4>, dim3(a->tokens, (a->q_heads + 1) / 2), 128, 0, st, *a, p.s, narrow, wide);
+        if ((long)a->tokens * a->q_heads < 8192)
+            e = launch_k(prefix_merge_kernel<4>, dim3(a->tokens, (a->q_heads + 1) / 2), 128, 0, st, *a, p.s);
         else
-            e = launch_k(prefix_merge_kernel<1>, dim3(a->tokens, (a->q_heads + 7) / 8), 128, 0, st, *a, p.s, narrow, wide);
+            e = launch_k(prefix_merge_kernel<1>, dim3(a->tokens, (a->q_heads + 7) / 8), 128, 0, st, *a, p.s);
     }
     if (e != cudaSuccess) mono_set_error("%s: %s", who, cudaGetErrorString(e));
     return (int)e;

@@ -88,6 +88,9 @@ __device__ __forceinline__ Work entry_work(const mono_prefix_attn_args& a, const
     return w;
 }
 
+// Every CTA takes `part_size` units, the last of them what is left: no part in use is empty.
+__device__ __forceinline__ uint32_t part_size(uint32_t U, uint32_t ctas) { return max((U + ctas - 1) / ctas, 1u); }
+
 // What the merge has to know of an entry, from the kernel that has the entry.
 struct alignas(16) Record {
     int tok0, ntok;
@@ -98,7 +101,7 @@ struct alignas(16) Record {
 // two segments share a number.  `entry`: per token its group (or what an earlier launch left) and its sequence.
 struct Scratch {
     Record* rec;           // [entries]
-    uint32_t* total[2];    // units and items of one kv head
+    uint32_t* total[2];    // units and items of one kv head (narrow: head group), units of a CTA's part and 2^32 over that
     int* entry[2];         // [tokens]
     float* seg[2];
     uint8_t* q_image;      // the wide kernel's queries: [2][kv heads][tokens][q heads per kv head][128], and per row
@@ -149,8 +152,11 @@ __device__ __forceinline__ void make_plan(const mono_prefix_attn_args& a, const 
         off[E] = bad ? 0 : bu + su;  // refused: nobody has work
         item[E] = bi + si;
         if (blockIdx.x == 0) {
+            const uint32_t per = part_size(off[E] * (WIDE ? a.kv_heads : head_groups(a.kv_heads)), gridDim.x);
             s.total[WIDE][0] = off[E];
             s.total[WIDE][1] = item[E];
+            s.total[WIDE][2] = per;
+            s.total[WIDE][3] = per == 1 ? 0xFFFFFFFFu : 0xFFFFFFFFu / per + 1;
             if (bad) guard_fail(a.guard, MONO_ERR_ARG, kSiteTables);
         }
     }
@@ -183,9 +189,6 @@ __device__ __forceinline__ Place place_of(const uint32_t* off, int E, uint32_t u
     p.local = u - off[lo];
     return p;
 }
-// Every CTA takes `part_size` units, the last of them what is left: no part in use is empty.
-__device__ __forceinline__ uint32_t part_size(uint32_t U, uint32_t ctas) { return max((U + ctas - 1) / ctas, 1u); }
-
 struct alignas(64) Params {
     CUtensorMap kmap, vmap, kmap1, vmap1, qmap;  // boxes of a head group, of one head's page, of 128 query rows
     mono_prefix_attn_args a;

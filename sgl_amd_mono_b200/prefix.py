@@ -72,13 +72,22 @@ def _caches(a, k_cache, v_cache, kv_heads: int, dev) -> None:
     a.n_pages = shape[0]
 
 
+def _front(views: dict, n: int) -> torch.Tensor:
+    """The first ``n`` rows of an op's buffer (``views[0]``), each view made once: a slice costs what a launch costs."""
+    v = views.get(n)
+    if v is None:
+        v = views[n] = views[0][:n]
+    return v
+
+
 def _launch(fn, a, index: int, what: str) -> None:
     """Enqueues on the current stream of device ``index``, whichever device is current."""
+    stream = torch._C._cuda_getCurrentRawStream(index)  # (the Stream object around it costs a microsecond)
     if torch.cuda.current_device() == index:
-        rc = fn(C.byref(a), torch.cuda.current_stream(index).cuda_stream)
+        rc = fn(C.byref(a), stream)
     else:
         with torch.cuda.device(index):
-            rc = fn(C.byref(a), torch.cuda.current_stream(index).cuda_stream)
+            rc = fn(C.byref(a), stream)
     if rc:
         L.check(rc, what)
 
@@ -105,6 +114,7 @@ class QkvAppendOp:
         self.q_heads, self.kv_heads, self.max_tokens = q_heads, kv_heads, max_tokens
         self.rot_dim, self.interleaved, self.eps = rot_dim, bool(interleaved), float(eps)
         self.q = torch.zeros(max_tokens, q_heads, HEAD_DIM, dtype=torch.bfloat16, device=self.dev)
+        self._views = {0: self.q}
         self.width = (q_heads + 2 * kv_heads) * HEAD_DIM
         self._fn = L.load().mono_qkv_append_launch
         self._fixed = f = L.QkvAppendArgs()  # what no call changes
@@ -120,8 +130,7 @@ class QkvAppendOp:
         (page * 64 + offset) outside the cache inserts nothing, and the slots inside it must differ.
         Returns q ``[tokens, q_heads, 128]`` (the op's own buffer)."""
         width, dev = self.width, self.dev
-        a = L.QkvAppendArgs()
-        C.memmove(C.byref(a), C.byref(self._fixed), C.sizeof(a))
+        a = L.QkvAppendArgs.from_buffer_copy(self._fixed)
         if not isinstance(qkv, torch.Tensor) or qkv.device != dev:
             raise ValueError(f"qkv: must be a tensor on {dev} (there is no CPU path)")
         shape = qkv.shape
@@ -164,7 +173,7 @@ class QkvAppendOp:
         _caches(a, k_cache, v_cache, self.kv_heads, dev)
         a.tokens = n
         _launch(self._fn, a, dev.index, "mono_qkv_append_launch")
-        return self.q[:n]
+        return _front(self._views, n)
 
 
 @dataclass
@@ -207,7 +216,11 @@ class SharedPrefixAttnOp:
             nbytes = L.load().mono_prefix_attn_scratch_bytes(max_tokens, q_heads, kv_heads, max_seqs, max_groups)
         self.scratch = torch.zeros(nbytes, dtype=torch.uint8, device=self.dev)
         self.out = torch.zeros(max_tokens, q_heads, HEAD_DIM, dtype=torch.bfloat16, device=self.dev)
+        self._views = {0: self.out}
         self.guard = guard if guard is not None else torch.zeros(L.GUARD_WORDS, dtype=torch.int32, device=self.dev)
+        _on(self.guard, "guard", self.dev, torch.int32)
+        if self.guard.numel() < L.GUARD_WORDS:
+            raise ValueError(f"guard: {self.guard.numel()} words, needs {L.GUARD_WORDS}")
         self._fn = L.load().mono_prefix_attn_launch
         self._fixed = f = L.PrefixAttnArgs()  # what no call changes
         f.q_heads, f.kv_heads, f.k_scale, f.v_scale, f.sm_scale = q_heads, kv_heads, self.k_scale, self.v_scale, self.sm_scale
@@ -239,8 +252,7 @@ class SharedPrefixAttnOp:
         ld = strides[0] if n > 1 else width
         if strides[2] != 1 or (self.q_heads > 1 and strides[1] != HEAD_DIM) or ld < width or ld % 8:
             raise ValueError(f"q: strides {strides}, needs contiguous heads and token rows a multiple of 8 values apart")
-        a = L.PrefixAttnArgs()
-        C.memmove(C.byref(a), C.byref(self._fixed), C.sizeof(a))
+        a = L.PrefixAttnArgs.from_buffer_copy(self._fixed)
         a.tokens, a.q, a.q_ld = n, _aligned(q.data_ptr(), "q"), ld
         _caches(a, k_cache, v_cache, self.kv_heads, dev)
         a.lens = _on(t.lens, "lens", dev, torch.int32)
@@ -261,7 +273,7 @@ class SharedPrefixAttnOp:
         elif t.group_start is not None or t.prefix_table is not None:
             raise ValueError("prefix_lens: missing beside group_start / prefix_table")
         if out is None:
-            out = self.out[:n]
+            out = _front(self._views, n)
         else:
             a.out = _aligned(_on(out, "out", dev, torch.bfloat16, (n, self.q_heads, HEAD_DIM)), "out")
         _launch(self._fn, a, dev.index, "mono_prefix_attn_launch")

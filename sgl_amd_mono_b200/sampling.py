@@ -11,12 +11,11 @@ captured into a CUDA graph.  The returned tensors are overwritten by the next ca
 
 from __future__ import annotations
 
-import ctypes as C
 
 import torch
 
 from . import _lib as L
-from .prefix import _device, _launch, _on
+from .prefix import _device, _front, _launch, _on
 
 
 class SampleOp:
@@ -30,6 +29,7 @@ class SampleOp:
         self.vocab, self.max_rows = vocab, max_rows
         self.tokens = torch.zeros(max_rows, dtype=torch.int64, device=self.dev)
         self.logprobs = torch.zeros(max_rows, dtype=torch.float32, device=self.dev)
+        self._tokens, self._logprobs = {0: self.tokens}, {0: self.logprobs}  # and their views by rows
         self._fn, self._out = L.load().mono_sample_launch, (self.tokens.data_ptr(), self.logprobs.data_ptr())
 
     def __call__(self, logits: torch.Tensor, u: torch.Tensor, temperature=None, top_k=None, top_p=None, min_p=None):
@@ -64,4 +64,4 @@ class SampleOp:
             a.min_p = _on(min_p, "min_p", dev, torch.float32, n)
         a.tokens, a.logprobs = self._out
         _launch(self._fn, a, dev.index, "mono_sample_launch")
-        return self.tokens[:rows], self.logprobs[:rows]
+        return _front(self._tokens, rows), _front(self._logprobs, rows)

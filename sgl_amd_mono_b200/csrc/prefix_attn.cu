@@ -123,14 +123,18 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_narrow_kernel(const __grid
         prefetch_tmap(&p.vmap);
     }
     MONO_TL(tl_narrow, 0);
+    // Beside the wide kernel, whose CTAs let this one start once all that was launched before them is done: what they
+    // leave is not read here, and the wait for them is at the end (the merge waits for this kernel alone).
     pdl_launch_dependents();
-    pdl_wait();
+    if (p.beside) __threadfence(); else pdl_wait();
+    const uint32_t ctas = p.beside ? __ldcg(p.s.share + 1) : gridDim.x;
     MONO_TL(tl_narrow, 1);
     if (tid == 0 && guard_failed(a.guard)) abort_flag = 1;
-    make_plan<false, kThreads>(a, p.s, off, item, red);
+    const bool used = blockIdx.x < ctas;
+    if (used) make_plan<false, kThreads>(a, p.s, off, item, red, ctas);
     MONO_TL(tl_narrow, 2);
     const int G = a.q_heads / a.kv_heads, hg = group_heads(a.kv_heads), keys = unit_keys(a.kv_heads);
-    const uint32_t U = off[E] * head_groups(a.kv_heads), per = part_size(U, gridDim.x), u0 = min(blockIdx.x * per, U), u1 = min(u0 + per, U);
+    const uint32_t U = used ? off[E] * head_groups(a.kv_heads) : 0, per = part_size(U, ctas), u0 = min(blockIdx.x * per, U), u1 = min(u0 + per, U);
     const uint64_t wait_ns = a.wait_ns ? a.wait_ns : kWaitLimitNs;
     if (u0 < u1) {
         if (warp == kConsumers) {
@@ -433,6 +437,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_narrow_kernel(const __grid
     }
     __syncthreads();
     MONO_TL(tl_narrow, 15);
+    if (p.beside) pdl_wait();
     if (*abortp) {
         for (int i = 0; i < 64; ++i) __nanosleep(1000);  // copies in flight land before the CTA's memory goes
         if (tid == 0 && !guard_failed(a.guard)) guard_fail(a.guard, MONO_ERR_DEADLINE, kSiteWait);
@@ -660,6 +665,8 @@ extern "C" int mono_prefix_attn_launch(const mono_prefix_attn_args* a, void* str
     p.s.rec = reinterpret_cast<Record*>(at);
     at += up256((size_t)(a->seqs + a->groups) * sizeof(Record));
     for (int w = 0; w < 2; ++w) p.s.total[w] = reinterpret_cast<uint32_t*>(at) + 4 * w;
+    p.s.share = reinterpret_cast<uint32_t*>(at) + 8;
+    p.beside = wide > 0;
     at += 256;
     for (int w = 0; w < 2; ++w) {
         p.s.entry[w] = reinterpret_cast<int*>(at);

@@ -88,6 +88,37 @@ __device__ __forceinline__ Work entry_work(const mono_prefix_attn_args& a, const
     return w;
 }
 
+// How the SMs are shared between the two kernels, which run side by side: the wide one is bound by its SMs, the narrow one by
+// HBM, and one after the other each leaves idle what the other wants.  In proportion to their work, a wide unit taken as
+// kWideCost and a narrow one as kNarrowCost for every eight rows of its tile (measured: 64 samples of a long prompt took 84, 84, 94
+// and 107 us at ratios 5, 6, 4 and 3 to 9; 24 samples in tiles of 16 rows 47 to 53 at 6 to 13 to 9, 62 at 4); each has at least one CTA, which leaves the merge's records.
+constexpr int kWideCost = 3, kNarrowCost = 2;
+__device__ __forceinline__ void make_share(const mono_prefix_attn_args& a, uint32_t* share, uint32_t ctas) {
+    __shared__ float s_wide[32], s_narrow[32];
+    float wide = 0.f, narrow = 0.f;
+    for (int e = threadIdx.x; e < a.groups + a.seqs; e += blockDim.x) {
+        const Entry n = entry_of(a, e);
+        const Work w = entry_work<true>(a, n), x = entry_work<false>(a, n);
+        if (w.tiles) wide += (float)w.per_head();
+        if (x.tiles) narrow += (float)x.per_head();
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        wide += __shfl_down_sync(0xffffffffu, wide, o);
+        narrow += __shfl_down_sync(0xffffffffu, narrow, o);
+    }
+    if ((threadIdx.x & 31) == 0) { s_wide[threadIdx.x >> 5] = wide; s_narrow[threadIdx.x >> 5] = narrow; }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < (int)blockDim.x / 32; ++w) { wide += s_wide[w]; narrow += s_narrow[w]; }
+        wide *= (float)(a.kv_heads * kWideCost);
+        narrow *= (float)(head_groups(a.kv_heads) * kNarrowCost * narrow_tile(a) / 8);
+        const int n = clamp_int((int)((float)ctas * (wide / fmaxf(wide + narrow, 1.f)) + 0.5f), 1, max((int)ctas - 1, 1));
+        share[0] = (uint32_t)n;
+        share[1] = max(ctas - (uint32_t)n, 1u);
+    }
+}
+
 // Every CTA takes `part_size` units, the last of them what is left: no part in use is empty.
 __device__ __forceinline__ uint32_t part_size(uint32_t U, uint32_t ctas) { return max((U + ctas - 1) / ctas, 1u); }
 
@@ -102,6 +133,7 @@ struct alignas(16) Record {
 struct Scratch {
     Record* rec;           // [entries]
     uint32_t* total[2];    // units and items of one kv head (narrow: head group), units of a CTA's part and 2^32 over that
+    uint32_t* share;       // how many of its CTAs the wide and the narrow kernel use, where both run
     int* entry[2];         // [tokens]
     float* seg[2];
     uint8_t* q_image;      // the wide kernel's queries: [2][kv heads][tokens][q heads per kv head][128], and per row
@@ -110,9 +142,9 @@ struct Scratch {
 
 // off[0..E]: units of one kv head (narrow: head group) before entry e (off[E]: all of them); item[0..E]: items likewise.  The
 // list of units runs through all entries for kv head 0, then for kv head 1, ...  Called by all threads of a block; the
-// blocks together leave the merge's records.
+// blocks together (`ctas` of them) leave the merge's records.
 template <bool WIDE, int THREADS>
-__device__ __forceinline__ void make_plan(const mono_prefix_attn_args& a, const Scratch& s, uint32_t* off, uint32_t* item, uint32_t* red /* [2 * 32] */) {
+__device__ __forceinline__ void make_plan(const mono_prefix_attn_args& a, const Scratch& s, uint32_t* off, uint32_t* item, uint32_t* red /* [2 * 32] */, uint32_t ctas) {
     const int E = a.groups + a.seqs, per = (E + THREADS - 1) / THREADS;
     const int e0 = min((int)threadIdx.x * per, E), e1 = min(e0 + per, E);
     uint32_t su = 0, si = 0;
@@ -129,8 +161,8 @@ __device__ __forceinline__ void make_plan(const mono_prefix_attn_args& a, const 
         if (w.tiles) su += (uint32_t)w.per_head();
         si += (uint32_t)w.tiles;
         if (!WIDE) {  // this block's share of the tokens
-            int t = n.tok0 + (int)((blockIdx.x + gridDim.x - (uint32_t)n.tok0 % gridDim.x) % gridDim.x);
-            for (; t < n.tok0 + n.ntok; t += gridDim.x) s.entry[e >= a.groups][t] = e;
+            int t = n.tok0 + (int)((blockIdx.x + ctas - (uint32_t)n.tok0 % ctas) % ctas);
+            for (; t < n.tok0 + n.ntok; t += ctas) s.entry[e >= a.groups][t] = e;
         }
     }
     // the sums of the threads before this one
@@ -152,7 +184,7 @@ __device__ __forceinline__ void make_plan(const mono_prefix_attn_args& a, const 
         off[E] = bad ? 0 : bu + su;  // refused: nobody has work
         item[E] = bi + si;
         if (blockIdx.x == 0) {
-            const uint32_t per = part_size(off[E] * (WIDE ? a.kv_heads : head_groups(a.kv_heads)), gridDim.x);
+            const uint32_t per = part_size(off[E] * (WIDE ? a.kv_heads : head_groups(a.kv_heads)), ctas);
             s.total[WIDE][0] = off[E];
             s.total[WIDE][1] = item[E];
             s.total[WIDE][2] = per;
@@ -193,6 +225,7 @@ struct alignas(64) Params {
     CUtensorMap kmap, vmap, kmap1, vmap1, qmap;  // boxes of a head group, of one head's page, of 128 query rows
     mono_prefix_attn_args a;
     Scratch s;
+    int beside;  // the narrow kernel runs beside the wide one
 };
 
 // Makes the query image and runs the wide kernel on `ctas` CTAs (prefix_attn_tc.cu).

@@ -133,11 +133,15 @@ __device__ __forceinline__ uint32_t widen2(uint32_t lo16) {
 // ends at 448), and what undoes the scale.  Image: [plane][kv head][token][head of the kv head][128 bytes].  Half a warp
 // per row.  (The rows are wanted by every CTA that has a part of their prefix: made by each of them, on its own rows, at
 // its start, they cost 4 to 7 us of it.)
-__global__ void __launch_bounds__(256) prefix_split_kernel(const mono_prefix_attn_args a, uint8_t* image, float* back_scale) {
+__global__ void __launch_bounds__(256) prefix_split_kernel(const mono_prefix_attn_args a, uint8_t* image, float* back_scale, uint32_t* share, int ctas) {
     pdl_prologue();
+    if (blockIdx.x == 0) {
+        make_share(a, share, (uint32_t)ctas);
+        return;
+    }
     const int lane = threadIdx.x & 31, sub = lane & 15;
     const unsigned G = a.q_heads / a.kv_heads, rows = (unsigned)a.tokens * a.q_heads;
-    const unsigned r = (blockIdx.x * 8 + (threadIdx.x >> 5)) * 2 + (lane >> 4);  // row of the image
+    const unsigned r = ((blockIdx.x - 1) * 8 + (threadIdx.x >> 5)) * 2 + (lane >> 4);  // row of the image
     const unsigned k = min(r, rows - 1), per = (unsigned)a.tokens * G, kh = k / per, tok = (k - kh * per) / G, g = k - kh * per - tok * G;
     const uint4 v = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(a.q) + (size_t)tok * a.q_ld + (size_t)(kh * G + g) * kDim) + sub);
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -258,13 +262,15 @@ __global__ void __launch_bounds__(kThreadsWide, 1) prefix_wide_kernel(const __gr
     fence_after();
     const uint32_t tmem = tmem_base_s;
     MONO_TL(tl_wide, 0);
-    pdl_launch_dependents();
     pdl_wait();
+    pdl_launch_dependents();  // only now: the narrow kernel starts on what the wait above waited for
+    const uint32_t ctas = p.s.share[0];
     if (tid == 0 && guard_failed(a.guard)) abort_flag = 1;
     MONO_TL(tl_wide, 1);
-    make_plan<true, kThreadsWide>(a, p.s, off, item, red);
+    const bool used = blockIdx.x < ctas;
+    if (used) make_plan<true, kThreadsWide>(a, p.s, off, item, red, ctas);
     MONO_TL(tl_wide, 2);
-    const uint32_t U = off[E] * a.kv_heads, per = part_size(U, gridDim.x), u0 = min(blockIdx.x * per, U), u1 = min(u0 + per, U);
+    const uint32_t U = used ? off[E] * a.kv_heads : 0, per = part_size(U, ctas), u0 = min(blockIdx.x * per, U), u1 = min(u0 + per, U);
     const uint64_t wait_ns = a.wait_ns ? a.wait_ns : kWaitLimitNs;
     if (warp >= kTmaWarp) {
         regs_down<kRegsFetch>();
@@ -606,7 +612,7 @@ cudaError_t launch_wide(const Params& p, int ctas, cudaStream_t st) {
         attr_done(attr_once);
     }
     const unsigned rows = (unsigned)p.a.tokens * p.a.q_heads;
-    const cudaError_t e = launch_k(prefix_split_kernel, (rows + 15) / 16, 256, 0, st, p.a, p.s.q_image, p.s.q_scale);
+    const cudaError_t e = launch_k(prefix_split_kernel, 1 + (rows + 15) / 16, 256, 0, st, p.a, p.s.q_image, p.s.q_scale, p.s.share, ctas);
     if (e != cudaSuccess) return e;
     return launch_k(prefix_wide_kernel, ctas, kThreadsWide, kSmemFixed + 2 * (size_t)(p.a.seqs + p.a.groups + 1) * 4, st, p);
 }

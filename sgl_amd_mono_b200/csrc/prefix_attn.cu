@@ -6,6 +6,8 @@
 // A prefix is read once for all tokens of its group: the rows of a tile come from every sequence of the group.
 // prefix_attn.cuh says how the work is cut.  This file holds the kernel for few rows and the merge; prefix_attn_tc.cu
 // the kernel for many.
+#include <algorithm>
+
 #include "prefix_attn.cuh"
 
 extern void mono_set_error(const char* fmt, ...);
@@ -67,7 +69,7 @@ __device__ __forceinline__ void load_q(const mono_prefix_attn_args& a, const Ent
     const __nv_bfloat16* src = reinterpret_cast<const __nv_bfloat16*>(a.q) + (size_t)(n.tok0 + r / G) * a.q_ld + (size_t)(head * G + r % G) * kDim + t * 32;
     uint4 raw[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) raw[j] = live ? __ldg(reinterpret_cast<const uint4*>(src) + j) : make_uint4(0, 0, 0, 0);
+    for (int j = 0; j < 4; ++j) raw[j] = live ? __ldcg(reinterpret_cast<const uint4*>(src) + j) : make_uint4(0, 0, 0, 0);
     const uint32_t* w = reinterpret_cast<const uint32_t*>(raw);
     float amax = 0.f;
 #pragma unroll
@@ -591,14 +593,14 @@ static size_t narrow_segments(size_t tokens, size_t q_heads, size_t kv_heads, si
     return group_heads((int)kv_heads) * ((size_t)sm_or_default() + head_groups((int)kv_heads) * (2 * tiles + seqs + groups));
 }
 // The wide kernel's entries have kWideRows rows at least, so there are at most 2 rows / kWideRows of them.
-static size_t wide_segments(size_t tokens, size_t q_heads, size_t kv_heads) {
+static size_t wide_segments(size_t tokens, size_t q_heads, size_t kv_heads, size_t seqs, size_t groups) {
     const size_t rows = tokens * (q_heads / kv_heads);
-    if (rows < kWideRows) return 0;
-    return (size_t)sm_or_default() + kv_heads * 2 * (rows / kWideTile + rows / kWideRows);
+    if (!wide_step((int)tokens, (int)(q_heads / kv_heads))) return 0;
+    return (size_t)sm_or_default() + kv_heads * (2 * (rows / kWideTile) + std::min(2 * (rows / kWideRows), seqs + groups));
 }
 // The wide kernel's queries (two planes of 128 bytes a row) and their scales; none where no entry can have so many rows.
 static size_t image_bytes(size_t tokens, size_t q_heads, size_t kv_heads) {
-    return tokens * (q_heads / kv_heads) < kWideRows ? 0 : up256(tokens * q_heads * 256) + up256(tokens * q_heads * 4);
+    return !wide_step((int)tokens, (int)(q_heads / kv_heads)) ? 0 : up256(tokens * q_heads * 256) + up256(tokens * q_heads * 4);
 }
 static size_t narrow_bytes(int tokens, int q_heads, int kv_heads, int seqs, int groups) {
     return up256(narrow_segments(tokens, q_heads, kv_heads, seqs, groups) * seg_floats(kNarrowTile) * sizeof(float));
@@ -610,7 +612,7 @@ extern "C" size_t mono_prefix_attn_scratch_bytes(int tokens, int q_heads, int kv
     using namespace prefix_attn;
     if (tokens < 1 || q_heads < 1 || kv_heads < 1 || seqs < 1 || groups < 0 || q_heads % kv_heads) return 0;
     return up256((size_t)(seqs + groups) * sizeof(Record)) + 256 + 2 * up256((size_t)tokens * 4) + image_bytes(tokens, q_heads, kv_heads) + narrow_bytes(tokens, q_heads, kv_heads, seqs, groups) +
-           wide_segments(tokens, q_heads, kv_heads) * seg_floats(kWideTile) * sizeof(float);
+           wide_segments(tokens, q_heads, kv_heads, seqs, groups) * seg_floats(kWideTile) * sizeof(float);
 }
 
 extern "C" int mono_prefix_attn_launch(const mono_prefix_attn_args* a, void* stream) {
@@ -652,7 +654,7 @@ extern "C" int mono_prefix_attn_launch(const mono_prefix_attn_args* a, void* str
     }
     Params p;
     const uint64_t inner = (uint64_t)a->kv_heads * kDim, rows = (uint64_t)a->n_pages * kPage;
-    const int wide = (long)a->tokens * (a->q_heads / a->kv_heads) >= kWideRows ? sm_or_default() : 0;  // no entry has more rows than the step
+    const int wide = wide_step(a->tokens, a->q_heads / a->kv_heads) ? sm_or_default() : 0;
     const int hg = group_heads(a->kv_heads), span = unit_keys(a->kv_heads) < kPage ? unit_keys(a->kv_heads) : kPage;
     for (int v = 0; v < 2; ++v) {  // boxes of the narrow kernel (the group's heads) and of the wide one (a head of a page)
         const uint8_t* cache = v ? a->v_cache : a->k_cache;

@@ -68,8 +68,16 @@ constexpr int kWideHalf = 128;
 __host__ __device__ __forceinline__ int group_heads(int kv_heads) { return kv_heads >= 8 ? 8 : kv_heads >= 4 ? 4 : kv_heads >= 2 ? 2 : 1; }
 __host__ __device__ __forceinline__ int head_groups(int kv_heads) { return (kv_heads + group_heads(kv_heads) - 1) / group_heads(kv_heads); }
 __host__ __device__ __forceinline__ int unit_keys(int kv_heads) { return 128 / group_heads(kv_heads); }
-// rows of an entry from which the wide kernel takes it
-constexpr int kWideRows = 48;
+// Rows of an entry from which the wide kernel takes it.  An entry of a few tiles reads its keys once per tile, the wide
+// kernel once: it wins from three tiles of 8 rows (a prefix of 11312 keys, 10 rows: 49 us wide, 41 narrow; 256 samples of
+// prompts with 17 to 48 rows: 149 wide, 158 narrow) and from one of 16 that is more than half full (30499 keys, 14 rows: 77
+// wide, 112 narrow).  A step of fewer rows than kWideStep in all stays narrow: the wide kernel's launch and start cost it
+// more (24 rows: 21 us wide, 16 narrow).
+constexpr int kWideRows = 9, kWideStep = 33;
+__host__ __device__ __forceinline__ bool wide_step(int tokens, int G) { return (long)tokens * G >= kWideStep; }
+__device__ __forceinline__ bool is_wide(const mono_prefix_attn_args& a, int rows) {
+    return rows >= (narrow_tile(a) == 8 ? 17 : kWideRows) && wide_step(a.tokens, a.q_heads / a.kv_heads);
+}
 
 struct Work {
     int tiles, units, last;  // row tiles; units of a tile, and of the last one
@@ -79,7 +87,7 @@ template <bool WIDE>
 __device__ __forceinline__ Work entry_work(const mono_prefix_attn_args& a, const Entry& n) {
     const int rows = n.ntok * (a.q_heads / a.kv_heads);
     Work w = {0, 0, 0};
-    if ((rows >= kWideRows) != WIDE || rows <= 0 || n.len <= 0) return w;
+    if (is_wide(a, rows) != WIDE || rows <= 0 || n.len <= 0) return w;
     const int tile = WIDE ? kWideTile : narrow_tile(a);
     w.tiles = (rows + tile - 1) / tile;
     const int keys = WIDE ? kPage : unit_keys(a.kv_heads);
@@ -195,7 +203,7 @@ __device__ __forceinline__ void make_plan(const mono_prefix_attn_args& a, const 
     if (blockIdx.x == 0) {
         for (int e = e0; e < e1; ++e) {
             const Entry n = entry_of(a, e);
-            const bool wide = n.ntok * (a.q_heads / a.kv_heads) >= kWideRows;
+            const bool wide = is_wide(a, n.ntok * (a.q_heads / a.kv_heads));
             if (wide != WIDE) continue;
             const Work w = entry_work<WIDE>(a, n);
             s.rec[e] = Record{n.tok0, n.ntok, off[e], item[e], w.tiles, w.units, w.last, wide};

@@ -51,7 +51,8 @@ __device__ __forceinline__ float below_or_at(uint32_t key) { return logit_of(key
 constexpr uint32_t kKeyNegInf = 0x007FFFFFu, kKeyInf = 0xFF800000u;
 
 constexpr int kTable = 32, kCopies = 16;  // a copy of the table per pair of banks: looked up by all lanes, it has no conflicts
-constexpr double kTwo52 = 4503599627370496.0;
+constexpr double kTwo52 = 4503599627370496.0;             // 2^52: a number below it, added, leaves its whole part in the mantissa
+constexpr double kRound32 = 6755399441055744.0 / kTable;  // (2^52 + 2^51) / 32
 
 struct Row {
     float mx;           // largest logit (finite)
@@ -62,13 +63,14 @@ struct Row {
     const double* tab;  // 2^(44 + i / 32), this lane's copy
 };
 
-// round(2^44 exp((x - mx) / T)), an f64 whole number.  y = (x - mx) log2(e) / T = n + i / 32 + r, 0 <= i < 32, |r| <= 1/64:
-// 2^y = 2^n 2^(i/32) 2^r, the last by its series in r ln 2 (at most 0.0109: the sixth power's term is below 2^-48).
-__device__ __forceinline__ double weight_f64(float x, const Row& r) {
+// round(2^44 exp((x - mx) / T)).  y = (x - mx) log2(e) / T = n + i / 32 + r, 0 <= i < 32, |r| <= 1/64:
+// 2^y = 2^n 2^(i/32) 2^r, the last by its series in r ln 2 (at most 0.0109: the sixth power's term is below 2^-48).  The
+// f64 pipe bounds the passes that weigh, so what integers can do they do: the sign tests, the exponent, the sums.
+__device__ __forceinline__ u64 weight_of(float x, const Row& r) {
     const double y = ((double)x - r.mx64) * r.c64;
-    const double shifted = fma(y, (double)kTable, 6755399441055744.0);  // + 2^52 + 2^51: the low word holds round(32 y)
+    const double shifted = y + kRound32;  // rounded to a multiple of 1/32: the low word holds 32 y
     const int q = __double2loint(shifted);
-    const double t = fma(shifted - 6755399441055744.0, -1.0 / kTable, y);
+    const double t = y - (shifted - kRound32);
     constexpr double L = 0.69314718055994530942;
     double e = fma(t, L * L * L * L * L / 120, L * L * L * L / 24);
     e = fma(t, e, L * L * L / 6);
@@ -76,14 +78,12 @@ __device__ __forceinline__ double weight_f64(float x, const Row& r) {
     e = fma(t, e, L);
     e = fma(t, e, 1.0);
     e *= r.tab[(q & (kTable - 1)) * kCopies];
-    // times 2^n, by the exponent.  Below 2^-45 (and for -inf) the exponent may leave its range: a high word of 0 leaves a
-    // number next to 0.
+    // times 2^n, by the exponent.  At -45 and below (and for -inf) the exponent may leave its range: a high word of 0 leaves
+    // a number next to 0.  y <= 0, so its high word, unsigned, grows with |y|.
     const int hi = __double2hiint(e) + ((q & ~(kTable - 1)) << 15);
-    e = __hiloint2double(y > -45.0 ? hi : 0, __double2loint(e));
-    return (e + kTwo52) - kTwo52;  // to a whole number
+    e = __hiloint2double((uint32_t)__double2hiint(y) < 0xC0468000u ? hi : 0, __double2loint(e));
+    return (u64)__double_as_longlong(e + kTwo52) - (u64)__double_as_longlong(kTwo52);  // to a whole number, below 2^52
 }
-__device__ __forceinline__ u64 whole(double w) { return (u64)__double_as_longlong(w + kTwo52) & 0xFFFFFFFFFFFFFull; }  // below 2^52
-__device__ __forceinline__ u64 weight_of(float x, const Row& r) { return whole(weight_f64(x, r)); }
 // floor(u W) for 0 <= u < 1
 __device__ __forceinline__ u64 share_of(float u, u64 W) {
     const int e = (int)((__float_as_uint(u) >> 23) & 0xFF);
@@ -104,12 +104,21 @@ __device__ __forceinline__ u64 warp_sum_u64(u64 v) {
 struct Hist {
     uint32_t n[2][kBins], lo[2][kBins], hi[2][kBins];  // counts, and masses in two words; two sets, used in turn
 };
+constexpr int kRank = 256;  // tokens that are ranked one against another
+constexpr int kList = 64;  // logits of the border's first range that a warp lists
+constexpr size_t kAfter = sizeof(Hist) + kWarps * kList * sizeof(uint16_t);  // shared memory behind the slice
 // One word atomics are native in shared memory, 64-bit ones are not: the carry is taken from the value that was there.
 __device__ __forceinline__ void hist_add(Hist& h, int set, int bin, uint32_t n, u64 w) {
     atomicAdd(&h.n[set][bin], n);
     const uint32_t wl = (uint32_t)w, old = atomicAdd(&h.lo[set][bin], wl);
     const uint32_t wh = (uint32_t)(w >> 32) + (old + wl < old ? 1u : 0u);
     if (wh) atomicAdd(&h.hi[set][bin], wh);
+}
+
+// CTA c's keys of the tokens to be ranked, in a set of the histograms that is not in use (the rest of it holds the ranked).
+__device__ __forceinline__ uint32_t* candidates(Hist& h, int set, int c) {
+    static_assert(kRank * kCtas <= 2 * kBins && kRank * 3 <= kBins, "fits a set");
+    return c < kCtas / 2 ? &h.n[set][c * kRank] : &h.lo[set][(c - kCtas / 2) * kRank];
 }
 
 __device__ __forceinline__ uint32_t peer_address(const void* p, int rank) {
@@ -183,19 +192,20 @@ __device__ __forceinline__ A block_before(A v, A* red) {
 // `slice`: logits of a CTA (a multiple of 4); runs: a warp's consecutive logits (a multiple of 128)
 template <typename T>
 __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 2) sample_kernel(const mono_sample_args a, int slice, int run) {
-    extern __shared__ __align__(16) float xs[];  // [slice], then the histograms
+    extern __shared__ __align__(16) float xs[];  // [slice], then the histograms and the warps' lists
     Hist& h = *reinterpret_cast<Hist*>(xs + slice);
     __shared__ u64 s_wsum[kWarps], red64[kWarps], s_z[kCtas], s_part[kCtas], s_cut[2];
     __shared__ uint32_t s_wties[kWarps], red32[kWarps], s_key[kCtas], s_num[kCtas], s_cnt[2];
     __shared__ float redf[2][kWarps];
     __shared__ int s_bin[2];
+    __shared__ uint32_t s_found, s_cand[kCtas], s_border;
     __shared__ double s_tab[kTable * kCopies];
     cg::cluster_group cluster = cg::this_cluster();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, row = blockIdx.x / kCtas, V = a.vocab;
     const int rank = (int)cluster.block_rank();
     if (tid < kTable * kCopies) s_tab[tid] = exp2((tid / kCopies) / (double)kTable) * kOne;
     for (int i = tid; i < kBins; i += kThreads) { h.n[0][i] = 0; h.lo[0][i] = 0; h.hi[0][i] = 0; }
-    if (tid == 0) { s_bin[0] = kBins; s_bin[1] = kBins; }
+    if (tid == 0) { s_bin[0] = kBins; s_bin[1] = kBins; s_found = 0; s_border = 0; }
     MONO_TL(tl_sample, 0);
     pdl_prologue();
     MONO_TL(tl_sample, 1);
@@ -279,22 +289,22 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 2) sam
     const double p = !greedy && tp < 1.f ? fmax((double)tp, 0.0) : 1.0;
     r.floor_w = !greedy && mp > 0.f ? (u64)ceil((double)fminf(mp, 1.f) * kOne) : 0ull;
     const bool filtered = r.k < (u64)V || p < 1.0 || r.floor_w;
+    const bool search = filtered && r.k != 1;  // with rank 0 alone the border is the largest logit
     // ---- Z, and the histogram of counts over steps of log2 w
     const int i0 = min(warp * run, slice), i1 = min(i0 + run, slice);
     {
-        // whole numbers up to 2^44 add exactly in f64 to 2^53: a thread has at most 96
-        double zd = 0.0;
+        u64 z = 0;
         for (int i = i0 + lane * 4; i < i1; i += 256) {  // eight weights at a time: f64 arithmetic answers late
             const bool second = i + 128 < i1;
             const float4 a4 = *reinterpret_cast<const float4*>(xs + i), b4 = second ? *reinterpret_cast<const float4*>(xs + i + 128) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
             const float v[8] = {a4.x, a4.y, a4.z, a4.w, b4.x, b4.y, b4.z, b4.w};
-            double w[8];
+            u64 w[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) w[j] = weight_f64(v[j], r);
+            for (int j = 0; j < 8; ++j) w[j] = weight_of(v[j], r);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                zd += w[j];
-                if (filtered && w[j] > 0.0) {
+                z += w[j];
+                if (search && w[j] != 0) {
                     uint32_t within;
                     const int b = step_of(v[j], r, &within);
                     atomicAdd(&h.n[0][b], 1u);
@@ -302,7 +312,6 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 2) sam
                 }
             }
         }
-        u64 z = whole(zd);
         z = warp_sum_u64(z);
         if (lane == 0) s_wsum[warp] = z;
     }
@@ -313,7 +322,7 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 2) sam
         for (int i = 0; i < kWarps; ++i) z += s_wsum[i];
         *cluster.map_shared_rank(&s_z[rank], tid) = z;
     }
-    if (filtered) hist_merge(h, 0, rank, cluster); else cluster.sync();
+    if (search) hist_merge(h, 0, rank, cluster); else cluster.sync();
     MONO_TL(tl_sample, 5);
     u64 Z = 0;
     for (int i = 0; i < kCtas; ++i) Z += s_z[i];
@@ -323,10 +332,20 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 2) sam
     bool all = !filtered;
     u64 run_above = 0;       // of this warp's run: the mass above the range that the keys were first searched in,
     float first_hi = 0.f;    // which ends here
-    if (filtered) {
+    // The run's logits of that range, as places in the run: a few of a hundred as a rule, and all that later steps look at.
+    uint16_t* list = reinterpret_cast<uint16_t*>(&h + 1) + warp * kList;
+    int listed = kList + 1;  // more than kList: not all are there, and later steps walk the run
+    if (filtered && !search) {
+        khi = klo = kmax;
+        kept = tie_w = (u64)kOne;
+        ties = 1;
+        tied = 2;  // or more, or no more than one
+    }
+    if (search) {
         // "mass before < p Z", for masses in whole units
         const u64 limit = p < 1.0 ? max((u64)ceil(p * (double)Z), 1ull) : ~0ull;
         // ---- bounds of the border among the steps
+        uint32_t n_before[kPerThread + 1];
         {
             const uint2 n2 = *reinterpret_cast<const uint2*>(&h.n[1][tid * kPerThread]);
             const uint32_t n[kPerThread] = {n2.x, n2.y};
@@ -351,6 +370,7 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 2) sam
             const float lim = limit == ~0ull ? INFINITY : (float)((double)limit / kOne), fl = (float)((double)r.floor_w / kOne);
 #pragma unroll
             for (int j = 0; j < kPerThread; ++j) {
+                n_before[j] = c;
                 c += n[j];
                 hi += m_hi[j];
                 lo += m_lo[j];
@@ -358,10 +378,14 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 2) sam
                 if (c > r.k || hi * up >= lim || top[j + 1] * down < fl) atomicMin(&s_bin[0], b);  // may not be kept whole
                 if (c > r.k || lo * down >= lim || top[j] * up < fl) atomicMin(&s_bin[1], b);      // the border is not behind it
             }
+            n_before[kPerThread] = c;
         }
         __syncthreads();
         const int b0 = s_bin[0], b1 = min(s_bin[1], kBins - 1);
+        if (b0 / kPerThread == tid) s_cnt[0] = b0 % kPerThread ? n_before[1] : n_before[0];
+        if (b1 / kPerThread == tid) s_cnt[1] = b1 % kPerThread ? n_before[2] : n_before[1];
         __syncthreads();
+        uint32_t in_range = s_cnt[1] - s_cnt[0];  // as the steps were counted
         if (b0 >= kBins) {
             all = true;
         } else {
@@ -377,75 +401,197 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 2) sam
             u64 above = 0;
             uint32_t n_above = 0;
             MONO_TL(tl_sample, 6);
+            int idle = 0;  // the histograms' set that no CTA of the row reads now
+            // One key, or one token, holds the border: of its `tied` the first `ties` are kept.
+            auto settle = [&]() {
+                // rank and mass before the j-th of them are n_above + j and above + j tie_w
+                u64 t = tied;
+                if (tie_w < r.floor_w) t = 0;
+                t = min(t, r.k - n_above);
+                if (limit != ~0ull) t = above >= limit ? 0 : min(t, (limit - above + tie_w - 1) / tie_w);
+                if (n_above + t == 0) t = 1;
+                ties = (uint32_t)t;
+                kept = above + t * tie_w;
+            };
             for (int level = 1;; ++level) {
-                const int set = (level & 1) ^ 1;  // the one that does not hold the sums of the step before
-                const uint32_t width = khi - klo;
-                const int sh = width < kBins ? 0 : 22 - __clz(width);
-                for (int i = tid; i < kBins; i += kThreads) { h.n[set][i] = 0; h.lo[set][i] = 0; h.hi[set][i] = 0; }
-                if (tid == 0) s_bin[set] = kBins;  // not the one that slower threads may still read
-                __syncthreads();
-                uint32_t n_ab = 0;
                 const float fhi = below_or_at(khi), flo = logit_of(klo);  // order as the keys do, and cost nothing to compare
-                double above_d = 0.0;
-                for (int b = i0; b < i1; b += 128) {  // whole warps: the lanes vote
-                    const int i = b + lane * 4;
-                    const float4 v4 = i < i1 ? *reinterpret_cast<const float4*>(xs + i) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-                    const float v[4] = {v4.x, v4.y, v4.z, v4.w};
-                    bool wanted = false;  // the first level also weighs what is above the range
+                if (level == 1) {  // what is above the range is weighed, what is in it listed
+                    u64 m_ab = 0;
+                    uint32_t n_ab = 0;
+                    int found = 0;
+                    for (int b = i0; b < i1; b += 256) {  // whole warps: the lanes vote
+                        float v[8];
+                        bool over = false, near = false;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) wanted = wanted || (v[j] >= flo && (level == 1 || v[j] <= fhi));
-                    if (!__any_sync(0xffffffffu, wanted)) continue;
-                    double w[4];
+                        for (int q = 0; q < 2; ++q) {
+                            const int i = b + q * 128 + lane * 4;
+                            const float4 v4 = i < i1 ? *reinterpret_cast<const float4*>(xs + i) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+                            v[4 * q] = v4.x; v[4 * q + 1] = v4.y; v[4 * q + 2] = v4.z; v[4 * q + 3] = v4.w;
+                        }
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) w[j] = weight_f64(v[j], r);
+                        for (int j = 0; j < 8; ++j) {
+                            over = over || v[j] > fhi;
+                            near = near || (v[j] >= flo && v[j] <= fhi);
+                        }
+                        if (__any_sync(0xffffffffu, over)) {
+                            u64 w[8];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        if (level == 1 && v[j] > fhi) {  // surely kept
-                            above_d += w[j];
-                            n_ab += w[j] > 0.0;
+                            for (int j = 0; j < 8; ++j) w[j] = weight_of(v[j], r);
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) {
+                                const u64 kept_w = v[j] > fhi ? w[j] : 0;  // surely kept
+                                m_ab += kept_w;
+                                n_ab += kept_w != 0;
+                            }
+                        }
+                        if (!__any_sync(0xffffffffu, near)) continue;
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const bool here = v[j] >= flo && v[j] <= fhi;
+                            const unsigned in = __ballot_sync(0xffffffffu, here);
+                            const int at = found + __popc(in & ((1u << lane) - 1));
+                            if (here && at < kList) list[at] = (uint16_t)(b - i0 + (j >> 2) * 128 + lane * 4 + (j & 3));
+                            found += __popc(in);
                         }
                     }
-                    bool near = false;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) near = near || (v[j] >= flo && v[j] <= fhi);
-                    if (!__any_sync(0xffffffffu, near)) continue;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const bool here = v[j] >= flo && v[j] <= fhi && w[j] > 0.0;
-                        const unsigned in = __ballot_sync(0xffffffffu, here);
-                        if (in == 0) continue;
-                        const int bin = (int)((khi - key_of(v[j])) >> sh), lead = __ffs(in) - 1;
-                        const int lb = __shfl_sync(0xffffffffu, bin, lead);
-                        const u64 wi = here ? whole(w[j]) : 0;
-                        if (__popc(in) > 4 && __all_sync(0xffffffffu, !here || bin == lb)) {  // many equal logits: one addition for all
-                            const u64 sum = warp_sum_u64(wi);
-                            if (lane == lead) hist_add(h, set, bin, __popc(in), sum);
-                        } else if (here) {
-                            hist_add(h, set, bin, 1, wi);
-                        }
-                        __syncwarp();
-                    }
-                }
-                u64 m_ab = whole(above_d);
-                if (level == 1) {
+                    listed = found;
                     m_ab = warp_sum_u64(m_ab);
                     n_ab = __reduce_add_sync(0xffffffffu, n_ab);
                     if (lane == 0) { red64[warp] = m_ab; red32[warp] = n_ab; }
                     run_above = m_ab;
                     first_hi = fhi;
+                    __syncwarp();
                 }
-                __syncthreads();
-                if (level == 1 && tid < kCtas) {
+                bool summed = level > 1;
+                auto sum_above = [&]() {
+                    for (int i = 0; i < kCtas; ++i) { above += s_part[i]; n_above += s_num[i]; }
+                    summed = true;
+                };
+                auto send_above = [&]() {
                     u64 m = 0;
                     uint32_t n = 0;
                     for (int i = 0; i < kWarps; ++i) { m += red64[i]; n += red32[i]; }
                     *cluster.map_shared_rank(&s_part[rank], tid) = m;
                     *cluster.map_shared_rank(&s_num[rank], tid) = n;
+                };
+                // ---- few tokens left: all CTAs get all of them, and rank them
+                if (in_range <= kRank) {
+                    if (listed <= kList) {
+                        for (int b = 0; b < listed; b += 32) {
+                            const float v = b + lane < listed ? xs[i0 + list[b + lane]] : -INFINITY;
+                            const bool here = v >= flo && v <= fhi && weight_of(v, r) != 0;
+                            const unsigned in = __ballot_sync(0xffffffffu, here);
+                            uint32_t at = lane == 0 && in ? atomicAdd(&s_found, __popc(in)) : 0;
+                            at = __shfl_sync(0xffffffffu, at, 0) + __popc(in & ((1u << lane) - 1));
+                            if (here && at < kRank) {
+#pragma unroll
+                                for (int c = 0; c < kCtas; ++c) st_peer(candidates(h, idle, rank) + at, c, key_of(v));
+                            }
+                        }
+                    } else if (lane == 0) {
+                        atomicAdd(&s_found, kRank + 1);
+                    }
+                    __syncthreads();
+                    if (tid < kCtas) {
+                        *cluster.map_shared_rank(&s_cand[rank], tid) = s_found;
+                        if (level == 1) send_above();
+                    }
+                    cluster.sync();
+                    if (tid == 0) s_found = 0;
+                    if (!summed) sum_above();
+                    uint32_t total = 0;
+                    for (int c = 0; c < kCtas; ++c) total += min(s_cand[c], (uint32_t)kRank + 1);
+                    if (total <= kRank) {
+                        uint32_t* keys = h.hi[idle];
+                        u64* ws = reinterpret_cast<u64*>(h.hi[idle] + kRank);
+                        uint32_t from = 0;
+                        for (int c = 0; c < kCtas; ++c) {
+                            if (tid < (int)s_cand[c]) {
+                                const uint32_t key = candidates(h, idle, c)[tid];
+                                keys[from + tid] = key;
+                                ws[from + tid] = weight_of(logit_of(key), r);
+                            }
+                            from += s_cand[c];
+                        }
+                        __syncthreads();
+                        static_assert(2 * kRank <= kThreads, "two threads per token");
+                        const int i = tid >> 1;
+                        uint32_t n_more = 0, alike = 0;
+                        u64 m_more = 0;
+                        const uint32_t key = i < (int)total ? keys[i] : 0xFFFFFFFFu;
+                        for (int j = tid & 1; j < (int)total; j += 2) {
+                            const uint32_t kj = keys[j];
+                            if (kj > key) { ++n_more; m_more += ws[j]; }
+                            alike += kj == key;
+                        }
+                        n_more += __shfl_xor_sync(0xffffffffu, n_more, 1);
+                        alike += __shfl_xor_sync(0xffffffffu, alike, 1);
+                        m_more += __shfl_xor_sync(0xffffffffu, m_more, 1);
+                        const u64 w = i < (int)total ? ws[i] : 0, m_to = above + m_more + alike * w;
+                        const uint32_t n_to = n_above + n_more + alike;  // rank and mass up to this key
+                        if (i < (int)total) {
+                            if (n_to > r.k || m_to >= limit || w < r.floor_w) atomicMax(&s_border, key);
+                            if (n_more + alike == total) s_part[0] = m_to;
+                        } else if (total == 0 && tid == 0) {
+                            s_part[0] = above;
+                        }
+                        __syncthreads();
+                        if (s_border == 0) {  // everything in the range is kept
+                            kept = s_part[0];
+                            khi = klo - 1;  // and nobody is tied
+                            break;
+                        }
+                        if (i < (int)total && key == s_border) {
+                            red32[0] = alike;
+                            red32[1] = n_above + n_more;
+                            red64[0] = w;
+                            red64[1] = above + m_more;
+                        }
+                        __syncthreads();
+                        khi = klo = s_border;
+                        tied = red32[0];
+                        n_above = red32[1];
+                        tie_w = red64[0];
+                        above = red64[1];
+                        settle();
+                        break;
+                    }
                 }
+                const int set = (level & 1) ^ 1;
+                const uint32_t width = khi - klo;
+                const int sh = width < kBins ? 0 : 22 - __clz(width);
+                for (int i = tid; i < kBins; i += kThreads) { h.n[set][i] = 0; h.lo[set][i] = 0; h.hi[set][i] = 0; }
+                if (tid == 0) s_bin[set] = kBins;
+                __syncthreads();
+                // adds the logits of the range that a warp's lanes hold
+                auto add = [&](float v) {
+                    bool here = v >= flo && v <= fhi;
+                    if (!__any_sync(0xffffffffu, here)) return;
+                    const u64 wi = weight_of(v, r);
+                    here = here && wi > 0;
+                    const unsigned in = __ballot_sync(0xffffffffu, here);
+                    if (in == 0) return;
+                    const int bin = (int)((khi - key_of(v)) >> sh), lead = __ffs(in) - 1;
+                    const int lb = __shfl_sync(0xffffffffu, bin, lead);
+                    if (__popc(in) > 4 && __all_sync(0xffffffffu, !here || bin == lb)) {  // many equal logits: one addition for all
+                        const u64 sum = warp_sum_u64(here ? wi : 0);
+                        if (lane == lead) hist_add(h, set, bin, __popc(in), sum);
+                    } else if (here) {
+                        hist_add(h, set, bin, 1, wi);
+                    }
+                    __syncwarp();
+                };
+                if (listed <= kList) {
+                    for (int b = 0; b < listed; b += 32) add(b + lane < listed ? xs[i0 + list[b + lane]] : -INFINITY);
+                } else {
+                    for (int b = i0; b < i1; b += 32) add(b + lane < i1 ? xs[b + lane] : -INFINITY);
+                }
+                __syncthreads();
+                if (!summed && tid < kCtas) send_above();
                 hist_merge(h, set, rank, cluster);
+                idle = set;
                 MONO_TL(tl_sample, 5 + 2 * level);
-                if (level == 1)
-                    for (int i = 0; i < kCtas; ++i) { above += s_part[i]; n_above += s_num[i]; }
+                if (!summed) sum_above();
                 const uint2 n2 = *reinterpret_cast<const uint2*>(&h.n[set ^ 1][tid * kPerThread]), l2 = *reinterpret_cast<const uint2*>(&h.lo[set ^ 1][tid * kPerThread]),
                             h2 = *reinterpret_cast<const uint2*>(&h.hi[set ^ 1][tid * kPerThread]);
                 const uint32_t n[kPerThread] = {n2.x, n2.y};
@@ -494,16 +640,10 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 2) sam
                 klo = khi - klo < (1u << sh) ? klo : khi - ((1u << sh) - 1);
                 if (sh == 0 || tied == 1) {
                     tie_w = bin_m / tied;
-                    // rank and mass before the j-th of them are n_above + j and above + j tie_w
-                    u64 t = tied;
-                    if (tie_w < r.floor_w) t = 0;
-                    t = min(t, r.k - n_above);
-                    if (limit != ~0ull) t = above >= limit ? 0 : min(t, (limit - above + tie_w - 1) / tie_w);
-                    if (n_above + t == 0) t = 1;
-                    ties = (uint32_t)t;
-                    kept = above + t * tie_w;
+                    settle();
                     break;
                 }
+                in_range = tied;
                 __syncthreads();  // red32 / red64 have been read
             }
         }
@@ -515,27 +655,27 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 2) sam
     const bool some = !all && ties > 0 && ties < tied;
     if (!all && !some && ties == tied) khi = klo - 1;  // all of the tied are kept: so is every key from klo on
     if (!all) {
-        double md = 0.0;
+        u64 m = 0;
         uint32_t t = 0;
         const float fhi = below_or_at(khi), flo = logit_of(klo);
-        for (int i = i0 + lane * 4; i < i1; i += 128) {
-            const float4 v4 = *reinterpret_cast<const float4*>(xs + i);
-            const float v[4] = {v4.x, v4.y, v4.z, v4.w};
-            // what lies above the first range has been added up
-            bool wanted = false;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) wanted = wanted || (v[j] <= first_hi && v[j] >= (some ? flo : fhi));
-            if (!wanted) continue;
-            double w[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) w[j] = weight_f64(v[j], r);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if (v[j] > fhi) md += v[j] <= first_hi ? w[j] : 0.0;
-                else if (some && v[j] >= flo) ++t;
+        auto take = [&](float v) {  // what lies above the first range has been added up
+            if (v > fhi) {
+                if (v <= first_hi) m += weight_of(v, r);
+            } else if (some && v >= flo) {
+                ++t;
+            }
+        };
+        if (listed <= kList) {
+            for (int b = lane; b < listed; b += 32) take(xs[i0 + list[b]]);
+        } else {
+            for (int i = i0 + lane * 4; i < i1; i += 128) {
+                const float4 v4 = *reinterpret_cast<const float4*>(xs + i);
+                take(v4.x);
+                take(v4.y);
+                take(v4.z);
+                take(v4.w);
             }
         }
-        u64 m = whole(md);
         m = warp_sum_u64(m) + run_above;
         t = __reduce_add_sync(0xffffffffu, t);
         if (lane == 0) { s_wsum[warp] = m; s_wties[warp] = t; }
@@ -621,10 +761,10 @@ static cudaError_t launch(const mono_sample_args* a, cudaStream_t st) {
     slice = (slice + 7) & ~7;  // slices start on 16-byte addresses where the row does
     int run = (slice + kWarps - 1) / kWarps;
     run = (run + 127) & ~127;
-    const size_t smem = (size_t)slice * 4 + sizeof(Hist);
+    const size_t smem = (size_t)slice * 4 + kAfter;
     static std::atomic<uint64_t> attr_once{0};  // bit d: set on device d
     if (attr_needed(attr_once)) {
-        const cudaError_t e = cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, MONO_SAMPLE_MAX_VOCAB / kCtas * 4 + (int)sizeof(Hist));
+        const cudaError_t e = cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, MONO_SAMPLE_MAX_VOCAB / kCtas * 4 + (int)kAfter);
         if (e != cudaSuccess) return e;
         attr_done(attr_once);
     }

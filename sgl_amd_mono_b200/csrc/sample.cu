@@ -22,6 +22,8 @@
 // Then each warp's run of kept mass says which warp walks to the token.
 #include <cooperative_groups.h>
 
+#include <cmath>
+
 #include "mono_common.cuh"
 
 extern void mono_set_error(const char* fmt, ...);
@@ -54,6 +56,9 @@ constexpr int kTable = 32, kCopies = 16;  // a copy of the table per pair of ban
 constexpr double kTwo52 = 4503599627370496.0;             // 2^52: a number below it, added, leaves its whole part in the mantissa
 constexpr double kRound32 = 6755399441055744.0 / kTable;  // (2^52 + 2^51) / 32
 
+struct Powers {
+    double p[kTable];  // 2^(44 + i / 32)
+};
 struct Row {
     float mx;           // largest logit (finite)
     float c;            // log2(e) / T, f32: for histogram steps only
@@ -191,7 +196,7 @@ __device__ __forceinline__ A block_before(A v, A* red) {
 
 // `slice`: logits of a CTA (a multiple of 4); runs: a warp's consecutive logits (a multiple of 128)
 template <typename T>
-__global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 2) sample_kernel(const mono_sample_args a, int slice, int run) {
+__global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 2) sample_kernel(const mono_sample_args a, int slice, int run, const __grid_constant__ Powers powers) {
     extern __shared__ __align__(16) float xs[];  // [slice], then the histograms and the warps' lists
     Hist& h = *reinterpret_cast<Hist*>(xs + slice);
     __shared__ u64 s_wsum[kWarps], red64[kWarps], s_z[kCtas], s_part[kCtas], s_cut[2];
@@ -203,7 +208,7 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 2) sam
     cg::cluster_group cluster = cg::this_cluster();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, row = blockIdx.x / kCtas, V = a.vocab;
     const int rank = (int)cluster.block_rank();
-    if (tid < kTable * kCopies) s_tab[tid] = exp2((tid / kCopies) / (double)kTable) * kOne;
+    if (tid < kTable * kCopies) s_tab[tid] = powers.p[tid / kCopies];
     for (int i = tid; i < kBins; i += kThreads) { h.n[0][i] = 0; h.lo[0][i] = 0; h.hi[0][i] = 0; }
     if (tid == 0) { s_bin[0] = kBins; s_bin[1] = kBins; s_found = 0; s_border = 0; }
     MONO_TL(tl_sample, 0);
@@ -768,7 +773,12 @@ static cudaError_t launch(const mono_sample_args* a, cudaStream_t st) {
         if (e != cudaSuccess) return e;
         attr_done(attr_once);
     }
-    return launch_k(sample_kernel<T>, a->rows * kCtas, kThreads, smem, st, *a, slice, run);
+    static const Powers powers = [] {  // (made by every CTA, they cost its start a microsecond)
+        Powers w;
+        for (int i = 0; i < kTable; ++i) w.p[i] = std::exp2(44.0 + i / (double)kTable);
+        return w;
+    }();
+    return launch_k(sample_kernel<T>, a->rows * kCtas, kThreads, smem, st, *a, slice, run, powers);
 }
 
 }  // namespace sampling

@@ -316,6 +316,14 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_narrow_kernel(const __grid
                         for (int z = 0; z < 2; ++z) {
                             if (!on[z]) continue;
                             const uint32_t vb = kb[z] + kTileBytes;
+                            if (lim_all < en.len && key0[z] + 16 > lim_all) {
+#pragma unroll 1
+                                for (int i4 = 0; i4 < 4; ++i4) {
+                                    const int kr = 2 * t + (i4 & 1) + (i4 >> 1) * 8, key = key0[z] + kr;
+                                    if (key >= lim_all && key < en.len) drop_nan(vb + kr * 128 + ((g ^ (kr & 7)) << 4), p.s.share + 2);
+                                }
+                                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the next unit comes here
+                            }
                             uint32_t vw[4][4];
 #pragma unroll
                             for (int i4 = 0; i4 < 4; ++i4) {
@@ -481,6 +489,23 @@ __device__ __forceinline__ Parts parts_of(const mono_prefix_attn_args& a, const 
     return r;
 }
 
+// NaN for those of this lane's eight dims that are NaN in a key which the token sees and the first row of its tile does not
+// (prefix_attn.cuh).  Apart from the kernel's body, which it would take registers from.
+static __device__ __noinline__ void mark_nan(const mono_prefix_attn_args& a, int e, int token, int head, int tile_rows) {
+    const Entry n = entry_of(a, e);
+    const int G = a.q_heads / a.kv_heads, kh = head / G, row = (token - n.tok0) * G + head - kh * G, dim = (threadIdx.x & 15) * 8;
+    const int end = min(row_limit(n, row, G), n.len);
+    for (int key = max(row_limit(n, row & ~(tile_rows - 1), G), 0); key < end; ++key) {
+        const int page = n.table[key / kPage];
+        if (page < 0 || page >= a.n_pages) continue;
+        const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.v_cache) + (((size_t)page * kPage + key % kPage) * a.kv_heads + kh) * kDim + dim);
+        const uint32_t nan[2] = {nan_bytes(v.x), nan_bytes(v.y)};
+        if (!(nan[0] | nan[1])) continue;
+        for (int q = 0; q < 8; ++q)
+            if (nan[q >> 2] >> (8 * (q & 3) + 7) & 1) reinterpret_cast<uint16_t*>(a.out)[((size_t)token * a.q_heads + head) * kDim + dim + q] = 0x7FC0;
+    }
+}
+
 // Half a warp per (token, head): a lane holds eight dims, and the rows of neighbouring heads, which lie side by side in a
 // wide segment, are read together.  SPLIT warps of a CTA share a pair of heads' parts; a batch of parts is requested at
 // once and added to a running maximum, so a row of few parts costs one round trip.
@@ -503,6 +528,9 @@ __global__ void __launch_bounds__(128) prefix_merge_kernel(const __grid_constant
         in[k] = in[k] && token >= rec[k].tok0 && token < rec[k].tok0 + rec[k].ntok;
     }
     if (!in[1]) return;  // a token of no sequence: the row stays as it was
+    // keys with NaN that this row may see and others of its tile do not: steps without the kernel for many rows have few of
+    // them, and look without having been told to
+    const bool look = rec[1].ntok > 1 && (!wide_step(a.tokens, a.q_heads / a.kv_heads) || s.share[2]);
     const int G = a.q_heads / a.kv_heads, kh = head / G;
     float M = -INFINITY, den = 0.f, num[8] = {};
     if (head < a.q_heads) {
@@ -579,6 +607,7 @@ __global__ void __launch_bounds__(128) prefix_merge_kernel(const __grid_constant
         o[q] = *reinterpret_cast<const uint32_t*>(&b);
     }
     reinterpret_cast<uint4*>(a.out)[((size_t)token * a.q_heads + head) * (kDim / 8) + sub] = make_uint4(o[0], o[1], o[2], o[3]);
+    if (look) mark_nan(a, s.entry[1][token], token, head, s.rec[s.entry[1][token]].wide ? kWideTile : narrow_tile(a));
 }
 
 // ------------------------------------------------------------------ host

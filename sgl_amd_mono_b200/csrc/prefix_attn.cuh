@@ -53,6 +53,22 @@ __device__ __forceinline__ int row_limit(const Entry& n, int row, int G) {
     return n.causal ? n.len - n.ntok + 1 + row / G : n.len;
 }
 
+// E4M3 bytes of NaN, as bit 7 of each.
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u; }
+// A weight of zero does not hide a NaN value from a matrix product.  So values of keys that not all rows of a tile see go to the
+// product without their NaN bytes (taken out of the 16 bytes at `at` in shared memory before they are read, out of the way
+// of the blocks without such keys), and the merge gives their NaN to the rows that do see them.
+__device__ __forceinline__ void drop_nan(uint32_t at, uint32_t* found) {
+    uint32_t w[4];
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
+    const uint32_t nan[4] = {nan_bytes(w[0]), nan_bytes(w[1]), nan_bytes(w[2]), nan_bytes(w[3])};
+    if (!(nan[0] | nan[1] | nan[2] | nan[3])) return;
+    *found = 1;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] &= ~((nan[i] >> 7) * 0xFFu);
+    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+}
+
 // A kernel's view of the work: narrow (8- or 16-row tiles, for a group of up to 8 kv heads at once) or wide (256-row tiles, one kv
 // head).  A narrow unit is 128 rows of K and V, (keys x heads of the group): a token's heads lie side by side in the
 // cache, and read together they come from HBM at its full rate, which they do not head by head.  A wide unit is one page;
@@ -124,6 +140,7 @@ __device__ __forceinline__ void make_share(const mono_prefix_attn_args& a, uint3
         const int n = clamp_int((int)((float)ctas * (wide / fmaxf(wide + narrow, 1.f)) + 0.5f), 1, max((int)ctas - 1, 1));
         share[0] = (uint32_t)n;
         share[1] = max(ctas - (uint32_t)n, 1u);
+        share[2] = 0;
     }
 }
 
@@ -141,7 +158,7 @@ struct alignas(16) Record {
 struct Scratch {
     Record* rec;           // [entries]
     uint32_t* total[2];    // units and items of one kv head (narrow: head group), units of a CTA's part and 2^32 over that
-    uint32_t* share;       // how many of its CTAs the wide and the narrow kernel use, where both run
+    uint32_t* share;       // how many of its CTAs the wide and the narrow kernel use, where both run; whether one took NaN bytes out
     int* entry[2];         // [tokens]
     float* seg[2];
     uint8_t* q_image;      // the wide kernel's queries: [2][kv heads][tokens][q heads per kv head][128], and per row

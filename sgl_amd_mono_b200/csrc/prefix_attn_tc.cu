@@ -27,7 +27,7 @@ constexpr int kConvWarp0 = 8, kTmaWarp = 12, kMmaWarp = 13;  // 13 and 14: the p
 constexpr int kThreadsWide = 16 * 32;                         // (warp 15 only fills the warpgroup)
 // Registers per thread: 128 at launch, moved from the warpgroups that need few to the two softmax ones, which hold a
 // block's 64 scores: 2 x 152 + 88 + 120 = 4 x 128.
-constexpr int kRegsSoftmax = 152, kRegsConv = 88, kRegsFetch = 120;
+constexpr int kRegsSoftmax = 152, kRegsConv = 104, kRegsFetch = 104;
 constexpr int kKStages = 6, kVStages = 4, kWStages = 4;  // K bytes, V bytes, widened V
 constexpr int kQPlane = 128 * 128;                       // [128 rows][128 B]
 constexpr int kKTile = kPage * 128, kVTile = kPage * 128, kWTile = 2 * kPage * 128;
@@ -393,6 +393,7 @@ __global__ void __launch_bounds__(kThreadsWide, 1) prefix_wide_kernel(const __gr
             bool live = true;
             for (uint32_t u = u0; u < u1 && live;) {
                 const Item x = item_at(a, off, item, u, u1);
+                const int every = row_limit(x.en, x.row0, G);  // keys below this are seen by all rows
                 for (int i = 0; i < x.blocks && live; ++i, ++it) {
                     const int vs = it % kVStages, ws = it % kWStages;
                     live = wait_on(&v_full[vs], (it / kVStages) & 1, abortp, wait_ns) &&
@@ -400,6 +401,14 @@ __global__ void __launch_bounds__(kThreadsWide, 1) prefix_wide_kernel(const __gr
                     if (!live) break;
                     const uint32_t src = smem_u32(vbuf + vs * kVTile), dst = smem_u32(wbuf + ws * kWTile);
                     const int have = page_ok[it % kOkRing] ? x.en.len - (x.b0 + i) * kPage : 0;
+                    const int all = every - (x.b0 + i) * kPage;
+                    if (all < min(have, kPage)) {
+#pragma unroll 1
+                        for (int j = 0; j < 4; ++j) {
+                            const int key = (ct & 7) + 8 * j + 32 * (ct >> 6), c16 = (ct >> 3) & 7;
+                            if (key >= all && key < have) drop_nan(src + key * 128 + ((c16 ^ (key & 7)) << 4), p.s.share + 2);
+                        }
+                    }
                     uint4 v[4];
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {  // eight lanes: eight keys, no bank twice

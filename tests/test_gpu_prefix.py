@@ -420,3 +420,150 @@ def test_ops_refuse_other_shapes_types_and_devices():
     with pytest.raises(ValueError, match="out"):
         att(q, kc, vc, dt, out=torch.zeros(2, 12, 128, device=DEV))
     assert L.load().mono_prefix_attn_scratch_bytes(8, 12, 2, 2, 1) == att.scratch.numel()
+
+
+# ---------------------------------------------------------------- entries of many rows, and both kinds in one launch
+@pytest.mark.parametrize("hq,hk,ntok,own,starts,prefix", [
+    (12, 2, [3] * 20, [5 + 13 * i for i in range(20)], [0, 20], [333]),        # 18 rows a sequence, 360 a prefix
+    (4, 2, [5] * 7, [5, 64, 65, 6, 300, 129, 9], [0, 2, 7], [640, 63]),        # 10 rows a sequence: half a tile and more
+    (4, 2, [4] * 9, [4, 5, 63, 64, 65, 66, 130, 200, 7], [0, 9], [100]),       # 8 rows a sequence: less than that
+    (8, 8, [1] * 17, [1 + 9 * i for i in range(17)], [0, 17], [700]),          # 17 rows of a prefix in tiles of 8
+    (8, 8, [1] * 16, [1 + 9 * i for i in range(16)], [0, 16], [700]),          # 16 of them
+    (16, 1, [3], [3], [0, 1], [1]),                                            # 48 rows, four keys
+    (16, 1, [2], [2], [0, 1], [64]),                                           # 32 rows in the whole step
+    (33, 3, [12, 1, 24], [12, 1, 90], [0, 2, 3], [65, 1000]),                  # 132 and 264 rows: a tile's halves and borders
+    (5, 1, [52], [1600], [], []),                                              # no prefix
+    (6, 1, [43, 1], [43, 2000], [0, 2], [5])])
+def test_attend_many_rows(hq, hk, ntok, own, starts, prefix):
+    _attend(hq, hk, ntok, own, starts, prefix, columns=1)
+
+
+def test_attend_many_rows_scores_far_apart_and_nan_rows():
+    """Maxima that rise by hundreds between blocks, and a NaN and an infinite query: their own rows only."""
+    hq, hk = 12, 2
+    t, pages = _tables([1] * 30 + [40], [9] * 30 + [400], [0, 30], [1500])
+    caches = _caches(pages, hk)
+    q = (torch.randn(70, hq, 128, generator=_gen(2)) * 30).bfloat16()
+    q[3, 7], q[50, 2, 5], q[12, 1, 100] = float("nan"), float("nan"), float("inf")
+    q[1, 5] *= 1e-30
+    q[1, 6] = 0
+    op = SharedPrefixAttnOp(hq, hk, DEV, max_tokens=70, max_seqs=31, k_scale=K_SCALE, v_scale=V_SCALE)
+    out = op(q.to(DEV), *(c.to(DEV) for c in caches), _dev(t))
+    bad = torch.isnan(out).any(-1).cpu()
+    assert bad[3, 7] and bad[50, 2] and int(bad.sum()) <= 3
+    keep = ~bad[..., None].expand_as(out).clone()
+    keep[12, 1] = False  # infinite scores have no restated value
+    _check_attend(out, q, caches, t, op, rows=keep)
+
+
+@pytest.mark.parametrize("hq,hk,ntok,own,starts,prefix", [
+    (12, 2, [5, 2, 1], [70, 130, 20], [0, 3], [200]),   # tiles of few rows (and 30 rows of one sequence)
+    (3, 1, [2, 3, 2], [20, 80, 64], [], []),
+    (8, 8, [6, 7], [9, 200], [0, 2], [64]),
+    (12, 2, [70, 3], [150, 66], [0, 2], [129]),         # prompt chunks
+    (16, 1, [20], [20], [], [])])
+def test_attend_nan_keys_and_values_of_later_tokens(hq, hk, ntok, own, starts, prefix):
+    """A NaN in a key (or in one dim of a value) of a token reaches the tokens that see it, and no earlier one."""
+    t, pages = _tables(ntok, own, starts, prefix)
+    caches = _caches(pages, hk)
+    for b, (n, ln) in enumerate(zip(ntok, own)):
+        for back, dim, which, head in ((0, 3, 1, 0), (max(n - 2, 0), 77, 1, hk - 1), (n // 2, 5, 0, 0)):
+            if n == 1 and which == 0:
+                continue
+            key = ln - 1 - back
+            caches[which][int(t.page_table[b, key // 64]), key % 64, head, dim] = 0xFF if back else 0x7F
+    tokens = sum(ntok)
+    q = torch.randn(tokens, hq, 128, generator=_gen(11)).bfloat16()
+    op = SharedPrefixAttnOp(hq, hk, DEV, max_tokens=tokens, max_seqs=len(own), max_groups=max(1, len(prefix)), k_scale=K_SCALE, v_scale=V_SCALE)
+    out = op(q.to(DEV), *(c.to(DEV) for c in caches), _dev(t))
+    ref = _check_attend(out, q, caches, t, op)
+    assert torch.equal(torch.isnan(out).cpu(), torch.isnan(ref))
+    assert torch.isnan(ref).any() and torch.isfinite(ref[0]).all() == (ntok[0] > 2)
+
+
+def test_attend_many_rows_ignore_masked_places_and_bad_pages():
+    hq, hk = 12, 2
+    op, q, caches, dc, t, out = _attend(hq, hk, [20, 1, 30], [33, 70, 129], [0, 3], [200])
+    want = out.clone()
+    n = [c.clone() for c in caches]
+    for tab, lens in ((t.page_table, t.lens), (t.prefix_table, t.prefix_lens)):
+        for row, ln in zip(tab, lens):
+            full, part = divmod(int(ln), 64)
+            if part:
+                for c in n:
+                    c[int(row[full]), part:] = 0x7F
+    assert torch.equal(op(q.to(DEV), *(c.to(DEV) for c in n), _dev(t)), want)
+    t2 = PrefixTables(t.q_start, t.page_table.clone(), t.lens, t.group_start, t.prefix_table.clone(), t.prefix_lens)
+    t2.prefix_table[0, 1] = caches[0].shape[0]
+    t2.page_table[2, 0] = -5
+    _check_attend(op(q.to(DEV), *dc, _dev(t2)), q, caches, t2, op)
+
+
+def test_attend_steps_of_other_sizes_share_an_op():
+    """Steps with and without entries of many rows, one after another on one op's buffers, each as on fresh ones."""
+    hq, hk = 12, 2
+    op = SharedPrefixAttnOp(hq, hk, DEV, max_tokens=200, max_seqs=40, max_groups=3, k_scale=K_SCALE, v_scale=V_SCALE)
+    for seed, (ntok, own, starts, prefix) in enumerate([
+            ([1] * 40, [9 + i for i in range(40)], [0, 20, 39, 40], [500, 77, 3]), ([1], [700], [], []), ([3] * 10, [40] * 10, [0, 10], [300]),
+            ([150, 2], [150, 2], [0, 1, 2], [64, 900]), ([1] * 2, [5, 6], [0, 2], [2000])]):
+        t, pages = _tables(ntok, own, starts, prefix, seed)
+        caches = _caches(pages, hk)
+        q = torch.randn(sum(ntok), hq, 128, generator=_gen(seed)).bfloat16()
+        _check_attend(op(q.to(DEV), *(c.to(DEV) for c in caches), _dev(t)), q, caches, t, op)
+        assert ops.guard_read(op.guard)[0] == 0
+
+
+def test_a_decode_step_in_one_graph():
+    """Append, attention, LM head and draw captured as one step; the replays follow the tables and the random numbers."""
+    from sgl_amd_mono_b200.sampling import SampleOp
+    from sgl_amd_mono_b200.tail import LmHeadOp
+
+    hq, hk, seqs, vocab, prompt = 12, 2, 6, 1000, 100
+    hidden, width = hq * 128, (hq + 2 * hk) * 128
+    g = _gen(21)
+    ang = torch.arange(256, dtype=torch.float64)[:, None] / 1e4 ** (torch.arange(0, 64, 2, dtype=torch.float64) / 64)
+    cos, sin = ang.cos().bfloat16().to(DEV), ang.sin().bfloat16().to(DEV)
+    pages = 2 + seqs
+    kc, vc = (c.to(DEV) for c in _caches(pages, hk))
+    app = QkvAppendOp(hq, hk, DEV, max_tokens=seqs, k_scale=K_SCALE, v_scale=V_SCALE)
+    att = SharedPrefixAttnOp(hq, hk, DEV, max_tokens=seqs, max_seqs=seqs, k_scale=K_SCALE, v_scale=V_SCALE)
+    w = (torch.randn(vocab, hidden, generator=g) * hidden**-0.5).bfloat16().to(DEV)
+    head = LmHeadOp(hidden, w, torch.zeros(hidden, dtype=torch.bfloat16, device=DEV), 1e-6, DEV)
+    draw = SampleOp(vocab, DEV, max_rows=seqs)
+    x = torch.zeros(seqs, width, dtype=torch.bfloat16, device=DEV)
+    positions, slots = (torch.zeros(seqs, dtype=torch.int64, device=DEV) for _ in range(2))
+    u, temp = torch.zeros(seqs, device=DEV), torch.full((seqs,), 0.8, device=DEV)
+    top_p = torch.full((seqs,), 0.9, device=DEV)
+    own = torch.arange(2, pages)
+    t = PrefixTables(torch.arange(seqs + 1, dtype=torch.int32), own.to(torch.int32).view(seqs, 1), torch.ones(seqs, dtype=torch.int32),
+                     torch.tensor([0, seqs], dtype=torch.int32), torch.tensor([[1, 0]], dtype=torch.int32), torch.tensor([prompt], dtype=torch.int32))
+    dt = _dev(t)
+
+    def step():
+        out = att(app(x, None, None, cos, sin, positions, slots, kc, vc), kc, vc, dt)
+        logits = head(out.view(seqs, hidden))
+        return out, logits, *draw(logits, u, temp, None, top_p)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            res = step()
+    torch.cuda.current_stream().wait_stream(side)
+    for k in range(3):
+        x.copy_(torch.randn(seqs, width, generator=g))
+        u.copy_(torch.rand(seqs, generator=g))
+        positions.fill_(prompt + k)
+        slots.copy_(own * 64 + k)
+        t.lens.fill_(k + 1)
+        dt.lens.copy_(t.lens)
+        graph.replay()
+        torch.cuda.synchronize()
+        out, logits, tokens, logprobs = (r.cpu() for r in res)
+        _check_attend(out, app.q.cpu(), [kc.cpu(), vc.cpu()], t, att)
+        for r in range(seqs):
+            token, lp, gap = OP.sample_row(logits[r].numpy(), float(u[r]), 0.8, 0, float(top_p[r]), 0.0)
+            # the draw decides to 2^-44 of the largest weight; sums in the restatement round at 2^-52 of theirs
+            assert gap < 1e-9 or (int(tokens[r]) == token and abs(float(logprobs[r]) - lp) <= abs(lp) * 2.0**-23 + 1e-9)

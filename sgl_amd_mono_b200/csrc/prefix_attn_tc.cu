@@ -232,7 +232,7 @@ __global__ void __launch_bounds__(kThreadsWide, 1) prefix_wide_kernel(const __gr
     uint32_t* off = reinterpret_cast<uint32_t*>(wbuf + kWStages * kWTile);
     uint32_t* item = off + E + 1;
     __shared__ uint64_t k_full[kKStages], k_empty[kKStages], v_full[kVStages], v_empty[kVStages], w_full[kWStages], w_empty[kWStages];
-    __shared__ uint64_t q_full[2], q_free[2], s_full[2], s_free[2], p_full[2][2], o_done[2], j_free, j_full, j_done;
+    __shared__ uint64_t q_full[2], q_free[2], s_full[2], s_free[2], p_full[2][2], o_done[2][2], j_free, j_full, j_done;
     __shared__ float s_join[2][128];  // stream 1's maxima and sums
     __shared__ int page_ok[kOkRing];
     __shared__ uint32_t red[64], tmem_base_s;
@@ -244,7 +244,7 @@ __global__ void __launch_bounds__(kThreadsWide, 1) prefix_wide_kernel(const __gr
         for (int i = 0; i < kKStages; ++i) { mbar_init(&k_full[i], 1); mbar_init(&k_empty[i], 2); }
         for (int i = 0; i < kVStages; ++i) { mbar_init(&v_full[i], 1); mbar_init(&v_empty[i], 4); }
         for (int i = 0; i < kWStages; ++i) { mbar_init(&w_full[i], 128); mbar_init(&w_empty[i], 2); }
-        for (int i = 0; i < 2; ++i) { mbar_init(&q_full[i], 1); mbar_init(&q_free[i], 1); mbar_init(&s_full[i], 1); mbar_init(&s_free[i], 4); mbar_init(&p_full[0][i], 4); mbar_init(&p_full[1][i], 4); mbar_init(&o_done[i], 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&q_full[i], 1); mbar_init(&q_free[i], 1); mbar_init(&s_full[i], 1); mbar_init(&s_free[i], 4); mbar_init(&p_full[0][i], 4); mbar_init(&p_full[1][i], 4); mbar_init(&o_done[0][i], 1); mbar_init(&o_done[1][i], 1); }
         mbar_init(&j_free, 128);
         mbar_init(&j_full, 128);
         mbar_init(&j_done, 128);
@@ -339,8 +339,8 @@ __global__ void __launch_bounds__(kThreadsWide, 1) prefix_wide_kernel(const __gr
                 const Item x = item_at(a, off, item, u, u1);
                 const int count = x.count(st), step = x.step();
                 // A block's scores are asked for as soon as the softmax has the scores before in registers, ahead of that
-                // block's values.  One thread's products are done in order: when S of block t + 2 is there, P of block t
-                // has been used.
+                // block's values.  (The two products are of different kinds and end in no certain order: that P of block t is
+                // used, and that O holds it, is asked of o_done, a barrier for even blocks and one for odd ones.)
                 for (int t = -1; t < count && live; ++t) {
                     if (t + 1 < count) {  // S = Q K^T of block t + 1
                         const int i = it0 + x.first(st) + (t + 1) * step, ks = i % kKStages, g = g0 + t + 1;
@@ -371,7 +371,7 @@ __global__ void __launch_bounds__(kThreadsWide, 1) prefix_wide_kernel(const __gr
                         if (elect_one()) {
 #pragma unroll
                             for (int s = 0; s < 4; ++s) mma_f16_ts(o_at, s_at + 64 + (g & 1) * 32 + s * 8, wd + s * (16 * 128 / 16), kIdescO, s > 0 || t > 0);
-                            mma_commit(&o_done[st]);
+                            mma_commit(&o_done[st][g & 1]);
                             mma_commit(&w_empty[ws]);
                             if (x.split) mma_commit(&w_empty[ws]);
                         }
@@ -491,7 +491,7 @@ __global__ void __launch_bounds__(kThreadsWide, 1) prefix_wide_kernel(const __gr
                         if (__any_sync(0xffffffffu, up != 1.f)) {
                             l *= up;
                             if (t > 0) {
-                                live = wait_on(&o_done[st], (g - 1) & 1, abortp, wait_ns);  // the block before is in O
+                                live = wait_on(&o_done[st][(g - 1) & 1], ((g - 1) >> 1) & 1, abortp, wait_ns);  // the block before is in O
                                 if (!live) break;
                                 fence_after();
 #pragma unroll 1
@@ -506,6 +506,11 @@ __global__ void __launch_bounds__(kThreadsWide, 1) prefix_wide_kernel(const __gr
                             }
                             sum = weights(s, qs, kBias - (m == -INFINITY ? 0.f : m), w, &mx);
                         }
+                        if (t > 1) {  // the place of these weights has been read
+                            live = wait_on(&o_done[st][g & 1], ((g >> 1) - 1) & 1, abortp, wait_ns);
+                            if (!live) break;
+                            fence_after();
+                        }
                         tmem_st16(s_addr + 64 + (g & 1) * 32, w);
                         tmem_st16(s_addr + 64 + (g & 1) * 32 + 16, w + 16);
                         l += sum;
@@ -517,7 +522,7 @@ __global__ void __launch_bounds__(kThreadsWide, 1) prefix_wide_kernel(const __gr
                     }
                     if (!live) break;
                     g0 += count;
-                    live = wait_on(&o_done[st], (g0 - 1) & 1, abortp, wait_ns);
+                    live = wait_on(&o_done[st][(g0 - 1) & 1], ((g0 - 1) >> 1) & 1, abortp, wait_ns);
                     MONO_TL(tl_wide, 13);
                     if (!live) break;
                     fence_after();

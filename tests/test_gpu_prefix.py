@@ -567,3 +567,12 @@ def test_a_decode_step_in_one_graph():
             token, lp, gap = OP.sample_row(logits[r].numpy(), float(u[r]), 0.8, 0, float(top_p[r]), 0.0)
             # the draw decides to 2^-44 of the largest weight; sums in the restatement round at 2^-52 of theirs
             assert gap < 1e-9 or (int(tokens[r]) == token and abs(float(logprobs[r]) - lp) <= abs(lp) * 2.0**-23 + 1e-9)
+
+
+@pytest.mark.parametrize("qmul", [1.0, 3.0])
+def test_attend_long_prefix_of_many_rows(qmul):
+    """Single keys that hold much of a row's weight, anywhere in a long prefix: none may be lost when a maximum rises."""
+    op, q, caches, dc, t, out = _attend(12, 2, [1] * 64, [33] * 64, [0, 64], [7000], seed=3, qmul=qmul)
+    qd, dt, want = q.to(DEV), _dev(t), out.clone()
+    for _ in range(20):
+        assert torch.equal(op(qd, *dc, dt), want)

@@ -91,8 +91,12 @@ __device__ __forceinline__ void load_q(const mono_prefix_attn_args& a, const Ent
 // Up to 8 NT rows per tile, of every head of a group.  A unit's 128 rows of K and V arrive by one TMA box each, head after
 // head (128-byte swizzle, which makes the 16-byte shared loads below free of bank conflicts); each of the eight warps
 // takes 16 keys of one head, with a running maximum and sum of its own.  Where a head has several warps they join their
-// parts at the segment's end.  The ninth warp keeps the ring of units full.  Bound: HBM; K and V stay bytes until a warp
-// has them in registers, where they become f16 exactly.
+// parts at the segment's end.  The ninth warp keeps the ring of units full.  K and V stay bytes until a warp has them in
+// registers, where they become f16 exactly.
+//
+// Bound: on all SMs HBM (80 us for 256 sequences of 512 keys, 48 heads on 8: fetching alone took 64); on the share of them
+// that it has beside the wide kernel, latency: of 1600 cycles a unit, 335 go to the first product, 205 to the softmax, 430 to
+// the second and 450 to waiting for the unit.
 //
 // Both products are formed transposed: S^T[key][row] = K Q^T and O^T[dim][row] += V^T P^T, with keys and dims as the 16
 // rows of the fragments and NT times 8 query rows as their columns: one token's heads are at most eight as a rule, and as
@@ -508,7 +512,8 @@ static __device__ __noinline__ void mark_nan(const mono_prefix_attn_args& a, int
 
 // Half a warp per (token, head): a lane holds eight dims, and the rows of neighbouring heads, which lie side by side in a
 // wide segment, are read together.  SPLIT warps of a CTA share a pair of heads' parts; a batch of parts is requested at
-// once and added to a running maximum, so a row of few parts costs one round trip.
+// once and added to a running maximum, so a row of few parts costs one round trip.  Bound: latency, of tables, then parts
+// (7 us for 48 rows, 11 us for 192 rows of 74 parts, 15 us for 12288 rows of 7 to 10).
 template <int SPLIT>
 __global__ void __launch_bounds__(128) prefix_merge_kernel(const __grid_constant__ mono_prefix_attn_args a, const __grid_constant__ Scratch s) {
     pdl_prologue();
@@ -728,7 +733,8 @@ extern "C" int mono_prefix_attn_launch(const mono_prefix_attn_args* a, void* str
         if (int rc = mono_tmap_encode_box(reinterpret_cast<mono_tmap_t*>(&p.qmap), p.s.q_image, 128, q_rows, 2, 128, q_rows * 128, 128)) return rc;
     cudaError_t e = wide ? launch_wide(p, wide, st) : cudaSuccess;
     if (e == cudaSuccess) e = launch_k(narrow_tile(*a) == 8 ? prefix_narrow_kernel<1> : prefix_narrow_kernel<2>, narrow, kThreads, smem, st, p);
-    // Few rows: four warps share two heads' segments (a long prefix leaves many of them); many rows: a warp each.
+    // Few rows: four warps share two heads' segments (a long prefix leaves many of them); many rows: a warp each.  (3072 rows:
+    // 103 us the whole step with four, 117 with one; 12288 rows: 184 with four, 176 with two, 175 with one.)
     if (e == cudaSuccess) {
         if ((long)a->tokens * a->q_heads < 8192)
             e = launch_k(prefix_merge_kernel<4>, dim3(a->tokens, (a->q_heads + 1) / 2), 128, 0, st, *a, p.s);

@@ -85,9 +85,9 @@ __host__ __device__ __forceinline__ int group_heads(int kv_heads) { return kv_he
 __host__ __device__ __forceinline__ int head_groups(int kv_heads) { return (kv_heads + group_heads(kv_heads) - 1) / group_heads(kv_heads); }
 __host__ __device__ __forceinline__ int unit_keys(int kv_heads) { return 128 / group_heads(kv_heads); }
 // Rows of an entry from which the wide kernel takes it.  An entry of a few tiles reads its keys once per tile, the wide
-// kernel once: it wins from three tiles of 8 rows (a prefix of 11312 keys, 10 rows: 49 us wide, 41 narrow; 256 samples of
-// prompts with 17 to 48 rows: 149 wide, 158 narrow) and from one of 16 that is more than half full (30499 keys, 14 rows: 77
-// wide, 112 narrow).  A step of fewer rows than kWideStep in all stays narrow: the wide kernel's launch and start cost it
+// kernel once: that wins from three tiles of 8 rows (256 samples of prompts with 17 to 48 rows: 149 us wide, 158 narrow; 10
+// rows of a prefix of 11312 keys: 49 wide, 41 narrow) and from one of 16 that is more than half full (14 rows, 30499 keys:
+// 77 wide, 112 narrow).  A step of fewer rows than kWideStep in all stays narrow: the wide kernel's launch and start cost it
 // more (24 rows: 21 us wide, 16 narrow).
 constexpr int kWideRows = 9, kWideStep = 33;
 __host__ __device__ __forceinline__ bool wide_step(int tokens, int G) { return (long)tokens * G >= kWideStep; }
@@ -112,10 +112,11 @@ __device__ __forceinline__ Work entry_work(const mono_prefix_attn_args& a, const
     return w;
 }
 
-// How the SMs are shared between the two kernels, which run side by side: the wide one is bound by its SMs, the narrow one by
-// HBM, and one after the other each leaves idle what the other wants.  In proportion to their work, a wide unit taken as
-// kWideCost and a narrow one as kNarrowCost for every eight rows of its tile (measured: 64 samples of a long prompt took 84, 84, 94
-// and 107 us at ratios 5, 6, 4 and 3 to 9; 24 samples in tiles of 16 rows 47 to 53 at 6 to 13 to 9, 62 at 4); each has at least one CTA, which leaves the merge's records.
+// How the SMs are shared between the two kernels, which run side by side: a start, a plan and an end cost each of them some
+// 8 us, and what one leaves of HBM or of the SMs the other uses (one after the other 64 samples of a long prompt took 103
+// us, side by side 80).  In proportion to their work, a wide unit taken as kWideCost and a narrow one as kNarrowCost for
+// every eight rows of its tile (64 samples: 84, 84, 94 and 107 us at ratios of 5, 6, 4 and 3 to 9; 24 samples in tiles of
+// 16 rows: 47 to 53 at 6 to 13 to 9, 62 at 4).  Each has at least one CTA, which leaves the merge's records.
 constexpr int kWideCost = 3, kNarrowCost = 2;
 __device__ __forceinline__ void make_share(const mono_prefix_attn_args& a, uint32_t* share, uint32_t ctas) {
     __shared__ float s_wide[32], s_narrow[32];

@@ -7,7 +7,9 @@
 // bf16 after the norm and after the rotation instead.
 //
 // Bound: memory.  A token's row is read once and written once (bf16 q, one byte per K and V value).  Sixteen lanes hold
-// a head, eight dims (16 bytes) each, so a warp takes two heads at a time and a norm is four shuffles.
+// a head, eight dims (16 bytes) each, so a warp takes two heads at a time and a norm is four shuffles.  Four pairs of heads
+// are in flight, and what a token and kind multiply by is made once for all its heads.  Measured (48 q heads on 8, B200):
+// 16384 tokens 88 us, 5771 GB/s, 88 % of a copy; 2001 tokens 20.8 us; 16 tokens of 12 heads on 2 2.5 us, a launch.
 #include "mono_common.cuh"
 
 extern void mono_set_error(const char* fmt, ...);

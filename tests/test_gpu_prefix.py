@@ -576,3 +576,21 @@ def test_attend_long_prefix_of_many_rows(qmul):
     qd, dt, want = q.to(DEV), _dev(t), out.clone()
     for _ in range(20):
         assert torch.equal(op(qd, *dc, dt), want)
+
+
+def test_attend_as_many_entries_as_a_launch_takes():
+    n = 2047
+    _attend(1, 1, [1] * n, [1 + i % 5 for i in range(n)], [0, n], [70])
+    _attend(2, 1, [0] * 1023 + [1] * 1024, [0] * 1023 + [1 + i % 70 for i in range(1024)], [], [])
+
+
+def test_attend_one_launch_after_another_without_overlap():
+    """The same bits whether a launch's kernels may start before the one before has ended or not."""
+    cases = [_attend(12, 2, [3] * 20, [40] * 20, [0, 20], [900]), _attend(12, 2, [1] * 3, [70] * 3, [0, 3], [300])]
+    want = [out.clone() for *_, out in cases]
+    try:
+        L.load().mono_set_pdl(0)
+        for (op, q, caches, dc, t, _), w in zip(cases, want):
+            assert torch.equal(op(q.to(DEV), *dc, _dev(t)), w)
+    finally:
+        L.load().mono_set_pdl(1)

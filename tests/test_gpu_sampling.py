@@ -28,7 +28,9 @@ def _check(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, op=N
         assert gap > 2.0**-36, "the test's own numbers lie on a border"
         assert int(token[r]) == want, f"row {r}: token {int(token[r])}, expected {want}"
         if want >= 0:
-            assert abs(float(logprob[r]) - lp) <= abs(lp) * 2.0**-24 + 2.0**-40, f"row {r}"
+            # every weight is rounded by at most 2^-45 of the largest, so their sum Z, which is at least the largest, by at
+            # most vocab 2^-45 of itself, and log Z by as much
+            assert abs(float(logprob[r]) - lp) <= abs(lp) * 2.0**-24 + 2.0**-40 + vocab * 2.0**-45, f"row {r}"
         else:
             assert float(logprob[r]) == -np.inf
     return token
@@ -201,3 +203,28 @@ def test_refusals():
     for name, bad in (("u", u.double()), ("u", u[:3]), ("top_k", u), ("top_p", u.int()), ("temperature", u.cpu()), ("min_p", u.repeat(2))):
         with pytest.raises(ValueError, match=name):
             op(**{"logits": x, "u": u, name: bad})
+
+
+@pytest.mark.parametrize("together", [True, False])
+@pytest.mark.parametrize("n", [1, 63, 64, 65, 127, 255, 256, 257, 700])
+def test_borders_among_many_close_logits(n, together):
+    """``n`` logits within a thousandth of each other (some equal) hold nearly all the mass, in one run or all over the
+    row: the border lies among them, whether they are few enough to be ranked at once or not."""
+    vocab, rows = 20000, 8
+    g = torch.Generator().manual_seed(n)
+    x = torch.randn(rows, vocab, generator=g) - 12
+    for r in range(rows):
+        at = torch.arange(n) + 4100 if together else torch.randperm(vocab, generator=g)[:n]
+        x[r, at] = 3 + torch.randint(0, 8, (n,), generator=g) * 1e-4
+    k = torch.tensor([1, max(1, n // 2), n, n + 1, 0, max(1, n - 1), 1, n // 3 + 1], dtype=torch.int32)
+    p = torch.tensor([1.0, 1.0, 0.999, 1.0, 0.37, 0.5, 0.0, 0.9])
+    mp = torch.tensor([0.0, 0.0, 0.0, 0.5, 0.0, 0.9997, 1.0, 0.0])
+    _check(x, _u(rows, seed=n + 1), torch.tensor([0.7, 1.0, 1.3, 1.0, 2.0, 1.0, 1.0, 0.5]), k, p, mp)
+
+
+def test_rank_zero_alone_is_the_first_of_the_largest():
+    x = _logits(4, 5000, seed=3)
+    x[:, [77, 4000]] = 9.0
+    one = torch.ones(4, dtype=torch.int32)
+    token = _check(x, torch.tensor([0.0, 0.5, 0.999, 0.3]), torch.tensor([1.0, 0.3, 5.0, 0.0]), one, torch.tensor([1.0, 0.0, 0.5, 1.0]), torch.tensor([0.0, 1.0, 0.2, 0.0]))
+    assert (token == 77).all()

@@ -9,7 +9,7 @@
 // Bound: memory.  A token's row is read once and written once (bf16 q, one byte per K and V value).  Sixteen lanes hold
 // a head, eight dims (16 bytes) each, so a warp takes two heads at a time and a norm is four shuffles.  Four pairs of heads
 // are in flight, and what a token and kind multiply by is made once for all its heads.  Measured (48 q heads on 8, B200):
-// 16384 tokens 84 us, 6022 GB/s, 92 % of a copy; 2001 tokens 17.1 us; 16 tokens of 12 heads on 2 2.5 us, a launch.
+// 16384 tokens 84 us, 6022 GB/s, 92 % of a copy; 2001 tokens 16.5 us; 16 tokens of 12 heads on 2 2.3 us, a launch.
 #include "mono_common.cuh"
 
 extern void mono_set_error(const char* fmt, ...);
@@ -18,7 +18,10 @@ namespace qkv_append {
 using namespace mono;
 
 constexpr int kDim = 128;
-constexpr int kThreads = 256, kCtasPerSm = 4;
+constexpr int kThreads = 256;
+// CTAs of an SM: with four, halves that turn with one another (their partners come by shuffles) do not fit 64 registers
+// (16384 tokens 101 us, with three 92), interleaved pairs do (84 us, with three 87).  Partial sums have at most 16 rows.
+constexpr int ctas_per_sm(bool interleaved, bool f32) { return f32 ? 2 : interleaved ? 4 : 3; }
 
 typedef unsigned long long f32x2;  // two f32 that one instruction works on
 __device__ __forceinline__ f32x2 pair(float lo, float hi) {
@@ -186,7 +189,7 @@ __device__ __forceinline__ void do_heads(const mono_qkv_append_args& a, const La
 // A warp takes `pairs` pairs of heads of one token (q pairs, then k, then v); lanes 0..15 hold the even head of a pair,
 // 16..31 the odd one.
 template <bool INTERLEAVED, bool F32SRC>
-__global__ void __launch_bounds__(kThreads, kCtasPerSm) qkv_append_kernel(const __grid_constant__ mono_qkv_append_args a, int chunks, int pairs) {
+__global__ void __launch_bounds__(kThreads, ctas_per_sm(INTERLEAVED, F32SRC)) qkv_append_kernel(const __grid_constant__ mono_qkv_append_args a, int chunks, int pairs) {
     pdl_prologue();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const unsigned work = blockIdx.x * (kThreads / 32) + warp;
@@ -218,10 +221,10 @@ template <bool INTERLEAVED>
 static cudaError_t launch(const mono_qkv_append_args* a, cudaStream_t st) {
     const int pairs = (a->q_heads + 1) / 2 + 2 * ((a->kv_heads + 1) / 2);
     // How many warps share a token: what takes least, reckoned as rounds of the warps that the GPU holds, a round as long as a
-    // warp's pairs of heads and kStart more (angles and latency).  2001 tokens of 48 heads on 8: two warps, one round, 17 us
-    // (five warps, which fill it 2.1 times, 20.6); 3000: three warps 23 us, one 28; 6000: two 41, one 45.
+    // warp's pairs of heads and kStart more (angles and latency).  With 32 warps an SM and 48 heads on 8: 2001 tokens, two
+    // warps, one round, 17 us (five warps, which fill it 2.1 times, 20.6); 3000: three warps 23 us, one 28; 6000: two 41, one 45.
     constexpr int kStart = 4;
-    const long long held = (mono_sm_count() > 0 ? mono_sm_count() : 148) * kCtasPerSm * (kThreads / 32);
+    const long long held = (mono_sm_count() > 0 ? mono_sm_count() : 148) * ctas_per_sm(INTERLEAVED, a->src_f32 != nullptr) * (kThreads / 32);
     int chunks = 1;
     long long least = -1;
     for (int c = 1; c <= pairs && (c == 1 || a->tokens * (long long)c <= 8 * held); ++c) {

@@ -733,8 +733,8 @@ extern "C" int mono_prefix_attn_launch(const mono_prefix_attn_args* a, void* str
         if (int rc = mono_tmap_encode_box(reinterpret_cast<mono_tmap_t*>(&p.qmap), p.s.q_image, 128, q_rows, 2, 128, q_rows * 128, 128)) return rc;
     cudaError_t e = wide ? launch_wide(p, wide, st) : cudaSuccess;
     if (e == cudaSuccess) e = launch_k(narrow_tile(*a) == 8 ? prefix_narrow_kernel<1> : prefix_narrow_kernel<2>, narrow, kThreads, smem, st, p);
-    // Few rows: four warps share two heads' segments (a long prefix leaves many of them); many rows: a warp each.  (3072 rows:
-    // 103 us the whole step with four, 117 with one; 12288 rows: 184 with four, 176 with two, 175 with one.)
+    // Few rows: four warps share two heads' segments (a long prefix leaves many of them); many rows: a warp each.  (64 tokens
+    // of 48 heads: 103 us the whole step with four, 117 with one; 256 tokens: 184 with four, 176 with two, 175 with one.)
     if (e == cudaSuccess) {
         if ((long)a->tokens * a->q_heads < 8192)
             e = launch_k(prefix_merge_kernel<4>, dim3(a->tokens, (a->q_heads + 1) / 2), 128, 0, st, *a, p.s);

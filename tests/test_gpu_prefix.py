@@ -417,6 +417,9 @@ def test_ops_refuse_other_shapes_types_and_devices():
                        ("prefix_table", dt.prefix_table[0]), ("prefix_lens", None), ("prefix_lens", dt.prefix_lens.repeat(2))]:
         with pytest.raises(ValueError, match=field):
             att(q, kc, vc, PrefixTables(**{**dt.__dict__, field: bad}))
+    for guard in (torch.zeros(L.GUARD_WORDS, device=DEV), torch.zeros(1, dtype=torch.int32, device=DEV), torch.zeros(L.GUARD_WORDS, dtype=torch.int32)):
+        with pytest.raises(ValueError, match="guard"):
+            SharedPrefixAttnOp(12, 2, DEV, max_tokens=8, max_seqs=2, guard=guard)
     with pytest.raises(ValueError, match="out"):
         att(q, kc, vc, dt, out=torch.zeros(2, 12, 128, device=DEV))
     assert L.load().mono_prefix_attn_scratch_bytes(8, 12, 2, 2, 1) == att.scratch.numel()

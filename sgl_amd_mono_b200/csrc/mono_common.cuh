@@ -353,6 +353,8 @@ inline int current_device_bit(uint64_t* bit) {
     *bit = 1ull << dev;
     return dev;
 }
+// A scale whose inverse is a normal number too.
+inline bool scale_ok(float s) { return s >= 0x1p-100f && s <= 0x1p100f; }
 inline bool attr_needed(const std::atomic<uint64_t>& once) {
     uint64_t bit = 0;
     if (current_device_bit(&bit) < 0) return true;

@@ -668,8 +668,8 @@ extern "C" int mono_prefix_attn_launch(const mono_prefix_attn_args* a, void* str
         return MONO_E_ARG;
     }
     if (a->q_ld < (long)a->q_heads * kDim || (a->q_ld & 7) || ((reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->out)) & 15) ||
-        (reinterpret_cast<uintptr_t>(a->scratch) & 255) || !(a->k_scale > 0.f) || !(a->v_scale > 0.f) || !(a->sm_scale > 0.f)) {
-        mono_set_error("%s: q rows at least q_heads * 128 values apart (a multiple of 8) on 16-byte addresses, scratch on a 256-byte address and positive scales required", who);
+        (reinterpret_cast<uintptr_t>(a->scratch) & 255) || !mono::scale_ok(a->k_scale) || !mono::scale_ok(a->v_scale) || !mono::scale_ok(a->sm_scale)) {
+        mono_set_error("%s: q rows at least q_heads * 128 values apart (a multiple of 8) on 16-byte addresses, scratch on a 256-byte address and scales of 2^-100 .. 2^100 required", who);
         return MONO_E_ARG;
     }
     if (a->n_pages < 1 || a->n_pages > (1ll << 31) / kPage - 1 || a->pt_ld > (1 << 24) || a->prefix_ld > (1 << 24)) {

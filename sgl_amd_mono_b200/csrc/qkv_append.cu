@@ -263,9 +263,8 @@ extern "C" int mono_qkv_append_launch(const mono_qkv_append_args* a, void* strea
     const uintptr_t all = reinterpret_cast<uintptr_t>(a->g_q) | reinterpret_cast<uintptr_t>(a->g_k) | reinterpret_cast<uintptr_t>(a->cos) |
                           reinterpret_cast<uintptr_t>(a->sin) | reinterpret_cast<uintptr_t>(a->q_out) | reinterpret_cast<uintptr_t>(a->k_cache) |
                           reinterpret_cast<uintptr_t>(a->v_cache);
-    if (!a->cos || !a->sin || a->table_rows < 1 || !a->positions || !a->q_out || !a->k_cache || !a->v_cache || a->n_pages < 1 || !(a->k_scale > 0.f) ||
-        !(a->v_scale > 0.f) || !(a->eps >= 0.f) || (all & 15)) {
-        mono_set_error("%s: rope tables, positions, q output and caches with positive scales required, 16-byte aligned", who);
+    if (!a->cos || !a->sin || a->table_rows < 1 || !a->positions || !a->q_out || !a->k_cache || !a->v_cache || a->n_pages < 1 || !mono::scale_ok(a->k_scale) || !mono::scale_ok(a->v_scale) || !(a->eps >= 0.f) || (all & 15)) {
+        mono_set_error("%s: rope tables, positions, q output and caches with scales of 2^-100 .. 2^100 required, 16-byte aligned", who);
         return MONO_E_ARG;
     }
     const cudaError_t e = a->interleaved ? qkv_append::launch<true>(a, (cudaStream_t)stream) : qkv_append::launch<false>(a, (cudaStream_t)stream);

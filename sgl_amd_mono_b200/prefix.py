@@ -42,8 +42,8 @@ def _heads(q_heads: int, kv_heads: int) -> None:
 
 def _scale(x: float, name: str) -> float:
     x = float(x)
-    if not 0.0 < x < float("inf"):
-        raise ValueError(f"{name}: {x}, needs a positive finite number")
+    if not 2.0**-100 <= x <= 2.0**100:
+        raise ValueError(f"{name}: {x}, needs a positive number, 2**-100 .. 2**100")
     return x
 
 

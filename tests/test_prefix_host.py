@@ -32,7 +32,7 @@ def _append_args(**kw):
 @pytest.mark.parametrize("bad", [
     dict(tokens=0), dict(q_heads=0), dict(kv_heads=0), dict(rot_dim=8), dict(rot_dim=72), dict(rot_dim=144), dict(src_bf16=None),
     dict(src_f32=4096), dict(src_ld=2040), dict(src_ld=2052), dict(src_bf16=4098), dict(cos=None), dict(table_rows=0), dict(positions=None),
-    dict(q_out=None), dict(k_cache=None), dict(v_cache=4100), dict(n_pages=0), dict(k_scale=0.0), dict(v_scale=-1.0), dict(eps=float("nan")),
+    dict(q_out=None), dict(k_cache=None), dict(v_cache=4100), dict(n_pages=0), dict(k_scale=0.0), dict(v_scale=-1.0), dict(k_scale=1e-39), dict(eps=float("nan")),
     dict(src_bf16=None, src_f32=4096, nsum=0), dict(src_bf16=None, src_f32=4096, nsum=2, tokens=17), dict(src_bf16=None, src_f32=4096, nsum=2, sum_stride=6)])
 def test_append_refuses(lib, bad):
     assert lib.mono_qkv_append_launch(C.byref(_append_args(**bad)), None) == -1
@@ -52,7 +52,7 @@ def _attn_args(**kw):
 @pytest.mark.parametrize("bad", [
     dict(tokens=0), dict(q_heads=13), dict(q_heads=34), dict(kv_heads=0), dict(seqs=0), dict(groups=-1), dict(seqs=2048), dict(q=None),
     dict(q_ld=1528), dict(q_ld=1540), dict(q=4104), dict(out=4104), dict(scratch=4112), dict(scratch=None), dict(scratch_bytes=1000), dict(lens=None),
-    dict(pt_ld=0), dict(prefix_ld=0), dict(group_start=None), dict(k_scale=0.0), dict(n_pages=0), dict(n_pages=1 << 26),
+    dict(pt_ld=0), dict(prefix_ld=0), dict(group_start=None), dict(k_scale=0.0), dict(v_scale=float("inf")), dict(sm_scale=1e-40), dict(n_pages=0), dict(n_pages=1 << 26),
     dict(tokens=1 << 20, pt_ld=1 << 20)])
 def test_attention_refuses(lib, bad):
     assert lib.mono_prefix_attn_launch(C.byref(_attn_args(**bad)), None) == -1

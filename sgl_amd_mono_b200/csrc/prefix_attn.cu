@@ -100,8 +100,8 @@ __device__ __forceinline__ void load_q(const mono_prefix_attn_args& a, const Ent
 // registers, where they become f16 exactly.
 //
 // Bound: on all SMs HBM (80 us for 256 sequences of 512 keys, 48 heads on 8: fetching alone took 64); on the share of them
-// that it has beside the wide kernel, mma.sync: of 1600 cycles a unit, 335 go to the first product, 205 to the softmax, 430 to
-// the second, and 450 to waiting for the unit; a product of 16 x 8 x 16 occupies a quadrant's tensor pipe for 32 cycles,
+// that it has beside the wide kernel, mma.sync: of 1530 cycles a unit, 330 go to the first product, 200 to the softmax, 430 to
+// the second, and 460 to the wait for the unit and the turn's start; a product of 16 x 8 x 16 occupies a quadrant's tensor pipe for 32 cycles,
 // which are 1024 a unit.
 //
 // Both products are formed transposed: S^T[key][row] = K Q^T and O^T[dim][row] += V^T P^T, with keys and dims as the 16

@@ -246,11 +246,16 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_narrow_kernel(const __grid
                     uint32_t kb[2];
                     bool on[2];
                     int key0[2];  // this warp's first key of each unit
+                    const int s0 = it % kStages, s1 = s0 + 1 == kStages ? 0 : s0 + 1;
+                    const uint32_t ph0 = (it / kStages) & 1, ph1 = s1 == 0 ? ph0 ^ 1 : ph0;
+                    // both asked at once, and waited for only where one is not there
+                    const bool h0 = mbar_test(&full[s0], ph0), h1 = np < 2 || mbar_test(&full[s1], ph1);
                     bool have = true;
+                    if (!h0) have = mbar_wait(&full[s0], ph0, abortp, wait_ns);
+                    if (!h1) have = have && mbar_wait(&full[s1], ph1, abortp, wait_ns);
 #pragma unroll
                     for (int z = 0; z < 2; ++z) {
-                        const int st = (it + z) % kStages;
-                        if (z < np) have = have && mbar_wait(&full[st], ((it + z) / kStages) & 1, abortp, wait_ns);
+                        const int st = z ? s1 : s0;
                         kb[z] = smem_u32(ring + st * 2 * kTileBytes) + rows_at * 128;
                         key0[z] = (p0 + i + z) * keys + slot * 16;
                         on[z] = z < np && have && mine && (page_ok[st] >> ok_bit & 1) && key0[z] < en.len;
@@ -371,8 +376,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_narrow_kernel(const __grid
                     }
                     __syncwarp();
                     if (lane == 0) {
-                        mbar_arrive(&empty[it % kStages]);
-                        if (np == 2) mbar_arrive(&empty[(it + 1) % kStages]);
+                        mbar_arrive(&empty[s0]);
+                        if (np == 2) mbar_arrive(&empty[s1]);
                     }
                     it += np;
                 }

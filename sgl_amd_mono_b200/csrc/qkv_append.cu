@@ -9,7 +9,7 @@
 // Bound: memory.  A token's row is read once and written once (bf16 q, one byte per K and V value).  Sixteen lanes hold
 // a head, eight dims (16 bytes) each, so a warp takes two heads at a time and a norm is four shuffles.  Four pairs of heads
 // are in flight, and what a token and kind multiply by is made once for all its heads.  Measured (48 q heads on 8, B200):
-// 16384 tokens 84 us, 6022 GB/s, 92 % of a copy; 2001 tokens 16.5 us; 16 tokens of 12 heads on 2 2.3 us, a launch.
+// 16384 tokens 87 us, 5827 GB/s, 89 % of a copy; 2001 tokens 16.3 us; 16 tokens of 12 heads on 2 2.3 us, a launch.
 #include "mono_common.cuh"
 
 extern void mono_set_error(const char* fmt, ...);
@@ -223,7 +223,7 @@ static cudaError_t launch(const mono_qkv_append_args* a, cudaStream_t st) {
     // How many warps share a token: what takes least, reckoned as rounds of the warps that the GPU holds, a round as long as a
     // warp's pairs of heads and kStart more (angles and latency).  With 32 warps an SM and 48 heads on 8: 2001 tokens, two
     // warps, one round, 17 us (five warps, which fill it 2.1 times, 20.6); 3000: three warps 23 us, one 28; 6000: two 41, one 45.
-    constexpr int kStart = 4;
+    constexpr int kStart = 6;
     const long long held = (mono_sm_count() > 0 ? mono_sm_count() : 148) * ctas_per_sm(INTERLEAVED, a->src_f32 != nullptr) * (kThreads / 32);
     int chunks = 1;
     long long least = -1;

@@ -10,7 +10,7 @@
 // to 2^-44 of the largest weight (f32 sums would decide it to 2^-20 or so, which draws other tokens where many are
 // alike).  A token whose weight rounds to 0 is never drawn, so it counts in no rank either.
 //
-// Layout: a cluster of eight CTAs per row; each reads its eighth of the row once from HBM into shared memory and all
+// Layout: a cluster of eight CTAs per row (many short rows: a CTA each); each reads its eighth of the row once from HBM into shared memory and all
 // passes run on that.  The border is found in steps that all eight CTAs decide alike from merged histograms (read over
 // distributed shared memory; one cluster barrier a step):
 //   1. the largest logit;
@@ -116,6 +116,7 @@ struct Hist {
     uint32_t n[2][kBins], lo[2][kBins], hi[2][kBins];  // counts, and masses in two words; two sets, used in turn
 };
 constexpr int kRank = 256;  // tokens that are ranked one against another (0.8 us; a round of bins takes 3.5)
+constexpr int kOneCta = 20480;  // logits of which one CTA holds a row, beside another CTA on its SM
 constexpr int kList = 64;  // logits of the border's first range that a warp lists
 constexpr size_t kAfter = sizeof(Hist) + kWarps * kList * sizeof(uint16_t);  // shared memory behind the slice
 // One word atomics are native in shared memory, 64-bit ones are not: the carry is taken from the value that was there.
@@ -148,7 +149,14 @@ __device__ __forceinline__ void st_peer(uint32_t* p, int rank, uint32_t v) {
 // The eight CTAs' histograms of set `set`, added into set `set ^ 1` of all of them: each CTA adds an eighth of the bins and
 // writes it to every CTA.  (Shared memory of other CTAs is read at some 8 bytes a cycle: with every CTA reading all
 // bins of all others a level took 3 us.)  Barriers before and after.
+template <int CTAS>
 __device__ __forceinline__ void hist_merge(Hist& h, int set, int rank, cg::cluster_group& cluster) {
+    if (CTAS == 1) {
+        __syncthreads();
+        for (int i = threadIdx.x; i < kBins; i += kThreads) { h.n[set ^ 1][i] = h.n[set][i]; h.lo[set ^ 1][i] = h.lo[set][i]; h.hi[set ^ 1][i] = h.hi[set][i]; }
+        __syncthreads();
+        return;
+    }
     constexpr int kShare = kBins / kCtas;
     static_assert(2 * kShare <= kThreads, "a thread per bin and kind");
     cluster.sync();
@@ -201,18 +209,18 @@ __device__ __forceinline__ A block_before(A v, A* red) {
 }
 
 // `slice`: logits of a CTA (a multiple of 4); runs: a warp's consecutive logits (a multiple of 128)
-template <typename T>
-__global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 2) sample_kernel(const mono_sample_args a, int slice, int run, const __grid_constant__ Powers powers) {
+template <typename T, int CTAS>
+__global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(kThreads, 2) sample_kernel(const mono_sample_args a, int slice, int run, const __grid_constant__ Powers powers) {
     extern __shared__ __align__(16) float xs[];  // [slice], then the histograms and the warps' lists
     Hist& h = *reinterpret_cast<Hist*>(xs + slice);
-    __shared__ u64 s_wsum[kWarps], red64[kWarps], s_z[kCtas], s_part[kCtas], s_cut[2];
-    __shared__ uint32_t s_wties[kWarps], red32[kWarps], s_key[kCtas], s_num[kCtas], s_cnt[2];
+    __shared__ u64 s_wsum[kWarps], red64[kWarps], s_z[CTAS], s_part[CTAS], s_cut[2];
+    __shared__ uint32_t s_wties[kWarps], red32[kWarps], s_key[CTAS], s_num[CTAS], s_cnt[2];
     __shared__ float redf[2][kWarps];
     __shared__ int s_bin[2];
-    __shared__ uint32_t s_found, s_cand[kCtas], s_border;
+    __shared__ uint32_t s_found, s_cand[CTAS], s_border;
     __shared__ double s_tab[kTable * kCopies];
     cg::cluster_group cluster = cg::this_cluster();
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, row = blockIdx.x / kCtas, V = a.vocab;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, row = blockIdx.x / CTAS, V = a.vocab;
     const int rank = (int)cluster.block_rank();
     if (tid < kTable * kCopies) s_tab[tid] = powers.p[tid / kCopies];
     for (int i = tid; i < kBins; i += kThreads) { h.n[0][i] = 0; h.lo[0][i] = 0; h.hi[0][i] = 0; }
@@ -268,14 +276,14 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 2) sam
     kmax = __reduce_max_sync(0xffffffffu, kmax);
     if (lane == 0) red32[warp] = kmax;
     __syncthreads();
-    if (tid < kCtas) {
+    if (tid < CTAS) {
         for (int i = 0; i < kWarps; ++i) kmax = max(kmax, red32[i]);
         *cluster.map_shared_rank(&s_key[rank], tid) = kmax;
     }
     cluster.sync();
     MONO_TL(tl_sample, 3);
     kmax = 0;
-    for (int i = 0; i < kCtas; ++i) kmax = max(kmax, s_key[i]);
+    for (int i = 0; i < CTAS; ++i) kmax = max(kmax, s_key[i]);
     if (kmax <= kKeyNegInf) {  // no logit above -inf: all CTAs of the row leave
         if (tid == 0 && rank == 0) {
             a.tokens[row] = -1;
@@ -328,15 +336,15 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 2) sam
     }
     __syncthreads();
     MONO_TL(tl_sample, 4);
-    if (tid < kCtas) {
+    if (tid < CTAS) {
         u64 z = 0;
         for (int i = 0; i < kWarps; ++i) z += s_wsum[i];
         *cluster.map_shared_rank(&s_z[rank], tid) = z;
     }
-    if (search) hist_merge(h, 0, rank, cluster); else cluster.sync();
+    if (search) hist_merge<CTAS>(h, 0, rank, cluster); else cluster.sync();
     MONO_TL(tl_sample, 5);
     u64 Z = 0;
-    for (int i = 0; i < kCtas; ++i) Z += s_z[i];
+    for (int i = 0; i < CTAS; ++i) Z += s_z[i];
     // kept: keys above khi; of the keys klo .. khi (one key, or one token) the first `ties` of `tied`
     uint32_t khi = 0, klo = 1, tied = 0, ties = 0;
     u64 kept = Z, tie_w = 0;
@@ -475,7 +483,7 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 2) sam
                 }
                 bool summed = level > 1;
                 auto sum_above = [&]() {
-                    for (int i = 0; i < kCtas; ++i) { above += s_part[i]; n_above += s_num[i]; }
+                    for (int i = 0; i < CTAS; ++i) { above += s_part[i]; n_above += s_num[i]; }
                     summed = true;
                 };
                 auto send_above = [&]() {
@@ -496,14 +504,14 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 2) sam
                             at = __shfl_sync(0xffffffffu, at, 0) + __popc(in & ((1u << lane) - 1));
                             if (here && at < kRank) {
 #pragma unroll
-                                for (int c = 0; c < kCtas; ++c) st_peer(candidates(h, idle, rank) + at, c, key_of(v));
+                                for (int c = 0; c < CTAS; ++c) st_peer(candidates(h, idle, rank) + at, c, key_of(v));
                             }
                         }
                     } else if (lane == 0) {
                         atomicAdd(&s_found, kRank + 1);
                     }
                     __syncthreads();
-                    if (tid < kCtas) {
+                    if (tid < CTAS) {
                         *cluster.map_shared_rank(&s_cand[rank], tid) = s_found;
                         if (level == 1) send_above();
                     }
@@ -511,12 +519,12 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 2) sam
                     if (tid == 0) s_found = 0;
                     if (!summed) sum_above();
                     uint32_t total = 0;
-                    for (int c = 0; c < kCtas; ++c) total += min(s_cand[c], (uint32_t)kRank + 1);
+                    for (int c = 0; c < CTAS; ++c) total += min(s_cand[c], (uint32_t)kRank + 1);
                     if (total <= kRank) {
                         uint32_t* keys = h.hi[idle];
                         u64* ws = reinterpret_cast<u64*>(h.hi[idle] + kRank);
                         uint32_t from = 0;
-                        for (int c = 0; c < kCtas; ++c) {
+                        for (int c = 0; c < CTAS; ++c) {
                             if (tid < (int)s_cand[c]) {
                                 const uint32_t key = candidates(h, idle, c)[tid];
                                 keys[from + tid] = key;
@@ -598,8 +606,8 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 2) sam
                     for (int b = i0; b < i1; b += 32) add(b + lane < i1 ? xs[b + lane] : -INFINITY);
                 }
                 __syncthreads();
-                if (!summed && tid < kCtas) send_above();
-                hist_merge(h, set, rank, cluster);
+                if (!summed && tid < CTAS) send_above();
+                hist_merge<CTAS>(h, set, rank, cluster);
                 idle = set;
                 MONO_TL(tl_sample, 5 + 2 * level);
                 if (!summed) sum_above();
@@ -691,7 +699,7 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 2) sam
         t = __reduce_add_sync(0xffffffffu, t);
         if (lane == 0) { s_wsum[warp] = m; s_wties[warp] = t; }
         __syncthreads();
-        if (tid < kCtas) {
+        if (tid < CTAS) {
             u64 sm = 0;
             uint32_t st = 0;
             for (int i = 0; i < kWarps; ++i) { sm += s_wsum[i]; st += s_wties[i]; }
@@ -766,16 +774,16 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads, 2) sam
     MONO_TL(tl_sample, 15);
 }
 
-template <typename T>
-static cudaError_t launch(const mono_sample_args* a, cudaStream_t st) {
-    int slice = (a->vocab + kCtas - 1) / kCtas;
+template <typename T, int CTAS>
+static cudaError_t launch_with(const mono_sample_args* a, cudaStream_t st) {
+    int slice = (a->vocab + CTAS - 1) / CTAS;
     slice = (slice + 7) & ~7;  // slices start on 16-byte addresses where the row does
     int run = (slice + kWarps - 1) / kWarps;
     run = (run + 127) & ~127;
     const size_t smem = (size_t)slice * 4 + kAfter;
     static std::atomic<uint64_t> attr_once{0};  // bit d: set on device d
     if (attr_needed(attr_once)) {
-        const cudaError_t e = cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, MONO_SAMPLE_MAX_VOCAB / kCtas * 4 + (int)kAfter);
+        const cudaError_t e = cudaFuncSetAttribute(sample_kernel<T, CTAS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (CTAS == 1 ? kOneCta : MONO_SAMPLE_MAX_VOCAB / kCtas) * 4 + (int)kAfter);
         if (e != cudaSuccess) return e;
         attr_done(attr_once);
     }
@@ -784,7 +792,15 @@ static cudaError_t launch(const mono_sample_args* a, cudaStream_t st) {
         for (int i = 0; i < kTable; ++i) w.p[i] = std::exp2(44.0 + i / (double)kTable);
         return w;
     }();
-    return launch_k(sample_kernel<T>, a->rows * kCtas, kThreads, smem, st, *a, slice, run, powers);
+    return launch_k(sample_kernel<T, CTAS>, a->rows * CTAS, kThreads, smem, st, *a, slice, run, powers);
+}
+// More rows than clusters run at once (two CTAs an SM), of a vocabulary that one CTA holds: a CTA per row, without the
+// cluster's barriers and merges (256 rows with all filters: of 1000 logits 14 us, by clusters 107; of 20000 41 and 120; 38
+// rows of 20000 25.5 and 24.6).
+template <typename T>
+static cudaError_t launch(const mono_sample_args* a, cudaStream_t st) {
+    const int sms = mono_sm_count() > 0 ? mono_sm_count() : 148;
+    return a->vocab <= kOneCta && a->rows * kCtas > 2 * sms ? launch_with<T, 1>(a, st) : launch_with<T, kCtas>(a, st);
 }
 
 }  // namespace sampling

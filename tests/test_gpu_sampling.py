@@ -228,3 +228,18 @@ def test_rank_zero_alone_is_the_first_of_the_largest():
     one = torch.ones(4, dtype=torch.int32)
     token = _check(x, torch.tensor([0.0, 0.5, 0.999, 0.3]), torch.tensor([1.0, 0.3, 5.0, 0.0]), one, torch.tensor([1.0, 0.0, 0.5, 1.0]), torch.tensor([0.0, 1.0, 0.2, 0.0]))
     assert (token == 77).all()
+
+
+@pytest.mark.parametrize("vocab", [7, 1000, 4099, 20480, 20481])
+@pytest.mark.parametrize("rounded", [False, True])
+def test_many_rows_of_small_vocabularies(vocab, rounded):
+    rows = 60
+    x, u = _logits(rows, vocab, vocab, rounded), _u(rows, vocab)
+    g = torch.Generator().manual_seed(5)
+    k = torch.randint(0, min(vocab, 300) + 1, (rows,), generator=g).to(torch.int32)
+    p = torch.where(torch.arange(rows) % 3 == 0, torch.ones(rows), torch.rand(rows, generator=g) * 0.98 + 0.01)
+    mp = torch.where(torch.arange(rows) % 4 == 0, torch.rand(rows, generator=g) * 0.2, torch.zeros(rows))
+    t = torch.where(torch.arange(rows) % 7 == 6, torch.zeros(rows), torch.rand(rows, generator=g) + 0.4)
+    x[1], x[2, : vocab // 2] = -float("inf"), float("nan")
+    _check(x, u)
+    _check(x.bfloat16() if rounded else x, u, t, k, p, mp)

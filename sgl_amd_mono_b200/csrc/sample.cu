@@ -10,7 +10,7 @@
 // to 2^-44 of the largest weight (f32 sums would decide it to 2^-20 or so, which draws other tokens where many are
 // alike).  A token whose weight rounds to 0 is never drawn, so it counts in no rank either.
 //
-// Layout: a cluster of eight CTAs per row (many short rows: a CTA each); each reads its eighth of the row once from HBM into shared memory and all
+// Layout: a cluster of eight CTAs per row (short rows: a CTA each); each reads its eighth of the row once from HBM into shared memory and all
 // passes run on that.  The border is found in steps that all eight CTAs decide alike from merged histograms (read over
 // distributed shared memory; one cluster barrier a step):
 //   1. the largest logit;
@@ -794,13 +794,15 @@ static cudaError_t launch_with(const mono_sample_args* a, cudaStream_t st) {
     }();
     return launch_k(sample_kernel<T, CTAS>, a->rows * CTAS, kThreads, smem, st, *a, slice, run, powers);
 }
-// More rows than clusters run at once (two CTAs an SM), of a vocabulary that one CTA holds: a CTA per row, without the
-// cluster's barriers and merges (256 rows with all filters: of 1000 logits 14 us, by clusters 107; of 20000 41 and 120; 38
-// rows of 20000 25.5 and 24.6).
+// A CTA per row, without the cluster's barriers and merges: where it holds the row and either the row is short, or there are
+// more rows than clusters run at once (two CTAs an SM; half of that for rows of up to 8192).  Measured with filters, us by
+// CTAs and by clusters: 1 row of 4000 logits 11.6 and 12.8, of 8000 14.8 and 13.2; 24 rows of 8000 16.7 and 18.1, of 16000
+// 24.4 and 19.1; 37 of 16000 24.3 and 24.3; 256 rows of 1000 14 and 107, of 20000 41 and 120.
 template <typename T>
 static cudaError_t launch(const mono_sample_args* a, cudaStream_t st) {
-    const int sms = mono_sm_count() > 0 ? mono_sm_count() : 148;
-    return a->vocab <= kOneCta && a->rows * kCtas > 2 * sms ? launch_with<T, 1>(a, st) : launch_with<T, kCtas>(a, st);
+    const int sms = mono_sm_count() > 0 ? mono_sm_count() : 148, ctas = a->rows * kCtas;
+    const bool one = a->vocab <= 4096 || ctas > (a->vocab <= 8192 ? sms : 2 * sms);
+    return one && a->vocab <= kOneCta ? launch_with<T, 1>(a, st) : launch_with<T, kCtas>(a, st);
 }
 
 }  // namespace sampling

@@ -10,7 +10,7 @@
 // to 2^-44 of the largest weight (f32 sums would decide it to 2^-20 or so, which draws other tokens where many are
 // alike).  A token whose weight rounds to 0 is never drawn, so it counts in no rank either.
 //
-// Layout: a cluster of eight CTAs per row (short rows: a CTA each); each reads its eighth of the row once from HBM into shared memory and all
+// Layout: a cluster of eight CTAs per row (short or many rows: fewer); each reads its share of the row once from HBM into shared memory and all
 // passes run on that.  The border is found in steps that all eight CTAs decide alike from merged histograms (read over
 // distributed shared memory; one cluster barrier a step):
 //   1. the largest logit;
@@ -38,7 +38,7 @@ namespace sampling {
 using namespace mono;
 namespace cg = cooperative_groups;
 
-constexpr int kCtas = 8;  // of a row: the portable cluster size; a slice of the largest vocabulary fits shared memory
+constexpr int kCtas = 8;  // of a row, at most: the portable cluster size; a slice of the largest vocabulary fits shared memory
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBins = 1024;
@@ -116,7 +116,7 @@ struct Hist {
     uint32_t n[2][kBins], lo[2][kBins], hi[2][kBins];  // counts, and masses in two words; two sets, used in turn
 };
 constexpr int kRank = 256;  // tokens that are ranked one against another (0.8 us; a round of bins takes 3.5)
-constexpr int kOneCta = 20480;  // logits of which one CTA holds a row, beside another CTA on its SM
+constexpr int kSlice = 20480;  // logits that a CTA holds beside another CTA on its SM
 constexpr int kList = 64;  // logits of the border's first range that a warp lists
 constexpr size_t kAfter = sizeof(Hist) + kWarps * kList * sizeof(uint16_t);  // shared memory behind the slice
 // One word atomics are native in shared memory, 64-bit ones are not: the carry is taken from the value that was there.
@@ -146,7 +146,7 @@ __device__ __forceinline__ uint32_t ld_peer(const uint32_t* p, int rank) {
 __device__ __forceinline__ void st_peer(uint32_t* p, int rank, uint32_t v) {
     asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(peer_address(p, rank)), "r"(v) : "memory");
 }
-// The eight CTAs' histograms of set `set`, added into set `set ^ 1` of all of them: each CTA adds an eighth of the bins and
+// The CTAs' histograms of set `set`, added into set `set ^ 1` of all of them: each CTA adds its share of the bins and
 // writes it to every CTA.  (Shared memory of other CTAs is read at some 8 bytes a cycle: with every CTA reading all
 // bins of all others a level took 3 us.)  Barriers before and after.
 template <int CTAS>
@@ -157,27 +157,28 @@ __device__ __forceinline__ void hist_merge(Hist& h, int set, int rank, cg::clust
         __syncthreads();
         return;
     }
-    constexpr int kShare = kBins / kCtas;
-    static_assert(2 * kShare <= kThreads, "a thread per bin and kind");
+    constexpr int kShare = kBins / CTAS;
     cluster.sync();
-    const int b = rank * kShare + (threadIdx.x & (kShare - 1)), what = threadIdx.x / kShare;
-    if (what == 0) {
-        uint32_t v[kCtas], n = 0;
+    for (int x = threadIdx.x; x < 2 * kShare; x += kThreads) {
+        const int b = rank * kShare + (x & (kShare - 1));
+        if (x < kShare) {
+            uint32_t v[CTAS], n = 0;
 #pragma unroll
-        for (int c = 0; c < kCtas; ++c) v[c] = ld_peer(&h.n[set][b], c);
+            for (int c = 0; c < CTAS; ++c) v[c] = ld_peer(&h.n[set][b], c);
 #pragma unroll
-        for (int c = 0; c < kCtas; ++c) n += v[c];
+            for (int c = 0; c < CTAS; ++c) n += v[c];
 #pragma unroll
-        for (int c = 0; c < kCtas; ++c) st_peer(&h.n[set ^ 1][b], c, n);
-    } else if (what == 1) {
-        uint32_t lo[kCtas], hi[kCtas];
-        u64 m = 0;
+            for (int c = 0; c < CTAS; ++c) st_peer(&h.n[set ^ 1][b], c, n);
+        } else {
+            uint32_t lo[CTAS], hi[CTAS];
+            u64 m = 0;
 #pragma unroll
-        for (int c = 0; c < kCtas; ++c) { lo[c] = ld_peer(&h.lo[set][b], c); hi[c] = ld_peer(&h.hi[set][b], c); }
+            for (int c = 0; c < CTAS; ++c) { lo[c] = ld_peer(&h.lo[set][b], c); hi[c] = ld_peer(&h.hi[set][b], c); }
 #pragma unroll
-        for (int c = 0; c < kCtas; ++c) m += ((u64)hi[c] << 32) + lo[c];
+            for (int c = 0; c < CTAS; ++c) m += ((u64)hi[c] << 32) + lo[c];
 #pragma unroll
-        for (int c = 0; c < kCtas; ++c) { st_peer(&h.lo[set ^ 1][b], c, (uint32_t)m); st_peer(&h.hi[set ^ 1][b], c, (uint32_t)(m >> 32)); }
+            for (int c = 0; c < CTAS; ++c) { st_peer(&h.lo[set ^ 1][b], c, (uint32_t)m); st_peer(&h.hi[set ^ 1][b], c, (uint32_t)(m >> 32)); }
+        }
     }
     cluster.sync();
 }
@@ -783,7 +784,7 @@ static cudaError_t launch_with(const mono_sample_args* a, cudaStream_t st) {
     const size_t smem = (size_t)slice * 4 + kAfter;
     static std::atomic<uint64_t> attr_once{0};  // bit d: set on device d
     if (attr_needed(attr_once)) {
-        const cudaError_t e = cudaFuncSetAttribute(sample_kernel<T, CTAS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (CTAS == 1 ? kOneCta : MONO_SAMPLE_MAX_VOCAB / kCtas) * 4 + (int)kAfter);
+        const cudaError_t e = cudaFuncSetAttribute(sample_kernel<T, CTAS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (CTAS < kCtas ? kSlice : MONO_SAMPLE_MAX_VOCAB / kCtas) * 4 + (int)kAfter);
         if (e != cudaSuccess) return e;
         attr_done(attr_once);
     }
@@ -794,15 +795,18 @@ static cudaError_t launch_with(const mono_sample_args* a, cudaStream_t st) {
     }();
     return launch_k(sample_kernel<T, CTAS>, a->rows * CTAS, kThreads, smem, st, *a, slice, run, powers);
 }
-// A CTA per row, without the cluster's barriers and merges: where it holds the row and either the row is short, or there are
-// more rows than clusters run at once (two CTAs an SM; half of that for rows of up to 8192).  Measured with filters, us by
-// CTAs and by clusters: 1 row of 4000 logits 11.6 and 12.8, of 8000 14.8 and 13.2; 24 rows of 8000 16.7 and 18.1, of 16000
-// 24.4 and 19.1; 37 of 16000 24.3 and 24.3; 256 rows of 1000 14 and 107, of 20000 41 and 120.
+// CTAs of a row.  One where it holds a short row: no barriers between CTAs, and nothing to merge.  Fewer than eight where there
+// are more rows than clusters run at once (two CTAs an SM) and a smaller cluster holds the row.  Measured with filters, us by
+// CTAs and by clusters of eight: 1 row of 4000 logits 11.6 and 12.8, of 8000 14.8 and 13.2; 24 rows of 8000 16.7 and 18.1, of
+// 16000 24.4 and 19.1; 256 rows of 1000 14 and 107, of 20000 41 and 120; by two CTAs 256 rows of 40000 75 and 153, by four 256
+// rows of 80000 129 and 188.
 template <typename T>
 static cudaError_t launch(const mono_sample_args* a, cudaStream_t st) {
-    const int sms = mono_sm_count() > 0 ? mono_sm_count() : 148, ctas = a->rows * kCtas;
-    const bool one = a->vocab <= 4096 || ctas > (a->vocab <= 8192 ? sms : 2 * sms);
-    return one && a->vocab <= kOneCta ? launch_with<T, 1>(a, st) : launch_with<T, kCtas>(a, st);
+    const int sms = mono_sm_count() > 0 ? mono_sm_count() : 148;
+    if (a->vocab <= 4096 || (a->vocab <= 8192 && a->rows * kCtas > sms)) return launch_with<T, 1>(a, st);
+    int ctas = kCtas;
+    while (ctas > 1 && a->rows * ctas > 2 * sms && a->vocab <= kSlice * (ctas / 2)) ctas /= 2;
+    return ctas == 1 ? launch_with<T, 1>(a, st) : ctas == 2 ? launch_with<T, 2>(a, st) : ctas == 4 ? launch_with<T, 4>(a, st) : launch_with<T, kCtas>(a, st);
 }
 
 }  // namespace sampling

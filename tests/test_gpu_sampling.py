@@ -230,10 +230,9 @@ def test_rank_zero_alone_is_the_first_of_the_largest():
     assert (token == 77).all()
 
 
-@pytest.mark.parametrize("vocab", [7, 1000, 4099, 20480, 20481])
+@pytest.mark.parametrize("rows,vocab", [(60, 7), (60, 1000), (60, 4099), (60, 20480), (60, 20481), (90, 8193), (90, 40960), (150, 9000), (40, 81920), (40, 81921)])
 @pytest.mark.parametrize("rounded", [False, True])
-def test_many_rows_of_small_vocabularies(vocab, rounded):
-    rows = 60
+def test_many_rows_of_small_vocabularies(rows, vocab, rounded):
     x, u = _logits(rows, vocab, vocab, rounded), _u(rows, vocab)
     g = torch.Generator().manual_seed(5)
     k = torch.randint(0, min(vocab, 300) + 1, (rows,), generator=g).to(torch.int32)

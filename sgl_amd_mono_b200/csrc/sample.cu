@@ -214,7 +214,7 @@ template <typename T, int CTAS>
 __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(kThreads, 2) sample_kernel(const mono_sample_args a, int slice, int run, const __grid_constant__ Powers powers) {
     extern __shared__ __align__(16) float xs[];  // [slice], then the histograms and the warps' lists
     Hist& h = *reinterpret_cast<Hist*>(xs + slice);
-    __shared__ u64 s_wsum[kWarps], red64[kWarps], s_z[CTAS], s_part[CTAS], s_cut[2];
+    __shared__ u64 s_wsum[kWarps], red64[kWarps], s_z[CTAS], s_kept[CTAS], s_part[CTAS], s_cut[2];
     __shared__ uint32_t s_wties[kWarps], red32[kWarps], s_key[CTAS], s_num[CTAS], s_cnt[2];
     __shared__ float redf[2][kWarps];
     __shared__ int s_bin[2];
@@ -704,7 +704,8 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(kThreads, 2) samp
             u64 sm = 0;
             uint32_t st = 0;
             for (int i = 0; i < kWarps; ++i) { sm += s_wsum[i]; st += s_wties[i]; }
-            *cluster.map_shared_rank(&s_z[rank], tid) = sm;  // Z has been taken
+            // (not into s_z: without a search no barrier lies behind the other CTAs' reading of Z)
+            *cluster.map_shared_rank(&s_kept[rank], tid) = sm;
             *cluster.map_shared_rank(&s_key[rank], tid) = st;
         }
         cluster.sync();
@@ -714,8 +715,9 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(kThreads, 2) samp
     u64 before = 0;
     uint32_t t_before = 0;
     auto kept_of = [&](uint32_t from, uint32_t n) { return some && from < ties ? (u64)min(n, ties - from) * tie_w : 0ull; };
+    const u64* sums = all ? s_z : s_kept;
     for (int c = 0; c < rank; ++c) {
-        before += s_z[c];
+        before += sums[c];
         if (some) { before += kept_of(t_before, s_key[c]); t_before += s_key[c]; }
     }
     for (int w = 0; w < warp; ++w) {

@@ -242,3 +242,18 @@ def test_many_rows_of_small_vocabularies(rows, vocab, rounded):
     x[1], x[2, : vocab // 2] = -float("inf"), float("nan")
     _check(x, u)
     _check(x.bfloat16() if rounded else x, u, t, k, p, mp)
+
+
+@pytest.mark.parametrize("rows,vocab", [(4, 129280), (90, 40000), (150, 40000), (40, 20000), (24, 9000)])
+def test_rows_of_rank_zero_alone_repeat_their_log_probability(rows, vocab):
+    """Greedy rows and rows with top_k = 1 need no search of a border: what their CTAs exchange must not meet."""
+    x, u = _logits(rows, vocab, vocab + rows), _u(rows, 3)
+    temperature = torch.where(torch.arange(rows) % 2 == 0, torch.zeros(rows), torch.full((rows,), 1.7))
+    k = torch.where(torch.arange(rows) % 2 == 0, torch.zeros(rows), torch.ones(rows)).to(torch.int32)
+    op = SampleOp(vocab, DEV, max_rows=rows)
+    args = [t.to(DEV) for t in (x, u, temperature, k)]
+    token, logprob = (t.clone() for t in op(*args))
+    _check(x, u, temperature, k, out=(token, logprob))
+    for _ in range(30):
+        again = op(*args)
+        assert torch.equal(again[0], token) and torch.equal(again[1], logprob)

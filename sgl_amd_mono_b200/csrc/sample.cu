@@ -223,6 +223,9 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(kThreads, 2) samp
     cg::cluster_group cluster = cg::this_cluster();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, row = blockIdx.x / CTAS, V = a.vocab;
     const int rank = (int)cluster.block_rank();
+    // The row's CTAs write into one another's shared memory once all of them are known to run: the wait for that comes
+    // after the load.
+    if (CTAS > 1) cluster.barrier_arrive();
     if (tid < kTable * kCopies) s_tab[tid] = powers.p[tid / kCopies];
     for (int i = tid; i < kBins; i += kThreads) { h.n[0][i] = 0; h.lo[0][i] = 0; h.hi[0][i] = 0; }
     if (tid == 0) { s_bin[0] = kBins; s_bin[1] = kBins; s_found = 0; s_border = 0; }
@@ -277,6 +280,7 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(kThreads, 2) samp
     kmax = __reduce_max_sync(0xffffffffu, kmax);
     if (lane == 0) red32[warp] = kmax;
     __syncthreads();
+    if (CTAS > 1) cluster.barrier_wait();
     if (tid < CTAS) {
         for (int i = 0; i < kWarps; ++i) kmax = max(kmax, red32[i]);
         *cluster.map_shared_rank(&s_key[rank], tid) = kmax;

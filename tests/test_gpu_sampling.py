@@ -257,3 +257,15 @@ def test_rows_of_rank_zero_alone_repeat_their_log_probability(rows, vocab):
     for _ in range(30):
         again = op(*args)
         assert torch.equal(again[0], token) and torch.equal(again[1], logprob)
+
+
+@pytest.mark.parametrize("rows,vocab", [(1, 8193), (18, 4097), (2, 40001)])
+def test_short_loads_of_whole_clusters(rows, vocab):
+    """Clusters of eight whose CTAs have next to nothing to load, one launch right after another."""
+    op = SampleOp(vocab, DEV, max_rows=rows)
+    x, u = _logits(rows, vocab, vocab), _u(rows, 5)
+    p = torch.full((rows,), 0.8)
+    args = [t.to(DEV) for t in (x, u)]
+    outs = [tuple(t.clone() for t in op(*args, top_p=p.to(DEV))) for _ in range(20)]
+    _check(x, u, top_p=p, out=outs[0])
+    assert all(torch.equal(t, outs[0][0]) and torch.equal(lp, outs[0][1]) for t, lp in outs)

@@ -2,6 +2,7 @@
 the restatement they are compared with against a second form of each definition."""
 
 import ctypes as C
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -118,3 +119,13 @@ def test_restated_draw_follows_its_definition():
     assert OP.sample_row(x, 0.0, min_p=0.2)[0] == 1 and OP.sample_row(x, 0.4, min_p=0.2)[0] == 1 and OP.sample_row(x, 0.999, min_p=0.5)[0] == 3
     assert OP.sample_row(x, 0.7, temperature=0.0)[0] == 1
     assert OP.sample_row(np.full(3, -np.inf), 0.5)[0] == -1
+
+
+def test_draw_waits_for_its_cluster_before_it_writes_to_peers():
+    """Another CTA's shared memory may be touched only once that CTA is known to run, so the kernel's first use of it lies
+    behind a wait for the whole cluster."""
+    src = (Path(L.__file__).parent / "csrc" / "sample.cu").read_text()
+    body = src[src.index("sample_kernel(") : src.index("static cudaError_t launch_with")]
+    first = min(body.index(use) for use in ("map_shared_rank(", "st_peer(", "ld_peer(", "hist_merge<"))
+    waits = [body.find(w) for w in ("cluster.barrier_wait()", "cluster.sync()")]
+    assert any(0 <= at < first for at in waits)

@@ -126,6 +126,6 @@ def test_draw_waits_for_its_cluster_before_it_writes_to_peers():
     behind a wait for the whole cluster."""
     src = (Path(L.__file__).parent / "csrc" / "sample.cu").read_text()
     body = src[src.index("sample_kernel(") : src.index("static cudaError_t launch_with")]
-    first = min(body.index(use) for use in ("map_shared_rank(", "st_peer(", "ld_peer(", "hist_merge<"))
+    first = min(body.index(use) for use in ("map_shared_rank(", "st_peer(", "hist_merge<"))
     waits = [body.find(w) for w in ("cluster.barrier_wait()", "cluster.sync()")]
     assert any(0 <= at < first for at in waits)

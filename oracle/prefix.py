@@ -110,7 +110,7 @@ def sample_row(x: np.ndarray, u: float, temperature: float = 1.0, top_k: int = 0
         if top_p < 1:
             front &= ahead < max(top_p, 0.0) * z
         if min_p > 0:
-            front &= w[order] >= min(min_p, 1.0)
+            front &= w[order] >= min_p
         front[0] = True
         kept = np.sort(order[front])
         c = np.cumsum(w[kept])

@@ -309,9 +309,9 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(kThreads, 2) samp
     r.c64 = greedy ? 1.4426950408889634 : 1.4426950408889634 / fmin(fmax((double)temp, 7.888609052210118e-31), 1.2676506002282294e30);
     r.c = (float)r.c64;
     r.mx64 = (double)r.mx;
-    r.k = greedy ? 1ull : tk < 1 || tk > V ? (u64)V : (u64)tk;
+    r.k = greedy || mp > 1.f ? 1ull : tk < 1 || tk > V ? (u64)V : (u64)tk;
     const double p = !greedy && tp < 1.f ? fmax((double)tp, 0.0) : 1.0;
-    r.floor_w = !greedy && mp > 0.f ? (u64)ceil((double)fminf(mp, 1.f) * kOne) : 0ull;
+    r.floor_w = !greedy && mp > 0.f ? (u64)ceil((double)fminf(mp, 1.f) * kOne) : 0ull;  // (above 1: no weight passes, and the first stays)
     const bool filtered = r.k < (u64)V || p < 1.0 || r.floor_w;
     const bool search = filtered && r.k != 1;  // with rank 0 alone the border is the largest logit
     // ---- Z, and the histogram of counts over steps of log2 w

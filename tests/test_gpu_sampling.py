@@ -269,3 +269,14 @@ def test_short_loads_of_whole_clusters(rows, vocab):
     outs = [tuple(t.clone() for t in op(*args, top_p=p.to(DEV))) for _ in range(20)]
     _check(x, u, top_p=p, out=outs[0])
     assert all(torch.equal(t, outs[0][0]) and torch.equal(lp, outs[0][1]) for t, lp in outs)
+
+
+@pytest.mark.parametrize("vocab", [4, 3000, 50001])
+def test_min_p_above_one_keeps_the_first_of_the_largest_alone(vocab):
+    x = torch.zeros(6, vocab)
+    x[:, 1:vocab:2] = 2.0
+    mp = torch.tensor([1.0, float(np.nextafter(np.float32(1), np.float32(2))), 1.5, float("inf"), 3.0, 1.5])
+    u = torch.tensor([0.9, 0.9, 0.9, 0.9, 0.0, 0.999])
+    token = _check(x, u, min_p=mp)
+    assert int(token[0]) > 1 and token[1:].tolist() == [1] * 5
+    _check(x, u, torch.full((6,), 0.3), torch.full((6,), 3, dtype=torch.int32), torch.full((6,), 0.9), mp)

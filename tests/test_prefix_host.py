@@ -2,6 +2,7 @@
 the restatement they are compared with against a second form of each definition."""
 
 import ctypes as C
+import math
 from pathlib import Path
 
 import numpy as np
@@ -129,3 +130,10 @@ def test_draw_waits_for_its_cluster_before_it_writes_to_peers():
     first = min(body.index(use) for use in ("map_shared_rank(", "st_peer(", "hist_merge<"))
     waits = [body.find(w) for w in ("cluster.barrier_wait()", "cluster.sync()")]
     assert any(0 <= at < first for at in waits)
+
+
+def test_restated_draw_keeps_the_first_alone_where_no_weight_passes():
+    x = np.array([0.0, 2.0, 1.0, 2.0], dtype=np.float32)
+    assert OP.sample_row(x, 0.9, min_p=1.0)[0] == 3
+    for min_p in (float(np.nextafter(np.float32(1), np.float32(2))), 1.5, math.inf):
+        assert OP.sample_row(x, 0.9, min_p=min_p)[0] == 1

@@ -663,7 +663,8 @@ int mono_qkv_append_launch(const mono_qkv_append_args* a, void* stream);
  * included) in pages page_table[b][..]; group g's sequences group_start[g] .. group_start[g + 1] - 1 share the first
  * prefix_lens[g] keys in pages prefix_table[g][..].  Token j of a sequence's n sees its group's prefix and the
  * sequence's keys 0 .. lens[b] - n + j.  out = softmax((q . k) k_scale sm_scale) v v_scale; a token that sees no key
- * gives zeros, tokens of no sequence keep their output row.  A page number outside the cache counts as a page without
+ * gives zeros, tokens of no sequence keep their output row.  Where many rows share their keys a query's values are exact
+ * within 2^13 of the row's largest, and held to 2^-21 of the largest below that; weights are f16 in their product with v.  A page number outside the cache counts as a page without
  * keys.  Lengths beyond their table's columns are cut.  Both starts must never fall and stay in range: otherwise the
  * guard's argument word is set and the output is not valid.  The tables are device data: a captured launch follows them. */
 typedef struct mono_prefix_attn_args {

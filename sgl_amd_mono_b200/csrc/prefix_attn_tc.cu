@@ -1,10 +1,10 @@
 // Shared-prefix attention for many rows on 5th-generation tensor cores (prefix_attn.cuh: how the work is cut).
 //
 // A block is one page (64 keys) of one kv head for up to 256 rows, which two streams of 128 rows (the TMEM lanes) work on:
-//   S[row][key] = sum_d Q[row][d] K[key][d]   kind::f8f6f4, M 128, N 64, K 128, twice: the bf16 queries as two E4M3 planes
+//   S[row][key] = sum_d Q[row][d] K[key][d]   kind::f8f6f4, M 128, N 64, K 128, twice: the bf16 queries as two planes
 //   O[row][dim] += sum_k P[row][k] V[k][dim]  kind::f16, M 128, N 128, K 64, P in tensor memory
-// K is used as the bytes that lie in the cache: a query row, scaled by a power of two, is split into hi + lo E4M3 values,
-// exactly for values within 2^12 of the row's largest.  P is f16 (11 bits, and with the bias below weights down to 2^-31 of
+// K is used as the bytes that lie in the cache: a query row, scaled by a power of two, is split into hi (E5M2) + lo (E4M3),
+// exactly for values within 2^13 of the row's largest, and to 2^-21 of the largest below that.  P is f16 (11 bits, and with the bias below weights down to 2^-31 of
 // the largest: two E4M3 planes would drop weights below 2^-18, which a long tail of small weights adds up), so four
 // warps widen V to f16 in shared memory, which is exact.  Each stream has a warpgroup of softmax threads, one row each.
 // The softmax takes a block's scores to registers at once, so the next block's are made while it works; P has two buffers,
@@ -108,7 +108,8 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t r[16]) 
 __device__ __forceinline__ uint64_t desc_sw128(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
     return (uint64_t)((saddr & 0x3FFFF) >> 4) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(sbo >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
-constexpr uint32_t kIdescS = (1u << 4) | ((64u >> 3) << 17) | ((128u >> 4) << 24);               // E4M3 x E4M3 -> f32, both K-major
+constexpr uint32_t kIdescLo = (1u << 4) | ((64u >> 3) << 17) | ((128u >> 4) << 24);              // E4M3 x E4M3 -> f32, both K-major
+constexpr uint32_t kIdescHi = kIdescLo | (1u << 7);                                               // E5M2 x E4M3
 constexpr uint32_t kIdescO = (1u << 4) | (1u << 16) | ((128u >> 3) << 17) | ((128u >> 4) << 24);  // f16 x f16 -> f32, B MN-major
 
 __device__ __forceinline__ float ex2(float x) {
@@ -131,10 +132,13 @@ __device__ __forceinline__ uint32_t widen2(uint32_t lo16) {
 }
 
 // ------------------------------------------------------------------ queries
-// Every query row as two planes of E4M3, scaled by the power of two that brings its largest value into [128, 256) (E4M3
-// ends at 448), and what undoes the scale.  Image: [plane][kv head][token][head of the kv head][128 bytes].  Half a warp
-// per row.  (The rows are wanted by every CTA that has a part of their prefix: made by each of them, on its own rows, at
-// its start, they cost 4 to 7 us of it.)
+// Every query row as two planes of bytes, scaled by the power of two that brings its largest value into [2^11, 2^12), and
+// what undoes the scale.  hi is the value's first three bits (E5M2, down to 2^-16); the rest has at most four more bits, is at
+// most 2^8 (E4M3 ends at 448) and ends at 2^-9 in E4M3: values of 2^-2 and more are exact, smaller ones off by 2^-10 at most.
+// (hi in E4M3 takes a largest value of 2^7 and is exact for 2^9 below it: scores of a row with one value of 1024 among
+// values of 1 were off by 0.026.)  Image: [plane][kv head][token][head of the kv head][128 bytes].  Half a warp per row.
+// (The rows are wanted by every CTA that has a part of their prefix: made by each of them, on its own rows, at its start, they
+// cost 4 to 7 us of it.)
 __global__ void __launch_bounds__(256) prefix_split_kernel(const mono_prefix_attn_args a, uint8_t* image, float* back_scale, uint32_t* share, int ctas) {
     pdl_prologue();
     if (blockIdx.x == 0) {
@@ -153,13 +157,13 @@ __global__ void __launch_bounds__(256) prefix_split_kernel(const mono_prefix_att
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
     const int ex = clamp_int((int)(top >> 23), 30, 254);
-    const float up = __uint_as_float((uint32_t)(261 - ex) << 23);  // 2^(134 - ex)
+    const float up = __uint_as_float((uint32_t)(265 - ex) << 23);  // 2^(11 - (ex - 127))
     uint32_t hi[2] = {0, 0}, lo[2] = {0, 0};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const float f0 = __uint_as_float(w[i] << 16) * up, f1 = __uint_as_float(w[i] & 0xFFFF0000u) * up;
-        const __nv_fp8x2_storage_t hb = __nv_cvt_float2_to_fp8x2(make_float2(f0, f1), __NV_SATFINITE, __NV_E4M3);
-        const __half2_raw hr = __nv_cvt_fp8x2_to_halfraw2(hb, __NV_E4M3);
+        const __nv_fp8x2_storage_t hb = __nv_cvt_float2_to_fp8x2(make_float2(f0, f1), __NV_SATFINITE, __NV_E5M2);
+        const __half2_raw hr = __nv_cvt_fp8x2_to_halfraw2(hb, __NV_E5M2);
         const float2 hf = __half22float2(*reinterpret_cast<const __half2*>(&hr));
         const __nv_fp8x2_storage_t lb = __nv_cvt_float2_to_fp8x2(make_float2(f0 - hf.x, f1 - hf.y), __NV_SATFINITE, __NV_E4M3);
         hi[i >> 1] |= (uint32_t)hb << (16 * (i & 1));
@@ -169,7 +173,7 @@ __global__ void __launch_bounds__(256) prefix_split_kernel(const mono_prefix_att
     *reinterpret_cast<uint2*>(image + (size_t)r * 128 + sub * 8) = make_uint2(hi[0], hi[1]);
     *reinterpret_cast<uint2*>(image + ((size_t)rows + r) * 128 + sub * 8) = make_uint2(lo[0], lo[1]);
     // infinite or NaN: saturation would hide it; a row of NaN
-    if (sub == 0) back_scale[r] = top == 0x7F800000u ? __uint_as_float(0x7FC00000u) : __uint_as_float((uint32_t)(ex - 7) << 23);
+    if (sub == 0) back_scale[r] = top == 0x7F800000u ? __uint_as_float(0x7FC00000u) : __uint_as_float((uint32_t)(ex - 11) << 23);
 }
 
 // ------------------------------------------------------------------ attention
@@ -356,7 +360,7 @@ __global__ void __launch_bounds__(kThreadsWide, 1) prefix_wide_kernel(const __gr
                         const uint64_t kd = desc_sw128(smem_u32(kbuf + ks * kKTile), 0, 1024);
                         if (elect_one()) {
 #pragma unroll
-                            for (int s = 0; s < 8; ++s) mma_f8(s_at, qd + (s >> 2) * (kQPlane / 16) + 2 * (s & 3), kd + 2 * (s & 3), kIdescS, s > 0);
+                            for (int s = 0; s < 8; ++s) mma_f8(s_at, qd + (s >> 2) * (kQPlane / 16) + 2 * (s & 3), kd + 2 * (s & 3), s < 4 ? kIdescHi : kIdescLo, s > 0);
                             mma_commit(&s_full[st]);
                             mma_commit(&k_empty[ks]);  // two arrivals free a stage: one per stream, or both from the only stream that uses it
                             if (x.split) mma_commit(&k_empty[ks]);

@@ -597,3 +597,32 @@ def test_attend_one_launch_after_another_without_overlap():
             assert torch.equal(op(q.to(DEV), *dc, _dev(t)), w)
     finally:
         L.load().mono_set_pdl(1)
+
+
+@pytest.mark.parametrize("spread", [9, 13, 20])
+@pytest.mark.parametrize("hq,hk,ntok,own,starts,prefix", [
+    (12, 2, [1] * 60, [30] * 60, [0, 60], [500]),     # one prefix of 360 rows
+    (6, 1, [100, 40], [100, 300], [], []),            # tiles of both sizes on their own keys
+    (12, 2, [1] * 4, [70] * 4, [0, 2, 4], [90, 64])])  # few rows
+def test_attend_queries_with_one_large_dim(hq, hk, ntok, own, starts, prefix, spread):
+    """A query dim up to 2^spread times the others, at a dim where the keys are zero, changes no score."""
+    t, pages = _tables(ntok, own, starts, prefix)
+    caches = _caches(pages, hk)
+    caches[0][..., 17] = 0
+    tokens = sum(ntok)
+    g = _gen(31)
+    sign = lambda *s: torch.randint(0, 2, s, generator=g) * 2.0 - 1.0  # noqa: E731
+    q = (sign(tokens, hq, 128) * (0.5 + 1.5 * torch.rand(tokens, hq, 128, generator=g))).bfloat16()  # 0.5 .. 2
+    q[..., 17] = (sign(tokens, hq) * 2.0 ** torch.randint(spread - 4, spread, (tokens, hq), generator=g)).bfloat16()
+    op = SharedPrefixAttnOp(hq, hk, DEV, max_tokens=tokens, max_seqs=len(own), max_groups=max(1, len(prefix)), k_scale=K_SCALE, v_scale=V_SCALE)
+    out = op(q.to(DEV), *(c.to(DEV) for c in caches), _dev(t))
+    if spread <= 13:
+        _check_attend(out, q, caches, t, op)
+        return
+    # beyond 2^13 a query value is held to 2^-21 of the row's largest: scores are off by that times the sum of a key's values,
+    # which enters numerator and denominator
+    ref, mag, big, seen = OP.attend(q, *caches, t.q_start, t.page_table, t.lens, t.group_start, t.prefix_table, t.prefix_lens, op.k_scale, op.v_scale, op.sm_scale)
+    most = float(OP.cache_values(caches[0]).abs().sum(-1).max()) * op.k_scale * op.sm_scale
+    score = 2.0**-21 * q.double().abs().amax(-1) * most + 128 * 2.0**-23 * big
+    tol = ref.abs() * 2.0**-8 + mag * (2.0**-11 + torch.expm1(2 * score)[..., None] + 2.0**-19 + (seen[:, None, None] / 16 + 16) * 2.0**-23)
+    assert ((out.cpu().double() - ref).abs() <= tol).all()

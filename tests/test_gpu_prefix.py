@@ -626,3 +626,24 @@ def test_attend_queries_with_one_large_dim(hq, hk, ntok, own, starts, prefix, sp
     score = 2.0**-21 * q.double().abs().amax(-1) * most + 128 * 2.0**-23 * big
     tol = ref.abs() * 2.0**-8 + mag * (2.0**-11 + torch.expm1(2 * score)[..., None] + 2.0**-19 + (seen[:, None, None] / 16 + 16) * 2.0**-23)
     assert ((out.cpu().double() - ref).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("hq,hk,ntok,own,starts,prefix", [
+    (6, 1, [2100], [2100], [], []),                                      # a prompt on its own keys
+    (12, 2, [4096, 1, 2001], [4096, 800, 3000], [], []),                 # prompts, one of them in a second chunk
+    (12, 2, [700, 442, 300], [1500, 442, 901], [0, 3], [4100])])         # prompt chunks behind a shared prefix
+def test_attend_long_prompts(hq, hk, ntok, own, starts, prefix):
+    t, pages = _tables(ntok, own, starts, prefix)
+    caches = _caches(pages, hk)
+    tokens = sum(ntok)
+    q = (torch.randn(tokens, hq, 128, generator=_gen(17)) * 2).bfloat16()
+    op = SharedPrefixAttnOp(hq, hk, DEV, max_tokens=tokens, max_seqs=len(own), max_groups=max(1, len(prefix)), k_scale=K_SCALE, v_scale=V_SCALE)
+    out = op(q.to(DEV), *(c.to(DEV) for c in caches), _dev(t)).cpu()
+    assert ops.guard_read(op.guard)[0] == 0
+    # some tokens, as sequences of one token each: token j of n sees its sequence's keys up to its own
+    pick = torch.unique(torch.cat([torch.arange(0, tokens, 97), torch.arange(40, 46), torch.tensor([tokens - 1]), torch.randperm(tokens, generator=_gen(1))[:40]]))
+    seq = torch.searchsorted(t.q_start[1:].long(), pick, right=True)
+    lens = t.lens[seq] - t.q_start[1:][seq] + pick.to(torch.int32) + 1
+    one = PrefixTables(torch.arange(len(pick) + 1, dtype=torch.int32), t.page_table[seq], lens.to(torch.int32),
+                       None if t.group_start is None else torch.tensor([0, len(pick)], dtype=torch.int32), t.prefix_table, t.prefix_lens)
+    _check_attend(out[pick], q[pick], caches, one, op)

@@ -682,7 +682,7 @@ typedef struct mono_prefix_attn_args {
     const int32_t* prefix_table; /* [groups][prefix_ld] */
     int prefix_ld;
     const int32_t* prefix_lens; /* [groups] */
-    float k_scale, v_scale, sm_scale;
+    float k_scale, v_scale, sm_scale; /* 2^-100 .. 2^100 each, k_scale sm_scale at most 2^100 */
     void* scratch; /* mono_prefix_attn_scratch_bytes(tokens, q_heads, kv_heads, seqs, groups); one launch at a time */
     size_t scratch_bytes;
     void* out; /* bf16 [tokens][q_heads][128] */

@@ -84,7 +84,7 @@ __device__ __forceinline__ void load_q(const mono_prefix_attn_args& a, const Ent
     // exponent field of the largest value, kept where 2^(13 - e) and its inverse are normal numbers
     const int e = clamp_int((int)(__float_as_uint(amax) >> 23), 30, 254);
     const float up = __uint_as_float((uint32_t)(267 - e) << 23);  // 2^(13 - (e - 127))
-    const float back = __uint_as_float((uint32_t)(e - 13) << 23) * (a.sm_scale * a.k_scale * 1.4426950408889634f);
+    const float back = score_scale(a, __uint_as_float((uint32_t)(e - 13) << 23));
 #pragma unroll
     for (int s = 0; s < 8; ++s)
 #pragma unroll
@@ -689,6 +689,10 @@ extern "C" int mono_prefix_attn_launch(const mono_prefix_attn_args* a, void* str
     if (a->q_ld < (long)a->q_heads * kDim || (a->q_ld & 7) || ((reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->out)) & 15) ||
         (reinterpret_cast<uintptr_t>(a->scratch) & 255) || !mono::scale_ok(a->k_scale) || !mono::scale_ok(a->v_scale) || !mono::scale_ok(a->sm_scale)) {
         mono_set_error("%s: q rows at least q_heads * 128 values apart (a multiple of 8) on 16-byte addresses, scratch on a 256-byte address and scales of 2^-100 .. 2^100 required", who);
+        return MONO_E_ARG;
+    }
+    if (a->k_scale * a->sm_scale > 0x1p100f) {
+        mono_set_error("%s: k_scale sm_scale of at most 2^100 required", who);
         return MONO_E_ARG;
     }
     if (a->n_pages < 1 || a->n_pages > (1ll << 31) / kPage - 1 || a->pt_ld > (1 << 24) || a->prefix_ld > (1 << 24)) {

@@ -53,6 +53,13 @@ __device__ __forceinline__ int row_limit(const Entry& n, int row, int G) {
     return n.causal ? n.len - n.ntok + 1 + row / G : n.len;
 }
 
+// What a product of a scaled query row is multiplied by to be a score in powers of two; `back` undoes the row's scale.  Not
+// 0, which would make NaN of the -inf of masked keys: products end at 2^30, so below 2^-126 every score is next to 0 anyway.
+__device__ __forceinline__ float score_scale(const mono_prefix_attn_args& a, float back) {
+    const float f = back * (a.sm_scale * a.k_scale * 1.4426950408889634f);
+    return f < 0x1p-126f ? 0x1p-126f : f;  // (NaN, of a row of NaN, stays)
+}
+
 // E4M3 bytes of NaN, as bit 7 of each.
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u; }
 // A weight of zero does not hide a NaN value from a matrix product.  So values of keys that not all rows of a tile see go to the

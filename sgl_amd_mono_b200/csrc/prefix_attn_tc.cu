@@ -460,7 +460,7 @@ __global__ void __launch_bounds__(kThreadsWide, 1) prefix_wide_kernel(const __gr
                 const bool join = x.join();  // stream 0 takes stream 1's part into its own
                 float m = -INFINITY, l = 0.f;
                 if (count > 0) {
-                    const float qs = mine ? __ldg(p.s.q_scale + x.image + row - x.row0) * (a.sm_scale * a.k_scale * 1.4426950408889634f) : 1.f;
+                    const float qs = mine ? score_scale(a, __ldg(p.s.q_scale + x.image + row - x.row0)) : 1.f;
                     const int lim = mine ? row_limit(x.en, row, G) : 0;
                     for (int t = 0; t < count; ++t) {
                         const int i = x.first(st) + t * x.step(), g = g0 + t;

@@ -210,10 +210,12 @@ class SharedPrefixAttnOp:
             raise ValueError(f"max_tokens {max_tokens}, max_seqs {max_seqs}, max_groups {max_groups}: needs at least one token and "
                              f"sequence, and at most {MAX_ENTRIES} sequences and groups")
         self.k_scale, self.v_scale = _scale(k_scale, "k_scale"), _scale(v_scale, "v_scale")
+        self.sm_scale = _scale(sm_scale, "sm_scale") if sm_scale is not None else HEAD_DIM ** -0.5
+        if self.k_scale * self.sm_scale > 2.0**100:
+            raise ValueError(f"sm_scale: {self.sm_scale}, needs at most 2**100 / k_scale")
         self.dev = _device(device)
         self.q_heads, self.kv_heads = q_heads, kv_heads
         self.max_tokens, self.max_seqs, self.max_groups = max_tokens, max_seqs, max_groups
-        self.sm_scale = _scale(sm_scale, "sm_scale") if sm_scale is not None else HEAD_DIM ** -0.5
         with torch.cuda.device(self.dev):
             nbytes = L.load().mono_prefix_attn_scratch_bytes(max_tokens, q_heads, kv_heads, max_seqs, max_groups)
         self.scratch = torch.zeros(nbytes, dtype=torch.uint8, device=self.dev)

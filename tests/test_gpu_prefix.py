@@ -647,3 +647,21 @@ def test_attend_long_prompts(hq, hk, ntok, own, starts, prefix):
     one = PrefixTables(torch.arange(len(pick) + 1, dtype=torch.int32), t.page_table[seq], lens.to(torch.int32),
                        None if t.group_start is None else torch.tensor([0, len(pick)], dtype=torch.int32), t.prefix_table, t.prefix_lens)
     _check_attend(out[pick], q[pick], caches, one, op)
+
+
+@pytest.mark.parametrize("k_scale,sm_scale", [(2.0**-40, None), (2.0**-100, 2.0**-100), (2.0**-100, 2.0**60), (2.0**100, 2.0**-100), (2.0**40, 2.0**-43)])
+def test_attend_small_scores_and_far_scales(k_scale, sm_scale):
+    """Scores next to 0 under the smallest scales weigh all visible keys alike, and masked keys not at all."""
+    hq, hk = 12, 2
+    t, pages = _tables([3, 1, 20], [40, 70, 30], [0, 3], [100])
+    caches = _caches(pages, hk)
+    q = torch.randn(24, hq, 128, generator=_gen(3)).bfloat16()
+    q[1, 4] = 0
+    q[2, 5] *= 2.0**-120
+    q[9, 7] = 0
+    q[13, 2] *= 2.0**-120
+    for n in (24, 4):  # entries of many rows, and of few
+        part = t if n == 24 else PrefixTables(t.q_start[:3], t.page_table[:2], t.lens[:2], torch.tensor([0, 2], dtype=torch.int32), t.prefix_table, t.prefix_lens)
+        op = SharedPrefixAttnOp(hq, hk, DEV, max_tokens=24, max_seqs=3, k_scale=k_scale, v_scale=V_SCALE, sm_scale=sm_scale)
+        out = op(q[:n].to(DEV), *(c.to(DEV) for c in caches), _dev(part))
+        _check_attend(out, q[:n], caches, part, op)

@@ -137,3 +137,10 @@ def test_restated_draw_keeps_the_first_alone_where_no_weight_passes():
     assert OP.sample_row(x, 0.9, min_p=1.0)[0] == 3
     for min_p in (float(np.nextafter(np.float32(1), np.float32(2))), 1.5, math.inf):
         assert OP.sample_row(x, 0.9, min_p=min_p)[0] == 1
+
+
+def test_attention_refuses_scales_whose_product_leaves_no_room_for_scores(lib):
+    assert lib.mono_prefix_attn_launch(C.byref(_attn_args(k_scale=2.0**60, sm_scale=2.0**41)), None) == -1
+    assert b"2^100" in lib.mono_last_error()
+    with pytest.raises(ValueError, match="sm_scale"):
+        SharedPrefixAttnOp(12, 2, "cuda:0", max_tokens=4, max_seqs=4, k_scale=2.0**60, sm_scale=2.0**41)

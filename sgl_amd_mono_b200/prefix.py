@@ -102,8 +102,10 @@ class QkvAppendOp:
     def __init__(self, q_heads: int, kv_heads: int, device, max_tokens: int, rot_dim: int = 64, interleaved: bool = False,
                  eps: float = 1e-6, k_scale: float = 1.0, v_scale: float = 1.0):
         _heads(q_heads, kv_heads)
-        if max_tokens < 1:
-            raise ValueError(f"max_tokens: {max_tokens}, needs at least 1")
+        if q_heads > 256:
+            raise ValueError(f"q_heads: {q_heads}, needs at most 256")
+        if not 1 <= max_tokens <= 1 << 24:
+            raise ValueError(f"max_tokens: {max_tokens}, needs 1..2**24")
         if rot_dim % 16 or not 16 <= rot_dim <= HEAD_DIM:
             raise ValueError(f"rot_dim: {rot_dim}, needs a multiple of 16 in 16..{HEAD_DIM}")
         if not float(eps) >= 0.0:
@@ -206,9 +208,9 @@ class SharedPrefixAttnOp:
                  k_scale: float = 1.0, v_scale: float = 1.0, sm_scale: float | None = None, guard: torch.Tensor | None = None,
                  deadline_s: float = 5.0):
         _heads(q_heads, kv_heads)
-        if max_tokens < 1 or max_seqs < 1 or max_groups < 0 or max_seqs + max_groups > MAX_ENTRIES:
-            raise ValueError(f"max_tokens {max_tokens}, max_seqs {max_seqs}, max_groups {max_groups}: needs at least one token and "
-                             f"sequence, and at most {MAX_ENTRIES} sequences and groups")
+        if not 1 <= max_tokens <= 1 << 20 or max_seqs < 1 or max_groups < 0 or max_seqs + max_groups > MAX_ENTRIES:
+            raise ValueError(f"max_tokens {max_tokens}, max_seqs {max_seqs}, max_groups {max_groups}: needs 1..2**20 tokens, at least "
+                             f"one sequence, and at most {MAX_ENTRIES} sequences and groups")
         self.k_scale, self.v_scale = _scale(k_scale, "k_scale"), _scale(v_scale, "v_scale")
         self.sm_scale = _scale(sm_scale, "sm_scale") if sm_scale is not None else HEAD_DIM ** -0.5
         if self.k_scale * self.sm_scale > 2.0**100:

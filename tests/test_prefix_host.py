@@ -144,3 +144,18 @@ def test_attention_refuses_scales_whose_product_leaves_no_room_for_scores(lib):
     assert b"2^100" in lib.mono_last_error()
     with pytest.raises(ValueError, match="sm_scale"):
         SharedPrefixAttnOp(12, 2, "cuda:0", max_tokens=4, max_seqs=4, k_scale=2.0**60, sm_scale=2.0**41)
+
+
+def test_ops_are_not_built_for_what_every_launch_refuses(lib):
+    """Each size at its largest passes the launch's check of it (and fails at the next), and so does the op."""
+    assert lib.mono_qkv_append_launch(C.byref(_append_args(q_heads=257)), None) == -1 and b"256 q heads" in lib.mono_last_error()
+    with pytest.raises(ValueError, match="q_heads"):
+        QkvAppendOp(272, 17, "cuda:0", max_tokens=4)
+    with pytest.raises(ValueError, match="device"):  # (what comes after the sizes)
+        QkvAppendOp(256, 16, "cpu", max_tokens=1 << 24)
+    with pytest.raises(ValueError, match="max_tokens"):
+        QkvAppendOp(12, 2, "cuda:0", max_tokens=(1 << 24) + 1)
+    with pytest.raises(ValueError, match="max_tokens"):
+        SharedPrefixAttnOp(12, 2, "cuda:0", max_tokens=(1 << 20) + 1, max_seqs=4)
+    with pytest.raises(ValueError, match="device"):
+        SharedPrefixAttnOp(12, 2, "cpu", max_tokens=1 << 20, max_seqs=4)

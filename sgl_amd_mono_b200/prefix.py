@@ -126,7 +126,9 @@ class QkvAppendOp:
     def __call__(self, qkv: torch.Tensor, g_q, g_k, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor, slots,
                  k_cache: torch.Tensor, v_cache: torch.Tensor, tokens: int | None = None) -> torch.Tensor:
         """``qkv``: bf16 ``[tokens, (q_heads + 2 kv_heads) * 128]`` (rows may lie further apart), or f32 partial sums
-        ``[nsum, rows, ..]`` of at most 16 ``tokens`` as the projection's GEMV leaves them (``tokens`` is then required).
+        ``[nsum, rows, ..]`` of at most 16 ``tokens`` as the projection's GEMV leaves them (``tokens`` is then required).  Of
+        wider rows, such as those of ``gqa.GqaConfig.qkv_rows`` with index heads at their end, the q | k | v part is given,
+        ``qkv[..., : (q_heads + 2 * kv_heads) * 128]``.
         ``g_q`` / ``g_k``: bf16 ``[128]``, None for no norm.  ``cos`` / ``sin``: bf16 or f32 ``[positions, rot_dim / 2]``.
         ``positions``, ``slots``: int64 ``[tokens]``; a position outside the table is taken to its nearest row, a slot
         (page * 64 + offset) outside the cache inserts nothing, and the slots inside it must differ.
@@ -147,12 +149,15 @@ class QkvAppendOp:
                 raise ValueError(f"qkv: rows {ld} values apart, needs a multiple of 8")
             a.src_bf16, a.src_ld = _aligned(qkv.data_ptr(), "qkv"), ld
         elif qkv.dtype is torch.float32:
-            if len(shape) != 3 or not qkv.is_contiguous() or shape[2] != width:
-                raise ValueError(f"qkv: shape {tuple(shape)}, needs contiguous f32 partial sums [nsum, rows, {width}]")
+            if len(shape) != 3 or shape[0] < 1 or shape[2] != width or qkv.stride(2) != 1 or (shape[1] > 1 and qkv.stride(1) < width):
+                raise ValueError(f"qkv: shape {tuple(shape)} strides {qkv.stride()}, needs f32 partial sums [nsum, rows, {width}] with contiguous rows")
             if tokens is None or not 1 <= tokens <= min(L.MAX_ROWS, shape[1]):
                 raise ValueError(f"tokens: {tokens}, partial sums of {shape[1]} rows serve 1..{min(L.MAX_ROWS, shape[1])}")
             n = tokens
-            a.src_f32, a.nsum, a.src_ld, a.sum_stride = _aligned(qkv.data_ptr(), "qkv"), shape[0], width, shape[1] * width
+            ld, apart = qkv.stride(1) if shape[1] > 1 else width, qkv.stride(0) if shape[0] > 1 else 0
+            if ld % 8 or apart % 4:
+                raise ValueError(f"qkv: rows {ld} and partial sums {apart} values apart, needs multiples of 8 and 4")
+            a.src_f32, a.nsum, a.src_ld, a.sum_stride = _aligned(qkv.data_ptr(), "qkv"), shape[0], ld, apart
         else:
             raise ValueError(f"qkv: dtype {qkv.dtype}, needs bfloat16 rows or float32 partial sums")
         if not 1 <= n <= self.max_tokens:

@@ -665,3 +665,34 @@ def test_attend_small_scores_and_far_scales(k_scale, sm_scale):
         op = SharedPrefixAttnOp(hq, hk, DEV, max_tokens=24, max_seqs=3, k_scale=k_scale, v_scale=V_SCALE, sm_scale=sm_scale)
         out = op(q[:n].to(DEV), *(c.to(DEV) for c in caches), _dev(part))
         _check_attend(out, q[:n], caches, part, op)
+
+
+@pytest.mark.parametrize("tokens,nsum,rows", [(1, 1, 1), (16, 3, 16), (9, 2, 9), (1, 4, 1)])
+def test_append_from_partial_sums_of_wider_rows(tokens, nsum, rows):
+    """The block-sparse layer's projection leaves its index heads behind q | k | v: the rows are taken where they lie."""
+    from sgl_amd_mono_b200.gqa import CFG_GQA
+
+    hq, hk, width = CFG_GQA.q_local, CFG_GQA.kv_local, CFG_GQA.qkv_rows
+    d, caches = _append_inputs(tokens, hq, hk, 64)
+    parts = torch.randn(nsum, rows, width, generator=_gen(3))
+    op = QkvAppendOp(hq, hk, DEV, max_tokens=16, k_scale=K_SCALE, v_scale=V_SCALE)
+    w = [d[k].to(DEV) for k in ("g_q", "g_k", "cos", "sin", "positions", "slots")]
+    kc, vc = (c.to(DEV) for c in caches)
+    part = parts.to(DEV)[..., : (hq + 2 * hk) * 128]
+    q = op(part, *w, kc, vc, tokens=tokens).clone()
+    x = torch.zeros(rows, (hq + 2 * hk) * 128)
+    for p in parts:
+        x = x + p[:, : x.shape[1]]
+    _check_append(q, kc, vc, x[:tokens], d, caches, hq, hk, False)
+    # the same bits as of rows that lie close
+    k2, v2 = (c.to(DEV) for c in caches)
+    assert torch.equal(op(part.contiguous(), *w, k2, v2, tokens=tokens), q) and torch.equal(k2, kc) and torch.equal(v2, vc)
+    for bad in (parts.to(DEV), parts.to(DEV)[..., 1 : 1 + x.shape[1]], part[0]):
+        with pytest.raises(ValueError, match="qkv"):
+            op(bad, *w, kc, vc, tokens=tokens)
+    if rows > 1:
+        odd = torch.zeros(nsum, rows, x.shape[1] + 4, device=DEV)[..., : x.shape[1]]
+        turned = part.transpose(1, 2).contiguous().transpose(1, 2)  # (of a single row that is the row itself)
+        for bad in (odd, turned):
+            with pytest.raises(ValueError, match="qkv"):
+                op(bad, *w, kc, vc, tokens=tokens)

@@ -26,6 +26,7 @@ HEAD_DIM = 128
 PAGE = 64
 MAX_GROUP = 16  # q heads per kv head
 MAX_ENTRIES = 2048  # sequences + prefix groups of one launch
+_VIEWS = 64  # views that an op keeps of one of its buffers
 
 
 def _device(device) -> torch.device:
@@ -73,9 +74,14 @@ def _caches(a, k_cache, v_cache, kv_heads: int, dev) -> None:
 
 
 def _front(views: dict, n: int) -> torch.Tensor:
-    """The first ``n`` rows of an op's buffer (``views[0]``), each view made once: a slice costs what a launch costs."""
+    """The first ``n`` rows of an op's buffer (``views[0]``), the views of some row counts kept: a slice costs what a launch
+    costs, and prompts come in any length."""
     v = views.get(n)
     if v is None:
+        if len(views) > _VIEWS:
+            base = views[0]
+            views.clear()
+            views[0] = base
         v = views[n] = views[0][:n]
     return v
 

@@ -11,6 +11,7 @@ import torch
 
 from oracle import prefix as OP
 from sgl_amd_mono_b200 import _lib as L
+from sgl_amd_mono_b200 import prefix
 from sgl_amd_mono_b200.build import build_library
 from sgl_amd_mono_b200.prefix import QkvAppendOp, SharedPrefixAttnOp
 from sgl_amd_mono_b200.sampling import SampleOp
@@ -159,3 +160,12 @@ def test_ops_are_not_built_for_what_every_launch_refuses(lib):
         SharedPrefixAttnOp(12, 2, "cuda:0", max_tokens=(1 << 20) + 1, max_seqs=4)
     with pytest.raises(ValueError, match="device"):
         SharedPrefixAttnOp(12, 2, "cpu", max_tokens=1 << 20, max_seqs=4)
+
+
+def test_an_op_keeps_few_views_of_its_buffers():
+    base = torch.arange(4000).view(1000, 4)
+    views = {0: base}
+    for n in list(range(1, 1001)) + [7, 7, 1000]:
+        v = prefix._front(views, n)
+        assert v.shape == (n, 4) and v.data_ptr() == base.data_ptr() and len(views) <= 100
+    assert prefix._front(views, 7) is prefix._front(views, 7) and views[0] is base

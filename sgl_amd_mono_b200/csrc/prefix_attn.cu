@@ -641,23 +641,26 @@ static int sm_or_default() {
     return n > 0 ? n : 148;
 }
 static size_t up256(size_t v) { return (v + 255) & ~size_t(255); }
-// Segments a launch may leave: one per CTA and one per item, for each head of a group.
-static size_t narrow_segments(size_t tokens, size_t q_heads, size_t kv_heads, size_t seqs, size_t groups) {
-    const size_t tiles = (tokens * (q_heads / kv_heads)) / 16 + 1;
-    return group_heads((int)kv_heads) * ((size_t)sm_or_default() + head_groups((int)kv_heads) * (2 * tiles + seqs + groups));
+// Segments a launch may leave: one per CTA and one per item, for each head of a group.  Tiles of 16 rows: an entry that the
+// narrow kernel has in a step of kWideStep rows or more fits one (two of half the size, if they have 8 rows); smaller steps
+// have at most kWideStep - 1 rows of sequences and as many of groups, so two full tiles of each beside one per entry.
+static size_t narrow_segments(size_t kv_heads, size_t seqs, size_t groups) {
+    static_assert(kWideRows <= kNarrowTile + 1 && 17 <= kNarrowTile + 1 && kWideStep - 1 <= 2 * kNarrowTile, "what the count says");
+    return group_heads((int)kv_heads) * ((size_t)sm_or_default() + head_groups((int)kv_heads) * (4 + seqs + groups));
 }
-// The wide kernel's entries have kWideRows rows at least, so there are at most 2 rows / kWideRows of them.
+// A token's rows lie in a sequence and, with groups, in a group.  The wide kernel's entries have kWideRows rows at least,
+// which bounds their number.
 static size_t wide_segments(size_t tokens, size_t q_heads, size_t kv_heads, size_t seqs, size_t groups) {
-    const size_t rows = tokens * (q_heads / kv_heads);
+    const size_t rows = tokens * (q_heads / kv_heads), kinds = groups ? 2 : 1;
     if (!wide_step((int)tokens, (int)(q_heads / kv_heads))) return 0;
-    return (size_t)sm_or_default() + kv_heads * (2 * (rows / kWideTile) + std::min(2 * (rows / kWideRows), seqs + groups));
+    return (size_t)sm_or_default() + kv_heads * (kinds * (rows / kWideTile) + std::min(kinds * (rows / kWideRows), seqs + groups));
 }
 // The wide kernel's queries (two planes of 128 bytes a row) and their scales; none where no entry can have so many rows.
 static size_t image_bytes(size_t tokens, size_t q_heads, size_t kv_heads) {
     return !wide_step((int)tokens, (int)(q_heads / kv_heads)) ? 0 : up256(tokens * q_heads * 256) + up256(tokens * q_heads * 4);
 }
-static size_t narrow_bytes(int tokens, int q_heads, int kv_heads, int seqs, int groups) {
-    return up256(narrow_segments(tokens, q_heads, kv_heads, seqs, groups) * seg_floats(kNarrowTile) * sizeof(float));
+static size_t narrow_bytes(int kv_heads, int seqs, int groups) {
+    return up256(narrow_segments(kv_heads, seqs, groups) * seg_floats(kNarrowTile) * sizeof(float));
 }
 
 }  // namespace prefix_attn
@@ -665,7 +668,7 @@ static size_t narrow_bytes(int tokens, int q_heads, int kv_heads, int seqs, int 
 extern "C" size_t mono_prefix_attn_scratch_bytes(int tokens, int q_heads, int kv_heads, int seqs, int groups) {
     using namespace prefix_attn;
     if (tokens < 1 || q_heads < 1 || kv_heads < 1 || seqs < 1 || groups < 0 || q_heads % kv_heads) return 0;
-    return up256((size_t)(seqs + groups) * sizeof(Record)) + 256 + 2 * up256((size_t)tokens * 4) + image_bytes(tokens, q_heads, kv_heads) + narrow_bytes(tokens, q_heads, kv_heads, seqs, groups) +
+    return up256((size_t)(seqs + groups) * sizeof(Record)) + 256 + 2 * up256((size_t)tokens * 4) + image_bytes(tokens, q_heads, kv_heads) + narrow_bytes(kv_heads, seqs, groups) +
            wide_segments(tokens, q_heads, kv_heads, seqs, groups) * seg_floats(kWideTile) * sizeof(float);
 }
 
@@ -736,7 +739,7 @@ extern "C" int mono_prefix_attn_launch(const mono_prefix_attn_args* a, void* str
     p.s.q_scale = reinterpret_cast<float*>(at + up256((size_t)a->tokens * a->q_heads * 256));
     at += image_bytes(a->tokens, a->q_heads, a->kv_heads);
     p.s.seg[0] = reinterpret_cast<float*>(at);
-    p.s.seg[1] = reinterpret_cast<float*>(at + narrow_bytes(a->tokens, a->q_heads, a->kv_heads, a->seqs, a->groups));
+    p.s.seg[1] = reinterpret_cast<float*>(at + narrow_bytes(a->kv_heads, a->seqs, a->groups));
     const cudaStream_t st = (cudaStream_t)stream;
     constexpr size_t fixed = 1024 + kStages * 2 * kTileBytes + 4 * kNarrowTile * kPitch * sizeof(float);
     const size_t smem = fixed + 2 * (size_t)(a->seqs + a->groups + 1) * 4;

@@ -696,3 +696,26 @@ def test_append_from_partial_sums_of_wider_rows(tokens, nsum, rows):
         for bad in (odd, turned):
             with pytest.raises(ValueError, match="qkv"):
                 op(bad, *w, kc, vc, tokens=tokens)
+
+
+@pytest.mark.parametrize("hq,hk,ntok,own,starts,prefix", [
+    (72, 9, [2, 0] * 20, [9, 0] * 20, list(range(0, 41, 2)), [5] * 20),   # two full tiles of 8 rows of every sequence and group
+    (8, 8, [16] + [0] * 15 + [1] * 3, [40] + [0] * 15 + [300] * 3, [0, 16, 19], [70, 90]),
+    (32, 2, [1] * 2, [700, 800], [0, 1, 2], [900, 300]),                  # fewer rows than the other kernel is started for
+    (7, 7, [4] * 8, [10 + i for i in range(8)], [0, 4, 8], [65, 200]),
+    (16, 1, [16, 1, 15, 1], [16, 40, 500, 1], [], [])])
+def test_attend_scratch_holds_what_a_step_leaves(hq, hk, ntok, own, starts, prefix):
+    """Steps of as many parts of tiles as their sizes allow, on a scratch of just the size asked for."""
+    t, pages = _tables(ntok, own, starts, prefix)
+    caches = _caches(pages, hk)
+    tokens = sum(ntok)
+    q = torch.randn(tokens, hq, 128, generator=_gen(8)).bfloat16()
+    op = SharedPrefixAttnOp(hq, hk, DEV, max_tokens=tokens, max_seqs=len(own), max_groups=len(prefix), k_scale=K_SCALE, v_scale=V_SCALE)
+    size = op.scratch.numel()
+    room = torch.full((size + 8192,), 0xA5, dtype=torch.uint8, device=DEV)
+    op._fixed.scratch = room.data_ptr()
+    assert room.data_ptr() % 256 == 0
+    out = op(q.to(DEV), *(c.to(DEV) for c in caches), _dev(t))
+    assert ops.guard_read(op.guard)[0] == 0
+    _check_attend(out, q, caches, t, op)
+    assert (room[size:] == 0xA5).all()

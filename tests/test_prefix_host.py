@@ -169,3 +169,18 @@ def test_an_op_keeps_few_views_of_its_buffers():
         v = prefix._front(views, n)
         assert v.shape == (n, 4) and v.data_ptr() == base.data_ptr() and len(views) <= 100
     assert prefix._front(views, 7) is prefix._front(views, 7) and views[0] is base
+
+
+def test_attention_scratch_of_long_prompts(lib):
+    """What 16384 tokens of 48 heads need: their rows in f32 once for a sequence and once for a group, and their queries."""
+    f = lib.mono_prefix_attn_scratch_bytes
+    rows = 16384 * 48
+    assert f(16384, 48, 8, 1, 0) < 1.25 * rows * (128 * 4 + 256)
+    assert f(16384, 48, 8, 4, 1) < 1.25 * rows * (2 * 128 * 4 + 256)
+    # a step of fewer tokens, sequences or groups fits what was reserved for more
+    sizes = [(t, s, g) for t in (1, 2, 5, 6, 33, 200, 3001) for s in (1, 3, 40) for g in (0, 1, 7)]
+    for hq, hk in ((12, 2), (48, 8), (72, 9), (5, 5)):
+        for a in sizes:
+            for b in sizes:
+                if all(x <= y for x, y in zip(a, b)):
+                    assert f(a[0], hq, hk, a[1], a[2]) <= f(b[0], hq, hk, b[1], b[2])

@@ -107,6 +107,7 @@ __device__ __forceinline__ void load_q(const mono_prefix_attn_args& a, const Ent
 // Both products are formed transposed: S^T[key][row] = K Q^T and O^T[dim][row] += V^T P^T, with keys and dims as the 16
 // rows of the fragments and NT times 8 query rows as their columns: one token's heads are at most eight as a rule, and as
 // the 16 rows they left most of the work empty.  P^T is turned from result to operand by two 8 x 8 transpositions.
+// (Two tiles of eight rows take all 168 registers, and 72 bytes a thread are spilled.)
 template <int NT>
 __global__ void __launch_bounds__(kThreads, 1) prefix_narrow_kernel(const __grid_constant__ Params p) {
     constexpr int kTile = 8 * NT;

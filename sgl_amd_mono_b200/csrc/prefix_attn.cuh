@@ -121,7 +121,7 @@ __device__ __forceinline__ Work entry_work(const mono_prefix_attn_args& a, const
 
 // How the SMs are shared between the two kernels, which run side by side: a start, a plan and an end cost each of them some
 // 8 us, and what one leaves of HBM or of the SMs the other uses (one after the other 64 samples of a long prompt took 103
-// us, side by side 80).  In proportion to their work, a wide unit taken as kWideCost and a narrow one as kNarrowCost for
+// us, side by side 80, and 83 since the wide kernel waits for a block's values by a barrier of its own).  In proportion to their work, a wide unit taken as kWideCost and a narrow one as kNarrowCost for
 // every eight rows of its tile (64 samples: 84, 84, 94 and 107 us at ratios of 5, 6, 4 and 3 to 9; 24 samples in tiles of
 // 16 rows: 47 to 53 at 6 to 13 to 9, 62 at 4).  Each has at least one CTA, which leaves the merge's records.
 constexpr int kWideCost = 3, kNarrowCost = 2;

@@ -9,7 +9,8 @@
 // Bound: memory.  A token's row is read once and written once (bf16 q, one byte per K and V value).  Sixteen lanes hold
 // a head, eight dims (16 bytes) each, so a warp takes two heads at a time and a norm is four shuffles.  Four pairs of heads
 // are in flight, and what a token and kind multiply by is made once for all its heads.  Measured (48 q heads on 8, B200):
-// 16384 tokens 87 us, 5827 GB/s, 89 % of a copy; 2001 tokens 16.3 us; 16 tokens of 12 heads on 2 2.3 us, a launch.
+// 16384 tokens 87 us, 5804 GB/s, 89 % of a copy (pairs by halves 91 us); 2001 tokens 16.3 us; 16 tokens of 12 heads on 2
+// 2.3 us, a launch, from four partial sums 2.8 us.
 #include "mono_common.cuh"
 
 extern void mono_set_error(const char* fmt, ...);
@@ -20,7 +21,7 @@ using namespace mono;
 constexpr int kDim = 128;
 constexpr int kThreads = 256;
 // CTAs of an SM: with four, halves that turn with one another (their partners come by shuffles) do not fit 64 registers
-// (16384 tokens 101 us, with three 92), interleaved pairs do (84 us, with three 87).  Partial sums have at most 16 rows.
+// (16384 tokens 100 us, with three 91), interleaved pairs do (87 us either way).  Partial sums have at most 16 rows.
 constexpr int ctas_per_sm(bool interleaved, bool f32) { return f32 ? 2 : interleaved ? 4 : 3; }
 
 typedef unsigned long long f32x2;  // two f32 that one instruction works on

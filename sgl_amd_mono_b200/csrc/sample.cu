@@ -22,10 +22,13 @@
 //      bins with counts and masses, and the bin that holds the border is searched again.
 // Then each warp's run of kept mass says which warp walks to the token.
 //
-// Bound: latency for few rows (the cluster's barriers, and code that a launch runs once); for many the f64 pipe and issue
-// slots (some 12 f64 operations a weight).  Measured, 129280 f32 logits: 1 row 22 us, 16 rows with all filters 36 us, 256
-// rows, one in eight with top-p, 157 us (843 GB/s).  A row's CTAs live 12 us without a filter: 4 for the load, 1 for the
-// maximum, 5 to 7 for Z; 30 with a top-p border deep in the bulk, whose rows are weighed a second time.
+// Bound: latency.  For few rows of the cluster's barriers, and of code that a launch runs once.  Many rows go in waves of
+// clusters, two CTAs an SM, whose loads, maxima and weights take turns and hardly cover each other: HBM alone would take 20
+// us for 256 rows, the f64 pipe (some 12 operations a weight) 22.  Measured, 129280 f32 logits: 1 row 22 us, 16 rows with all
+// filters 36 us, 256 rows, one in eight with top-p, 158 us (835 GB/s); without a filter 121 us, of bf16 logits 102 us; 129281
+// logits, rows at any address, as 129280.  A row's CTAs live 12 us without a filter: 4 for the load, 1 for the maximum, 5 to
+// 7 for Z; 30 with a top-p border deep in the bulk, whose rows are weighed a second time.  (Two CTAs an SM leave 64 registers a
+// thread; the kernel of two CTAs a row spills 44 bytes of them.)
 #include <cooperative_groups.h>
 
 #include <cmath>

@@ -280,3 +280,14 @@ def test_min_p_above_one_keeps_the_first_of_the_largest_alone(vocab):
     token = _check(x, u, min_p=mp)
     assert int(token[0]) > 1 and token[1:].tolist() == [1] * 5
     _check(x, u, torch.full((6,), 0.3), torch.full((6,), 3, dtype=torch.int32), torch.full((6,), 0.9), mp)
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_the_largest_vocabulary(rows):
+    vocab = 393216
+    x, u = _logits(rows, vocab, 21), _u(rows, 22)
+    x[0] = 1.25  # all alike
+    p = torch.where(torch.arange(rows) % 2 == 0, torch.full((rows,), 0.9), torch.ones(rows))
+    k = torch.where(torch.arange(rows) % 3 == 2, torch.full((rows,), 200000), torch.zeros(rows)).to(torch.int32)
+    _check(x, u)
+    _check(x, u, top_k=k, top_p=p)

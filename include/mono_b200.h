@@ -664,7 +664,8 @@ int mono_qkv_append_launch(const mono_qkv_append_args* a, void* stream);
  * prefix_lens[g] keys in pages prefix_table[g][..].  Token j of a sequence's n sees its group's prefix and the
  * sequence's keys 0 .. lens[b] - n + j.  out = softmax((q . k) k_scale sm_scale) v v_scale; a token that sees no key
  * gives zeros, tokens of no sequence keep their output row.  Where many rows share their keys a query's values are exact
- * within 2^13 of the row's largest, and held to 2^-21 of the largest below that; weights are f16 in their product with v.  A page number outside the cache counts as a page without
+ * within 2^13 of the row's largest, and held to 2^-21 of the largest below that; weights are f16 in their product with v
+ * (2^-11 of themselves; below 2^-21 of a row's largest, 2^-32 of the largest).  A page number outside the cache counts as a page without
  * keys.  Lengths beyond their table's columns are cut.  Both starts must never fall and stay in range: otherwise the
  * guard's argument word is set and the output is not valid.  The tables are device data: a captured launch follows them. */
 typedef struct mono_prefix_attn_args {

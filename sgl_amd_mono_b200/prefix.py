@@ -212,7 +212,8 @@ class SharedPrefixAttnOp:
     ``softmax((q . k) k_scale sm_scale) v v_scale``; a token that sees no key gives zeros, and rows of ``out`` behind
     the last sequence's tokens keep what they held.  Scores are f32; where many rows share their keys, a query's values are
     held exactly within 2^13 of the row's largest, and to 2^-21 of the largest below that.  Weights are rounded to f16 for
-    their product with the values.  ``guard`` holds the error words (``ops.guard_read``): starts that
+    their product with the values: to 2^-11 of themselves, those below 2^-21 of a row's largest to 2^-32 of the largest.
+    ``guard`` holds the error words (``ops.guard_read``): starts that
     fall or leave their range set the argument word."""
 
     def __init__(self, q_heads: int, kv_heads: int, device, max_tokens: int, max_seqs: int, max_groups: int = 1,
